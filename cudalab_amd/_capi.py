@@ -30,6 +30,7 @@ CQ_OP_GEMV_F32 = 3
 
 CQ_DTYPE_F16 = 0
 CQ_DTYPE_F32 = 1
+CQ_DTYPE_BF16 = 2
 
 # quantizer scale forms: amax / qmax (torch on the CPU) or amax * fl(1/qmax)
 # (torch on a GPU)
@@ -85,7 +86,46 @@ class CqPrepared(ctypes.Structure):
 
 
 _vp = ctypes.c_void_p
+_i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
+
+
+class CqNormRope(ctypes.Structure):
+    """cq_norm_rope_t"""
+    _fields_ = [(n, _vp) for n in ("q", "k", "q_out", "k_out")] + [
+        (n, _i64) for n in ("q_token_stride", "q_head_stride", "k_token_stride",
+                            "k_head_stride", "q_out_token_stride", "q_out_head_stride",
+                            "k_out_token_stride", "k_out_head_stride")] + [
+        (n, _vp) for n in ("q_weight", "k_weight", "cos_table", "sin_table",
+                           "positions")] + [
+        (n, _i64) for n in ("tokens", "table_rows")] + [
+        (n, _i32) for n in ("q_heads", "k_heads", "head_dim", "rot_dim", "dtype",
+                            "weight_dtype", "positions_64", "interleaved")] + [
+        ("eps", ctypes.c_float)]
+
+
+class CqKvCache(ctypes.Structure):
+    """cq_kv_cache_t"""
+    _fields_ = [("k", _vp), ("v", _vp), ("scales", _vp), ("pages", _i64),
+                ("heads", _i32), ("head_dim", _i32), ("page_size", _i32), ("bits", _i32)]
+
+
+class CqKvSlots(ctypes.Structure):
+    """cq_kv_slots_t"""
+    _fields_ = [("table", _vp), ("starts", _vp), ("counts", _vp), ("table_stride", _i64),
+                ("table_cols", _i32), ("batch", _i32), ("tokens", _i32)]
+
+
+class CqAttention(ctypes.Structure):
+    """cq_attention_t"""
+    _fields_ = [("q", _vp), ("out", _vp)] + [
+        (n, _i64) for n in ("q_batch_stride", "q_token_stride", "q_head_stride")] + [
+        (n, _vp) for n in ("table", "lengths", "counts", "prefix_table")] + [
+        ("table_stride", _i64), ("workspace", _vp), ("workspace_bytes", _i64)] + [
+        (n, _i32) for n in ("table_cols", "prefix_cols", "prefix_len", "batch", "tokens",
+                            "q_heads", "dtype")] + [("softmax_scale", ctypes.c_float)]
+
+
 _cstr = ctypes.c_char_p
 
 # name -> (restype, argtypes); must match include/cdnaqgemv.h
@@ -144,6 +184,16 @@ SIGNATURES = {
     "cq_prepare": (ctypes.c_int, [ctypes.c_int, _cstr, _vp, _vp, _vp, _vp,
                                   _i64, _i64, ctypes.POINTER(CqPrepared)]),
     "cq_launch_prepared": (ctypes.c_int, [_vp, _vp]),
+    "cq_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(CqNormRope), _vp]),
+    "cq_kv_append": (ctypes.c_int, [
+        ctypes.POINTER(CqKvCache), ctypes.POINTER(CqKvSlots), ctypes.c_int, _vp, _i64,
+        _i64, _i64, _vp, _i64, _i64, _i64, _vp]),
+    "cq_kv_read": (ctypes.c_int, [ctypes.POINTER(CqKvCache), ctypes.POINTER(CqKvSlots),
+                                  ctypes.c_int, _vp, _vp, _vp]),
+    "cq_attention": (ctypes.c_int, [ctypes.POINTER(CqKvCache),
+                                    ctypes.POINTER(CqAttention), _vp]),
+    "cq_attention_workspace": (_i64, [ctypes.POINTER(CqKvCache),
+                                      ctypes.POINTER(CqAttention)]),
     "cq_last_error": (ctypes.c_char_p, []),
     "cq_version": (ctypes.c_char_p, []),
 }

@@ -45,7 +45,8 @@ LIB_NAME = "libcdnaqgemv.so"
 LIB_PATH = LIB_DIR / LIB_NAME
 
 ARCH = "gfx950"
-SOURCES = ("cq_kernels.hip", "cq_quantize.hip", "cq_capi.cpp")
+SOURCES = ("cq_kernels.hip", "cq_quantize.hip", "cq_norm_rope.hip", "cq_kvcache.hip",
+           "cq_attention.hip", "cq_capi.cpp", "cq_attn_capi.cpp")
 # the Python binding of the eager fast path (host code only, built with the
 # host compiler against torch's headers; it calls the library by address)
 FAST_SOURCE = "cq_pyfast.cpp"
@@ -184,8 +185,8 @@ def build_library(verbose: bool = False) -> Path:
 
 
 def build(op: str):
-    """Extension object for `op` ("int4gemv" | "qgemv" | "gemv"), bound to the built
-    library.  Mirrors `cudalab/build.py:build(op)` (which returned the JIT
+    """Extension object for `op` ("int4gemv" | "qgemv" | "gemv" | "attention"), bound
+    to the built library.  Mirrors `cudalab/build.py:build(op)` (which returned the JIT
     module); raises if the library has not been built."""
     from . import ext
     return ext.get_ext(op)

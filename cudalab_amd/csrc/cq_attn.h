@@ -1,0 +1,38 @@
+// Internal interface of the operators around attention: the C entry points
+// (cq_attn_capi.cpp) check a call's arguments and hand them on unchanged to
+// the launchers (cq_kvcache.hip, cq_attention.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <cstdint>
+#include <string>
+
+#include "cdnaqgemv.h"
+
+namespace cq {
+
+// Sets the calling thread's cq_last_error() text and returns `code`
+// (cq_capi.cpp).
+int set_error(int code, const std::string& msg);
+
+// Workgroups a launch may have (the grid's x dimension).
+constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+
+// Launchers: arguments are checked, sizes are positive.  A launcher that
+// finds its grid beyond kMaxGrid returns hipErrorInvalidValue unlaunched.
+hipError_t launch_norm_rope(const cq_norm_rope_t& a, hipStream_t stream);
+// Element strides of k or v [batch, tokens, heads, head_dim].
+struct KvStrides {
+    int64_t batch, token, head;
+};
+hipError_t launch_kv_append(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int dtype,
+                            const void* k, KvStrides ks, const void* v, KvStrides vs,
+                            hipStream_t stream);
+hipError_t launch_kv_read(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int dtype,
+                          void* k_out, void* v_out, hipStream_t stream);
+
+int64_t attention_workspace(const cq_kv_cache_t& c, const cq_attention_t& a);
+hipError_t launch_attention(const cq_kv_cache_t& c, const cq_attention_t& a,
+                            hipStream_t stream);
+
+}  // namespace cq

@@ -12,6 +12,7 @@
 // tensors; this layer sees only pointers and sizes.
 
 #include "cdnaqgemv.h"
+#include "cq_attn.h"
 #include "cq_internal.h"
 
 #include <hip/hip_runtime.h>
@@ -540,6 +541,10 @@ int timed_window(Go go, hipStream_t s, const Window& w, float* kernel_us,
 }
 
 }  // namespace
+
+namespace cq {
+int set_error(int code, const std::string& msg) { return fail(code, msg); }
+}  // namespace cq
 
 extern "C" {
 

@@ -1,0 +1,272 @@
+// Per-head RMS norm of queries and keys with the position rotation in the
+// same pass (gfx950).
+//
+//   n = x * (1 / sqrt(mean(x^2) + eps)) * weight
+//   a' = a cos - b sin, b' = b cos + a sin  for the pairs the rotation turns
+//
+// in FP32, rounded once.  Rounding the normed value to the element type before
+// the rotation, as a chain of separate calls would, is left out: one rounding
+// is closer to the formula.
+//
+// Bound by memory: each element is read and written once, and the tables'
+// rows of a token serve all its heads.  LANES lanes take a head, eight
+// elements each: the lane that holds a holds its b too, so the rotation needs
+// no exchange, and the only one is the sum of squares.
+
+#include <algorithm>
+
+#include "cq_attn.h"
+#include "cq_elem.h"
+
+namespace cq {
+namespace {
+
+constexpr int kBlock = 256;
+
+__device__ __forceinline__ float load_weight(const void* p, int dtype, int i) {
+    if (dtype == CQ_DTYPE_F16) return (float)static_cast<const _Float16*>(p)[i];
+    if (dtype == CQ_DTYPE_BF16) return (float)static_cast<const __bf16*>(p)[i];
+    return static_cast<const float*>(p)[i];
+}
+
+// Row of the cos/sin tables of a token, or -1 for a position outside them.
+__device__ __forceinline__ int64_t table_row(const cq_norm_rope_t& a, int64_t token) {
+    const int64_t p = a.positions_64 ? static_cast<const int64_t*>(a.positions)[token]
+                                     : static_cast<const int32_t*>(a.positions)[token];
+    return p >= 0 && p < a.table_rows ? p : -1;
+}
+
+// One head's place: heads count through q's, then k's.
+template <class T>
+struct Head {
+    const T* src;
+    T* dst;
+    bool is_q;
+    __device__ __forceinline__ Head(const cq_norm_rope_t& a, int64_t token, int h) {
+        is_q = h < a.q_heads;
+        if (is_q) {
+            src = static_cast<const T*>(a.q) + token * a.q_token_stride + h * a.q_head_stride;
+            dst = static_cast<T*>(a.q_out) + token * a.q_out_token_stride +
+                  h * a.q_out_head_stride;
+        } else {
+            h -= a.q_heads;
+            src = static_cast<const T*>(a.k) + token * a.k_token_stride + h * a.k_head_stride;
+            dst = static_cast<T*>(a.k_out) + token * a.k_out_token_stride +
+                  h * a.k_out_head_stride;
+        }
+    }
+};
+
+// Vector kernel: head_dim and rot_dim multiples of 8, head_dim <= 8 * LANES,
+// rows and weights aligned to four elements, tables to 16 bytes.  A group of
+// LANES lanes takes heads part, part + parts, ... of one token, BATCH loads in
+// flight; lane l holds elements e0..e0+3 and e1..e1+3, in the half style the
+// two ends of pairs 4l..4l+3, else eight neighbours.
+template <class T, bool PAIRS, int LANES, int BATCH>
+__global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uint32_t parts,
+                                                           uint32_t iters) {
+    using V = Vec<T, 4>;
+    const int lane = threadIdx.x % LANES;
+    const uint32_t group = blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+    const int heads = a.q_heads + a.k_heads;
+    // groups past the last token repeat it and store nothing
+    const bool live = group / parts < a.tokens;
+    const int64_t token = live ? group / parts : a.tokens - 1;
+    const uint32_t part = group % parts;
+    const bool active = 8 * lane < a.head_dim;
+    const bool turn = a.cos_table != nullptr && 8 * lane < a.rot_dim;
+    const bool halves = turn && !PAIRS;
+    const int e0 = !active ? 0 : halves ? 4 * lane : 8 * lane;
+    const int e1 = !active ? 4 : halves ? a.rot_dim / 2 + 4 * lane : 8 * lane + 4;
+
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (turn) {
+        const int64_t row = table_row(a, token);
+        if (row >= 0) {
+            const int64_t at = row * (a.rot_dim / 2) + 4 * lane;
+            const Vec<float, 4> cv = *reinterpret_cast<const Vec<float, 4>*>(a.cos_table + at);
+            const Vec<float, 4> sv = *reinterpret_cast<const Vec<float, 4>*>(a.sin_table + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = cv[i], s[i] = sv[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = s[i] = __builtin_nanf("");
+        }
+    }
+    const bool norm = a.q_weight != nullptr || a.k_weight != nullptr;
+    float wq[8], wk[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int e = i < 4 ? e0 + i : e1 + i - 4;
+        wq[i] = a.q_weight != nullptr ? load_weight(a.q_weight, a.weight_dtype, e) : 1.f;
+        wk[i] = a.k_weight != nullptr ? load_weight(a.k_weight, a.weight_dtype, e) : 1.f;
+    }
+    const float mean = 1.f / (float)a.head_dim;
+
+    for (uint32_t it = 0; it < iters; it += BATCH) {
+        V x0[BATCH], x1[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            const int h = (int)min(part + (it + u) * parts, (uint32_t)heads - 1);
+            const Head<T> head(a, token, h);
+            x0[u] = *reinterpret_cast<const V*>(head.src + e0);
+            x1[u] = *reinterpret_cast<const V*>(head.src + e1);
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            const uint32_t h = part + (it + u) * parts;
+            const Head<T> head(a, token, (int)min(h, (uint32_t)heads - 1));
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = (float)x0[u][i], f[4 + i] = (float)x1[u][i];
+            if (norm) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
+                ss = lanes_sum<LANES>(active ? ss : 0.f);
+                const bool has = head.is_q ? a.q_weight != nullptr : a.k_weight != nullptr;
+                const float r = has ? 1.f / sqrtf(ss * mean + a.eps) : 1.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = f[i] * r * (head.is_q ? wq[i] : wk[i]);
+            }
+            if (turn) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float& p = f[PAIRS ? 2 * i : i];
+                    float& q = f[PAIRS ? 2 * i + 1 : 4 + i];
+                    const float t = p * c[i] - q * s[i];
+                    q = q * c[i] + p * s[i];
+                    p = t;
+                }
+            }
+            V y0, y1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y0[i] = (T)f[i], y1[i] = (T)f[4 + i];
+            if (live && active && h < (uint32_t)heads) {
+                *reinterpret_cast<V*>(head.dst + e0) = y0;
+                *reinterpret_cast<V*>(head.dst + e1) = y1;
+            }
+        }
+    }
+}
+
+// Element kernel (any even dims, any alignment): one wave per head, pairs
+// lane, lane + 64, ... held between the sum and the rotation.
+constexpr int kMaxPairs = 8;      // head_dim <= 1024
+
+template <class T>
+__global__ __launch_bounds__(kBlock) void norm_rope_any_kernel(cq_norm_rope_t a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
+    const int heads = a.q_heads + a.k_heads;
+    const int64_t token = unit / heads;
+    if (token >= a.tokens) return;                 // uniform over the wave
+    const Head<T> head(a, token, (int)(unit % heads));
+    const void* weight = head.is_q ? a.q_weight : a.k_weight;
+    const int half = a.cos_table != nullptr ? a.rot_dim / 2 : 0;
+    const int64_t row = half > 0 ? table_row(a, token) : 0;
+    float p[kMaxPairs], q[kMaxPairs];
+    float ss = 0.f;
+    auto places = [&](int pair, int& e0, int& e1) {
+        const bool halves = pair < half && !a.interleaved;
+        e0 = halves ? pair : 2 * pair;
+        e1 = halves ? pair + half : 2 * pair + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < kMaxPairs; ++i) {
+        const int pair = lane + 64 * i;
+        p[i] = q[i] = 0.f;
+        if (2 * pair < a.head_dim) {
+            int e0, e1;
+            places(pair, e0, e1);
+            p[i] = (float)head.src[e0];
+            q[i] = (float)head.src[e1];
+            ss = __builtin_fmaf(p[i], p[i], ss);
+            ss = __builtin_fmaf(q[i], q[i], ss);
+        }
+    }
+    ss = lanes_sum<64>(ss);
+    const float r = weight != nullptr ? 1.f / sqrtf(ss * (1.f / (float)a.head_dim) + a.eps) : 1.f;
+#pragma unroll
+    for (int i = 0; i < kMaxPairs; ++i) {
+        const int pair = lane + 64 * i;
+        if (2 * pair >= a.head_dim) continue;
+        int e0, e1;
+        places(pair, e0, e1);
+        float x = p[i], y = q[i];
+        if (weight != nullptr) {
+            x = x * r * load_weight(weight, a.weight_dtype, e0);
+            y = y * r * load_weight(weight, a.weight_dtype, e1);
+        }
+        if (pair < half) {
+            const float c = row >= 0 ? a.cos_table[row * half + pair] : __builtin_nanf("");
+            const float s = row >= 0 ? a.sin_table[row * half + pair] : __builtin_nanf("");
+            const float t = x * c - y * s;
+            y = y * c + x * s;
+            x = t;
+        }
+        head.dst[e0] = (T)x;
+        head.dst[e1] = (T)y;
+    }
+}
+
+bool multiple(int64_t v, int64_t m) { return v % m == 0; }
+
+// Whether the vector kernel may run: everything it reads or writes as four
+// elements starts at a multiple of them.
+bool vector_ok(const cq_norm_rope_t& a, int64_t elem) {
+    auto rows_ok = [&](const void* p, int64_t ts, int64_t hs) {
+        return multiple((int64_t)(uintptr_t)p, 4 * elem) && multiple(ts, 4) && multiple(hs, 4);
+    };
+    if (a.head_dim % 8 != 0 || a.head_dim > 512) return false;
+    if (a.cos_table != nullptr &&
+        (a.rot_dim % 8 != 0 || !multiple((int64_t)(uintptr_t)a.cos_table, 16) ||
+         !multiple((int64_t)(uintptr_t)a.sin_table, 16)))
+        return false;
+    if (a.q_heads > 0 && !(rows_ok(a.q, a.q_token_stride, a.q_head_stride) &&
+                           rows_ok(a.q_out, a.q_out_token_stride, a.q_out_head_stride)))
+        return false;
+    return a.k_heads == 0 || (rows_ok(a.k, a.k_token_stride, a.k_head_stride) &&
+                              rows_ok(a.k_out, a.k_out_token_stride, a.k_out_head_stride));
+}
+
+template <class T, bool PAIRS>
+hipError_t launch_typed(const cq_norm_rope_t& a, hipStream_t stream) {
+    const int64_t heads = (int64_t)a.q_heads + a.k_heads;
+    if (!vector_ok(a, sizeof(T))) {
+        const int64_t units = a.tokens * heads, grid = (units + kBlock / 64 - 1) / (kBlock / 64);
+        if (grid > kMaxGrid) return hipErrorInvalidValue;
+        norm_rope_any_kernel<T><<<dim3((unsigned)grid), dim3(kBlock), 0, stream>>>(a);
+        return hipGetLastError();
+    }
+    const int lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : a.head_dim <= 256 ? 32 : 64;
+    const int batch = 1;
+    const int64_t iters = 1, parts = (heads + iters - 1) / iters;
+    const int64_t groups = a.tokens * parts, per = kBlock / lanes;
+    const int64_t grid = (groups + per - 1) / per;
+    if (groups + per > kMaxGrid) return hipErrorInvalidValue;
+    auto go = [&](auto* kernel) {
+        kernel<<<dim3((unsigned)grid), dim3(kBlock), 0, stream>>>(a, (uint32_t)parts,
+                                                                  (uint32_t)iters);
+        return hipGetLastError();
+    };
+    (void)batch;
+    if (lanes == 8) return go(&norm_rope_kernel<T, PAIRS, 8, 1>);
+    if (lanes == 16) return go(&norm_rope_kernel<T, PAIRS, 16, 1>);
+    if (lanes == 32) return go(&norm_rope_kernel<T, PAIRS, 32, 1>);
+    return go(&norm_rope_kernel<T, PAIRS, 64, 1>);
+}
+
+}  // namespace
+
+hipError_t launch_norm_rope(const cq_norm_rope_t& a, hipStream_t stream) {
+    auto go = [&](auto elem) {
+        using T = decltype(elem);
+        return a.interleaved ? launch_typed<T, true>(a, stream) : launch_typed<T, false>(a, stream);
+    };
+    if (a.dtype == CQ_DTYPE_F16) return go(_Float16{});
+    if (a.dtype == CQ_DTYPE_BF16) return go(__bf16{});
+    return go(float{});
+}
+
+}  // namespace cq

@@ -675,8 +675,12 @@ _EXTS: dict[str, _OpExt] = {}
 _EXT_TYPES = {"int4gemv": Int4gemvExt, "qgemv": QgemvExt, "gemv": GemvExt}
 
 
-def get_ext(op: str) -> _OpExt:
-    """Singleton extension object for "int4gemv", "qgemv" or "gemv"."""
+def get_ext(op: str):
+    """Singleton extension object for "int4gemv", "qgemv", "gemv" or
+    "attention"."""
+    if op == "attention":
+        from .attention import get_attention
+        return get_attention()
     if op not in _EXT_TYPES:
         raise KeyError(f"no extension for operator {op!r}")
     e = _EXTS.get(op)

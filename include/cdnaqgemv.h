@@ -28,7 +28,10 @@
  *     y[n] = sum_k w[n,k] * x[k] in FP32, cast once to the dtype.
  *
  * Plus the on-device quantizers that produce the first two operators'
- * weights from fp16 W (cq_int4_quantize, cq_q8_quantize).
+ * weights from fp16 W (cq_int4_quantize, cq_q8_quantize), and what a decoder
+ * runs between these projections: per-head norms with the rotation
+ * (cq_qk_norm_rope), a quantized paged key/value cache (cq_kv_append,
+ * cq_kv_read) and attention over it (cq_attention).
  *
  * All pointers are device pointers on the current HIP device; `stream` is a
  * hipStream_t (NULL = the null stream).  Calls are asynchronous: a kernel is
@@ -83,9 +86,10 @@ extern "C" {
 #define CQ_OP_GEMV_F16 2
 #define CQ_OP_GEMV_F32 3
 
-/* gemv element types */
+/* element types */
 #define CQ_DTYPE_F16 0
 #define CQ_DTYPE_F32 1
+#define CQ_DTYPE_BF16 2   /* the operators around attention only */
 
 /* quantizer scale forms (cq_int4_quantize, cq_q8_quantize): the reference
  * computes the scale as `amax / qmax` in torch, which is one correctly
@@ -422,6 +426,133 @@ int cq_prepare(int op, const char* variant, const void* w, const void* scale,
  * bit-identical to the direct call.  Returns CQ_OK or CQ_ERR_HIP.
  */
 int cq_launch_prepared(const cq_prepared_t* prepared, void* stream);
+
+/*
+ * The operators between the q/k/v projections and the o projection of a
+ * decoder: per-head norms with the position rotation, a quantized paged
+ * key/value cache, and attention over it.  No counterpart in the reference
+ * (its path ends at the projections).  Element types are CQ_DTYPE_*; strides
+ * count elements; innermost dimensions are contiguous.  As everywhere in
+ * this library the calls are asynchronous on `stream`, allocate nothing and
+ * keep nothing between calls.  Lengths, positions and page numbers live on
+ * the device: the kernels check them against the buffers' sizes given here,
+ * as each declaration says, and never access memory outside them.
+ */
+
+/* Per-head RMS norm and rotation of q [tokens, q_heads, head_dim] and
+ * k [tokens, k_heads, head_dim], in FP32, rounded once to `dtype`:
+ *   n = x * (1 / sqrt(mean(x^2) + eps)) * weight     (no norm if weight NULL)
+ *   a' = a cos - b sin, b' = b cos + a sin            (no rotation if cos NULL)
+ * for the pairs (a, b) = (n[i], n[i + rot_dim / 2]), or (n[2i], n[2i + 1]) if
+ * `interleaved`, with cos, sin = table[position, i], i < rot_dim / 2; dims from
+ * rot_dim on are not turned.  An output may be its own input (same pointer and
+ * strides); otherwise no output shares a byte with an operand.  A position
+ * outside [0, table_rows) turns that token's rotated dims into NaN. */
+typedef struct cq_norm_rope {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_token_stride, k_head_stride;
+    int64_t q_out_token_stride, q_out_head_stride;
+    int64_t k_out_token_stride, k_out_head_stride;
+    const void* q_weight;      /* [head_dim] of weight_dtype, or NULL */
+    const void* k_weight;
+    const float* cos_table;    /* [table_rows, rot_dim / 2], or NULL */
+    const float* sin_table;
+    const void* positions;     /* int32 or int64 [tokens] */
+    int64_t tokens, table_rows;
+    int32_t q_heads, k_heads;  /* either may be 0 (its pointers unused) */
+    int32_t head_dim;          /* even, 2..1024 */
+    int32_t rot_dim;           /* even, 2..head_dim */
+    int32_t dtype;             /* CQ_DTYPE_F16, _F32 or _BF16 */
+    int32_t weight_dtype;      /* likewise */
+    int32_t positions_64;      /* 1: positions are int64 */
+    int32_t interleaved;
+    float eps;
+} cq_norm_rope_t;
+int cq_qk_norm_rope(const cq_norm_rope_t* args, void* stream);
+
+/* A paged key/value cache: `pages` pages of `page_size` tokens of every head.
+ *   8 bits: k int8 [pages, heads, page_size, head_dim],
+ *           v int8 [pages, heads, page_size / 16, head_dim, 16]
+ *   4 bits: k u8 [pages, heads, page_size, head_dim / 2],
+ *           v u8 [pages, heads, page_size / 16, head_dim / 2, 16],
+ *           dim 2j in the low nibble of byte j and 2j + 1 in the high one
+ *   scales f32 [pages, heads, 2, page_size]: K's, then V's
+ * A value is code * scale of its token and head.  V keeps 16 tokens of a dim
+ * side by side: attention multiplies it over the tokens and reads them as one
+ * matrix operand.  k, v and scales are contiguous and 16-byte aligned. */
+typedef struct cq_kv_cache {
+    void* k;
+    void* v;
+    float* scales;
+    int64_t pages;             /* 1..2^31-1 */
+    int32_t heads;             /* 1..65535 */
+    int32_t head_dim;          /* 64, 128 or 256 */
+    int32_t page_size;         /* 16, 32, 64, 128 or 256 */
+    int32_t bits;              /* 4 or 8 */
+} cq_kv_cache_t;
+
+/* Which tokens of which sequences a call means: sequence b's token t is at
+ * position starts[b] + t for 0 <= t < counts[b] (tokens, if counts is NULL or
+ * says more), in page table[b * table_stride + position / page_size]. */
+typedef struct cq_kv_slots {
+    const int32_t* table;      /* [batch, table_cols], rows table_stride apart */
+    const int32_t* starts;     /* [batch] */
+    const int32_t* counts;     /* [batch] or NULL */
+    int64_t table_stride;
+    int32_t table_cols;
+    int32_t batch;
+    int32_t tokens;
+} cq_kv_slots_t;
+
+/* Quantizes k and v [batch, tokens, heads, head_dim] into the cache; per token
+ * and head, with qmax = 127 or 7 and every operation rounded to FP32:
+ *   scale = amax * fl(1 / qmax), code = clamp(rint(x * fl(1 / scale)), +-qmax)
+ * An amax below 2^-100 gives scale 0 and codes 0, one that is not finite scale
+ * NaN and codes 0.  A token whose position or page is out of range is not
+ * written.  The pages written belong to one sequence each. */
+int cq_kv_append(const cq_kv_cache_t* cache, const cq_kv_slots_t* slots, int dtype,
+                 const void* k, int64_t k_batch_stride, int64_t k_token_stride,
+                 int64_t k_head_stride, const void* v, int64_t v_batch_stride,
+                 int64_t v_token_stride, int64_t v_head_stride, void* stream);
+
+/* The values of the cached tokens into contiguous k_out and v_out
+ * [batch, tokens, heads, head_dim], rounded once to `dtype`; 0 for tokens past
+ * the count and for positions and pages out of range. */
+int cq_kv_read(const cq_kv_cache_t* cache, const cq_kv_slots_t* slots, int dtype,
+               void* k_out, void* v_out, void* stream);
+
+/* Attention of q [batch, tokens, q_heads, head_dim] over the cache, q head h
+ * on cache head h / (q_heads / heads).  Sequence b holds lengths[b] tokens, of
+ * which the last counts[b] (tokens, if NULL or more) are the call's: its query
+ * t is at position p = lengths[b] - count + t and sees the sequence's positions
+ * 0..p and all prefix_len tokens of the prefix, whose pages are
+ * prefix_table[0 .. prefix_cols).  Positions without a page in range are not
+ * seen.  out = sum_j softmax_j(softmax_scale * q . k_j) v_j, FP32 scores,
+ * statistics and sums, rounded once to `dtype` (F16 or BF16); 0 for a row that
+ * sees nothing and for rows t >= count. */
+typedef struct cq_attention {
+    const void* q;             /* 16-byte aligned; strides multiples of 8 */
+    void* out;                 /* contiguous, 16-byte aligned */
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    const int32_t* table;      /* [batch, table_cols], rows table_stride apart */
+    const int32_t* lengths;    /* [batch] */
+    const int32_t* counts;     /* [batch] or NULL */
+    const int32_t* prefix_table;  /* [prefix_cols] or NULL */
+    int64_t table_stride;
+    void* workspace;           /* cq_attention_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int32_t table_cols, prefix_cols, prefix_len;
+    int32_t batch, tokens, q_heads;
+    int32_t dtype;
+    float softmax_scale;
+} cq_attention_t;
+int cq_attention(const cq_kv_cache_t* cache, const cq_attention_t* args, void* stream);
+/* Bytes of workspace that call needs (0 or more), or a negative CQ_* status. */
+int64_t cq_attention_workspace(const cq_kv_cache_t* cache, const cq_attention_t* args);
 
 /*
  * Message of the last failed call on this thread ("" if none).  Replaces
