@@ -3,9 +3,36 @@
 //   s_j = scale * (q . kcode_j) * kscale_j, p = softmax(s) over what the row
 //   sees, out_d = sum_j p_j * vscale_j * vcode_jd
 //
-// One pass over the keys with the running maximum and sum: a wave keeps
-// (m, l, o) = (max s, sum e^(s - m), sum e^(s - m) v) and rescales l and o
-// when m grows; partial triples of disjoint key ranges join the same way.
+// One pass over the keys with a running reference M and sum l: with
+// vscale_j = f_j 2^e_j (f in [1/2, 1)) a wave keeps
+//   l = sum_j 2^(s_j log2(e) - M),  o_d = sum_j w_j vcode_jd,
+//   w_j = 2^(s_j log2(e) + e_j - M) f_j
+// and raises M (scaling l and o down) when an exponent passes kRaise; triples
+// (M, l, o) of disjoint keys join the same way.  Folding V's exponent into
+// that of the softmax keeps w_j, which the matrix instructions take as fp16,
+// in range for any scales: the largest w of a row lies in [1/2, 2^kRaise), and
+// what fp16 then rounds off is 2^-11 of each weight, or 2^-24 of 1.  The codes
+// are exact in fp16; scores, sums and statistics are FP32.
+//
+// Matrix form, 64 keys at a time (v_mfma_f32_16x16x32_f16, FP32 sums):
+//   S^T [keys x rows] = K [keys x D] Q^T [D x rows]
+//   O^T [D x rows]   += V^T [D x keys] W^T [keys x rows]
+// Rows are the query heads of a key head (times the new tokens), 16 to a
+// matrix.  S comes out with a row's keys in the four lanes row + 16 g, four
+// keys of each matrix in a lane, which is just how W goes in if lane group g
+// owns keys 16 g .. 16 g + 15 of the 64: K's rows are loaded in that order, V
+// is stored with 16 tokens of a dim together, and nothing crosses lanes but a
+// raise of M and the last sums.  Both operands are loaded once from memory as
+// codes, 16 bytes to a lane, and turned into fp16 in registers.
+//
+// Work is dealt out on the device, where the lengths are: the (sequence, row
+// group, head) units are laid end to end as tiles of 64 keys, and each
+// workgroup takes an equal run of tiles, wherever units begin and end.  A unit
+// that lies in one run is finished there; a longer one leaves a triple per run
+// in the workspace, which join_kernel joins.  Equal runs keep every workgroup
+// busy to the end for any mix of lengths, and the grid never depends on them.
+
+#include <algorithm>
 
 #include "cq_attn.h"
 #include "cq_elem.h"
@@ -14,98 +41,865 @@ namespace cq {
 namespace {
 
 constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / 64;
+constexpr int kTile = 64;               // keys of a tile
 constexpr float kNegInf = -__builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 8.f;
+constexpr int kLeastExp = -100;         // a V scale below 2^-100 counts as 0
 
-// One workgroup per row (sequence, new token, query head); its four waves
-// take every fourth key, a lane E dims.
-template <class T, int BITS, int D>
-__global__ __launch_bounds__(kBlock) void row_kernel(cq_kv_cache_t c, cq_attention_t a) {
+using h8 = Vec<_Float16, 8>;
+using h2 = Vec<_Float16, 2>;
+using f4 = Vec<float, 4>;
+using u4 = Vec<uint32_t, 4>;
+using u2 = Vec<uint32_t, 2>;
+
+// One launch over one source of keys (the sequences' own, or the prefix).
+struct Source {
+    cq_kv_cache_t c;
+    cq_attention_t a;
+    int32_t group;         // query heads per key head
+    int32_t rows;          // rows of a unit's sequence (or of the whole batch)
+    int32_t row_groups;    // of rows_per_unit rows
+    int32_t rows_per_unit;
+    int32_t prefix;        // 1: the prefix's keys
+    int32_t least;         // tiles that a run has at least
+    uint32_t runs;         // workgroups
+    int32_t finish;        // 1: units of one run write `out`; 0: their home
+    // workspace: triples of broken units, two per run, and of whole units
+    float* broken_o;       // [runs * 2 * rows_per_unit, D]
+    float* broken_ml;      // [.., 2]
+    float* home_o;         // [batch * tokens * q_heads, D]
+    float* home_ml;
+};
+
+// -------------------------------------------------------------- the units
+__device__ __forceinline__ int new_tokens(const cq_attention_t& a, int b) {
+    return a.counts != nullptr ? max(0, min(a.tokens, a.counts[b])) : a.tokens;
+}
+
+// Own positions that query t of sequence b sees (0 for t past the count).
+__device__ __forceinline__ int own_limit(const Source& s, int length, int count, int t) {
+    if (t >= count) return 0;
+    const int64_t last = (int64_t)length - count + t + 1;
+    return (int)max((int64_t)0, min(last, (int64_t)s.a.table_cols * s.c.page_size));
+}
+
+// Tiles of entry e: (sequence, row group), or the prefix's row group.
+__device__ __forceinline__ int tiles_of(const Source& s, int e) {
+    if (s.prefix) return (s.a.prefix_len + kTile - 1) / kTile;
+    const int b = e / s.row_groups, rg = e % s.row_groups;
+    const int count = new_tokens(s.a, b);
+    const int first = rg * s.rows_per_unit / s.group;
+    if (first >= count) return 0;
+    const int last = min((rg * s.rows_per_unit + s.rows_per_unit - 1) / s.group, count - 1);
+    return (own_limit(s, s.a.lengths[b], count, last) + kTile - 1) / kTile;
+}
+
+__device__ __forceinline__ int entries_of(const Source& s) {
+    return s.prefix ? s.row_groups : s.a.batch * s.row_groups;
+}
+
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {     // inclusive
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t up = __shfl_up(v, off);
+        if (lane >= off) v += up;
+    }
+    return v;
+}
+
+// Tiles (of one head) before entry `at`, in all, and, if `find` is not
+// negative, the entry that holds tile `find` of the heads' sequence: every
+// lane of the wave gets the same.  heads * tiles of a call fit 63 bits.
+struct Deal {
+    int64_t total = 0;      // tiles of all entries, one head
+    int64_t before = 0;     // tiles ahead of the entry, one head
+    int entry = 0;
+};
+
+__device__ __forceinline__ Deal deal_at(const Source& s, int at, int lane) {
+    Deal d;
+    d.entry = at;
+    const int n = entries_of(s);
+    if (s.prefix) {
+        const int t = tiles_of(s, 0);
+        d.total = (int64_t)t * n;
+        d.before = (int64_t)t * at;
+        return d;
+    }
+    for (int base = 0; base < n; base += 64) {
+        const int e = base + lane;
+        const uint32_t sum = wave_scan(e < n ? tiles_of(s, e) : 0, lane);
+        if (at >= base && at < base + 64)
+            d.before = d.total + (at > base ? __shfl(sum, at - base - 1) : 0u);
+        d.total += __shfl(sum, 63);
+    }
+    return d;
+}
+
+// The entry that holds position `pos` (below heads * total).
+__device__ __forceinline__ Deal deal_find(const Source& s, int64_t pos, int64_t total, int lane) {
+    Deal d;
+    d.total = total;
+    const int n = entries_of(s), heads = s.c.heads;
+    if (s.prefix) {
+        const int t = tiles_of(s, 0);
+        d.entry = (int)(pos / ((int64_t)t * heads));
+        d.before = (int64_t)t * d.entry;
+        return d;
+    }
+    int64_t done = 0;
+    for (int base = 0; base < n; base += 64) {
+        const int e = base + lane;
+        const uint32_t sum = wave_scan(e < n ? tiles_of(s, e) : 0, lane);
+        const uint64_t past = __ballot((done + sum) * heads > pos);
+        if (past != 0) {
+            const int first = __builtin_ctzll(past);
+            d.entry = base + first;
+            d.before = done + (first > 0 ? __shfl(sum, first - 1) : 0u);
+            return d;
+        }
+        done += __shfl(sum, 63);
+    }
+    return d;
+}
+
+__device__ __forceinline__ int64_t run_length(const Source& s, int64_t total) {
+    const int64_t all = total * s.c.heads;
+    return max((int64_t)s.least, (all + s.runs - 1) / s.runs);
+}
+
+// ----------------------------------------------------------- small pieces
+__device__ __forceinline__ uint32_t pk_sub_f16(uint32_t a, float b) {
+    const h2 v = __builtin_bit_cast(h2, a) - h2{(_Float16)b, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// Four int8 of a word as fp16 pairs (0, 2), (1, 3): the byte under the
+// exponent of 1024, sign bit flipped, is 1152 + code.
+__device__ __forceinline__ void fp16_of_bytes(uint32_t w, uint32_t& a, uint32_t& b) {
+    a = pk_sub_f16((w & 0x00FF00FFu) ^ 0x64806480u, 1152.f);
+    b = pk_sub_f16(((w >> 8) & 0x00FF00FFu) ^ 0x64806480u, 1152.f);
+}
+
+// Eight int4 of a word as fp16 pairs (0, 4), (1, 5), (2, 6), (3, 7); the high
+// nibble of a byte stays in place under the exponent of 64, whose last bits
+// are sixteenths.
+__device__ __forceinline__ void fp16_of_nibbles(uint32_t w, uint32_t (&p)[4]) {
+    const uint32_t x = w >> 8;
+    p[0] = pk_sub_f16((w & 0x000F000Fu) ^ 0x64086408u, 1032.f);
+    p[1] = pk_sub_f16((w & 0x00F000F0u) ^ 0x54805480u, 72.f);
+    p[2] = pk_sub_f16((x & 0x000F000Fu) ^ 0x64086408u, 1032.f);
+    p[3] = pk_sub_f16((x & 0x00F000F0u) ^ 0x54805480u, 72.f);
+}
+
+// Maximum and sum over the four lanes l, l + 16, l + 32, l + 48, in each.
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// What a triple's sums are multiplied with to stand at reference `top`.  One
+// that has seen no number has M = -Inf and sums of 0, or of NaN where it saw
+// only NaN: l itself then.
+__device__ __forceinline__ float factor(float m, float l, float top) {
+    return m == kNegInf ? l : __builtin_amdgcn_exp2f(m - top);
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, f4 v) {
+    Vec<T, 4> o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (T)v[i];
+    *reinterpret_cast<Vec<T, 4>*>(p) = o;
+}
+
+// ------------------------------------------------------------- the kernel
+// NB row matrices to a wave.  SHARE: the four waves take the same keys for
+// four times 16 NB rows; otherwise the same 16 NB rows, and every fourth tile
+// each.
+template <class T, int BITS, int D, int NB, bool SHARE>
+struct Tiles {
+    static constexpr int kRow = D * BITS / 8;              // bytes of a token's row
+    static constexpr int kLane = kRow / 4;                 // K bytes of a lane and row
+    static constexpr int kChunk = kLane < 16 ? kLane : 16;
+    static constexpr int kChunks = kLane / kChunk;
+    static constexpr int kWords = kChunk / 4;
+    static constexpr int kSteps = D / 32;                  // products over D
+    static constexpr int kVTiles = kRow / 16;              // 16 rows of V bytes
+    static constexpr int kOTiles = D / 16;
+    static constexpr int kUnitRows = 16 * NB * (SHARE ? kWaves : 1);
+    static constexpr bool kHalf = sizeof(T) == 2 && std::is_same_v<T, _Float16>;
+
+    // Where dims of product step u of lane group g start, and their order:
+    // the unpacking leaves pairs of bytes or nibbles apart.
+    static __device__ __forceinline__ int step_dim(int u, int g) {
+        constexpr int per = kChunk / BITS;                 // steps of a chunk
+        return ((u / per) * 4 * kChunk + g * kChunk) * 8 / BITS + (u % per) * 8;
+    }
+    static constexpr int order(int i) {
+        constexpr int o8[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+        constexpr int o4[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+        return BITS == 8 ? o8[i] : o4[i];
+    }
+
+    h8 q[NB][kSteps];
+    float qscale[NB];                    // scale log2(e) over q's own factor
+    int limit[NB];                       // keys that the lane's row sees
+    int full;                            // tiles of which every row sees all
+    f4 o[NB][kOTiles];
+    float l[NB], ref[NB], raise[NB];
+
+    Vec<uint32_t, kWords> kq[4][kChunks];
+    u4 vq[kVTiles];
+    f4 ks[4], vs[4];
+    bool there;                          // the lane group's 16 keys have a page
+
+    // Row r of the unit's source: its query and where its result goes.
+    static __device__ __forceinline__ int64_t row_index(const Source& s, int b, int r, int h,
+                                                        int& t) {
+        if (s.prefix) {
+            const int per = s.a.tokens * s.group;
+            b = r / per;
+            r -= b * per;
+        }
+        t = r / s.group;
+        return ((int64_t)b * s.a.tokens + t) * s.a.q_heads + h * s.group + r % s.group;
+    }
+
+    __device__ __forceinline__ void load_q(const Source& s, int b, int first_row, int h,
+                                           int lane) {
+        const int g = lane >> 4;
+        int least = 0x7FFFFFFF;
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+            // rows past the last repeat it (nobody stores them)
+            const int r = min(first_row + 16 * rb + (lane & 15), s.rows - 1);
+            int t;
+            const int64_t at = row_index(s, b, r, h, t);
+            const int hq = (int)(at % s.a.q_heads);
+            const int bb = (int)(at / s.a.q_heads / s.a.tokens);
+            const int count = new_tokens(s.a, bb);
+            limit[rb] = s.prefix ? (t < count ? s.a.prefix_len : 0)
+                                 : own_limit(s, s.a.lengths[bb], count, t);
+            least = min(least, limit[rb]);
+            const T* p = static_cast<const T*>(s.a.q) + bb * s.a.q_batch_stride +
+                         t * s.a.q_token_stride + hq * s.a.q_head_stride;
+            qscale[rb] = s.a.softmax_scale * kLog2e;
+            Vec<T, 8> raw[kSteps];
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u)
+                raw[u] = *reinterpret_cast<const Vec<T, 8>*>(p + step_dim(u, g));
+            float by = 1.f;
+            if constexpr (!kHalf) {
+                // bfloat16 goes into fp16 times a power of two that brings the
+                // row's largest into [2^14, 2^15): exact down to 2^-28 of it
+                float top = 0.f;
+#pragma unroll
+                for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf((float)raw[u][i]));
+                top = quad_max(top);
+                int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
+                if (top == 0.f || top > 3.4e38f) e = 0;
+                by = ldexpf(1.f, -e);
+                if (e < -126) {                    // 2^-e is no FP32 number
+                    by = 0x1p126f;
+                    e = -126;
+                }
+                qscale[rb] *= ldexpf(1.f, e);
+            }
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const T x = raw[u][order(i)];
+                    if constexpr (kHalf) q[rb][u][i] = x;
+                    else q[rb][u][i] = (_Float16)((float)x * by);
+                }
+        }
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) least = min(least, __shfl_xor(least, off));
+        full = __builtin_amdgcn_readfirstlane(least) / kTile;
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+            l[rb] = ref[rb] = 0.f;
+            raise[rb] = kNegInf;
+#pragma unroll
+            for (int i = 0; i < kOTiles; ++i) o[rb][i] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // Table entry of 16 keys `sub` of a tile (any entry past the table).
+    static __device__ __forceinline__ int32_t entry(const Source& s, const int32_t* table,
+                                                    int cols, int tile, int sub) {
+        return table[min((int)(((int64_t)tile * kTile + sub * 16) / s.c.page_size), cols - 1)];
+    }
+
+    __device__ __forceinline__ void load_k(const Source& s, int32_t entry, int tile, int h,
+                                           int lane) {
+        const int g = lane >> 4, r = lane & 15;
+        const int64_t page = max((int64_t)0, page_in(entry, s.c.pages));
+        const int in = (tile * kTile + (r >> 2) * 16) & (s.c.page_size - 1);
+        const uint8_t* p = static_cast<const uint8_t*>(s.c.k) +
+                           ((page * s.c.heads + h) * s.c.page_size + in + (r & 3)) * kRow +
+                           g * kChunk;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+                kq[t][c] = *reinterpret_cast<const Vec<uint32_t, kWords>*>(
+                    p + t * 4 * kRow + c * 4 * kChunk);
+    }
+
+    __device__ __forceinline__ void load_scales(const Source& s, int32_t entry, int tile, int h,
+                                                int lane) {
+        const int g = lane >> 4;
+        const int64_t page = max((int64_t)0, page_in(entry, s.c.pages));
+        there = page_in(entry, s.c.pages) >= 0;
+        const int in = (tile * kTile + g * 16) & (s.c.page_size - 1);
+        const float* p = s.c.scales + (page * s.c.heads + h) * 2 * s.c.page_size + in;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            ks[t] = *reinterpret_cast<const f4*>(p + 4 * t);
+            vs[t] = *reinterpret_cast<const f4*>(p + s.c.page_size + 4 * t);
+        }
+    }
+
+    __device__ __forceinline__ void load_v(const Source& s, int32_t entry, int tile, int h,
+                                           int lane) {
+        const int g = lane >> 4, r = lane & 15;
+        const int64_t page = max((int64_t)0, page_in(entry, s.c.pages));
+        const int in = (tile * kTile + g * 16) & (s.c.page_size - 1);
+        const uint8_t* p = static_cast<const uint8_t*>(s.c.v) +
+                           ((page * s.c.heads + h) * s.c.page_size + in) * kRow + r * 16;
+#pragma unroll
+        for (int i = 0; i < kVTiles; ++i) vq[i] = *reinterpret_cast<const u4*>(p + i * 256);
+    }
+
+    static __device__ __forceinline__ h8 unpack_k(const Vec<uint32_t, kWords> (&row)[kChunks],
+                                                  int u) {
+        constexpr int per = kChunk / BITS;
+        u4 w;
+        if constexpr (BITS == 8) {
+            uint32_t a, b, c, d;
+            fp16_of_bytes(row[u / per][2 * (u % per)], a, b);
+            fp16_of_bytes(row[u / per][2 * (u % per) + 1], c, d);
+            w = u4{a, b, c, d};
+        } else {
+            // pairs (0, 4), (1, 5), (2, 6), (3, 7) of the word's nibbles
+            uint32_t p[4];
+            fp16_of_nibbles(row[u / per][u % per], p);
+            w = u4{p[0], p[1], p[2], p[3]};
+        }
+        return __builtin_bit_cast(h8, w);
+    }
+
+    // One tile of keys.  `next`: issues the loads that the registers freed
+    // here can take.
+    template <class NextK, class NextV>
+    __device__ __forceinline__ void step(int tile, int lane, NextK&& next_k, NextV&& next_v) {
+        f4 sc[NB][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int rb = 0; rb < NB; ++rb) sc[rb][t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u) {
+                const h8 k = unpack_k(kq[t], u);
+#pragma unroll
+                for (int rb = 0; rb < NB; ++rb)
+                    sc[rb][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rb][u], sc[rb][t], 0,
+                                                                      0, 0);
+            }
+        }
+        next_k();
+        // V's scales as f 2^e
+        float f[16], ef[16], back[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float v = vs[j / 4][j % 4];
+            const int e = max((int)((__float_as_uint(v) >> 23) & 0xFF) - 126, kLeastExp);
+            f[j] = __builtin_amdgcn_ldexpf(v, -e);
+            ef[j] = (float)e;
+            back[j] = __builtin_amdgcn_ldexpf(1.f, -e);
+        }
+        const bool masked = tile >= full || !__all(there);
+        h8 w[NB][2];
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+            float x[16];
+            float top = kNegInf;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                x[j] = __builtin_fmaf(sc[rb][j / 4][j % 4], ks[j / 4][j % 4] * qscale[rb],
+                                      ef[j] - ref[rb]);
+            uint32_t seen = 0xFFFFu;
+            if (masked) {
+                const int n = there ? limit[rb] - tile * kTile - (lane >> 4) * 16 : 0;
+                seen = n <= 0 ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (!((seen >> j) & 1)) x[j] = kNegInf;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
+            if (__any(top > raise[rb])) {
+                top = quad_max(top);
+                const bool first = raise[rb] == kNegInf;
+                if (top > (first ? kNegInf : 0.f)) {
+                    const float keep = first ? 1.f : __builtin_amdgcn_exp2f(-top);
+                    ref[rb] += top;
+                    raise[rb] = kRaise;
+                    l[rb] *= keep;
+#pragma unroll
+                    for (int i = 0; i < kOTiles; ++i) o[rb][i] *= keep;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[j] -= top;
+                }
+            }
+            float p[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float y = __builtin_amdgcn_exp2f(x[j]);
+                l[rb] = __builtin_fmaf(y, back[j], l[rb]);
+                p[j] = y * f[j];
+            }
+            if (masked) {
+                // what is not seen may have a scale of NaN or Inf
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (!((seen >> j) & 1)) p[j] = 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    // keys of a word as its bytes come out: 0, 2, 1, 3
+                    constexpr int at[4] = {0, 2, 1, 3};
+                    w[rb][u][i] = (_Float16)p[8 * u + (i & 4) + at[i & 3]];
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < kVTiles; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if constexpr (BITS == 8) {
+                    uint32_t a, b, c, d;
+                    fp16_of_bytes(vq[i][2 * u], a, b);
+                    fp16_of_bytes(vq[i][2 * u + 1], c, d);
+                    const h8 v = __builtin_bit_cast(h8, u4{a, b, c, d});
+#pragma unroll
+                    for (int rb = 0; rb < NB; ++rb)
+                        o[rb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[rb][u], o[rb][i],
+                                                                         0, 0, 0);
+                } else {
+                    // bytes are tokens here: low nibbles the even dim's, high
+                    // ones the odd dim's
+                    uint32_t p0[4], p1[4];
+                    fp16_of_nibbles(vq[i][2 * u], p0);
+                    fp16_of_nibbles(vq[i][2 * u + 1], p1);
+                    const h8 even = __builtin_bit_cast(h8, u4{p0[0], p0[2], p1[0], p1[2]});
+                    const h8 odd = __builtin_bit_cast(h8, u4{p0[1], p0[3], p1[1], p1[3]});
+#pragma unroll
+                    for (int rb = 0; rb < NB; ++rb) {
+                        o[rb][2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            even, w[rb][u], o[rb][2 * i], 0, 0, 0);
+                        o[rb][2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            odd, w[rb][u], o[rb][2 * i + 1], 0, 0, 0);
+                    }
+                }
+            }
+        next_v();
+    }
+
+    __device__ __forceinline__ void run(const Source& s, int b, int h, int tile, int end,
+                                        int stride, int lane) {
+        const int32_t* table = s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride;
+        const int cols = s.prefix ? s.a.prefix_cols : s.a.table_cols;
+        const int ksub = (lane & 15) >> 2, vsub = lane >> 4;
+        if (tile >= end) return;
+        int32_t ke = entry(s, table, cols, tile, ksub), ve = entry(s, table, cols, tile, vsub);
+        load_k(s, ke, tile, h, lane);
+        load_scales(s, ve, tile, h, lane);
+        load_v(s, ve, tile, h, lane);
+        for (; tile < end; tile += stride) {
+            const int next = tile + stride;
+            if (next < end) {
+                ke = entry(s, table, cols, next, ksub);
+                ve = entry(s, table, cols, next, vsub);
+            }
+            step(tile, lane, [&] { if (next < end) load_k(s, ke, next, h, lane); },
+                 [&] {
+                     if (next < end) {
+                         load_scales(s, ve, next, h, lane);
+                         load_v(s, ve, next, h, lane);
+                     }
+                 });
+        }
+    }
+
+    // Dims of o[.][i] start: four from 16 i + 4 g, or (4 bits) every other of
+    // eight from 32 (i / 2) + 8 g.
+    // f(dim, four values): the lane's part of row matrix rb, four dims a call.
+    template <class F>
+    __device__ __forceinline__ void each_four(int rb, int lane, F&& f) const {
+        const int g = lane >> 4;
+        if constexpr (BITS == 8) {
+#pragma unroll
+            for (int i = 0; i < kOTiles; ++i) f(16 * i + 4 * g, o[rb][i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kOTiles; i += 2) {
+                const f4 a = o[rb][i], b = o[rb][i + 1];
+                f(16 * i + 8 * g, f4{a[0], b[0], a[1], b[1]});
+                f(16 * i + 8 * g + 4, f4{a[2], b[2], a[3], b[3]});
+            }
+        }
+    }
+};
+
+// Least waves per SIMD (registers) and workgroups that a CU is dealt.
+constexpr int waves_of(int d, int nb) { return d * nb <= 128 ? 2 : 1; }
+
+template <class T, int BITS, int D, int NB, bool SHARE>
+__global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s) {
+    using W = Tiles<T, BITS, D, NB, SHARE>;
+    constexpr int kRows = W::kUnitRows;
+    // waves that split a unit's keys join here
+    __shared__ __attribute__((aligned(16))) float sm_o[SHARE ? 1 : kRows][SHARE ? 4 : D + 4];
+    __shared__ float sm_m[kWaves][SHARE ? 1 : kRows], sm_l[kWaves][SHARE ? 1 : kRows];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t total = deal_at(s, 0, lane).total;
+    const int64_t per = run_length(s, total);
+    int64_t pos = (int64_t)blockIdx.x * per;
+    const int64_t stop = min(pos + per, total * s.c.heads);
+    if (pos >= stop) return;
+    Deal d = deal_find(s, pos, total, lane);
+    int e = __builtin_amdgcn_readfirstlane(d.entry);
+    int n = __builtin_amdgcn_readfirstlane(tiles_of(s, e));
+    const int64_t in_entry = pos - d.before * s.c.heads;
+    int h = __builtin_amdgcn_readfirstlane((int)(in_entry / n));
+    int tile = __builtin_amdgcn_readfirstlane((int)(in_entry % n));
+    int64_t left = stop - pos;
+    W work;
+    for (;;) {
+        const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(n - tile), left));
+        const int b = s.prefix ? 0 : e / s.row_groups;
+        const int row0 = (s.prefix ? e : e % s.row_groups) * kRows;
+        const int mine = row0 + (SHARE ? wave * 16 * NB : 0);
+        const bool whole = take == n;
+        const int64_t slot = ((int64_t)blockIdx.x * 2 + (tile > 0 ? 0 : 1)) * kRows;
+        // where a row's triple or result goes
+        auto put_ml = [&](int r, float m, float l) {
+            int t;
+            const int64_t at = whole ? W::row_index(s, b, r, h, t) : slot + r - row0;
+            float* ml = whole ? s.home_ml : s.broken_ml;
+            ml[2 * at] = m;
+            ml[2 * at + 1] = l;
+        };
+        auto put_o = [&](int r, int dim, f4 v, float l) {
+            int t;
+            if (!whole) {
+                *reinterpret_cast<f4*>(s.broken_o + (slot + r - row0) * D + dim) = v;
+                return;
+            }
+            const int64_t at = W::row_index(s, b, r, h, t) * D + dim;
+            if (s.finish) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                store4(static_cast<T*>(s.a.out) + at, l == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * inv);
+            } else {
+                *reinterpret_cast<f4*>(s.home_o + at) = v;
+            }
+        };
+        const bool triple = !whole || !s.finish;
+        if (SHARE) {
+            if (mine < s.rows) {
+                work.load_q(s, b, mine, h, lane);
+                work.run(s, b, h, tile, tile + take, 1, lane);
+#pragma unroll
+                for (int rb = 0; rb < NB; ++rb) {
+                    const int r = mine + 16 * rb + (lane & 15);
+                    const float l = quad_sum(work.l[rb]);
+                    if (r < s.rows) {
+                        if (triple && lane < 16)
+                            put_ml(r, work.raise[rb] == kNegInf ? kNegInf : work.ref[rb], l);
+                        work.each_four(rb, lane, [&](int dim, f4 v) { put_o(r, dim, v, l); });
+                    }
+                }
+            }
+        } else {
+            work.load_q(s, b, mine, h, lane);
+            work.run(s, b, h, tile + wave, tile + take, kWaves, lane);
+            float m[NB], l[NB];
+#pragma unroll
+            for (int rb = 0; rb < NB; ++rb) {
+                l[rb] = quad_sum(work.l[rb]);
+                m[rb] = work.raise[rb] == kNegInf ? kNegInf : work.ref[rb];
+                if (lane < 16) {
+                    sm_m[wave][16 * rb + lane] = m[rb];
+                    sm_l[wave][16 * rb + lane] = l[rb];
+                }
+            }
+            __syncthreads();
+            // the waves' sums, brought to one reference, one wave after another
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                if (wave == v) {
+#pragma unroll
+                    for (int rb = 0; rb < NB; ++rb) {
+                        const int r = 16 * rb + (lane & 15);
+                        float top = sm_m[0][r];
+#pragma unroll
+                        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, sm_m[i][r]);
+                        const float keep = factor(m[rb], l[rb], top);
+                        work.each_four(rb, lane, [&](int dim, f4 x) {
+                            f4* at = reinterpret_cast<f4*>(&sm_o[r][dim]);
+                            *at = v == 0 ? x * keep : *at + x * keep;
+                        });
+                    }
+                }
+                __syncthreads();
+            }
+            for (int i = threadIdx.x; i < kRows * (D / 4); i += kBlock) {
+                const int r = i / (D / 4), dim = i % (D / 4) * 4;
+                if (row0 + r >= s.rows) break;
+                float top = sm_m[0][r], sum = 0.f;
+#pragma unroll
+                for (int v = 1; v < kWaves; ++v) top = fmaxf(top, sm_m[v][r]);
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v)
+                    sum += sm_l[v][r] * factor(sm_m[v][r], sm_l[v][r], top);
+                if (triple && dim == 0) put_ml(row0 + r, top, sum);
+                put_o(row0 + r, dim, *reinterpret_cast<const f4*>(&sm_o[r][dim]), sum);
+            }
+            __syncthreads();
+        }
+        left -= take;
+        if (left <= 0) break;
+        tile = 0;
+        if (++h == s.c.heads) {
+            h = 0;
+            do {
+                if (++e >= entries_of(s)) return;
+                n = __builtin_amdgcn_readfirstlane(tiles_of(s, e));
+            } while (n == 0);
+        }
+    }
+}
+
+// Joins the triples of a row: those of its own keys' runs and, with a prefix,
+// those of the prefix's.  One wave per row.  Rows that a run has finished are
+// left alone; rows without any keys become zeros.
+template <class T, int D>
+__global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead) {
     constexpr int E = D / 64;
-    constexpr int R = BITS == 8 ? D : D / 2;
-    __shared__ float part[4][D + 2];
-    const int hq = blockIdx.x % a.q_heads;
-    const int64_t bt = blockIdx.x / a.q_heads;
-    const int b = (int)(bt / a.tokens), t = (int)(bt % a.tokens);
-    const int h = hq / (a.q_heads / c.heads);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const T* q = static_cast<const T*>(a.q) + b * a.q_batch_stride + t * a.q_token_stride +
-                 hq * a.q_head_stride;
-    float qf[E], o[E] = {};
-#pragma unroll
-    for (int e = 0; e < E; ++e) qf[e] = (float)q[lane * E + e];
-    int count = a.tokens;
-    if (a.counts != nullptr) count = min(count, a.counts[b]);
-    float m = kNegInf, l = 0.f;
-    auto walk = [&](const int32_t* table, int64_t cols, int64_t n) {
-        n = min(n, cols * c.page_size);
-        for (int64_t j = wave; j < n; j += 4) {
-            const int64_t page = page_in(table[j / c.page_size], c.pages);
-            if (page < 0) continue;
-            const int64_t ph = page * c.heads + h;
-            const int in = (int)(j % c.page_size);
-            const uint8_t* kr = static_cast<const uint8_t*>(c.k) + (ph * c.page_size + in) * R;
-            const uint8_t* vr = static_cast<const uint8_t*>(c.v) +
-                                (ph * (c.page_size / 16) + in / 16) * R * 16 + in % 16;
-            auto code = [&](const uint8_t* p, int step, int d) {
-                if (BITS == 8) return (float)(int8_t)p[d * step];
-                return (float)((int)((uint32_t)p[(d / 2) * step] << (28 - 4 * (d & 1))) >> 28);
-            };
-            const float* sc = c.scales + ph * 2 * c.page_size + in;
-            float s = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) s = __builtin_fmaf(qf[e], code(kr, 1, lane * E + e), s);
-            s = lanes_sum<64>(s) * (sc[0] * a.softmax_scale);
-            const float top = fmaxf(m, s);
-            const float ref = top == kNegInf ? 0.f : top;
-            const float keep = __expf(m - ref), p = __expf(s - ref);
-            m = top;
-            l = l * keep + p;
-            const float pv = p * sc[c.page_size];
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = o[e] * keep + pv * code(vr, 16, lane * E + e);
-        }
+    using VE = Vec<float, E>;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+    const cq_attention_t& a = own.a;
+    if (row >= (int64_t)a.batch * a.tokens * a.q_heads) return;     // uniform over the wave
+    const int hq = (int)(row % a.q_heads), t = (int)(row / a.q_heads % a.tokens);
+    const int b = (int)(row / a.q_heads / a.tokens);
+    const int h = hq / own.group, r = t * own.group + hq % own.group;
+
+    // a source's triples of the row: `count` of them, the first at `first`,
+    // later ones `stride` rows on (from the run after the first)
+    struct Parts {
+        int count = 0;
+        bool home = false;
+        int64_t run = 0;
+        int local = 0;
     };
-    if (t < count) {
-        if (a.prefix_len > 0) walk(a.prefix_table, a.prefix_cols, a.prefix_len);
-        walk(a.table + b * a.table_stride, a.table_cols, (int64_t)a.lengths[b] - count + t + 1);
+    auto parts_of = [&](const Source& s, int entry, int local) {
+        Parts p;
+        const int n = tiles_of(s, entry);
+        if (n == 0) return p;
+        const Deal d = deal_at(s, entry, lane);
+        const int64_t per = run_length(s, d.total);
+        const int64_t from = d.before * s.c.heads + (int64_t)h * n;
+        p.run = from / per;
+        p.count = (int)((from + n - 1) / per - p.run) + 1;
+        p.home = p.count == 1;
+        p.local = local;
+        return p;
+    };
+    auto place = [&](const Source& s, const Parts& p, int i) -> int64_t {
+        if (p.home) return row;
+        return ((p.run + i) * 2 + (i == 0 ? 1 : 0)) * s.rows_per_unit + p.local;
+    };
+    const Parts mine = parts_of(own, b * own.row_groups + r / own.rows_per_unit,
+                                r % own.rows_per_unit);
+    if (own.finish && mine.home) return;
+    Parts pre;
+    if (!own.finish) {
+        const int pr = b * a.tokens * own.group + r;
+        pre = parts_of(ahead, pr / ahead.rows_per_unit, pr % ahead.rows_per_unit);
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) part[wave][lane * E + e] = o[e];
-    if (lane == 0) part[wave][D] = m, part[wave][D + 1] = l;
-    __syncthreads();
+    const int count = mine.count + pre.count;
+    auto at = [&](int i, const float*& o, const float*& ml) {
+        const bool first = i < mine.count;
+        const Source& s = first ? own : ahead;
+        const Parts& p = first ? mine : pre;
+        const int64_t x = place(s, p, first ? i : i - mine.count);
+        o = (p.home ? s.home_o : s.broken_o) + x * D;
+        ml = (p.home ? s.home_ml : s.broken_ml) + x * 2;
+    };
     float top = kNegInf;
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][D]);
-    const float ref = top == kNegInf ? 0.f : top;
-    for (int d = threadIdx.x; d < D; d += kBlock) {
-        float sum = 0.f, out = 0.f;
-        for (int w = 0; w < 4; ++w) {
-            const float keep = __expf(part[w][D] - ref);
-            sum += part[w][D + 1] * keep;
-            out += part[w][d] * keep;
+    for (int base = 0; base < count; base += 64) {
+        float m = kNegInf;
+        if (base + lane < count) {
+            const float *o, *ml;
+            at(base + lane, o, ml);
+            m = ml[0];
         }
-        static_cast<T*>(a.out)[(int64_t)blockIdx.x * D + d] = (T)(sum == 0.f ? 0.f : out / sum);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+        top = fmaxf(top, m);
     }
+    float sum = 0.f;
+    VE acc = {};
+    for (int base = 0; base < count; base += 64) {
+        float keep = 0.f;
+        if (base + lane < count) {
+            const float *o, *ml;
+            at(base + lane, o, ml);
+            keep = factor(ml[0], ml[1], top);
+            sum += keep * ml[1];
+        }
+        const int n = min(64, count - base);
+        for (int i = 0; i < n; ++i) {
+            const float *o, *ml;
+            at(base + i, o, ml);
+            const float k = __shfl(keep, i);
+            const VE v = *reinterpret_cast<const VE*>(o + lane * E);
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[j] += v[j] * k;
+        }
+    }
+    sum = lanes_sum<64>(sum);
+    T* out = static_cast<T*>(a.out) + row * D + lane * E;
+#pragma unroll
+    for (int j = 0; j < E; ++j) out[j] = (T)(sum == 0.f ? 0.f : acc[j] / sum);
+}
+
+// ------------------------------------------------------------------- host
+constexpr int kCus = 256;
+
+struct Shape {
+    int nb;
+    bool share;
+};
+
+// Rows that share keys fill one wave's matrices; many of them go to all four
+// waves of a workgroup.
+Shape shape_of(int64_t rows, int d) {
+    if (rows <= 16) return {1, false};
+    if (d > 128) return {1, true};
+    if (rows <= 32) return {2, false};
+    return {2, true};
+}
+
+Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, Shape* shape) {
+    Source s{};
+    s.c = c;
+    s.a = a;
+    s.prefix = prefix;
+    s.group = a.q_heads / c.heads;
+    const int64_t rows = (int64_t)a.tokens * s.group * (prefix ? a.batch : 1);
+    s.rows = (int32_t)rows;
+    *shape = shape_of(rows, c.head_dim);
+    s.rows_per_unit = 16 * shape->nb * (shape->share ? kWaves : 1);
+    s.row_groups = (int32_t)((rows + s.rows_per_unit - 1) / s.rows_per_unit);
+    s.least = shape->share ? 1 : kWaves;
+    s.finish = a.prefix_len == 0;
+    // no more runs than tiles, as far as the tables' sizes tell
+    const int64_t keys = prefix ? a.prefix_len : (int64_t)a.table_cols * c.page_size;
+    const int64_t entries = (int64_t)s.row_groups * (prefix ? 1 : a.batch);
+    const __int128 tiles = (__int128)((keys + kTile - 1) / kTile) * entries * c.heads;
+    const __int128 most = (tiles + s.least - 1) / s.least;
+    const int64_t room = (int64_t)kCus * waves_of(c.head_dim, shape->nb);
+    s.runs = (uint32_t)(most < room ? (most < 1 ? 1 : (int64_t)most) : room);
+    return s;
+}
+
+// Lays out the workspace from `base` (null: only sizes); returns its bytes.
+int64_t lay_out(const cq_kv_cache_t& c, const cq_attention_t& a, Source* own, Source* ahead,
+                char* base) {
+    int64_t used = 0;
+    auto take = [&](int64_t rows, float** o, float** ml) {
+        *o = reinterpret_cast<float*>(base + used);
+        used += rows * c.head_dim * 4;
+        *ml = reinterpret_cast<float*>(base + used);
+        used += (rows * 8 + 15) / 16 * 16;
+    };
+    const int64_t all = (int64_t)a.batch * a.tokens * a.q_heads;
+    for (Source* s : {own, ahead}) {
+        if (s->rows == 0) continue;
+        take((int64_t)s->runs * 2 * s->rows_per_unit, &s->broken_o, &s->broken_ml);
+        if (!s->finish) take(all, &s->home_o, &s->home_ml);
+    }
+    return used;
+}
+
+template <class T, int BITS, int D>
+hipError_t launch_tiles(const Source& s, Shape shape, hipStream_t stream) {
+    auto go = [&](auto* kernel) {
+        kernel<<<dim3(s.runs), dim3(kBlock), 0, stream>>>(s);
+        return hipGetLastError();
+    };
+    if constexpr (D > 128) {
+        return shape.share ? go(&tile_kernel<T, BITS, D, 1, true>)
+                           : go(&tile_kernel<T, BITS, D, 1, false>);
+    } else {
+        if (shape.nb == 1) return go(&tile_kernel<T, BITS, D, 1, false>);
+        return shape.share ? go(&tile_kernel<T, BITS, D, 2, true>)
+                           : go(&tile_kernel<T, BITS, D, 2, false>);
+    }
+}
+
+template <class T, int D>
+hipError_t launch_typed(const Source& own, Shape os, const Source& ahead, Shape as,
+                        hipStream_t stream) {
+    hipError_t e = hipSuccess;
+    const bool wide = own.c.bits == 8;
+    if (ahead.rows > 0)
+        e = wide ? launch_tiles<T, 8, D>(ahead, as, stream) : launch_tiles<T, 4, D>(ahead, as, stream);
+    if (e != hipSuccess) return e;
+    e = wide ? launch_tiles<T, 8, D>(own, os, stream) : launch_tiles<T, 4, D>(own, os, stream);
+    if (e != hipSuccess) return e;
+    const int64_t rows = (int64_t)own.a.batch * own.a.tokens * own.a.q_heads;
+    join_kernel<T, D><<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kBlock), 0, stream>>>(
+        own, ahead);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t attention_workspace(const cq_kv_cache_t&, const cq_attention_t&) { return 0; }
+int64_t attention_workspace(const cq_kv_cache_t& c, const cq_attention_t& a) {
+    Shape os{}, as{};
+    Source own = source_of(c, a, false, &os), ahead{};
+    if (a.prefix_len > 0) ahead = source_of(c, a, true, &as);
+    return lay_out(c, a, &own, &ahead, nullptr);
+}
 
 hipError_t launch_attention(const cq_kv_cache_t& c, const cq_attention_t& a,
                             hipStream_t stream) {
-    const int64_t grid = (int64_t)a.batch * a.tokens * a.q_heads;
-    if (grid > kMaxGrid) return hipErrorInvalidValue;
-    auto go = [&](auto* kernel) {
-        kernel<<<dim3((unsigned)grid), dim3(kBlock), 0, stream>>>(c, a);
-        return hipGetLastError();
-    };
+    Shape os{}, as{};
+    Source own = source_of(c, a, false, &os), ahead{};
+    if (a.prefix_len > 0) ahead = source_of(c, a, true, &as);
+    lay_out(c, a, &own, &ahead, static_cast<char*>(a.workspace));
     auto typed = [&](auto elem) {
         using T = decltype(elem);
-        if (c.bits == 8)
-            return c.head_dim == 64 ? go(&row_kernel<T, 8, 64>)
-                   : c.head_dim == 128 ? go(&row_kernel<T, 8, 128>) : go(&row_kernel<T, 8, 256>);
-        return c.head_dim == 64 ? go(&row_kernel<T, 4, 64>)
-               : c.head_dim == 128 ? go(&row_kernel<T, 4, 128>) : go(&row_kernel<T, 4, 256>);
+        if (c.head_dim == 64) return launch_typed<T, 64>(own, os, ahead, as, stream);
+        if (c.head_dim == 128) return launch_typed<T, 128>(own, os, ahead, as, stream);
+        return launch_typed<T, 256>(own, os, ahead, as, stream);
     };
     return a.dtype == CQ_DTYPE_F16 ? typed(_Float16{}) : typed(__bf16{});
 }
