@@ -11,8 +11,16 @@
 // (M, l, o) of disjoint keys join the same way.  Folding V's exponent into
 // that of the softmax keeps w_j, which the matrix instructions take as fp16,
 // in range for any scales: the largest w of a row lies in [1/2, 2^kRaise), and
-// what fp16 then rounds off is 2^-11 of each weight, or 2^-24 of 1.  The codes
-// are exact in fp16; scores, sums and statistics are FP32.
+// what fp16 then rounds off is 2^-11 of each weight, or 2^-24 of 1.
+// Scores, statistics and sums are FP32.
+//
+// A code of K goes into the matrix units as the fp16 subnormal
+// (code + 2^(bits-1)) 2^-24, which is the code's bits with the sign bit turned
+// and nothing else: one operation for two codes.  What the offset adds to a
+// score is the same for every key of a row, so the score sums start at minus
+// that.  V's codes go in as they are: there a common offset would cost digits
+// where a key of large weight has small codes.  q is brought to fp16 times a
+// power of two that puts the wave's largest finite element into [2^13, 2^14).
 //
 // Matrix form, 64 keys at a time (v_mfma_f32_16x16x32_f16, FP32 sums):
 //   S^T [keys x rows] = K [keys x D] Q^T [D x rows]
@@ -63,6 +71,7 @@ struct Source {
     int32_t row_groups;    // of rows_per_unit rows
     int32_t rows_per_unit;
     int32_t prefix;        // 1: the prefix's keys
+    int32_t page_shift;    // log2 of the page size
     int32_t least;         // tiles that a run has at least
     uint32_t runs;         // workgroups
     int32_t finish;        // 1: units of one run write `out`; 0: their home
@@ -100,13 +109,22 @@ __device__ __forceinline__ int entries_of(const Source& s) {
     return s.prefix ? s.row_groups : s.a.batch * s.row_groups;
 }
 
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lane) {     // inclusive
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t up = __shfl_up(v, off);
-        if (lane >= off) v += up;
-    }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {     // inclusive
+    v += row_dpp<0x111>(v);                                     // row_shr 1, 2, 4, 8
+    v += row_dpp<0x112>(v);
+    v += row_dpp<0x114>(v);
+    v += row_dpp<0x118>(v);
+    // the last lane of a row to the rows behind it
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
     return v;
+}
+
+// x / y of whole numbers >= 0, in 32 bits where they fit (a 64-bit division
+// takes a hundred instructions).
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+    if (((uint64_t)x | (uint64_t)y) >> 32 == 0) return (uint32_t)x / (uint32_t)y;
+    return x / y;
 }
 
 // Tiles (of one head) before entry `at`, in all, and, if `find` is not
@@ -130,7 +148,7 @@ __device__ __forceinline__ Deal deal_at(const Source& s, int at, int lane) {
     }
     for (int base = 0; base < n; base += 64) {
         const int e = base + lane;
-        const uint32_t sum = wave_scan(e < n ? tiles_of(s, e) : 0, lane);
+        const uint32_t sum = wave_scan(e < n ? tiles_of(s, e) : 0);
         if (at >= base && at < base + 64)
             d.before = d.total + (at > base ? __shfl(sum, at - base - 1) : 0u);
         d.total += __shfl(sum, 63);
@@ -145,14 +163,14 @@ __device__ __forceinline__ Deal deal_find(const Source& s, int64_t pos, int64_t 
     const int n = entries_of(s), heads = s.c.heads;
     if (s.prefix) {
         const int t = tiles_of(s, 0);
-        d.entry = (int)(pos / ((int64_t)t * heads));
+        d.entry = (int)quotient(pos, (int64_t)t * heads);
         d.before = (int64_t)t * d.entry;
         return d;
     }
     int64_t done = 0;
     for (int base = 0; base < n; base += 64) {
         const int e = base + lane;
-        const uint32_t sum = wave_scan(e < n ? tiles_of(s, e) : 0, lane);
+        const uint32_t sum = wave_scan(e < n ? tiles_of(s, e) : 0);
         const uint64_t past = __ballot((done + sum) * heads > pos);
         if (past != 0) {
             const int first = __builtin_ctzll(past);
@@ -167,41 +185,65 @@ __device__ __forceinline__ Deal deal_find(const Source& s, int64_t pos, int64_t 
 
 __device__ __forceinline__ int64_t run_length(const Source& s, int64_t total) {
     const int64_t all = total * s.c.heads;
-    return max((int64_t)s.least, (all + s.runs - 1) / s.runs);
+    return max((int64_t)s.least, quotient(all + s.runs - 1, s.runs));
 }
 
 // ----------------------------------------------------------- small pieces
-__device__ __forceinline__ uint32_t pk_sub_f16(uint32_t a, float b) {
+// K's codes of a word as fp16 pairs, offset and in units of 2^-24: bytes (0, 2),
+// (1, 3) of int8; of int4 the low and high nibbles of bytes (0, 2) and of
+// (1, 3), the high ones 16 times what they stand for.
+__device__ __forceinline__ void halves_of_bytes(uint32_t w, uint32_t& a, uint32_t& b) {
+    a = (w & 0x00FF00FFu) ^ 0x00800080u;
+    b = ((w >> 8) & 0x00FF00FFu) ^ 0x00800080u;
+}
+__device__ __forceinline__ void halves_of_nibbles(uint32_t w, uint32_t (&p)[4]) {
+    const uint32_t x = w >> 8;
+    p[0] = (w & 0x000F000Fu) ^ 0x00080008u;
+    p[1] = (w & 0x00F000F0u) ^ 0x00800080u;
+    p[2] = (x & 0x000F000Fu) ^ 0x00080008u;
+    p[3] = (x & 0x00F000F0u) ^ 0x00800080u;
+}
+
+// V's codes as fp16 pairs in the same order: under the exponent of 1024 (of 64
+// for a high nibble, whose last bits are then sixteenths), less the offset.
+__device__ __forceinline__ uint32_t less(uint32_t a, float b) {
     const h2 v = __builtin_bit_cast(h2, a) - h2{(_Float16)b, (_Float16)b};
     return __builtin_bit_cast(uint32_t, v);
 }
-
-// Four int8 of a word as fp16 pairs (0, 2), (1, 3): the byte under the
-// exponent of 1024, sign bit flipped, is 1152 + code.
-__device__ __forceinline__ void fp16_of_bytes(uint32_t w, uint32_t& a, uint32_t& b) {
-    a = pk_sub_f16((w & 0x00FF00FFu) ^ 0x64806480u, 1152.f);
-    b = pk_sub_f16(((w >> 8) & 0x00FF00FFu) ^ 0x64806480u, 1152.f);
+__device__ __forceinline__ void codes_of_bytes(uint32_t w, uint32_t& a, uint32_t& b) {
+    a = less((w & 0x00FF00FFu) ^ 0x64806480u, 1152.f);
+    b = less(((w >> 8) & 0x00FF00FFu) ^ 0x64806480u, 1152.f);
 }
-
-// Eight int4 of a word as fp16 pairs (0, 4), (1, 5), (2, 6), (3, 7); the high
-// nibble of a byte stays in place under the exponent of 64, whose last bits
-// are sixteenths.
-__device__ __forceinline__ void fp16_of_nibbles(uint32_t w, uint32_t (&p)[4]) {
+__device__ __forceinline__ void codes_of_nibbles(uint32_t w, uint32_t (&p)[4]) {
     const uint32_t x = w >> 8;
-    p[0] = pk_sub_f16((w & 0x000F000Fu) ^ 0x64086408u, 1032.f);
-    p[1] = pk_sub_f16((w & 0x00F000F0u) ^ 0x54805480u, 72.f);
-    p[2] = pk_sub_f16((x & 0x000F000Fu) ^ 0x64086408u, 1032.f);
-    p[3] = pk_sub_f16((x & 0x00F000F0u) ^ 0x54805480u, 72.f);
+    p[0] = less((w & 0x000F000Fu) ^ 0x64086408u, 1032.f);
+    p[1] = less((w & 0x00F000F0u) ^ 0x54805480u, 72.f);
+    p[2] = less((x & 0x000F000Fu) ^ 0x64086408u, 1032.f);
+    p[3] = less((x & 0x00F000F0u) ^ 0x54805480u, 72.f);
 }
 
 // Maximum and sum over the four lanes l, l + 16, l + 32, l + 48, in each.
+template <class F>
+__device__ __forceinline__ float quad_fold(float v, F&& f) {
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const uint32_t y = __float_as_uint(v);
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float quad_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    return quad_fold(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float quad_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    return quad_fold(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, row_dpp<0x128>(v));
+    v = fmaxf(v, row_dpp<0x124>(v));
+    v = fmaxf(v, row_dpp<0x122>(v));
+    v = fmaxf(v, row_dpp<0x121>(v));
+    return quad_max(v);
 }
 
 // What a triple's sums are multiplied with to stand at reference `top`.  One
@@ -219,6 +261,12 @@ __device__ __forceinline__ void store4(T* p, f4 v) {
     *reinterpret_cast<Vec<T, 4>*>(p) = o;
 }
 
+// What a wave's lanes know of a tile's keys, for the others: K's scale with all
+// that a score takes, V's as f 2^e, and 2^-e.
+struct Keys {
+    float k[kTile], e[kTile], f[kTile], back[kTile];
+};
+
 // ------------------------------------------------------------- the kernel
 // NB row matrices to a wave.  SHARE: the four waves take the same keys for
 // four times 16 NB rows; otherwise the same 16 NB rows, and every fourth tile
@@ -234,7 +282,9 @@ struct Tiles {
     static constexpr int kVTiles = kRow / 16;              // 16 rows of V bytes
     static constexpr int kOTiles = D / 16;
     static constexpr int kUnitRows = 16 * NB * (SHARE ? kWaves : 1);
-    static constexpr bool kHalf = sizeof(T) == 2 && std::is_same_v<T, _Float16>;
+    // a code's offset and unit as the matrix units see it
+    static constexpr float kOffset = BITS == 8 ? 128.f : 8.f;
+    static constexpr float kUnit = 0x1p-24f;
 
     // Where dims of product step u of lane group g start, and their order:
     // the unpacking leaves pairs of bytes or nibbles apart.
@@ -249,7 +299,8 @@ struct Tiles {
     }
 
     h8 q[NB][kSteps];
-    float qscale[NB];                    // scale log2(e) over q's own factor
+    float start[NB];                     // what the score sums start at
+    float qscale;                        // of a score sum: scale log2(e), units, q's factor
     int limit[NB];                       // keys that the lane's row sees
     int full;                            // tiles of which every row sees all
     f4 o[NB][kOTiles];
@@ -257,7 +308,7 @@ struct Tiles {
 
     Vec<uint32_t, kWords> kq[4][kChunks];
     u4 vq[kVTiles];
-    f4 ks[4], vs[4];
+    float ks, vs;                        // scales of key `lane` of the tile
     bool there;                          // the lane group's 16 keys have a page
 
     // Row r of the unit's source: its query and where its result goes.
@@ -276,6 +327,8 @@ struct Tiles {
                                            int lane) {
         const int g = lane >> 4;
         int least = 0x7FFFFFFF;
+        Vec<T, 8> raw[NB][kSteps];
+        float top = 0.f;
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
             // rows past the last repeat it (nobody stores them)
@@ -290,38 +343,35 @@ struct Tiles {
             least = min(least, limit[rb]);
             const T* p = static_cast<const T*>(s.a.q) + bb * s.a.q_batch_stride +
                          t * s.a.q_token_stride + hq * s.a.q_head_stride;
-            qscale[rb] = s.a.softmax_scale * kLog2e;
-            Vec<T, 8> raw[kSteps];
 #pragma unroll
-            for (int u = 0; u < kSteps; ++u)
-                raw[u] = *reinterpret_cast<const Vec<T, 8>*>(p + step_dim(u, g));
-            float by = 1.f;
-            if constexpr (!kHalf) {
-                // bfloat16 goes into fp16 times a power of two that brings the
-                // row's largest into [2^14, 2^15): exact down to 2^-28 of it
-                float top = 0.f;
+            for (int u = 0; u < kSteps; ++u) {
+                raw[rb][u] = *reinterpret_cast<const Vec<T, 8>*>(p + step_dim(u, g));
 #pragma unroll
-                for (int u = 0; u < kSteps; ++u)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf((float)raw[u][i]));
-                top = quad_max(top);
-                int e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
-                if (top == 0.f || top > 3.4e38f) e = 0;
-                by = ldexpf(1.f, -e);
-                if (e < -126) {                    // 2^-e is no FP32 number
-                    by = 0x1p126f;
-                    e = -126;
+                for (int i = 0; i < 8; ++i) {
+                    const float x = fabsf((float)raw[rb][u][i]);
+                    top = fmaxf(top, x < __builtin_inff() ? x : 0.f);
                 }
-                qscale[rb] *= ldexpf(1.f, e);
             }
+        }
+        // One factor for the wave: exact down to 2^-27 of its largest element,
+        // 2^-38 of that where fp16 is subnormal, so an error far below FP32's
+        // in the largest row's scores is all that a small row can show.
+        top = wave_max(top);
+        const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+        qscale = ldexpf(s.a.softmax_scale * kLog2e * (1.f / kUnit), e);
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+            float sum = 0.f;
 #pragma unroll
             for (int u = 0; u < kSteps; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const T x = raw[u][order(i)];
-                    if constexpr (kHalf) q[rb][u][i] = x;
-                    else q[rb][u][i] = (_Float16)((float)x * by);
+                    // high nibbles come as 16 times their code
+                    const int down = BITS == 4 && (order(i) & 1) ? 4 : 0;
+                    q[rb][u][i] = (_Float16)ldexpf((float)raw[rb][u][order(i)], -e - down);
+                    sum = __builtin_fmaf((float)q[rb][u][i], down ? 16.f : 1.f, sum);
                 }
+            start[rb] = -kOffset * kUnit * quad_sum(sum);
         }
 #pragma unroll
         for (int off = 1; off < 16; off <<= 1) least = min(least, __shfl_xor(least, off));
@@ -338,7 +388,7 @@ struct Tiles {
     // Table entry of 16 keys `sub` of a tile (any entry past the table).
     static __device__ __forceinline__ int32_t entry(const Source& s, const int32_t* table,
                                                     int cols, int tile, int sub) {
-        return table[min((int)(((int64_t)tile * kTile + sub * 16) / s.c.page_size), cols - 1)];
+        return table[min((tile * kTile + sub * 16) >> s.page_shift, cols - 1)];
     }
 
     __device__ __forceinline__ void load_k(const Source& s, int32_t entry, int tile, int h,
@@ -363,12 +413,9 @@ struct Tiles {
         const int64_t page = max((int64_t)0, page_in(entry, s.c.pages));
         there = page_in(entry, s.c.pages) >= 0;
         const int in = (tile * kTile + g * 16) & (s.c.page_size - 1);
-        const float* p = s.c.scales + (page * s.c.heads + h) * 2 * s.c.page_size + in;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            ks[t] = *reinterpret_cast<const f4*>(p + 4 * t);
-            vs[t] = *reinterpret_cast<const f4*>(p + s.c.page_size + 4 * t);
-        }
+        const float* p = s.c.scales + (page * s.c.heads + h) * 2 * s.c.page_size + in + (lane & 15);
+        ks = p[0];
+        vs = p[s.c.page_size];
     }
 
     __device__ __forceinline__ void load_v(const Source& s, int32_t entry, int tile, int h,
@@ -387,28 +434,38 @@ struct Tiles {
         constexpr int per = kChunk / BITS;
         u4 w;
         if constexpr (BITS == 8) {
-            uint32_t a, b, c, d;
-            fp16_of_bytes(row[u / per][2 * (u % per)], a, b);
-            fp16_of_bytes(row[u / per][2 * (u % per) + 1], c, d);
-            w = u4{a, b, c, d};
+            uint32_t x, y, z, v;
+            halves_of_bytes(row[u / per][2 * (u % per)], x, y);
+            halves_of_bytes(row[u / per][2 * (u % per) + 1], z, v);
+            w = u4{x, y, z, v};
         } else {
             // pairs (0, 4), (1, 5), (2, 6), (3, 7) of the word's nibbles
-            uint32_t p[4];
-            fp16_of_nibbles(row[u / per][u % per], p);
-            w = u4{p[0], p[1], p[2], p[3]};
+            uint32_t x[4];
+            halves_of_nibbles(row[u / per][u % per], x);
+            w = u4{x[0], x[1], x[2], x[3]};
         }
         return __builtin_bit_cast(h8, w);
     }
 
-    // One tile of keys.  `next`: issues the loads that the registers freed
-    // here can take.
+    // One tile of keys.  next_k and next_v issue the loads that the registers
+    // freed by then can take.  `keys`: LDS of the wave's own.
     template <class NextK, class NextV>
-    __device__ __forceinline__ void step(int tile, int lane, NextK&& next_k, NextV&& next_v) {
+    __device__ __forceinline__ void step(int tile, int lane, Keys& keys, NextK&& next_k,
+                                         NextV&& next_v) {
+        {
+            const int e = max((int)((__float_as_uint(vs) >> 23) & 0xFF) - 126, kLeastExp);
+            keys.k[lane] = ks * qscale;
+            keys.e[lane] = (float)e;
+            keys.f[lane] = __builtin_amdgcn_ldexpf(vs, -e);
+            keys.back[lane] = __builtin_amdgcn_ldexpf(1.f, -e);
+        }
+        const bool here = there;
         f4 sc[NB][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int rb = 0; rb < NB; ++rb) sc[rb][t] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int rb = 0; rb < NB; ++rb)
+                sc[rb][t] = f4{start[rb], start[rb], start[rb], start[rb]};
 #pragma unroll
             for (int u = 0; u < kSteps; ++u) {
                 const h8 k = unpack_k(kq[t], u);
@@ -419,17 +476,11 @@ struct Tiles {
             }
         }
         next_k();
-        // V's scales as f 2^e
-        float f[16], ef[16], back[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const float v = vs[j / 4][j % 4];
-            const int e = max((int)((__float_as_uint(v) >> 23) & 0xFF) - 126, kLeastExp);
-            f[j] = __builtin_amdgcn_ldexpf(v, -e);
-            ef[j] = (float)e;
-            back[j] = __builtin_amdgcn_ldexpf(1.f, -e);
-        }
-        const bool masked = tile >= full || !__all(there);
+        // the keys' quadruples come from other lanes of this wave
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int own = lane & 48;           // the lane's 16 keys
+        const bool masked = tile >= full || !__all(here);
         h8 w[NB][2];
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
@@ -437,15 +488,13 @@ struct Tiles {
             float top = kNegInf;
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                x[j] = __builtin_fmaf(sc[rb][j / 4][j % 4], ks[j / 4][j % 4] * qscale[rb],
-                                      ef[j] - ref[rb]);
-            uint32_t seen = 0xFFFFu;
+                x[j] = __builtin_fmaf(sc[rb][j / 4][j % 4], keys.k[own + j], keys.e[own + j] - ref[rb]);
+            int n = 16;
             if (masked) {
-                const int n = there ? limit[rb] - tile * kTile - (lane >> 4) * 16 : 0;
-                seen = n <= 0 ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1;
+                asm volatile("");       // a branch, not selects on every tile
+                n = here ? limit[rb] - tile * kTile - (lane >> 4) * 16 : 0;
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (!((seen >> j) & 1)) x[j] = kNegInf;
+                for (int j = 0; j < 16; ++j) x[j] = j < n ? x[j] : kNegInf;
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
@@ -463,18 +512,17 @@ struct Tiles {
                     for (int j = 0; j < 16; ++j) x[j] -= top;
                 }
             }
-            float p[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const float y = __builtin_amdgcn_exp2f(x[j]);
-                l[rb] = __builtin_fmaf(y, back[j], l[rb]);
-                p[j] = y * f[j];
+                l[rb] = __builtin_fmaf(y, keys.back[own + j], l[rb]);
+                x[j] = y * keys.f[own + j];
             }
             if (masked) {
                 // what is not seen may have a scale of NaN or Inf
+                asm volatile("");
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (!((seen >> j) & 1)) p[j] = 0.f;
+                for (int j = 0; j < 16; ++j) x[j] = j < n ? x[j] : 0.f;
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -482,17 +530,19 @@ struct Tiles {
                 for (int i = 0; i < 8; ++i) {
                     // keys of a word as its bytes come out: 0, 2, 1, 3
                     constexpr int at[4] = {0, 2, 1, 3};
-                    w[rb][u][i] = (_Float16)p[8 * u + (i & 4) + at[i & 3]];
+                    w[rb][u][i] = (_Float16)x[8 * u + (i & 4) + at[i & 3]];
                 }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < kVTiles; ++i)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 if constexpr (BITS == 8) {
                     uint32_t a, b, c, d;
-                    fp16_of_bytes(vq[i][2 * u], a, b);
-                    fp16_of_bytes(vq[i][2 * u + 1], c, d);
+                    codes_of_bytes(vq[i][2 * u], a, b);
+                    codes_of_bytes(vq[i][2 * u + 1], c, d);
                     const h8 v = __builtin_bit_cast(h8, u4{a, b, c, d});
 #pragma unroll
                     for (int rb = 0; rb < NB; ++rb)
@@ -502,8 +552,8 @@ struct Tiles {
                     // bytes are tokens here: low nibbles the even dim's, high
                     // ones the odd dim's
                     uint32_t p0[4], p1[4];
-                    fp16_of_nibbles(vq[i][2 * u], p0);
-                    fp16_of_nibbles(vq[i][2 * u + 1], p1);
+                    codes_of_nibbles(vq[i][2 * u], p0);
+                    codes_of_nibbles(vq[i][2 * u + 1], p1);
                     const h8 even = __builtin_bit_cast(h8, u4{p0[0], p0[2], p1[0], p1[2]});
                     const h8 odd = __builtin_bit_cast(h8, u4{p0[1], p0[3], p1[1], p1[3]});
 #pragma unroll
@@ -519,7 +569,7 @@ struct Tiles {
     }
 
     __device__ __forceinline__ void run(const Source& s, int b, int h, int tile, int end,
-                                        int stride, int lane) {
+                                        int stride, int lane, Keys& keys) {
         const int32_t* table = s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride;
         const int cols = s.prefix ? s.a.prefix_cols : s.a.table_cols;
         const int ksub = (lane & 15) >> 2, vsub = lane >> 4;
@@ -534,7 +584,7 @@ struct Tiles {
                 ke = entry(s, table, cols, next, ksub);
                 ve = entry(s, table, cols, next, vsub);
             }
-            step(tile, lane, [&] { if (next < end) load_k(s, ke, next, h, lane); },
+            step(tile, lane, keys, [&] { if (next < end) load_k(s, ke, next, h, lane); },
                  [&] {
                      if (next < end) {
                          load_scales(s, ve, next, h, lane);
@@ -544,9 +594,9 @@ struct Tiles {
         }
     }
 
-    // Dims of o[.][i] start: four from 16 i + 4 g, or (4 bits) every other of
-    // eight from 32 (i / 2) + 8 g.
-    // f(dim, four values): the lane's part of row matrix rb, four dims a call.
+    // f(dim, four values): the lane's part of the sums of row matrix rb, four
+    // dims a call.  Dims of o[.][i] are four from 16 i + 4 g, or (4 bits) every
+    // other of eight from 32 (i / 2) + 8 g.
     template <class F>
     __device__ __forceinline__ void each_four(int rb, int lane, F&& f) const {
         const int g = lane >> 4;
@@ -574,6 +624,7 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
     // waves that split a unit's keys join here
     __shared__ __attribute__((aligned(16))) float sm_o[SHARE ? 1 : kRows][SHARE ? 4 : D + 4];
     __shared__ float sm_m[kWaves][SHARE ? 1 : kRows], sm_l[kWaves][SHARE ? 1 : kRows];
+    __shared__ __attribute__((aligned(16))) Keys sm_keys[kWaves];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t total = deal_at(s, 0, lane).total;
@@ -585,8 +636,8 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
     int e = __builtin_amdgcn_readfirstlane(d.entry);
     int n = __builtin_amdgcn_readfirstlane(tiles_of(s, e));
     const int64_t in_entry = pos - d.before * s.c.heads;
-    int h = __builtin_amdgcn_readfirstlane((int)(in_entry / n));
-    int tile = __builtin_amdgcn_readfirstlane((int)(in_entry % n));
+    int h = __builtin_amdgcn_readfirstlane((int)quotient(in_entry, n));
+    int tile = __builtin_amdgcn_readfirstlane((int)(in_entry - (int64_t)h * n));
     int64_t left = stop - pos;
     W work;
     for (;;) {
@@ -622,7 +673,7 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
         if (SHARE) {
             if (mine < s.rows) {
                 work.load_q(s, b, mine, h, lane);
-                work.run(s, b, h, tile, tile + take, 1, lane);
+                work.run(s, b, h, tile, tile + take, 1, lane, sm_keys[wave]);
 #pragma unroll
                 for (int rb = 0; rb < NB; ++rb) {
                     const int r = mine + 16 * rb + (lane & 15);
@@ -636,7 +687,7 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
             }
         } else {
             work.load_q(s, b, mine, h, lane);
-            work.run(s, b, h, tile + wave, tile + take, kWaves, lane);
+            work.run(s, b, h, tile + wave, tile + take, kWaves, lane, sm_keys[wave]);
             float m[NB], l[NB];
 #pragma unroll
             for (int rb = 0; rb < NB; ++rb) {
@@ -697,6 +748,7 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
 // Joins the triples of a row: those of its own keys' runs and, with a prefix,
 // those of the prefix's.  One wave per row.  Rows that a run has finished are
 // left alone; rows without any keys become zeros.
+constexpr int kJoin = 8;                // triples in flight
 template <class T, int D>
 __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead) {
     constexpr int E = D / 64;
@@ -724,8 +776,8 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead) 
         const Deal d = deal_at(s, entry, lane);
         const int64_t per = run_length(s, d.total);
         const int64_t from = d.before * s.c.heads + (int64_t)h * n;
-        p.run = from / per;
-        p.count = (int)((from + n - 1) / per - p.run) + 1;
+        p.run = quotient(from, per);
+        p.count = (int)(quotient(from + n - 1, per) - p.run) + 1;
         p.home = p.count == 1;
         p.local = local;
         return p;
@@ -759,31 +811,30 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead) 
             at(base + lane, o, ml);
             m = ml[0];
         }
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
-        top = fmaxf(top, m);
+        top = fmaxf(top, wave_max(m));
     }
     float sum = 0.f;
     VE acc = {};
-    for (int base = 0; base < count; base += 64) {
-        float keep = 0.f;
-        if (base + lane < count) {
-            const float *o, *ml;
-            at(base + lane, o, ml);
-            keep = factor(ml[0], ml[1], top);
-            sum += keep * ml[1];
-        }
-        const int n = min(64, count - base);
-        for (int i = 0; i < n; ++i) {
-            const float *o, *ml;
-            at(base + i, o, ml);
-            const float k = __shfl(keep, i);
-            const VE v = *reinterpret_cast<const VE*>(o + lane * E);
+    for (int base = 0; base < count; base += kJoin) {
+        VE v[kJoin];
+        float k[kJoin], l[kJoin];
 #pragma unroll
-            for (int j = 0; j < E; ++j) acc[j] += v[j] * k;
+        for (int i = 0; i < kJoin; ++i) {
+            const float *o, *ml;
+            at(min(base + i, count - 1), o, ml);
+            v[i] = *reinterpret_cast<const VE*>(o + lane * E);
+            k[i] = ml[0];
+            l[i] = ml[1];
+        }
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) {
+            if (base + i >= count) break;
+            const float keep = factor(k[i], l[i], top);
+            sum += keep * l[i];
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[j] += v[i][j] * keep;
         }
     }
-    sum = lanes_sum<64>(sum);
     T* out = static_cast<T*>(a.out) + row * D + lane * E;
 #pragma unroll
     for (int j = 0; j < E; ++j) out[j] = (T)(sum == 0.f ? 0.f : acc[j] / sum);
@@ -812,6 +863,7 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
     s.a = a;
     s.prefix = prefix;
     s.group = a.q_heads / c.heads;
+    s.page_shift = __builtin_ctz((unsigned)c.page_size);
     const int64_t rows = (int64_t)a.tokens * s.group * (prefix ? a.batch : 1);
     s.rows = (int32_t)rows;
     *shape = shape_of(rows, c.head_dim);
