@@ -72,7 +72,8 @@ struct Source {
     int32_t rows_per_unit;
     int32_t prefix;        // 1: the prefix's keys
     int32_t page_shift;    // log2 of the page size
-    int32_t least;         // tiles that a run has at least
+    int32_t quantum;       // a run's length is a multiple of it
+    int32_t cost;          // of a unit besides its tiles, in tiles
     uint32_t runs;         // workgroups
     int32_t finish;        // 1: units of one run write `out`; 0: their home
     // workspace: triples of broken units, two per run, and of whole units
@@ -97,12 +98,16 @@ __device__ __forceinline__ int own_limit(const Source& s, int length, int count,
 // Tiles of entry e: (sequence, row group), or the prefix's row group.
 __device__ __forceinline__ int tiles_of(const Source& s, int e) {
     if (s.prefix) return (s.a.prefix_len + kTile - 1) / kTile;
-    const int b = e / s.row_groups, rg = e % s.row_groups;
+    int b = e, last = s.a.tokens - 1, first = 0;
+    if (s.row_groups > 1) {
+        b = e / s.row_groups;
+        const int row = (e - b * s.row_groups) * s.rows_per_unit;
+        first = row / s.group;
+        last = min(last, (row + s.rows_per_unit - 1) / s.group);
+    }
     const int count = new_tokens(s.a, b);
-    const int first = rg * s.rows_per_unit / s.group;
     if (first >= count) return 0;
-    const int last = min((rg * s.rows_per_unit + s.rows_per_unit - 1) / s.group, count - 1);
-    return (own_limit(s, s.a.lengths[b], count, last) + kTile - 1) / kTile;
+    return (own_limit(s, s.a.lengths[b], count, min(last, count - 1)) + kTile - 1) / kTile;
 }
 
 __device__ __forceinline__ int entries_of(const Source& s) {
@@ -127,65 +132,36 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
     return x / y;
 }
 
-// Tiles (of one head) before entry `at`, in all, and, if `find` is not
-// negative, the entry that holds tile `find` of the heads' sequence: every
-// lane of the wave gets the same.  heads * tiles of a call fit 63 bits.
-struct Deal {
-    int64_t total = 0;      // tiles of all entries, one head
-    int64_t before = 0;     // tiles ahead of the entry, one head
-    int entry = 0;
-};
-
-__device__ __forceinline__ Deal deal_at(const Source& s, int at, int lane) {
-    Deal d;
-    d.entry = at;
-    const int n = entries_of(s);
-    if (s.prefix) {
-        const int t = tiles_of(s, 0);
-        d.total = (int64_t)t * n;
-        d.before = (int64_t)t * at;
-        return d;
-    }
-    for (int base = 0; base < n; base += 64) {
-        const int e = base + lane;
-        const uint32_t sum = wave_scan(e < n ? tiles_of(s, e) : 0);
-        if (at >= base && at < base + 64)
-            d.before = d.total + (at > base ? __shfl(sum, at - base - 1) : 0u);
-        d.total += __shfl(sum, 63);
-    }
-    return d;
+// A unit's place in the deal: as many steps as its tiles, rounded up to the
+// quantum, and its cost.
+__device__ __forceinline__ int steps_of(const Source& s, int tiles) {
+    if (tiles == 0) return 0;
+    return (tiles + s.quantum - 1) / s.quantum * s.quantum + s.cost;
 }
 
-// The entry that holds position `pos` (below heads * total).
-__device__ __forceinline__ Deal deal_find(const Source& s, int64_t pos, int64_t total, int lane) {
-    Deal d;
-    d.total = total;
-    const int n = entries_of(s), heads = s.c.heads;
-    if (s.prefix) {
-        const int t = tiles_of(s, 0);
-        d.entry = (int)quotient(pos, (int64_t)t * heads);
-        d.before = (int64_t)t * d.entry;
-        return d;
+// Entries base .. base + 63, one to a lane: tiles, steps, and the steps up to
+// and with the lane's, of one head.
+struct Entries {
+    int base, tiles;
+    uint32_t steps, upto;
+    __device__ __forceinline__ Entries(const Source& s, int at, int lane) : base(at) {
+        tiles = at + lane < entries_of(s) ? tiles_of(s, at + lane) : 0;
+        steps = steps_of(s, tiles);
+        upto = wave_scan(steps);
     }
-    int64_t done = 0;
-    for (int base = 0; base < n; base += 64) {
-        const int e = base + lane;
-        const uint32_t sum = wave_scan(e < n ? tiles_of(s, e) : 0);
-        const uint64_t past = __ballot((done + sum) * heads > pos);
-        if (past != 0) {
-            const int first = __builtin_ctzll(past);
-            d.entry = base + first;
-            d.before = done + (first > 0 ? __shfl(sum, first - 1) : 0u);
-            return d;
-        }
-        done += __shfl(sum, 63);
-    }
-    return d;
+    __device__ __forceinline__ uint32_t all() const { return __builtin_amdgcn_readlane(upto, 63); }
+};
+
+// Steps of all units of one head; `first` holds entries 0 .. 63.
+__device__ __forceinline__ int64_t all_steps(const Source& s, const Entries& first, int lane) {
+    int64_t total = first.all();
+    for (int base = 64; base < entries_of(s); base += 64) total += Entries(s, base, lane).all();
+    return total;
 }
 
 __device__ __forceinline__ int64_t run_length(const Source& s, int64_t total) {
-    const int64_t all = total * s.c.heads;
-    return max((int64_t)s.least, quotient(all + s.runs - 1, s.runs));
+    const int64_t each = quotient(total * s.c.heads + s.runs - 1, s.runs);
+    return (max((int64_t)1, each) + s.quantum - 1) / s.quantum * s.quantum;
 }
 
 // ----------------------------------------------------------- small pieces
@@ -311,17 +287,25 @@ struct Tiles {
     float ks, vs;                        // scales of key `lane` of the tile
     bool there;                          // the lane group's 16 keys have a page
 
-    // Row r of the unit's source: its query and where its result goes.
-    static __device__ __forceinline__ int64_t row_index(const Source& s, int b, int r, int h,
-                                                        int& t) {
-        if (s.prefix) {
-            const int per = s.a.tokens * s.group;
-            b = r / per;
-            r -= b * per;
+    // Row r of the unit's source: its sequence, new token and query head.
+    struct RowAt {
+        int b, t, hq;
+        __device__ __forceinline__ RowAt(const Source& s, int unit_b, int r, int h)
+            : b(unit_b), t(0), hq(h * s.group + r) {
+            if (s.prefix || s.a.tokens > 1) {
+                const int all = r / s.group;
+                hq = h * s.group + r - all * s.group;
+                t = all;
+                if (s.prefix) {
+                    b = all / s.a.tokens;
+                    t = all - b * s.a.tokens;
+                }
+            }
         }
-        t = r / s.group;
-        return ((int64_t)b * s.a.tokens + t) * s.a.q_heads + h * s.group + r % s.group;
-    }
+        __device__ __forceinline__ int64_t flat(const Source& s) const {
+            return ((int64_t)b * s.a.tokens + t) * s.a.q_heads + hq;
+        }
+    };
 
     __device__ __forceinline__ void load_q(const Source& s, int b, int first_row, int h,
                                            int lane) {
@@ -333,16 +317,13 @@ struct Tiles {
         for (int rb = 0; rb < NB; ++rb) {
             // rows past the last repeat it (nobody stores them)
             const int r = min(first_row + 16 * rb + (lane & 15), s.rows - 1);
-            int t;
-            const int64_t at = row_index(s, b, r, h, t);
-            const int hq = (int)(at % s.a.q_heads);
-            const int bb = (int)(at / s.a.q_heads / s.a.tokens);
-            const int count = new_tokens(s.a, bb);
-            limit[rb] = s.prefix ? (t < count ? s.a.prefix_len : 0)
-                                 : own_limit(s, s.a.lengths[bb], count, t);
+            const RowAt at(s, b, r, h);
+            const int count = new_tokens(s.a, at.b);
+            limit[rb] = s.prefix ? (at.t < count ? s.a.prefix_len : 0)
+                                 : own_limit(s, s.a.lengths[at.b], count, at.t);
             least = min(least, limit[rb]);
-            const T* p = static_cast<const T*>(s.a.q) + bb * s.a.q_batch_stride +
-                         t * s.a.q_token_stride + hq * s.a.q_head_stride;
+            const T* p = static_cast<const T*>(s.a.q) + at.b * s.a.q_batch_stride +
+                         at.t * s.a.q_token_stride + at.hq * s.a.q_head_stride;
 #pragma unroll
             for (int u = 0; u < kSteps; ++u) {
                 raw[rb][u] = *reinterpret_cast<const Vec<T, 8>*>(p + step_dim(u, g));
@@ -568,16 +549,22 @@ struct Tiles {
         next_v();
     }
 
-    __device__ __forceinline__ void run(const Source& s, int b, int h, int tile, int end,
-                                        int stride, int lane, Keys& keys) {
+    // Keys from tile `tile`, every `stride`th up to `end`.  The first loads go
+    // out before the queries are fetched.
+    __device__ __forceinline__ void run(const Source& s, int b, int first_row, int h, int tile,
+                                        int end, int stride, int lane, Keys& keys) {
         const int32_t* table = s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride;
         const int cols = s.prefix ? s.a.prefix_cols : s.a.table_cols;
         const int ksub = (lane & 15) >> 2, vsub = lane >> 4;
-        if (tile >= end) return;
-        int32_t ke = entry(s, table, cols, tile, ksub), ve = entry(s, table, cols, tile, vsub);
-        load_k(s, ke, tile, h, lane);
-        load_scales(s, ve, tile, h, lane);
-        load_v(s, ve, tile, h, lane);
+        int32_t ke = 0, ve = 0;
+        if (tile < end) {
+            ke = entry(s, table, cols, tile, ksub);
+            ve = entry(s, table, cols, tile, vsub);
+            load_k(s, ke, tile, h, lane);
+            load_scales(s, ve, tile, h, lane);
+            load_v(s, ve, tile, h, lane);
+        }
+        load_q(s, b, first_row, h, lane);
         for (; tile < end; tile += stride) {
             const int next = tile + stride;
             if (next < end) {
@@ -622,58 +609,69 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
     using W = Tiles<T, BITS, D, NB, SHARE>;
     constexpr int kRows = W::kUnitRows;
     // waves that split a unit's keys join here
-    __shared__ __attribute__((aligned(16))) float sm_o[SHARE ? 1 : kRows][SHARE ? 4 : D + 4];
+    __shared__ __attribute__((aligned(16))) float
+        sm_o[SHARE ? 1 : kWaves][SHARE ? 1 : kRows][SHARE ? 4 : D + 4];
     __shared__ float sm_m[kWaves][SHARE ? 1 : kRows], sm_l[kWaves][SHARE ? 1 : kRows];
     __shared__ __attribute__((aligned(16))) Keys sm_keys[kWaves];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t total = deal_at(s, 0, lane).total;
+    Entries at(s, 0, lane);
+    const int64_t total = all_steps(s, at, lane);
     const int64_t per = run_length(s, total);
-    int64_t pos = (int64_t)blockIdx.x * per;
+    const int64_t pos = (int64_t)blockIdx.x * per;
     const int64_t stop = min(pos + per, total * s.c.heads);
     if (pos >= stop) return;
-    Deal d = deal_find(s, pos, total, lane);
-    int e = __builtin_amdgcn_readfirstlane(d.entry);
-    int n = __builtin_amdgcn_readfirstlane(tiles_of(s, e));
-    const int64_t in_entry = pos - d.before * s.c.heads;
-    int h = __builtin_amdgcn_readfirstlane((int)quotient(in_entry, n));
-    int tile = __builtin_amdgcn_readfirstlane((int)(in_entry - (int64_t)h * n));
+    int64_t before = 0;                 // steps of one head ahead of entry at.base
+    uint64_t past;
+    while ((past = __ballot((before + at.upto) * s.c.heads > pos)) == 0) {
+        before += at.all();
+        if (at.base + 64 >= entries_of(s)) return;
+        at = Entries(s, at.base + 64, lane);
+    }
+    int slot_e = __builtin_ctzll(past);
+    int n = __builtin_amdgcn_readlane(at.tiles, slot_e);
+    int steps = __builtin_amdgcn_readlane(at.steps, slot_e);
+    before += (uint32_t)__builtin_amdgcn_readlane(at.upto, slot_e) - (uint32_t)steps;
+    const int64_t in_entry = pos - before * s.c.heads;
+    int h = __builtin_amdgcn_readfirstlane((int)quotient(in_entry, steps));
+    int tile = __builtin_amdgcn_readfirstlane((int)(in_entry - (int64_t)h * steps));
     int64_t left = stop - pos;
     W work;
     for (;;) {
-        const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(n - tile), left));
-        const int b = s.prefix ? 0 : e / s.row_groups;
-        const int row0 = (s.prefix ? e : e % s.row_groups) * kRows;
+        const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(steps - tile), left));
+        const int end = min(tile + take, n);
+        const int e = at.base + slot_e;
+        const int b = s.prefix ? 0 : s.row_groups == 1 ? e : e / s.row_groups;
+        const int row0 = (e - b * s.row_groups) * kRows;
         const int mine = row0 + (SHARE ? wave * 16 * NB : 0);
-        const bool whole = take == n;
+        const bool whole = tile == 0 && end == n;
         const int64_t slot = ((int64_t)blockIdx.x * 2 + (tile > 0 ? 0 : 1)) * kRows;
         // where a row's triple or result goes
         auto put_ml = [&](int r, float m, float l) {
-            int t;
-            const int64_t at = whole ? W::row_index(s, b, r, h, t) : slot + r - row0;
+            const int64_t to = whole ? typename W::RowAt(s, b, r, h).flat(s) : slot + r - row0;
             float* ml = whole ? s.home_ml : s.broken_ml;
-            ml[2 * at] = m;
-            ml[2 * at + 1] = l;
+            ml[2 * to] = m;
+            ml[2 * to + 1] = l;
         };
         auto put_o = [&](int r, int dim, f4 v, float l) {
-            int t;
             if (!whole) {
                 *reinterpret_cast<f4*>(s.broken_o + (slot + r - row0) * D + dim) = v;
                 return;
             }
-            const int64_t at = W::row_index(s, b, r, h, t) * D + dim;
+            const int64_t to = typename W::RowAt(s, b, r, h).flat(s) * D + dim;
             if (s.finish) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                store4(static_cast<T*>(s.a.out) + at, l == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * inv);
+                store4(static_cast<T*>(s.a.out) + to, l == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * inv);
             } else {
-                *reinterpret_cast<f4*>(s.home_o + at) = v;
+                *reinterpret_cast<f4*>(s.home_o + to) = v;
             }
         };
         const bool triple = !whole || !s.finish;
-        if (SHARE) {
+        if (tile >= end) {
+            // the unit's cost alone
+        } else if (SHARE) {
             if (mine < s.rows) {
-                work.load_q(s, b, mine, h, lane);
-                work.run(s, b, h, tile, tile + take, 1, lane, sm_keys[wave]);
+                work.run(s, b, mine, h, tile, end, 1, lane, sm_keys[wave]);
 #pragma unroll
                 for (int rb = 0; rb < NB; ++rb) {
                     const int r = mine + 16 * rb + (lane & 15);
@@ -686,49 +684,35 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
                 }
             }
         } else {
-            work.load_q(s, b, mine, h, lane);
-            work.run(s, b, h, tile + wave, tile + take, kWaves, lane, sm_keys[wave]);
-            float m[NB], l[NB];
+            work.run(s, b, mine, h, tile + wave, end, kWaves, lane, sm_keys[wave]);
 #pragma unroll
             for (int rb = 0; rb < NB; ++rb) {
-                l[rb] = quad_sum(work.l[rb]);
-                m[rb] = work.raise[rb] == kNegInf ? kNegInf : work.ref[rb];
+                const int r = 16 * rb + (lane & 15);
+                const float l = quad_sum(work.l[rb]);
                 if (lane < 16) {
-                    sm_m[wave][16 * rb + lane] = m[rb];
-                    sm_l[wave][16 * rb + lane] = l[rb];
+                    sm_m[wave][r] = work.raise[rb] == kNegInf ? kNegInf : work.ref[rb];
+                    sm_l[wave][r] = l;
                 }
+                work.each_four(rb, lane, [&](int dim, f4 x) {
+                    *reinterpret_cast<f4*>(&sm_o[wave][r][dim]) = x;
+                });
             }
             __syncthreads();
-            // the waves' sums, brought to one reference, one wave after another
-#pragma unroll
-            for (int v = 0; v < kWaves; ++v) {
-                if (wave == v) {
-#pragma unroll
-                    for (int rb = 0; rb < NB; ++rb) {
-                        const int r = 16 * rb + (lane & 15);
-                        float top = sm_m[0][r];
-#pragma unroll
-                        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, sm_m[i][r]);
-                        const float keep = factor(m[rb], l[rb], top);
-                        work.each_four(rb, lane, [&](int dim, f4 x) {
-                            f4* at = reinterpret_cast<f4*>(&sm_o[r][dim]);
-                            *at = v == 0 ? x * keep : *at + x * keep;
-                        });
-                    }
-                }
-                __syncthreads();
-            }
-            for (int i = threadIdx.x; i < kRows * (D / 4); i += kBlock) {
+            const int rows = min(kRows, s.rows - row0);
+            for (int i = threadIdx.x; i < rows * (D / 4); i += kBlock) {
                 const int r = i / (D / 4), dim = i % (D / 4) * 4;
-                if (row0 + r >= s.rows) break;
                 float top = sm_m[0][r], sum = 0.f;
 #pragma unroll
                 for (int v = 1; v < kWaves; ++v) top = fmaxf(top, sm_m[v][r]);
+                f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int v = 0; v < kWaves; ++v)
-                    sum += sm_l[v][r] * factor(sm_m[v][r], sm_l[v][r], top);
+                for (int v = 0; v < kWaves; ++v) {
+                    const float keep = factor(sm_m[v][r], sm_l[v][r], top);
+                    sum += sm_l[v][r] * keep;
+                    x += *reinterpret_cast<const f4*>(&sm_o[v][r][dim]) * keep;
+                }
                 if (triple && dim == 0) put_ml(row0 + r, top, sum);
-                put_o(row0 + r, dim, *reinterpret_cast<const f4*>(&sm_o[r][dim]), sum);
+                put_o(row0 + r, dim, x, sum);
             }
             __syncthreads();
         }
@@ -738,106 +722,121 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
         if (++h == s.c.heads) {
             h = 0;
             do {
-                if (++e >= entries_of(s)) return;
-                n = __builtin_amdgcn_readfirstlane(tiles_of(s, e));
+                if (++slot_e == 64) {
+                    if (at.base + 64 >= entries_of(s)) return;
+                    at = Entries(s, at.base + 64, lane);
+                    slot_e = 0;
+                }
+                if (at.base + slot_e >= entries_of(s)) return;
+                n = __builtin_amdgcn_readlane(at.tiles, slot_e);
             } while (n == 0);
+            steps = __builtin_amdgcn_readlane(at.steps, slot_e);
         }
     }
 }
 
-// Joins the triples of a row: those of its own keys' runs and, with a prefix,
-// those of the prefix's.  One wave per row.  Rows that a run has finished are
-// left alone; rows without any keys become zeros.
+// Joins the triples of rows: those of their own keys' runs and, with a prefix,
+// those of the prefix's.  One wave per `each` rows of a unit.  Rows that a run
+// has finished are left alone; rows without any keys become zeros.
 constexpr int kJoin = 8;                // triples in flight
 template <class T, int D>
-__global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead) {
+__global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, int each) {
     constexpr int E = D / 64;
     using VE = Vec<float, E>;
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
     const cq_attention_t& a = own.a;
-    if (row >= (int64_t)a.batch * a.tokens * a.q_heads) return;     // uniform over the wave
-    const int hq = (int)(row % a.q_heads), t = (int)(row / a.q_heads % a.tokens);
-    const int b = (int)(row / a.q_heads / a.tokens);
-    const int h = hq / own.group, r = t * own.group + hq % own.group;
+    const uint32_t blocks = (own.rows + each - 1) / each;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
+    const uint32_t unit = wave / blocks;
+    const int r0 = (wave - unit * blocks) * each;
+    const int h = unit % own.c.heads, b = unit / own.c.heads;
+    if (b >= a.batch) return;                       // uniform over the wave
 
-    // a source's triples of the row: `count` of them, the first at `first`,
-    // later ones `stride` rows on (from the run after the first)
+    // a source's triples of the row at `local` in its unit: in runs run,
+    // run + 1, ..., or in the row's home
     struct Parts {
         int count = 0;
         bool home = false;
         int64_t run = 0;
-        int local = 0;
     };
-    auto parts_of = [&](const Source& s, int entry, int local) {
+    auto parts_of = [&](const Source& s, int entry) {
         Parts p;
-        const int n = tiles_of(s, entry);
+        Entries at(s, 0, lane);
+        const int64_t per = run_length(s, all_steps(s, at, lane));
+        int64_t before = 0;
+        while (at.base + 64 <= entry) {
+            before += at.all();
+            at = Entries(s, at.base + 64, lane);
+        }
+        const int n = __builtin_amdgcn_readlane(at.tiles, entry - at.base);
         if (n == 0) return p;
-        const Deal d = deal_at(s, entry, lane);
-        const int64_t per = run_length(s, d.total);
-        const int64_t from = d.before * s.c.heads + (int64_t)h * n;
+        const int steps = __builtin_amdgcn_readlane(at.steps, entry - at.base);
+        before += (uint32_t)__builtin_amdgcn_readlane(at.upto, entry - at.base) - (uint32_t)steps;
+        const int64_t from = before * s.c.heads + (int64_t)h * steps;
         p.run = quotient(from, per);
         p.count = (int)(quotient(from + n - 1, per) - p.run) + 1;
         p.home = p.count == 1;
-        p.local = local;
         return p;
     };
-    auto place = [&](const Source& s, const Parts& p, int i) -> int64_t {
-        if (p.home) return row;
-        return ((p.run + i) * 2 + (i == 0 ? 1 : 0)) * s.rows_per_unit + p.local;
-    };
-    const Parts mine = parts_of(own, b * own.row_groups + r / own.rows_per_unit,
-                                r % own.rows_per_unit);
+    const Parts mine = parts_of(own, b * own.row_groups + r0 / own.rows_per_unit);
     if (own.finish && mine.home) return;
-    Parts pre;
-    if (!own.finish) {
-        const int pr = b * a.tokens * own.group + r;
-        pre = parts_of(ahead, pr / ahead.rows_per_unit, pr % ahead.rows_per_unit);
-    }
-    const int count = mine.count + pre.count;
-    auto at = [&](int i, const float*& o, const float*& ml) {
-        const bool first = i < mine.count;
-        const Source& s = first ? own : ahead;
-        const Parts& p = first ? mine : pre;
-        const int64_t x = place(s, p, first ? i : i - mine.count);
-        o = (p.home ? s.home_o : s.broken_o) + x * D;
-        ml = (p.home ? s.home_ml : s.broken_ml) + x * 2;
-    };
-    float top = kNegInf;
-    for (int base = 0; base < count; base += 64) {
-        float m = kNegInf;
-        if (base + lane < count) {
-            const float *o, *ml;
-            at(base + lane, o, ml);
-            m = ml[0];
+    for (int r = r0; r < min(r0 + each, own.rows); ++r) {
+        const int t = r / own.group;
+        const int64_t row = ((int64_t)b * a.tokens + t) * a.q_heads + h * own.group +
+                            (r - t * own.group);
+        const int own_local = r % own.rows_per_unit;
+        Parts pre;
+        int pre_local = 0;
+        if (!own.finish) {
+            const int pr = b * own.rows + r;
+            pre = parts_of(ahead, pr / ahead.rows_per_unit);
+            pre_local = pr % ahead.rows_per_unit;
         }
-        top = fmaxf(top, wave_max(m));
-    }
-    float sum = 0.f;
-    VE acc = {};
-    for (int base = 0; base < count; base += kJoin) {
-        VE v[kJoin];
-        float k[kJoin], l[kJoin];
+        const int count = mine.count + pre.count;
+        auto at = [&](int i, const float*& o, const float*& ml) {
+            const bool first = i < mine.count;
+            const Source& s = first ? own : ahead;
+            const Parts& p = first ? mine : pre;
+            if (!first) i -= mine.count;
+            const int64_t x = p.home ? row : ((p.run + i) * 2 + (i == 0 ? 1 : 0)) * s.rows_per_unit +
+                                                 (first ? own_local : pre_local);
+            o = (p.home ? s.home_o : s.broken_o) + x * D;
+            ml = (p.home ? s.home_ml : s.broken_ml) + x * 2;
+        };
+        float ref = kNegInf, sum = 0.f;
+        VE acc = {};
+        for (int base = 0; base < count; base += kJoin) {
+            VE v[kJoin];
+            float m[kJoin], l[kJoin];
+            float top = ref;
 #pragma unroll
-        for (int i = 0; i < kJoin; ++i) {
-            const float *o, *ml;
-            at(min(base + i, count - 1), o, ml);
-            v[i] = *reinterpret_cast<const VE*>(o + lane * E);
-            k[i] = ml[0];
-            l[i] = ml[1];
+            for (int i = 0; i < kJoin; ++i) {
+                const float *o, *ml;
+                at(min(base + i, count - 1), o, ml);
+                v[i] = *reinterpret_cast<const VE*>(o + lane * E);
+                m[i] = ml[0];
+                l[i] = ml[1];
+            }
+#pragma unroll
+            for (int i = 0; i < kJoin; ++i) top = fmaxf(top, m[i]);
+            const float keep = factor(ref, sum, top);
+            sum *= keep;
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[j] *= keep;
+            ref = top;
+#pragma unroll
+            for (int i = 0; i < kJoin; ++i) {
+                if (base + i >= count) break;
+                const float by = factor(m[i], l[i], top);
+                sum += by * l[i];
+#pragma unroll
+                for (int j = 0; j < E; ++j) acc[j] += v[i][j] * by;
+            }
         }
+        T* out = static_cast<T*>(a.out) + row * D + lane * E;
 #pragma unroll
-        for (int i = 0; i < kJoin; ++i) {
-            if (base + i >= count) break;
-            const float keep = factor(k[i], l[i], top);
-            sum += keep * l[i];
-#pragma unroll
-            for (int j = 0; j < E; ++j) acc[j] += v[i][j] * keep;
-        }
+        for (int j = 0; j < E; ++j) out[j] = (T)(sum == 0.f ? 0.f : acc[j] / sum);
     }
-    T* out = static_cast<T*>(a.out) + row * D + lane * E;
-#pragma unroll
-    for (int j = 0; j < E; ++j) out[j] = (T)(sum == 0.f ? 0.f : acc[j] / sum);
 }
 
 // ------------------------------------------------------------------- host
@@ -854,7 +853,7 @@ Shape shape_of(int64_t rows, int d) {
     if (rows <= 16) return {1, false};
     if (d > 128) return {1, true};
     if (rows <= 32) return {2, false};
-    return {2, true};
+    return {d > 64 || rows <= 128 ? 2 : 4, true};
 }
 
 Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, Shape* shape) {
@@ -869,15 +868,17 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
     *shape = shape_of(rows, c.head_dim);
     s.rows_per_unit = 16 * shape->nb * (shape->share ? kWaves : 1);
     s.row_groups = (int32_t)((rows + s.rows_per_unit - 1) / s.rows_per_unit);
-    s.least = shape->share ? 1 : kWaves;
+    s.quantum = kWaves;
+    s.cost = shape->share ? kWaves : 2 * kWaves;
     s.finish = a.prefix_len == 0;
-    // no more runs than tiles, as far as the tables' sizes tell
+    // no more runs than quanta, as far as the tables' sizes tell
     const int64_t keys = prefix ? a.prefix_len : (int64_t)a.table_cols * c.page_size;
     const int64_t entries = (int64_t)s.row_groups * (prefix ? 1 : a.batch);
-    const __int128 tiles = (__int128)((keys + kTile - 1) / kTile) * entries * c.heads;
-    const __int128 most = (tiles + s.least - 1) / s.least;
+    const __int128 steps = (__int128)((keys + kTile - 1) / kTile + s.quantum + s.cost) * entries *
+                           c.heads;
     const int64_t room = (int64_t)kCus * waves_of(c.head_dim, shape->nb);
-    s.runs = (uint32_t)(most < room ? (most < 1 ? 1 : (int64_t)most) : room);
+    const __int128 most = steps / s.quantum;
+    s.runs = (uint32_t)(most < room ? (int64_t)most : room);
     return s;
 }
 
@@ -911,8 +912,10 @@ hipError_t launch_tiles(const Source& s, Shape shape, hipStream_t stream) {
                            : go(&tile_kernel<T, BITS, D, 1, false>);
     } else {
         if (shape.nb == 1) return go(&tile_kernel<T, BITS, D, 1, false>);
-        return shape.share ? go(&tile_kernel<T, BITS, D, 2, true>)
-                           : go(&tile_kernel<T, BITS, D, 2, false>);
+        if (!shape.share) return go(&tile_kernel<T, BITS, D, 2, false>);
+        if constexpr (D <= 64)
+            if (shape.nb == 4) return go(&tile_kernel<T, BITS, D, 4, true>);
+        return go(&tile_kernel<T, BITS, D, 2, true>);
     }
 }
 
@@ -926,9 +929,14 @@ hipError_t launch_typed(const Source& own, Shape os, const Source& ahead, Shape 
     if (e != hipSuccess) return e;
     e = wide ? launch_tiles<T, 8, D>(own, os, stream) : launch_tiles<T, 4, D>(own, os, stream);
     if (e != hipSuccess) return e;
-    const int64_t rows = (int64_t)own.a.batch * own.a.tokens * own.a.q_heads;
-    join_kernel<T, D><<<dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kBlock), 0, stream>>>(
-        own, ahead);
+    // a wave finds out for eight rows at once that they are finished, as most
+    // are where rows are many (1024 tokens x 64 heads: 62 us with one row, 35
+    // with eight); of few rows most have triples to join, one row a wave
+    const int64_t all = (int64_t)own.rows * own.a.batch * own.c.heads;
+    const int each = own.finish && os.share && all >= 32 * kWaves * kCus ? 8 : 1;
+    const int64_t waves = (int64_t)((own.rows + each - 1) / each) * own.a.batch * own.c.heads;
+    join_kernel<T, D><<<dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kBlock), 0, stream>>>(
+        own, ahead, each);
     return hipGetLastError();
 }
 
