@@ -13,6 +13,11 @@ numbers live on the device and are never read by the host: the kernels check
 them against the tensors' sizes (a token outside them is not written, reads as
 zeros and is not attended to).  Launches go on the current torch stream of the
 tensors' device, work inside a HIP graph, and keep nothing between calls.
+
+Each call is first offered to the fast path (csrc/cq_pyattn.h): one C++ call
+that applies the same rules to the tensors' metadata and makes the library
+call.  It launches nothing for a call it does not accept, and the checked path
+here then runs and raises.
 """
 from __future__ import annotations
 
@@ -22,7 +27,7 @@ from typing import Optional
 import torch
 
 from . import _capi
-from .ext import _on_device
+from .ext import _on_device, fast_module_or_none
 from .kvcache import KVCache
 
 _DTYPES = {torch.float16: _capi.CQ_DTYPE_F16, torch.float32: _capi.CQ_DTYPE_F32,
@@ -83,6 +88,10 @@ class AttentionExt:
 
     def __init__(self) -> None:
         self._lib = _capi.load()
+        mod = fast_module_or_none()
+        self._fast = mod and mod.AttentionCalls(*(_capi.entry_address(n) for n in (
+            "cq_qk_norm_rope", "cq_kv_append", "cq_kv_read", "cq_attention",
+            "cq_attention_workspace", "cq_last_error")))
 
     # ---- norms and rotation ----
     def qk_norm_rope(self, q: torch.Tensor, k: torch.Tensor,
@@ -96,13 +105,18 @@ class AttentionExt:
         """RMS norm of each head of q (tokens, Hq, D) and k (tokens, Hkv, D),
         then the rotation of its first R dims, into new contiguous tensors.
         See qk_norm_rope_into."""
+        if self._fast is not None:
+            got = self._fast.norm_rope(q, k, None, None, q_weight, k_weight, cos, sin,
+                                       positions, eps, interleaved)
+            if got is not None:
+                return got
         for name, t in (("q", q), ("k", k)):
             if not isinstance(t, torch.Tensor):
                 _fail(f"{name} must be a tensor, got {type(t).__name__}")
         qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        self.qk_norm_rope_into(q, k, qo, ko, q_weight, k_weight, cos, sin, positions,
-                               eps=eps, interleaved=interleaved)
+        self._norm_rope(q, k, qo, ko, q_weight, k_weight, cos, sin, positions, eps,
+                        interleaved)
         return qo, ko
 
     def qk_norm_rope_into(self, q, k, q_out, k_out, q_weight=None, k_weight=None,
@@ -118,6 +132,15 @@ class AttentionExt:
         row positions[token] (int32 or int64).  Tokens and heads may have any
         stride; a position outside the tables turns the token's rotated dims
         into NaN."""
+        if self._fast is not None and q_out is not None and k_out is not None \
+                and self._fast.norm_rope(q, k, q_out, k_out, q_weight, k_weight, cos, sin,
+                                         positions, eps, interleaved) is not None:
+            return
+        self._norm_rope(q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps,
+                        interleaved)
+
+    def _norm_rope(self, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps,
+                   interleaved) -> None:
         if not isinstance(q, torch.Tensor):
             _fail(f"q must be a tensor, got {type(q).__name__}")
         dev = q.device
@@ -208,6 +231,9 @@ class AttentionExt:
         written; pages written belong to one sequence each."""
         if not isinstance(cache, KVCache):
             _fail(f"cache must be a KVCache, got {type(cache).__name__}")
+        if self._fast is not None and cache.fast is not None \
+                and self._fast.append(cache.fast, k, v, block_table, starts, counts):
+            return
         for name, t in (("k", k), ("v", v)):
             _heads(name, t, 4, cache.device)
             if t.dtype != k.dtype or t.shape != k.shape:
@@ -233,6 +259,10 @@ class AttentionExt:
         zeros past the count and where no page is."""
         if not isinstance(cache, KVCache):
             _fail(f"cache must be a KVCache, got {type(cache).__name__}")
+        if self._fast is not None and cache.fast is not None:
+            got = self._fast.read(cache.fast, block_table, starts, counts, tokens, dtype)
+            if got is not None:
+                return got
         if dtype not in _DTYPES:
             _fail(f"dtype must be float16, bfloat16 or float32, got {dtype}")
         if isinstance(tokens, bool) or not isinstance(tokens, int) \
@@ -256,11 +286,13 @@ class AttentionExt:
                 scale: Optional[float] = None) -> torch.Tensor:
         """Attention of q (batch, tokens, Hq, D), float16 or bfloat16, over the
         cache, into a new tensor of q's shape and type.  See forward_into."""
+        got = self._fast_forward(q, cache, block_table, lengths, None, counts, prefix, scale)
+        if got is not None:
+            return got
         if not isinstance(q, torch.Tensor):
             _fail(f"q must be a tensor, got {type(q).__name__}")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        self.forward_into(q, cache, block_table, lengths, out, counts, prefix=prefix,
-                          scale=scale)
+        self._forward(q, cache, block_table, lengths, out, counts, prefix, scale)
         return out
 
     def forward_into(self, q: torch.Tensor, cache: KVCache, block_table: torch.Tensor,
@@ -279,6 +311,27 @@ class AttentionExt:
         and `lengths` does not count them.  `scale` multiplies the scores
         (default D ** -0.5).  FP32 scores, statistics and sums, one rounding; a
         query that sees nothing, or lies past counts[b], gives zeros."""
+        if out is not None and self._fast_forward(q, cache, block_table, lengths, out, counts,
+                                                  prefix, scale) is not None:
+            return
+        self._forward(q, cache, block_table, lengths, out, counts, prefix, scale)
+
+    def _fast_forward(self, q, cache, block_table, lengths, out, counts, prefix, scale):
+        if self._fast is None or not isinstance(cache, KVCache) or cache.fast is None:
+            return None
+        pages, n = None, 0
+        if prefix is not None:
+            pages, n = prefix
+            if type(n) is not int or not 0 <= n < 2 ** 31 or pages is None:
+                return None
+        if scale is None:
+            scale = cache.head_dim ** -0.5
+        elif not isinstance(scale, (int, float)):
+            return None
+        return self._fast.forward(cache.fast, q, block_table, lengths, counts, out, pages, n,
+                                  scale)
+
+    def _forward(self, q, cache, block_table, lengths, out, counts, prefix, scale) -> None:
         if not isinstance(cache, KVCache):
             _fail(f"cache must be a KVCache, got {type(cache).__name__}")
         dev = cache.device

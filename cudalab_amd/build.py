@@ -142,7 +142,7 @@ def _fast_module_cmd(out: Path, stamp: str) -> list[str]:
     return ["g++", *_FAST_FLAGS,
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
             stamp, f"-DCQ_FAST_ABI=\"{fast_abi_stamp()}\"",
-            *[f"-I{p}" for p in incs], str(CSRC / FAST_SOURCE),
+            *[f"-I{p}" for p in incs], f"-I{CSRC}", str(CSRC / FAST_SOURCE),
             "-o", str(out), *[f"-L{p}" for p in library_paths()], *_FAST_LIBS]
 
 

@@ -39,6 +39,7 @@
 #include <vector>
 
 #include "cdnaqgemv.h"
+#include "cq_pyattn.h"
 
 namespace py = pybind11;
 
@@ -397,4 +398,5 @@ PYBIND11_MODULE(_cqfast, m) {
         .def("knows", &Launcher::knows)
         .def("cached", &Launcher::cached)
         .def("clear", &Launcher::clear);
+    cqattn::bind(m);
 }

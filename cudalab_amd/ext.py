@@ -89,19 +89,27 @@ class _DeclineAll:
 _fast_warned = False
 
 
-def _fast_launcher(op: str, names: list[str]):
-    """The fast-path launcher of `op`, or a launcher that declines every
-    call (with one warning per process) when the fast-path module cannot
-    be used; the checked path is complete without it."""
+def fast_module_or_none():
+    """The fast-path module, or None (with one warning per process) where it
+    cannot be used."""
     global _fast_warned
-    grouped = _GROUPED_ENTRY.get(op)
     try:
-        mod = _capi.fast_module()
+        return _capi.fast_module()
     except (_capi.LibraryMissing, _capi.StaleLibrary, ImportError, OSError) as e:
         if not _fast_warned:
             _fast_warned = True
             warnings.warn(f"eager fast path unavailable, every call takes the "
                           f"checked path: {e}", RuntimeWarning, stacklevel=3)
+        return None
+
+
+def _fast_launcher(op: str, names: list[str]):
+    """The fast-path launcher of `op`, or a launcher that declines every
+    call when the fast-path module cannot be used; the checked path is
+    complete without it."""
+    grouped = _GROUPED_ENTRY.get(op)
+    mod = fast_module_or_none()
+    if mod is None:
         return _DeclineAll()
     return mod.Launcher(
         _FAST_KIND[op], names, _capi.entry_address("cq_prepare"),

@@ -31,6 +31,7 @@ from __future__ import annotations
 import torch
 
 from . import _capi
+from .ext import fast_module_or_none
 
 HEAD_DIMS = (64, 128, 256)
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -84,6 +85,9 @@ class KVCache:
         self.device = k.device
         self.c = _capi.CqKvCache(k.data_ptr(), v.data_ptr(), scales.data_ptr(), pages,
                                  heads, dim, page, bits)
+        mod = fast_module_or_none()
+        self.fast = mod and mod.Cache(k, v.data_ptr(), scales.data_ptr(), pages, heads, dim,
+                                      page, bits)
 
     @classmethod
     def empty(cls, pages: int, heads: int, head_dim: int, page_size: int = 64,
