@@ -22,11 +22,31 @@ namespace cq {
 namespace {
 
 constexpr int kBlock = 256;
+constexpr int64_t kManyHeads = 256 * 8 * 4 * 8;   // 256 CUs of eight waves of four groups, times 8
 
 __device__ __forceinline__ float load_weight(const void* p, int dtype, int i) {
     if (dtype == CQ_DTYPE_F16) return (float)static_cast<const _Float16*>(p)[i];
     if (dtype == CQ_DTYPE_BF16) return (float)static_cast<const __bf16*>(p)[i];
     return static_cast<const float*>(p)[i];
+}
+
+// Four weights from i, a multiple of four (all at once where `wide`).
+__device__ __forceinline__ void load_weights(const void* p, int dtype, int i, bool wide,
+                                             float (&w)[4]) {
+    if (wide && dtype == CQ_DTYPE_F16) {
+        const Vec<_Float16, 4> v = *reinterpret_cast<const Vec<_Float16, 4>*>(
+            static_cast<const _Float16*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = (float)v[j];
+    } else if (wide && dtype == CQ_DTYPE_BF16) {
+        const Vec<__bf16, 4> v = *reinterpret_cast<const Vec<__bf16, 4>*>(
+            static_cast<const __bf16*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = (float)v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = load_weight(p, dtype, i + j);
+    }
 }
 
 // Row of the cos/sin tables of a token, or -1 for a position outside them.
@@ -64,7 +84,7 @@ struct Head {
 // two ends of pairs 4l..4l+3, else eight neighbours.
 template <class T, bool PAIRS, int LANES, int BATCH>
 __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uint32_t parts,
-                                                           uint32_t iters) {
+                                                           uint32_t iters, bool wide) {
     using V = Vec<T, 4>;
     const int lane = threadIdx.x % LANES;
     const uint32_t group = blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
@@ -79,6 +99,28 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
     const int e0 = !active ? 0 : halves ? 4 * lane : 8 * lane;
     const int e1 = !active ? 4 : halves ? a.rot_dim / 2 + 4 * lane : 8 * lane + 4;
 
+    V x0[BATCH], x1[BATCH];
+    auto load = [&](uint32_t it) {
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+            const int h = (int)min(part + (it + u) * parts, (uint32_t)heads - 1);
+            const Head<T> head(a, token, h);
+            x0[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(head.src + e0));
+            x1[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(head.src + e1));
+        }
+    };
+    load(0);
+    float w[2][2][4];           // of q and k, at e0 and e1
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const void* p = i == 0 ? a.q_weight : a.k_weight;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[i][0][j] = w[i][1][j] = 1.f;
+        if (p != nullptr) {
+            load_weights(p, a.weight_dtype, e0, wide, w[i][0]);
+            load_weights(p, a.weight_dtype, e1, wide, w[i][1]);
+        }
+    }
     float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
     if (turn) {
         const int64_t row = table_row(a, token);
@@ -94,24 +136,9 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
         }
     }
     const bool norm = a.q_weight != nullptr || a.k_weight != nullptr;
-    float wq[8], wk[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int e = i < 4 ? e0 + i : e1 + i - 4;
-        wq[i] = a.q_weight != nullptr ? load_weight(a.q_weight, a.weight_dtype, e) : 1.f;
-        wk[i] = a.k_weight != nullptr ? load_weight(a.k_weight, a.weight_dtype, e) : 1.f;
-    }
     const float mean = 1.f / (float)a.head_dim;
 
-    for (uint32_t it = 0; it < iters; it += BATCH) {
-        V x0[BATCH], x1[BATCH];
-#pragma unroll
-        for (int u = 0; u < BATCH; ++u) {
-            const int h = (int)min(part + (it + u) * parts, (uint32_t)heads - 1);
-            const Head<T> head(a, token, h);
-            x0[u] = *reinterpret_cast<const V*>(head.src + e0);
-            x1[u] = *reinterpret_cast<const V*>(head.src + e1);
-        }
+    for (uint32_t it = 0;;) {
 #pragma unroll
         for (int u = 0; u < BATCH; ++u) {
             const uint32_t h = part + (it + u) * parts;
@@ -127,7 +154,8 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
                 const bool has = head.is_q ? a.q_weight != nullptr : a.k_weight != nullptr;
                 const float r = has ? 1.f / sqrtf(ss * mean + a.eps) : 1.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = f[i] * r * (head.is_q ? wq[i] : wk[i]);
+                for (int i = 0; i < 8; ++i)
+                    f[i] = f[i] * r * (head.is_q ? w[0][i / 4][i % 4] : w[1][i / 4][i % 4]);
             }
             if (turn) {
 #pragma unroll
@@ -143,10 +171,13 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
 #pragma unroll
             for (int i = 0; i < 4; ++i) y0[i] = (T)f[i], y1[i] = (T)f[4 + i];
             if (live && active && h < (uint32_t)heads) {
-                *reinterpret_cast<V*>(head.dst + e0) = y0;
-                *reinterpret_cast<V*>(head.dst + e1) = y1;
+                __builtin_nontemporal_store(y0, reinterpret_cast<V*>(head.dst + e0));
+                __builtin_nontemporal_store(y1, reinterpret_cast<V*>(head.dst + e1));
             }
         }
+        it += BATCH;
+        if (it >= iters) break;
+        load(it);
     }
 }
 
@@ -240,21 +271,30 @@ hipError_t launch_typed(const cq_norm_rope_t& a, hipStream_t stream) {
         return hipGetLastError();
     }
     const int lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : a.head_dim <= 256 ? 32 : 64;
-    const int batch = 1;
-    const int64_t iters = 1, parts = (heads + iters - 1) / iters;
-    const int64_t groups = a.tokens * parts, per = kBlock / lanes;
-    const int64_t grid = (groups + per - 1) / per;
-    if (groups + per > kMaxGrid) return hipErrorInvalidValue;
-    auto go = [&](auto* kernel) {
-        kernel<<<dim3((unsigned)grid), dim3(kBlock), 0, stream>>>(a, (uint32_t)parts,
-                                                                  (uint32_t)iters);
+    const int64_t per = kBlock / lanes;
+    auto weight_wide = [&](const void* p) {
+        return a.weight_dtype == CQ_DTYPE_F32 || (uintptr_t)p % 8 == 0;
+    };
+    const bool wide = weight_wide(a.q_weight) && weight_wide(a.k_weight);
+    auto go = [&](auto* kernel, int64_t iters) {
+        const int64_t parts = (heads + iters - 1) / iters, groups = a.tokens * parts;
+        if (groups + per > kMaxGrid) return hipErrorInvalidValue;
+        kernel<<<dim3((unsigned)((groups + per - 1) / per)), dim3(kBlock), 0, stream>>>(
+            a, (uint32_t)parts, (uint32_t)iters, wide);
         return hipGetLastError();
     };
-    (void)batch;
-    if (lanes == 8) return go(&norm_rope_kernel<T, PAIRS, 8, 1>);
-    if (lanes == 16) return go(&norm_rope_kernel<T, PAIRS, 16, 1>);
-    if (lanes == 32) return go(&norm_rope_kernel<T, PAIRS, 32, 1>);
-    return go(&norm_rope_kernel<T, PAIRS, 64, 1>);
+    // Few heads in all: one to a group, so that each wave has as little to wait
+    // for as can be.  Many: eight, four loads of each end in flight, and the
+    // weights and tables are fetched once for them.
+    const bool many = a.tokens * heads > kManyHeads;
+#define CQ_GO(L)                                                       \
+    (many ? go(&norm_rope_kernel<T, PAIRS, L, 4>, 8)                   \
+          : go(&norm_rope_kernel<T, PAIRS, L, 1>, 1))
+    if (lanes == 8) return CQ_GO(8);
+    if (lanes == 16) return CQ_GO(16);
+    if (lanes == 32) return CQ_GO(32);
+    return CQ_GO(64);
+#undef CQ_GO
 }
 
 }  // namespace
