@@ -41,6 +41,7 @@
 // busy to the end for any mix of lengths, and the grid never depends on them.
 
 #include <algorithm>
+#include <utility>
 
 #include "cq_attn.h"
 #include "cq_elem.h"
@@ -237,42 +238,71 @@ __device__ __forceinline__ void store4(T* p, f4 v) {
     *reinterpret_cast<Vec<T, 4>*>(p) = o;
 }
 
-// What a wave's lanes know of a tile's keys, for the others: K's scale with all
-// that a score takes, V's as f 2^e, and 2^-e.
-struct Keys {
-    float k[kTile], e[kTile], f[kTile], back[kTile];
+// Lane J of each row of 16 lanes, to the whole row (an operand of the
+// instruction that takes it, not one of its own).
+template <int J>
+__device__ __forceinline__ float of_lane(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x150 + J,
+                                                              0xF, 0xF, true));
+}
+template <class F, int... J>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, J...>) {
+    (f(std::integral_constant<int, J>{}), ...);
+}
+// f(integral_constant 0), ..., f(integral_constant 15)
+template <class F>
+__device__ __forceinline__ void sixteen(F&& f) {
+    each_of(f, std::make_integer_sequence<int, 16>{});
+}
+
+// --------------------------------------------------------------- the rows
+// Row r of a unit's source: its sequence, new token and query head.
+struct RowAt {
+    int b, t, hq;
+    __device__ __forceinline__ RowAt(const Source& s, int unit_b, int r, int h)
+        : b(unit_b), t(0), hq(h * s.group + r) {
+        if (s.prefix || s.a.tokens > 1) {
+            const int all = r / s.group;
+            hq = h * s.group + r - all * s.group;
+            t = all;
+            if (s.prefix) {
+                b = all / s.a.tokens;
+                t = all - b * s.a.tokens;
+            }
+        }
+    }
+    __device__ __forceinline__ int64_t flat(const Source& s) const {
+        return ((int64_t)b * s.a.tokens + t) * s.a.q_heads + hq;
+    }
 };
 
-// ------------------------------------------------------------- the kernel
-// NB row matrices to a wave.  SHARE: the four waves take the same keys for
-// four times 16 NB rows; otherwise the same 16 NB rows, and every fourth tile
-// each.
-template <class T, int BITS, int D, int NB, bool SHARE>
-struct Tiles {
-    static constexpr int kRow = D * BITS / 8;              // bytes of a token's row
-    static constexpr int kLane = kRow / 4;                 // K bytes of a lane and row
-    static constexpr int kChunk = kLane < 16 ? kLane : 16;
-    static constexpr int kChunks = kLane / kChunk;
-    static constexpr int kWords = kChunk / 4;
+// The unpacking of a word leaves pairs of bytes or nibbles apart: code order(i)
+// of eight comes i-th.
+template <int BITS>
+constexpr int order(int i) {
+    constexpr int o8[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+    constexpr int o4[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+    return BITS == 8 ? o8[i] : o4[i];
+}
+
+// Largest magnitude among fp16 or bfloat16 words, as its bits; Inf and NaN are
+// the largest of all.
+__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
+    using us2 = Vec<unsigned short, 2>;
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a),
+                                                                  __builtin_bit_cast(us2, b)));
+}
+
+// The state of a wave's 16 NB rows: queries, sums and references.  RAW: the
+// score products take K's codes as they lie in memory, offset and in units
+// (halves_of_*); else the codes themselves.
+template <class T, int BITS, int D, int NB, bool RAW>
+struct Rows {
     static constexpr int kSteps = D / 32;                  // products over D
-    static constexpr int kVTiles = kRow / 16;              // 16 rows of V bytes
     static constexpr int kOTiles = D / 16;
-    static constexpr int kUnitRows = 16 * NB * (SHARE ? kWaves : 1);
-    // a code's offset and unit as the matrix units see it
     static constexpr float kOffset = BITS == 8 ? 128.f : 8.f;
     static constexpr float kUnit = 0x1p-24f;
-
-    // Where dims of product step u of lane group g start, and their order:
-    // the unpacking leaves pairs of bytes or nibbles apart.
-    static __device__ __forceinline__ int step_dim(int u, int g) {
-        constexpr int per = kChunk / BITS;                 // steps of a chunk
-        return ((u / per) * 4 * kChunk + g * kChunk) * 8 / BITS + (u % per) * 8;
-    }
-    static constexpr int order(int i) {
-        constexpr int o8[8] = {0, 2, 1, 3, 4, 6, 5, 7};
-        constexpr int o4[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-        return BITS == 8 ? o8[i] : o4[i];
-    }
+    static constexpr uint32_t kInf = std::is_same_v<T, _Float16> ? 0x7C00u : 0x7F80u;
 
     h8 q[NB][kSteps];
     float start[NB];                     // what the score sums start at
@@ -282,37 +312,13 @@ struct Tiles {
     f4 o[NB][kOTiles];
     float l[NB], ref[NB], raise[NB];
 
-    Vec<uint32_t, kWords> kq[4][kChunks];
-    u4 vq[kVTiles];
-    float ks, vs;                        // scales of key `lane` of the tile
-    bool there;                          // the lane group's 16 keys have a page
-
-    // Row r of the unit's source: its sequence, new token and query head.
-    struct RowAt {
-        int b, t, hq;
-        __device__ __forceinline__ RowAt(const Source& s, int unit_b, int r, int h)
-            : b(unit_b), t(0), hq(h * s.group + r) {
-            if (s.prefix || s.a.tokens > 1) {
-                const int all = r / s.group;
-                hq = h * s.group + r - all * s.group;
-                t = all;
-                if (s.prefix) {
-                    b = all / s.a.tokens;
-                    t = all - b * s.a.tokens;
-                }
-            }
-        }
-        __device__ __forceinline__ int64_t flat(const Source& s) const {
-            return ((int64_t)b * s.a.tokens + t) * s.a.q_heads + hq;
-        }
-    };
-
-    __device__ __forceinline__ void load_q(const Source& s, int b, int first_row, int h,
-                                           int lane) {
-        const int g = lane >> 4;
+    // dim(u): where the eight dims of step u that this lane multiplies start.
+    template <class Dim>
+    __device__ __forceinline__ void load(const Source& s, int b, int first_row, int h, int lane,
+                                         Dim&& dim) {
         int least = 0x7FFFFFFF;
         Vec<T, 8> raw[NB][kSteps];
-        float top = 0.f;
+        uint32_t top2 = 0;
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
             // rows past the last repeat it (nobody stores them)
@@ -326,20 +332,35 @@ struct Tiles {
                          at.t * s.a.q_token_stride + at.hq * s.a.q_head_stride;
 #pragma unroll
             for (int u = 0; u < kSteps; ++u) {
-                raw[rb][u] = *reinterpret_cast<const Vec<T, 8>*>(p + step_dim(u, g));
+                raw[rb][u] = *reinterpret_cast<const Vec<T, 8>*>(p + dim(u));
+                const u4 w = __builtin_bit_cast(u4, raw[rb][u]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = fabsf((float)raw[rb][u][i]);
-                    top = fmaxf(top, x < __builtin_inff() ? x : 0.f);
-                }
+                for (int i = 0; i < 4; ++i) top2 = pk_max(top2, w[i] & 0x7FFF7FFFu);
             }
+        }
+        uint32_t bits = max(top2 & 0xFFFFu, top2 >> 16);
+        if (__any(bits >= kInf)) {
+            // the largest that is a number
+            bits = 0;
+#pragma unroll
+            for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+                for (int u = 0; u < kSteps; ++u) {
+                    const u4 w = __builtin_bit_cast(u4, raw[rb][u]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t x = (w[i / 2] >> (16 * (i & 1))) & 0x7FFFu;
+                        bits = x < kInf ? max(bits, x) : bits;
+                    }
+                }
         }
         // One factor for the wave: exact down to 2^-27 of its largest element,
         // 2^-38 of that where fp16 is subnormal, so an error far below FP32's
         // in the largest row's scores is all that a small row can show.
-        top = wave_max(top);
+        const float top =
+            wave_max((float)__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
         const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
-        qscale = ldexpf(s.a.softmax_scale * kLog2e * (1.f / kUnit), e);
+        qscale = ldexpf(s.a.softmax_scale * kLog2e * (RAW ? 1.f / kUnit : 1.f), e);
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
             float sum = 0.f;
@@ -347,12 +368,12 @@ struct Tiles {
             for (int u = 0; u < kSteps; ++u)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    // high nibbles come as 16 times their code
-                    const int down = BITS == 4 && (order(i) & 1) ? 4 : 0;
-                    q[rb][u][i] = (_Float16)ldexpf((float)raw[rb][u][order(i)], -e - down);
-                    sum = __builtin_fmaf((float)q[rb][u][i], down ? 16.f : 1.f, sum);
+                    // raw high nibbles come as 16 times their code
+                    const int down = RAW && BITS == 4 && (order<BITS>(i) & 1) ? 4 : 0;
+                    q[rb][u][i] = (_Float16)ldexpf((float)raw[rb][u][order<BITS>(i)], -e - down);
+                    if (RAW) sum = __builtin_fmaf((float)q[rb][u][i], down ? 16.f : 1.f, sum);
                 }
-            start[rb] = -kOffset * kUnit * quad_sum(sum);
+            start[rb] = RAW ? -kOffset * kUnit * quad_sum(sum) : 0.f;
         }
 #pragma unroll
         for (int off = 1; off < 16; off <<= 1) least = min(least, __shfl_xor(least, off));
@@ -366,114 +387,29 @@ struct Tiles {
         }
     }
 
-    // Table entry of 16 keys `sub` of a tile (any entry past the table).
-    static __device__ __forceinline__ int32_t entry(const Source& s, const int32_t* table,
-                                                    int cols, int tile, int sub) {
-        return table[min((tile * kTile + sub * 16) >> s.page_shift, cols - 1)];
-    }
-
-    __device__ __forceinline__ void load_k(const Source& s, int32_t entry, int tile, int h,
-                                           int lane) {
-        const int g = lane >> 4, r = lane & 15;
-        const int64_t page = max((int64_t)0, page_in(entry, s.c.pages));
-        const int in = (tile * kTile + (r >> 2) * 16) & (s.c.page_size - 1);
-        const uint8_t* p = static_cast<const uint8_t*>(s.c.k) +
-                           ((page * s.c.heads + h) * s.c.page_size + in + (r & 3)) * kRow +
-                           g * kChunk;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c)
-                kq[t][c] = *reinterpret_cast<const Vec<uint32_t, kWords>*>(
-                    p + t * 4 * kRow + c * 4 * kChunk);
-    }
-
-    __device__ __forceinline__ void load_scales(const Source& s, int32_t entry, int tile, int h,
-                                                int lane) {
-        const int g = lane >> 4;
-        const int64_t page = max((int64_t)0, page_in(entry, s.c.pages));
-        there = page_in(entry, s.c.pages) >= 0;
-        const int in = (tile * kTile + g * 16) & (s.c.page_size - 1);
-        const float* p = s.c.scales + (page * s.c.heads + h) * 2 * s.c.page_size + in + (lane & 15);
-        ks = p[0];
-        vs = p[s.c.page_size];
-    }
-
-    __device__ __forceinline__ void load_v(const Source& s, int32_t entry, int tile, int h,
-                                           int lane) {
-        const int g = lane >> 4, r = lane & 15;
-        const int64_t page = max((int64_t)0, page_in(entry, s.c.pages));
-        const int in = (tile * kTile + g * 16) & (s.c.page_size - 1);
-        const uint8_t* p = static_cast<const uint8_t*>(s.c.v) +
-                           ((page * s.c.heads + h) * s.c.page_size + in) * kRow + r * 16;
-#pragma unroll
-        for (int i = 0; i < kVTiles; ++i) vq[i] = *reinterpret_cast<const u4*>(p + i * 256);
-    }
-
-    static __device__ __forceinline__ h8 unpack_k(const Vec<uint32_t, kWords> (&row)[kChunks],
-                                                  int u) {
-        constexpr int per = kChunk / BITS;
-        u4 w;
-        if constexpr (BITS == 8) {
-            uint32_t x, y, z, v;
-            halves_of_bytes(row[u / per][2 * (u % per)], x, y);
-            halves_of_bytes(row[u / per][2 * (u % per) + 1], z, v);
-            w = u4{x, y, z, v};
-        } else {
-            // pairs (0, 4), (1, 5), (2, 6), (3, 7) of the word's nibbles
-            uint32_t x[4];
-            halves_of_nibbles(row[u / per][u % per], x);
-            w = u4{x[0], x[1], x[2], x[3]};
-        }
-        return __builtin_bit_cast(h8, w);
-    }
-
-    // One tile of keys.  next_k and next_v issue the loads that the registers
-    // freed by then can take.  `keys`: LDS of the wave's own.
-    template <class NextK, class NextV>
-    __device__ __forceinline__ void step(int tile, int lane, Keys& keys, NextK&& next_k,
-                                         NextV&& next_v) {
-        {
-            const int e = max((int)((__float_as_uint(vs) >> 23) & 0xFF) - 126, kLeastExp);
-            keys.k[lane] = ks * qscale;
-            keys.e[lane] = (float)e;
-            keys.f[lane] = __builtin_amdgcn_ldexpf(vs, -e);
-            keys.back[lane] = __builtin_amdgcn_ldexpf(1.f, -e);
-        }
-        const bool here = there;
-        f4 sc[NB][4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int rb = 0; rb < NB; ++rb)
-                sc[rb][t] = f4{start[rb], start[rb], start[rb], start[rb]};
-#pragma unroll
-            for (int u = 0; u < kSteps; ++u) {
-                const h8 k = unpack_k(kq[t], u);
-#pragma unroll
-                for (int rb = 0; rb < NB; ++rb)
-                    sc[rb][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rb][u], sc[rb][t], 0,
-                                                                      0, 0);
-            }
-        }
-        next_k();
-        // the keys' quadruples come from other lanes of this wave
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const int own = lane & 48;           // the lane's 16 keys
-        const bool masked = tile >= full || !__all(here);
-        h8 w[NB][2];
+    // From a tile's score sums to its weights w, raising the references and
+    // adding to l.  sc[.][t][i] is the lane's row against key 16 g + 4 t + i of
+    // the tile (lane group g = lane / 16); ks, vs are the scales of key `lane`,
+    // `there` whether the group's keys have a page.
+    __device__ __forceinline__ void weights(const f4 (&sc)[NB][4], float ks, float vs, bool there,
+                                            int tile, int lane, h8 (&w)[NB][2]) {
+        // Each lane prepares one key for the 16 lanes of its row, whose keys
+        // these are: K's scale with all that a score takes, V's as f 2^e.
+        const int e = max((int)((__float_as_uint(vs) >> 23) & 0xFF) - 126, kLeastExp);
+        const float kf = ks * qscale, ef = (float)e, vf = __builtin_amdgcn_ldexpf(vs, -e);
+        const float back = __builtin_amdgcn_ldexpf(1.f, -e);
+        const bool masked = tile >= full || !__all(there);
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
             float x[16];
             float top = kNegInf;
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                x[j] = __builtin_fmaf(sc[rb][j / 4][j % 4], keys.k[own + j], keys.e[own + j] - ref[rb]);
-            int n = 16;
+            sixteen([&](auto j) {
+                const float t = of_lane<j>(ef) - ref[rb];
+                x[j] = __builtin_fmaf(of_lane<j>(kf), sc[rb][j / 4][j % 4], t);
+            });
+            int n = 16;                  // keys of the lane's 16 that its row sees
             if (masked) {
-                asm volatile("");       // a branch, not selects on every tile
-                n = here ? limit[rb] - tile * kTile - (lane >> 4) * 16 : 0;
+                n = there ? limit[rb] - tile * kTile - (lane & 48) : 0;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) x[j] = j < n ? x[j] : kNegInf;
             }
@@ -493,29 +429,236 @@ struct Tiles {
                     for (int j = 0; j < 16; ++j) x[j] -= top;
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            sixteen([&](auto j) {
                 const float y = __builtin_amdgcn_exp2f(x[j]);
-                l[rb] = __builtin_fmaf(y, keys.back[own + j], l[rb]);
-                x[j] = y * keys.f[own + j];
-            }
+                l[rb] = __builtin_fmaf(of_lane<j>(back), y, l[rb]);
+                x[j] = of_lane<j>(vf) * y;
+            });
             if (masked) {
                 // what is not seen may have a scale of NaN or Inf
-                asm volatile("");
 #pragma unroll
                 for (int j = 0; j < 16; ++j) x[j] = j < n ? x[j] : 0.f;
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    // keys of a word as its bytes come out: 0, 2, 1, 3
-                    constexpr int at[4] = {0, 2, 1, 3};
-                    w[rb][u][i] = (_Float16)x[8 * u + (i & 4) + at[i & 3]];
-                }
+                for (int i = 0; i < 8; ++i) w[rb][u][i] = (_Float16)x[8 * u + order<8>(i)];
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+    }
+
+    __device__ __forceinline__ float reference(int rb) const {
+        return raise[rb] == kNegInf ? kNegInf : ref[rb];
+    }
+
+    // f(dim, four values): the lane's part of the sums of row matrix rb, four
+    // dims a call.  Dims of o[.][i] are four from 16 i + 4 g, or (4 bits) every
+    // other of eight from 32 (i / 2) + 8 g.
+    template <class F>
+    __device__ __forceinline__ void each_four(int rb, int lane, F&& f) const {
+        const int g = lane >> 4;
+        if constexpr (BITS == 8) {
+#pragma unroll
+            for (int i = 0; i < kOTiles; ++i) f(16 * i + 4 * g, o[rb][i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kOTiles; i += 2) {
+                const f4 a = o[rb][i], b = o[rb][i + 1];
+                f(16 * i + 8 * g, f4{a[0], b[0], a[1], b[1]});
+                f(16 * i + 8 * g + 4, f4{a[2], b[2], a[3], b[3]});
+            }
+        }
+    }
+};
+
+// ------------------------------------------------------- a run of a kernel
+// A run's way through its units: part(e, b, h, row0, tile, end, n) for each
+// part of a unit, tiles [tile, end) of its n.
+template <class Part>
+__device__ __forceinline__ void walk_run(const Source& s, int lane, Part&& part) {
+    Entries at(s, 0, lane);
+    const int64_t total = all_steps(s, at, lane);
+    const int64_t per = run_length(s, total);
+    const int64_t pos = (int64_t)blockIdx.x * per;
+    const int64_t stop = min(pos + per, total * s.c.heads);
+    if (pos >= stop) return;
+    int64_t before = 0;                 // steps of one head ahead of entry at.base
+    uint64_t past;
+    while ((past = __ballot((before + at.upto) * s.c.heads > pos)) == 0) {
+        before += at.all();
+        if (at.base + 64 >= entries_of(s)) return;
+        at = Entries(s, at.base + 64, lane);
+    }
+    int slot_e = __builtin_ctzll(past);
+    int n = __builtin_amdgcn_readlane(at.tiles, slot_e);
+    int steps = __builtin_amdgcn_readlane(at.steps, slot_e);
+    before += (uint32_t)__builtin_amdgcn_readlane(at.upto, slot_e) - (uint32_t)steps;
+    const int64_t in_entry = pos - before * s.c.heads;
+    int h = __builtin_amdgcn_readfirstlane((int)quotient(in_entry, steps));
+    int tile = __builtin_amdgcn_readfirstlane((int)(in_entry - (int64_t)h * steps));
+    int64_t left = stop - pos;
+    for (;;) {
+        const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(steps - tile), left));
+        const int end = min(tile + take, n);
+        const int e = at.base + slot_e;
+        const int b = s.prefix ? 0 : s.row_groups == 1 ? e : e / s.row_groups;
+        // (a unit's cost alone may be what is left of it)
+        if (tile < end) part(b, h, (e - b * s.row_groups) * s.rows_per_unit, tile, end, n);
+        left -= take;
+        if (left <= 0) return;
+        tile = 0;
+        if (++h == s.c.heads) {
+            h = 0;
+            do {
+                if (++slot_e == 64) {
+                    if (at.base + 64 >= entries_of(s)) return;
+                    at = Entries(s, at.base + 64, lane);
+                    slot_e = 0;
+                }
+                if (at.base + slot_e >= entries_of(s)) return;
+                n = __builtin_amdgcn_readlane(at.tiles, slot_e);
+            } while (n == 0);
+            steps = __builtin_amdgcn_readlane(at.steps, slot_e);
+        }
+    }
+}
+
+// Where the rows of a part of a unit go: `out` or the rows' home if the part
+// is the whole unit, else a slot of the run.
+template <class T, int D>
+struct Sink {
+    const Source& s;
+    int b, h, row0;
+    bool whole, triple;
+    int64_t slot;
+    __device__ __forceinline__ Sink(const Source& src, int b_, int h_, int row0_, int tile, int end,
+                                    int n)
+        : s(src), b(b_), h(h_), row0(row0_), whole(tile == 0 && end == n),
+          triple(!whole || !src.finish),
+          slot(((int64_t)blockIdx.x * 2 + (tile > 0 ? 0 : 1)) * src.rows_per_unit) {}
+    __device__ __forceinline__ void put_ml(int r, float m, float l) const {
+        const int64_t to = whole ? RowAt(s, b, r, h).flat(s) : slot + r - row0;
+        float* ml = whole ? s.home_ml : s.broken_ml;
+        ml[2 * to] = m;
+        ml[2 * to + 1] = l;
+    }
+    __device__ __forceinline__ void put_o(int r, int dim, f4 v, float l) const {
+        if (!whole) {
+            *reinterpret_cast<f4*>(s.broken_o + (slot + r - row0) * D + dim) = v;
+            return;
+        }
+        const int64_t to = RowAt(s, b, r, h).flat(s) * D + dim;
+        if (s.finish) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            store4(static_cast<T*>(s.a.out) + to, l == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * inv);
+        } else {
+            *reinterpret_cast<f4*>(s.home_o + to) = v;
+        }
+    }
+};
+
+// Table entry of 16 keys `sub` of a tile (any entry past the table), and the
+// page it means, 0 for none.
+__device__ __forceinline__ int32_t entry_at(const Source& s, const int32_t* table, int cols,
+                                            int tile, int sub) {
+    return table[min((tile * kTile + sub * 16) >> s.page_shift, cols - 1)];
+}
+__device__ __forceinline__ int64_t page_or_0(const Source& s, int32_t entry) {
+    return max((int64_t)0, page_in(entry, s.c.pages));
+}
+
+// ------------------------------------------------------- few rows: a wave's
+// The four waves of a workgroup take the same 16 NB rows and every fourth tile
+// each, codes from memory to registers, and join their sums in LDS.
+template <class T, int BITS, int D, int NB>
+struct Tiles : Rows<T, BITS, D, NB, true> {
+    using Base = Rows<T, BITS, D, NB, true>;
+    using Base::kSteps;
+    static constexpr int kRow = D * BITS / 8;              // bytes of a token's row
+    static constexpr int kLane = kRow / 4;                 // K bytes of a lane and row
+    static constexpr int kChunk = kLane < 16 ? kLane : 16;
+    static constexpr int kChunks = kLane / kChunk;
+    static constexpr int kWords = kChunk / 4;
+    static constexpr int kVTiles = kRow / 16;              // 16 rows of V bytes
+
+    Vec<uint32_t, kWords> kq[4][kChunks];
+    u4 vq[kVTiles];
+    float ks, vs;                        // scales of key `lane` of the tile
+    bool there;                          // the lane group's 16 keys have a page
+
+    // K's rows in the order that gives lane group g keys 16 g .. 16 g + 15.
+    __device__ __forceinline__ void load_k(const Source& s, int32_t entry, int tile, int h,
+                                           int lane) {
+        const int g = lane >> 4, r = lane & 15;
+        const int in = (tile * kTile + (r >> 2) * 16) & (s.c.page_size - 1);
+        const uint8_t* p =
+            static_cast<const uint8_t*>(s.c.k) +
+            ((page_or_0(s, entry) * s.c.heads + h) * s.c.page_size + in + (r & 3)) * kRow +
+            g * kChunk;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+                kq[t][c] = *reinterpret_cast<const Vec<uint32_t, kWords>*>(
+                    p + t * 4 * kRow + c * 4 * kChunk);
+    }
+
+    __device__ __forceinline__ void load_v(const Source& s, int32_t entry, int tile, int h,
+                                           int lane) {
+        const int g = lane >> 4, r = lane & 15;
+        there = page_in(entry, s.c.pages) >= 0;
+        const int64_t ph = page_or_0(s, entry) * s.c.heads + h;
+        const int in = (tile * kTile + g * 16) & (s.c.page_size - 1);
+        const float* sc = s.c.scales + ph * 2 * s.c.page_size + in + r;
+        ks = sc[0];
+        vs = sc[s.c.page_size];
+        const uint8_t* p =
+            static_cast<const uint8_t*>(s.c.v) + (ph * s.c.page_size + in) * kRow + r * 16;
+#pragma unroll
+        for (int i = 0; i < kVTiles; ++i) vq[i] = *reinterpret_cast<const u4*>(p + i * 256);
+    }
+
+    static __device__ __forceinline__ h8 unpack_k(const Vec<uint32_t, kWords> (&row)[kChunks],
+                                                  int u) {
+        constexpr int per = kChunk / BITS;                 // steps of a chunk
+        u4 w;
+        if constexpr (BITS == 8) {
+            uint32_t x, y, z, v;
+            halves_of_bytes(row[u / per][2 * (u % per)], x, y);
+            halves_of_bytes(row[u / per][2 * (u % per) + 1], z, v);
+            w = u4{x, y, z, v};
+        } else {
+            uint32_t x[4];
+            halves_of_nibbles(row[u / per][u % per], x);
+            w = u4{x[0], x[1], x[2], x[3]};
+        }
+        return __builtin_bit_cast(h8, w);
+    }
+
+    // One tile of keys.  next_k and next_v issue the loads that the registers
+    // freed by then can take.
+    template <class NextK, class NextV>
+    __device__ __forceinline__ void step(int tile, int lane, NextK&& next_k, NextV&& next_v) {
+        f4 sc[NB][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int rb = 0; rb < NB; ++rb) {
+                const float x = this->start[rb];
+                sc[rb][t] = f4{x, x, x, x};
+            }
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u) {
+                const h8 k = unpack_k(kq[t], u);
+#pragma unroll
+                for (int rb = 0; rb < NB; ++rb)
+                    sc[rb][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, this->q[rb][u],
+                                                                      sc[rb][t], 0, 0, 0);
+            }
+        }
+        next_k();
+        h8 w[NB][2];
+        this->weights(sc, ks, vs, there, tile, lane, w);
+        auto& o = this->o;
 #pragma unroll
         for (int i = 0; i < kVTiles; ++i)
 #pragma unroll
@@ -552,51 +695,29 @@ struct Tiles {
     // Keys from tile `tile`, every `stride`th up to `end`.  The first loads go
     // out before the queries are fetched.
     __device__ __forceinline__ void run(const Source& s, int b, int first_row, int h, int tile,
-                                        int end, int stride, int lane, Keys& keys) {
+                                        int end, int stride, int lane) {
         const int32_t* table = s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride;
         const int cols = s.prefix ? s.a.prefix_cols : s.a.table_cols;
-        const int ksub = (lane & 15) >> 2, vsub = lane >> 4;
+        const int g = lane >> 4, ksub = (lane & 15) >> 2;
         int32_t ke = 0, ve = 0;
         if (tile < end) {
-            ke = entry(s, table, cols, tile, ksub);
-            ve = entry(s, table, cols, tile, vsub);
+            ke = entry_at(s, table, cols, tile, ksub);
+            ve = entry_at(s, table, cols, tile, g);
             load_k(s, ke, tile, h, lane);
-            load_scales(s, ve, tile, h, lane);
             load_v(s, ve, tile, h, lane);
         }
-        load_q(s, b, first_row, h, lane);
+        this->load(s, b, first_row, h, lane, [&](int u) {
+            constexpr int per = kChunk / BITS;
+            return ((u / per) * 4 * kChunk + g * kChunk) * 8 / BITS + (u % per) * 8;
+        });
         for (; tile < end; tile += stride) {
             const int next = tile + stride;
             if (next < end) {
-                ke = entry(s, table, cols, next, ksub);
-                ve = entry(s, table, cols, next, vsub);
+                ke = entry_at(s, table, cols, next, ksub);
+                ve = entry_at(s, table, cols, next, g);
             }
-            step(tile, lane, keys, [&] { if (next < end) load_k(s, ke, next, h, lane); },
-                 [&] {
-                     if (next < end) {
-                         load_scales(s, ve, next, h, lane);
-                         load_v(s, ve, next, h, lane);
-                     }
-                 });
-        }
-    }
-
-    // f(dim, four values): the lane's part of the sums of row matrix rb, four
-    // dims a call.  Dims of o[.][i] are four from 16 i + 4 g, or (4 bits) every
-    // other of eight from 32 (i / 2) + 8 g.
-    template <class F>
-    __device__ __forceinline__ void each_four(int rb, int lane, F&& f) const {
-        const int g = lane >> 4;
-        if constexpr (BITS == 8) {
-#pragma unroll
-            for (int i = 0; i < kOTiles; ++i) f(16 * i + 4 * g, o[rb][i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kOTiles; i += 2) {
-                const f4 a = o[rb][i], b = o[rb][i + 1];
-                f(16 * i + 8 * g, f4{a[0], b[0], a[1], b[1]});
-                f(16 * i + 8 * g + 4, f4{a[2], b[2], a[3], b[3]});
-            }
+            step(tile, lane, [&] { if (next < end) load_k(s, ke, next, h, lane); },
+                 [&] { if (next < end) load_v(s, ve, next, h, lane); });
         }
     }
 };
@@ -604,135 +725,219 @@ struct Tiles {
 // Least waves per SIMD (registers) and workgroups that a CU is dealt.
 constexpr int waves_of(int d, int nb) { return d * nb <= 128 ? 2 : 1; }
 
-template <class T, int BITS, int D, int NB, bool SHARE>
+template <class T, int BITS, int D, int NB>
 __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s) {
-    using W = Tiles<T, BITS, D, NB, SHARE>;
-    constexpr int kRows = W::kUnitRows;
-    // waves that split a unit's keys join here
-    __shared__ __attribute__((aligned(16))) float
-        sm_o[SHARE ? 1 : kWaves][SHARE ? 1 : kRows][SHARE ? 4 : D + 4];
-    __shared__ float sm_m[kWaves][SHARE ? 1 : kRows], sm_l[kWaves][SHARE ? 1 : kRows];
-    __shared__ __attribute__((aligned(16))) Keys sm_keys[kWaves];
+    constexpr int kRows = 16 * NB;
+    __shared__ __attribute__((aligned(16))) float sm_o[kWaves][kRows][D + 4];
+    __shared__ float sm_m[kWaves][kRows], sm_l[kWaves][kRows];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Entries at(s, 0, lane);
-    const int64_t total = all_steps(s, at, lane);
-    const int64_t per = run_length(s, total);
-    const int64_t pos = (int64_t)blockIdx.x * per;
-    const int64_t stop = min(pos + per, total * s.c.heads);
-    if (pos >= stop) return;
-    int64_t before = 0;                 // steps of one head ahead of entry at.base
-    uint64_t past;
-    while ((past = __ballot((before + at.upto) * s.c.heads > pos)) == 0) {
-        before += at.all();
-        if (at.base + 64 >= entries_of(s)) return;
-        at = Entries(s, at.base + 64, lane);
-    }
-    int slot_e = __builtin_ctzll(past);
-    int n = __builtin_amdgcn_readlane(at.tiles, slot_e);
-    int steps = __builtin_amdgcn_readlane(at.steps, slot_e);
-    before += (uint32_t)__builtin_amdgcn_readlane(at.upto, slot_e) - (uint32_t)steps;
-    const int64_t in_entry = pos - before * s.c.heads;
-    int h = __builtin_amdgcn_readfirstlane((int)quotient(in_entry, steps));
-    int tile = __builtin_amdgcn_readfirstlane((int)(in_entry - (int64_t)h * steps));
-    int64_t left = stop - pos;
-    W work;
-    for (;;) {
-        const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(steps - tile), left));
-        const int end = min(tile + take, n);
-        const int e = at.base + slot_e;
-        const int b = s.prefix ? 0 : s.row_groups == 1 ? e : e / s.row_groups;
-        const int row0 = (e - b * s.row_groups) * kRows;
-        const int mine = row0 + (SHARE ? wave * 16 * NB : 0);
-        const bool whole = tile == 0 && end == n;
-        const int64_t slot = ((int64_t)blockIdx.x * 2 + (tile > 0 ? 0 : 1)) * kRows;
-        // where a row's triple or result goes
-        auto put_ml = [&](int r, float m, float l) {
-            const int64_t to = whole ? typename W::RowAt(s, b, r, h).flat(s) : slot + r - row0;
-            float* ml = whole ? s.home_ml : s.broken_ml;
-            ml[2 * to] = m;
-            ml[2 * to + 1] = l;
-        };
-        auto put_o = [&](int r, int dim, f4 v, float l) {
-            if (!whole) {
-                *reinterpret_cast<f4*>(s.broken_o + (slot + r - row0) * D + dim) = v;
-                return;
-            }
-            const int64_t to = typename W::RowAt(s, b, r, h).flat(s) * D + dim;
-            if (s.finish) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                store4(static_cast<T*>(s.a.out) + to, l == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * inv);
-            } else {
-                *reinterpret_cast<f4*>(s.home_o + to) = v;
-            }
-        };
-        const bool triple = !whole || !s.finish;
-        if (tile >= end) {
-            // the unit's cost alone
-        } else if (SHARE) {
-            if (mine < s.rows) {
-                work.run(s, b, mine, h, tile, end, 1, lane, sm_keys[wave]);
+    Tiles<T, BITS, D, NB> work;
+    walk_run(s, lane, [&](int b, int h, int row0, int tile, int end, int n) {
+        work.run(s, b, row0, h, tile + wave, end, kWaves, lane);
 #pragma unroll
-                for (int rb = 0; rb < NB; ++rb) {
-                    const int r = mine + 16 * rb + (lane & 15);
-                    const float l = quad_sum(work.l[rb]);
-                    if (r < s.rows) {
-                        if (triple && lane < 16)
-                            put_ml(r, work.raise[rb] == kNegInf ? kNegInf : work.ref[rb], l);
-                        work.each_four(rb, lane, [&](int dim, f4 v) { put_o(r, dim, v, l); });
+        for (int rb = 0; rb < NB; ++rb) {
+            const int r = 16 * rb + (lane & 15);
+            const float l = quad_sum(work.l[rb]);
+            if (lane < 16) {
+                sm_m[wave][r] = work.reference(rb);
+                sm_l[wave][r] = l;
+            }
+            work.each_four(rb, lane,
+                           [&](int dim, f4 x) { *reinterpret_cast<f4*>(&sm_o[wave][r][dim]) = x; });
+        }
+        __syncthreads();
+        const Sink<T, D> sink(s, b, h, row0, tile, end, n);
+        const int rows = min(kRows, s.rows - row0);
+        for (int i = threadIdx.x; i < rows * (D / 4); i += kBlock) {
+            const int r = i / (D / 4), dim = i % (D / 4) * 4;
+            float top = sm_m[0][r], sum = 0.f;
+#pragma unroll
+            for (int v = 1; v < kWaves; ++v) top = fmaxf(top, sm_m[v][r]);
+            f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                const float keep = factor(sm_m[v][r], sm_l[v][r], top);
+                sum += sm_l[v][r] * keep;
+                x += *reinterpret_cast<const f4*>(&sm_o[v][r][dim]) * keep;
+            }
+            if (sink.triple && dim == 0) sink.put_ml(row0 + r, top, sum);
+            sink.put_o(row0 + r, dim, x, sum);
+        }
+        __syncthreads();
+    });
+}
+
+// -------------------------------------------------- many rows: a workgroup's
+// W waves take 32 rows each and the same keys: the codes of a tile become fp16
+// once, in LDS, for all of them, two tiles in turn, while the next tile's codes
+// are on their way to registers.
+template <class T, int BITS, int D, int W>
+__global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kernel(Source s) {
+    constexpr int NB = 2, kThreads = 64 * W;
+    constexpr int kRow = D * BITS / 8;
+    constexpr int kParts = kRow / 16;                      // 16 bytes of a K row
+    constexpr int kPieces = kTile * kParts;                // of a tile's K, and of its V
+    constexpr int kEach = (kPieces + kThreads - 1) / kThreads;
+    constexpr int kCodes = 128 / BITS;                     // codes of a piece
+    // rows in LDS start 16 bytes apart from a multiple of the banks
+    constexpr int kKRow = D + 8, kVRow = kTile + 8;
+    __shared__ __attribute__((aligned(16))) _Float16 sm_k[2][kTile][kKRow];
+    __shared__ __attribute__((aligned(16))) _Float16 sm_v[2][D][kVRow];
+    const int lane = threadIdx.x & 63, g = lane >> 4, r16 = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Rows<T, BITS, D, NB, false> rows;
+    u4 kq[kEach], vq[kEach];
+
+    walk_run(s, lane, [&](int b, int h, int row0, int tile, int end, int n) {
+        const int32_t* table = s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride;
+        const int cols = s.prefix ? s.a.prefix_cols : s.a.table_cols;
+        const int mine = row0 + 32 * wave;
+        const bool live = mine < s.rows;
+        // pieces of a tile: K's by key and part, V's by 16 keys and row; their
+        // table entries are looked up a tile ahead
+        int32_t ke[kEach], ve[kEach], se;
+        auto look_up = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int c = threadIdx.x + i * kThreads;
+                ke[i] = entry_at(s, table, cols, t, min(c / kParts, kTile - 1) >> 4);
+                ve[i] = entry_at(s, table, cols, t, min(c / kRow, 3));
+            }
+        };
+        auto fetch = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int c = threadIdx.x + i * kThreads;
+                if (kPieces % kThreads != 0 && c >= kPieces) break;
+                const int key = c / kParts, sub = c / kRow;
+                const int64_t kp = page_or_0(s, ke[i]), vp = page_or_0(s, ve[i]);
+                const int kin = (t * kTile + key) & (s.c.page_size - 1);
+                const int vin = (t * kTile + sub * 16) & (s.c.page_size - 1);
+                kq[i] = *reinterpret_cast<const u4*>(
+                    static_cast<const uint8_t*>(s.c.k) +
+                    ((kp * s.c.heads + h) * s.c.page_size + kin) * kRow + (c % kParts) * 16);
+                vq[i] = *reinterpret_cast<const u4*>(
+                    static_cast<const uint8_t*>(s.c.v) +
+                    ((vp * s.c.heads + h) * s.c.page_size + vin) * kRow + (c % kRow) * 16);
+            }
+        };
+        auto spread = [&](int buf) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int c = threadIdx.x + i * kThreads;
+                if (kPieces % kThreads != 0 && c >= kPieces) break;
+                // key 16 s + 4 t + i lies in row 16 t + 4 s + i: the rows of
+                // product t are then 16 side by side
+                const int key = c / kParts, sub = c / kRow, vr = c % kRow;
+                const int kr = (key >> 2 & 3) * 16 + (key >> 4) * 4 + (key & 3);
+                u4* kd = reinterpret_cast<u4*>(&sm_k[buf][kr][(c % kParts) * kCodes]);
+                if constexpr (BITS == 8) {
+                    u4* vd = reinterpret_cast<u4*>(&sm_v[buf][vr][sub * 16]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t x[4], y[4];
+                        codes_of_bytes(kq[i][2 * j], x[0], x[1]);
+                        codes_of_bytes(kq[i][2 * j + 1], x[2], x[3]);
+                        codes_of_bytes(vq[i][2 * j], y[0], y[1]);
+                        codes_of_bytes(vq[i][2 * j + 1], y[2], y[3]);
+                        kd[j] = u4{x[0], x[1], x[2], x[3]};
+                        vd[j] = u4{y[0], y[1], y[2], y[3]};
+                    }
+                } else {
+                    // V's row is two dims: the even ones' tokens, the odd ones'
+                    u4* even = reinterpret_cast<u4*>(&sm_v[buf][vr / 16 * 32 + vr % 16][sub * 16]);
+                    u4* odd = reinterpret_cast<u4*>(&sm_v[buf][vr / 16 * 32 + 16 + vr % 16][sub * 16]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t x[4];
+                        codes_of_nibbles(kq[i][j], x);
+                        kd[j] = u4{x[0], x[1], x[2], x[3]};
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t x[4], y[4];
+                        codes_of_nibbles(vq[i][2 * j], x);
+                        codes_of_nibbles(vq[i][2 * j + 1], y);
+                        even[j] = u4{x[0], x[2], y[0], y[2]};
+                        odd[j] = u4{x[1], x[3], y[1], y[3]};
                     }
                 }
             }
-        } else {
-            work.run(s, b, mine, h, tile + wave, end, kWaves, lane, sm_keys[wave]);
+        };
+        float ks, vs;
+        bool there;
+        auto fetch_scales = [&](int t) {
+            there = page_in(se, s.c.pages) >= 0;
+            const int in = (t * kTile + g * 16) & (s.c.page_size - 1);
+            const float* sc = s.c.scales +
+                              (page_or_0(s, se) * s.c.heads + h) * 2 * s.c.page_size + in + r16;
+            ks = sc[0];
+            vs = sc[s.c.page_size];
+        };
+        look_up(tile);
+        se = entry_at(s, table, cols, tile, g);
+        fetch(tile);
+        fetch_scales(tile);
+        if (tile + 1 < end) look_up(tile + 1);
+        if (live) rows.load(s, b, mine, h, lane, [&](int u) { return u * 32 + g * 8; });
+        spread(0);
+        if (tile + 1 < end) fetch(tile + 1);
+        __syncthreads();
+        for (int t = tile; t < end; ++t) {
+            const int buf = (t - tile) & 1;
+            if (t + 2 < end) look_up(t + 2);
+            if (t + 1 < end) se = entry_at(s, table, cols, t + 1, g);
+            if (live) {
+                f4 sc[NB][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int rb = 0; rb < NB; ++rb) sc[rb][i] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int u = 0; u < D / 32; ++u) {
+                        const h8 k = *reinterpret_cast<const h8*>(
+                            &sm_k[buf][16 * i + r16][u * 32 + g * 8]);
+#pragma unroll
+                        for (int rb = 0; rb < NB; ++rb)
+                            sc[rb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                k, rows.q[rb][u], sc[rb][i], 0, 0, 0);
+                    }
+                }
+                h8 w[NB][2];
+                rows.weights(sc, ks, vs, there, t, lane, w);
+                if (t + 1 < end) fetch_scales(t + 1);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const h8 v = *reinterpret_cast<const h8*>(
+                            &sm_v[buf][16 * i + r16][g * 16 + u * 8]);
+#pragma unroll
+                        for (int rb = 0; rb < NB; ++rb)
+                            rows.o[rb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                v, w[rb][u], rows.o[rb][i], 0, 0, 0);
+                    }
+            }
+            if (t + 1 < end) {
+                spread(buf ^ 1);
+                if (t + 2 < end) fetch(t + 2);
+            }
+            __syncthreads();
+        }
+        if (live) {
+            const Sink<T, D> sink(s, b, h, row0, tile, end, n);
 #pragma unroll
             for (int rb = 0; rb < NB; ++rb) {
-                const int r = 16 * rb + (lane & 15);
-                const float l = quad_sum(work.l[rb]);
-                if (lane < 16) {
-                    sm_m[wave][r] = work.raise[rb] == kNegInf ? kNegInf : work.ref[rb];
-                    sm_l[wave][r] = l;
+                const int r = mine + 16 * rb + r16;
+                const float l = quad_sum(rows.l[rb]);
+                if (r < s.rows) {
+                    if (sink.triple && lane < 16) sink.put_ml(r, rows.reference(rb), l);
+                    rows.each_four(rb, lane, [&](int dim, f4 v) { sink.put_o(r, dim, v, l); });
                 }
-                work.each_four(rb, lane, [&](int dim, f4 x) {
-                    *reinterpret_cast<f4*>(&sm_o[wave][r][dim]) = x;
-                });
             }
-            __syncthreads();
-            const int rows = min(kRows, s.rows - row0);
-            for (int i = threadIdx.x; i < rows * (D / 4); i += kBlock) {
-                const int r = i / (D / 4), dim = i % (D / 4) * 4;
-                float top = sm_m[0][r], sum = 0.f;
-#pragma unroll
-                for (int v = 1; v < kWaves; ++v) top = fmaxf(top, sm_m[v][r]);
-                f4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int v = 0; v < kWaves; ++v) {
-                    const float keep = factor(sm_m[v][r], sm_l[v][r], top);
-                    sum += sm_l[v][r] * keep;
-                    x += *reinterpret_cast<const f4*>(&sm_o[v][r][dim]) * keep;
-                }
-                if (triple && dim == 0) put_ml(row0 + r, top, sum);
-                put_o(row0 + r, dim, x, sum);
-            }
-            __syncthreads();
         }
-        left -= take;
-        if (left <= 0) break;
-        tile = 0;
-        if (++h == s.c.heads) {
-            h = 0;
-            do {
-                if (++slot_e == 64) {
-                    if (at.base + 64 >= entries_of(s)) return;
-                    at = Entries(s, at.base + 64, lane);
-                    slot_e = 0;
-                }
-                if (at.base + slot_e >= entries_of(s)) return;
-                n = __builtin_amdgcn_readlane(at.tiles, slot_e);
-            } while (n == 0);
-            steps = __builtin_amdgcn_readlane(at.steps, slot_e);
-        }
-    }
+    });
 }
 
 // Joins the triples of rows: those of their own keys' runs and, with a prefix,
@@ -842,18 +1047,21 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
 // ------------------------------------------------------------------- host
 constexpr int kCus = 256;
 
+// Which kernel takes a source: the tile kernel with nb row matrices to a wave,
+// or the block kernel with `waves` waves.
 struct Shape {
-    int nb;
-    bool share;
+    int nb;          // 0: the block kernel
+    int waves;
+    int rows;        // of a unit
+    int resident;    // workgroups that a CU holds
 };
 
-// Rows that share keys fill one wave's matrices; many of them go to all four
-// waves of a workgroup.
 Shape shape_of(int64_t rows, int d) {
-    if (rows <= 16) return {1, false};
-    if (d > 128) return {1, true};
-    if (rows <= 32) return {2, false};
-    return {d > 64 || rows <= 128 ? 2 : 4, true};
+    if (rows <= 16) return {1, kWaves, 16, waves_of(d, 1)};
+    if (rows <= 32 && d <= 128) return {2, kWaves, 32, waves_of(d, 2)};
+    if (d == 256) return {0, 4, 128, 1};
+    if (rows <= 128) return {0, 4, 128, 2};
+    return {0, 8, 256, 1};
 }
 
 Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, Shape* shape) {
@@ -866,17 +1074,20 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
     const int64_t rows = (int64_t)a.tokens * s.group * (prefix ? a.batch : 1);
     s.rows = (int32_t)rows;
     *shape = shape_of(rows, c.head_dim);
-    s.rows_per_unit = 16 * shape->nb * (shape->share ? kWaves : 1);
+    s.rows_per_unit = shape->rows;
     s.row_groups = (int32_t)((rows + s.rows_per_unit - 1) / s.rows_per_unit);
-    s.quantum = kWaves;
-    s.cost = shape->share ? kWaves : 2 * kWaves;
+    // a workgroup of the tile kernel takes four tiles at a time; a unit's start
+    // and end take as long as two rounds of them, or two tiles of the block
+    // kernel
+    s.quantum = shape->nb > 0 ? kWaves : 2;
+    s.cost = shape->nb > 0 ? 2 * kWaves : 2;
     s.finish = a.prefix_len == 0;
     // no more runs than quanta, as far as the tables' sizes tell
     const int64_t keys = prefix ? a.prefix_len : (int64_t)a.table_cols * c.page_size;
     const int64_t entries = (int64_t)s.row_groups * (prefix ? 1 : a.batch);
     const __int128 steps = (__int128)((keys + kTile - 1) / kTile + s.quantum + s.cost) * entries *
                            c.heads;
-    const int64_t room = (int64_t)kCus * waves_of(c.head_dim, shape->nb);
+    const int64_t room = (int64_t)kCus * shape->resident;
     const __int128 most = steps / s.quantum;
     s.runs = (uint32_t)(most < room ? (int64_t)most : room);
     return s;
@@ -904,19 +1115,15 @@ int64_t lay_out(const cq_kv_cache_t& c, const cq_attention_t& a, Source* own, So
 template <class T, int BITS, int D>
 hipError_t launch_tiles(const Source& s, Shape shape, hipStream_t stream) {
     auto go = [&](auto* kernel) {
-        kernel<<<dim3(s.runs), dim3(kBlock), 0, stream>>>(s);
+        kernel<<<dim3(s.runs), dim3(64 * shape.waves), 0, stream>>>(s);
         return hipGetLastError();
     };
-    if constexpr (D > 128) {
-        return shape.share ? go(&tile_kernel<T, BITS, D, 1, true>)
-                           : go(&tile_kernel<T, BITS, D, 1, false>);
-    } else {
-        if (shape.nb == 1) return go(&tile_kernel<T, BITS, D, 1, false>);
-        if (!shape.share) return go(&tile_kernel<T, BITS, D, 2, false>);
-        if constexpr (D <= 64)
-            if (shape.nb == 4) return go(&tile_kernel<T, BITS, D, 4, true>);
-        return go(&tile_kernel<T, BITS, D, 2, true>);
+    if (shape.nb == 1) return go(&tile_kernel<T, BITS, D, 1>);
+    if constexpr (D <= 128) {
+        if (shape.nb == 2) return go(&tile_kernel<T, BITS, D, 2>);
+        if (shape.waves == 8) return go(&block_kernel<T, BITS, D, 8>);
     }
+    return go(&block_kernel<T, BITS, D, 4>);
 }
 
 template <class T, int D>
@@ -933,7 +1140,7 @@ hipError_t launch_typed(const Source& own, Shape os, const Source& ahead, Shape 
     // are where rows are many (1024 tokens x 64 heads: 62 us with one row, 35
     // with eight); of few rows most have triples to join, one row a wave
     const int64_t all = (int64_t)own.rows * own.a.batch * own.c.heads;
-    const int each = own.finish && os.share && all >= 32 * kWaves * kCus ? 8 : 1;
+    const int each = own.finish && os.nb == 0 && all >= 32 * kWaves * kCus ? 8 : 1;
     const int64_t waves = (int64_t)((own.rows + each - 1) / each) * own.a.batch * own.c.heads;
     join_kernel<T, D><<<dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kBlock), 0, stream>>>(
         own, ahead, each);
