@@ -10,8 +10,8 @@
 // and raises M (scaling l and o down) when an exponent passes kRaise; triples
 // (M, l, o) of disjoint keys join the same way.  Folding V's exponent into
 // that of the softmax keeps w_j, which the matrix instructions take as fp16,
-// in range for any scales: the largest w of a row lies in [1/2, 2^kRaise), and
-// what fp16 then rounds off is 2^-11 of each weight, or 2^-24 of 1.
+// in range for any scales: the largest w of a row lies in [2^-5, 2^kRaise), and
+// what fp16 then rounds off is 2^-11 of each weight, or 2^-25 of 1.
 // Scores, statistics and sums are FP32.
 //
 // A code of K goes into the matrix units as the fp16 subnormal
@@ -56,6 +56,7 @@ constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.f;
 constexpr int kLeastExp = -100;         // a V scale below 2^-100 counts as 0
+constexpr int kEven = 4;
 
 using h8 = Vec<_Float16, 8>;
 using h2 = Vec<_Float16, 2>;
@@ -390,29 +391,40 @@ struct Rows {
     // From a tile's score sums to its weights w, raising the references and
     // adding to l.  sc[.][t][i] is the lane's row against key 16 g + 4 t + i of
     // the tile (lane group g = lane / 16); ks, vs are the scales of key `lane`,
-    // `there` whether the group's keys have a page.
+    // `there` whether the group's keys have a page.  Each lane prepares one key
+    // for the 16 lanes of its row, whose keys these are: K's scale with all that
+    // a score takes, V's as f 2^e.
+    //
+    // Where every row sees every key and V's scales lie within 2^kEven of the
+    // largest, e is the tile's largest instead: the weight of the key with the
+    // largest p is then 2^-kEven at least, well inside fp16, and e and 2^-e are
+    // one addition for 16 keys instead of two operations for each.
     __device__ __forceinline__ void weights(const f4 (&sc)[NB][4], float ks, float vs, bool there,
                                             int tile, int lane, h8 (&w)[NB][2]) {
-        // Each lane prepares one key for the 16 lanes of its row, whose keys
-        // these are: K's scale with all that a score takes, V's as f 2^e.
         const int e = max((int)((__float_as_uint(vs) >> 23) & 0xFF) - 126, kLeastExp);
-        const float kf = ks * qscale, ef = (float)e, vf = __builtin_amdgcn_ldexpf(vs, -e);
-        const float back = __builtin_amdgcn_ldexpf(1.f, -e);
-        const bool masked = tile >= full || !__all(there);
+        const int most = __builtin_amdgcn_readfirstlane((int)wave_max((float)e));
+        const bool even = tile < full && most < 128 && __all(there && e >= most - kEven);
+        const int by = even ? most : e;
+        const float kf = ks * qscale, ef = (float)by, vf = __builtin_amdgcn_ldexpf(vs, -by);
+        const float back = __builtin_amdgcn_ldexpf(1.f, -by);
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
+            // keys of the lane's 16 that its row sees
+            const int n = there ? limit[rb] - tile * kTile - (lane & 48) : 0;
             float x[16];
-            float top = kNegInf;
-            sixteen([&](auto j) {
-                const float t = of_lane<j>(ef) - ref[rb];
-                x[j] = __builtin_fmaf(of_lane<j>(kf), sc[rb][j / 4][j % 4], t);
-            });
-            int n = 16;                  // keys of the lane's 16 that its row sees
-            if (masked) {
-                n = there ? limit[rb] - tile * kTile - (lane & 48) : 0;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = j < n ? x[j] : kNegInf;
+            if (even) {
+                const float t = ef - ref[rb];
+                sixteen([&](auto j) {
+                    x[j] = __builtin_fmaf(of_lane<j>(kf), sc[rb][j / 4][j % 4], t);
+                });
+            } else {
+                sixteen([&](auto j) {
+                    const float t = of_lane<j>(ef) - ref[rb];
+                    x[j] = __builtin_fmaf(of_lane<j>(kf), sc[rb][j / 4][j % 4], t);
+                    x[j] = j < n ? x[j] : kNegInf;
+                });
             }
+            float top = kNegInf;
 #pragma unroll
             for (int j = 0; j < 16; ++j) top = fmaxf(top, x[j]);
             if (__any(top > raise[rb])) {
@@ -429,15 +441,22 @@ struct Rows {
                     for (int j = 0; j < 16; ++j) x[j] -= top;
                 }
             }
-            sixteen([&](auto j) {
-                const float y = __builtin_amdgcn_exp2f(x[j]);
-                l[rb] = __builtin_fmaf(of_lane<j>(back), y, l[rb]);
-                x[j] = of_lane<j>(vf) * y;
-            });
-            if (masked) {
-                // what is not seen may have a scale of NaN or Inf
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = j < n ? x[j] : 0.f;
+            for (int j = 0; j < 16; ++j) x[j] = __builtin_amdgcn_exp2f(x[j]);
+            if (even) {
+                float sum = 0.f;
+                sixteen([&](auto j) {
+                    sum += x[j];
+                    x[j] = of_lane<j>(vf) * x[j];
+                });
+                l[rb] = __builtin_fmaf(sum, back, l[rb]);
+            } else {
+                sixteen([&](auto j) {
+                    l[rb] = __builtin_fmaf(of_lane<j>(back), x[j], l[rb]);
+                    // what is not seen may have a scale of NaN or Inf
+                    const float p = of_lane<j>(vf) * x[j];
+                    x[j] = j < n ? p : 0.f;
+                });
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -556,14 +575,23 @@ struct Sink {
     }
 };
 
-// Table entry of 16 keys `sub` of a tile (any entry past the table), and the
-// page it means, 0 for none.
-__device__ __forceinline__ int32_t entry_at(const Source& s, const int32_t* table, int cols,
-                                            int tile, int sub) {
-    return table[min((tile * kTile + sub * 16) >> s.page_shift, cols - 1)];
+// Table entry of 16 keys `sub` of a tile (any entry past the table), whether it
+// names a page, and which (0 for none).
+__device__ __forceinline__ uint32_t entry_at(const Source& s, const int32_t* table, int cols,
+                                             int tile, int sub) {
+    return (uint32_t)table[min((tile * kTile + sub * 16) >> s.page_shift, cols - 1)];
 }
-__device__ __forceinline__ int64_t page_or_0(const Source& s, int32_t entry) {
-    return max((int64_t)0, page_in(entry, s.c.pages));
+__device__ __forceinline__ bool is_page(const Source& s, uint32_t entry) {
+    return entry < (uint32_t)s.c.pages;
+}
+__device__ __forceinline__ uint32_t page_or_0(const Source& s, uint32_t entry) {
+    return is_page(s, entry) ? entry : 0;
+}
+
+// Bytes of K (or V) from the cache's start to a head of a page, and floats of
+// the scales; `unit` bytes (floats) to a token.
+__device__ __forceinline__ uint64_t head_of(const Source& s, uint32_t page, int h, int unit) {
+    return ((uint64_t)page * (uint32_t)s.c.heads + (uint32_t)h) * (uint32_t)(s.c.page_size * unit);
 }
 
 // ------------------------------------------------------- few rows: a wave's
@@ -586,14 +614,13 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
     bool there;                          // the lane group's 16 keys have a page
 
     // K's rows in the order that gives lane group g keys 16 g .. 16 g + 15.
-    __device__ __forceinline__ void load_k(const Source& s, int32_t entry, int tile, int h,
+    __device__ __forceinline__ void load_k(const Source& s, uint32_t entry, int tile, int h,
                                            int lane) {
         const int g = lane >> 4, r = lane & 15;
         const int in = (tile * kTile + (r >> 2) * 16) & (s.c.page_size - 1);
-        const uint8_t* p =
-            static_cast<const uint8_t*>(s.c.k) +
-            ((page_or_0(s, entry) * s.c.heads + h) * s.c.page_size + in + (r & 3)) * kRow +
-            g * kChunk;
+        const uint8_t* p = static_cast<const uint8_t*>(s.c.k) +
+                           head_of(s, page_or_0(s, entry), h, kRow) + (in + (r & 3)) * kRow +
+                           g * kChunk;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -602,17 +629,17 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
                     p + t * 4 * kRow + c * 4 * kChunk);
     }
 
-    __device__ __forceinline__ void load_v(const Source& s, int32_t entry, int tile, int h,
+    __device__ __forceinline__ void load_v(const Source& s, uint32_t entry, int tile, int h,
                                            int lane) {
         const int g = lane >> 4, r = lane & 15;
-        there = page_in(entry, s.c.pages) >= 0;
-        const int64_t ph = page_or_0(s, entry) * s.c.heads + h;
+        there = is_page(s, entry);
+        const uint32_t page = page_or_0(s, entry);
         const int in = (tile * kTile + g * 16) & (s.c.page_size - 1);
-        const float* sc = s.c.scales + ph * 2 * s.c.page_size + in + r;
+        const float* sc = s.c.scales + head_of(s, page, h, 2) + in + r;
         ks = sc[0];
         vs = sc[s.c.page_size];
-        const uint8_t* p =
-            static_cast<const uint8_t*>(s.c.v) + (ph * s.c.page_size + in) * kRow + r * 16;
+        const uint8_t* p = static_cast<const uint8_t*>(s.c.v) + head_of(s, page, h, kRow) +
+                           in * kRow + r * 16;
 #pragma unroll
         for (int i = 0; i < kVTiles; ++i) vq[i] = *reinterpret_cast<const u4*>(p + i * 256);
     }
@@ -699,7 +726,7 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
         const int32_t* table = s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride;
         const int cols = s.prefix ? s.a.prefix_cols : s.a.table_cols;
         const int g = lane >> 4, ksub = (lane & 15) >> 2;
-        int32_t ke = 0, ve = 0;
+        uint32_t ke = 0, ve = 0;
         if (tile < end) {
             ke = entry_at(s, table, cols, tile, ksub);
             ve = entry_at(s, table, cols, tile, g);
@@ -796,7 +823,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
         const bool live = mine < s.rows;
         // pieces of a tile: K's by key and part, V's by 16 keys and row; their
         // table entries are looked up a tile ahead
-        int32_t ke[kEach], ve[kEach], se;
+        uint32_t ke[kEach], ve[kEach], se;
         auto look_up = [&](int t) {
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
@@ -811,15 +838,15 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
                 const int c = threadIdx.x + i * kThreads;
                 if (kPieces % kThreads != 0 && c >= kPieces) break;
                 const int key = c / kParts, sub = c / kRow;
-                const int64_t kp = page_or_0(s, ke[i]), vp = page_or_0(s, ve[i]);
+                const uint32_t kp = page_or_0(s, ke[i]), vp = page_or_0(s, ve[i]);
                 const int kin = (t * kTile + key) & (s.c.page_size - 1);
                 const int vin = (t * kTile + sub * 16) & (s.c.page_size - 1);
-                kq[i] = *reinterpret_cast<const u4*>(
-                    static_cast<const uint8_t*>(s.c.k) +
-                    ((kp * s.c.heads + h) * s.c.page_size + kin) * kRow + (c % kParts) * 16);
-                vq[i] = *reinterpret_cast<const u4*>(
-                    static_cast<const uint8_t*>(s.c.v) +
-                    ((vp * s.c.heads + h) * s.c.page_size + vin) * kRow + (c % kRow) * 16);
+                kq[i] = *reinterpret_cast<const u4*>(static_cast<const uint8_t*>(s.c.k) +
+                                                     head_of(s, kp, h, kRow) + kin * kRow +
+                                                     (c % kParts) * 16);
+                vq[i] = *reinterpret_cast<const u4*>(static_cast<const uint8_t*>(s.c.v) +
+                                                     head_of(s, vp, h, kRow) + vin * kRow +
+                                                     (c % kRow) * 16);
             }
         };
         auto spread = [&](int buf) {
@@ -868,10 +895,9 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
         float ks, vs;
         bool there;
         auto fetch_scales = [&](int t) {
-            there = page_in(se, s.c.pages) >= 0;
+            there = is_page(s, se);
             const int in = (t * kTile + g * 16) & (s.c.page_size - 1);
-            const float* sc = s.c.scales +
-                              (page_or_0(s, se) * s.c.heads + h) * 2 * s.c.page_size + in + r16;
+            const float* sc = s.c.scales + head_of(s, page_or_0(s, se), h, 2) + in + r16;
             ks = sc[0];
             vs = sc[s.c.page_size];
         };
