@@ -77,6 +77,7 @@ struct Source {
     int32_t quantum;       // a run's length is a multiple of it
     int32_t cost;          // of a unit besides its tiles, in tiles
     uint32_t runs;         // workgroups
+    int32_t fits;          // the deal's sums fit 31 bits
     int32_t finish;        // 1: units of one run write `out`; 0: their home
     // workspace: triples of broken units, two per run, and of whole units
     float* broken_o;       // [runs * 2 * rows_per_unit, D]
@@ -127,13 +128,6 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {     // inclusive
     return v;
 }
 
-// x / y of whole numbers >= 0, in 32 bits where they fit (a 64-bit division
-// takes a hundred instructions).
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
-    if (((uint64_t)x | (uint64_t)y) >> 32 == 0) return (uint32_t)x / (uint32_t)y;
-    return x / y;
-}
-
 // A unit's place in the deal: as many steps as its tiles, rounded up to the
 // quantum, and its cost.
 __device__ __forceinline__ int steps_of(const Source& s, int tiles) {
@@ -154,16 +148,17 @@ struct Entries {
     __device__ __forceinline__ uint32_t all() const { return __builtin_amdgcn_readlane(upto, 63); }
 };
 
-// Steps of all units of one head; `first` holds entries 0 .. 63.
-__device__ __forceinline__ int64_t all_steps(const Source& s, const Entries& first, int lane) {
-    int64_t total = first.all();
+// Steps of all units of one head; `first` holds entries 0 .. 63.  (The host
+// sees to it that the steps of all heads stay below 2^31.)
+__device__ __forceinline__ uint32_t all_steps(const Source& s, const Entries& first, int lane) {
+    uint32_t total = first.all();
     for (int base = 64; base < entries_of(s); base += 64) total += Entries(s, base, lane).all();
     return total;
 }
 
-__device__ __forceinline__ int64_t run_length(const Source& s, int64_t total) {
-    const int64_t each = quotient(total * s.c.heads + s.runs - 1, s.runs);
-    return (max((int64_t)1, each) + s.quantum - 1) / s.quantum * s.quantum;
+__device__ __forceinline__ uint32_t run_length(const Source& s, uint32_t total) {
+    const uint32_t each = (total * s.c.heads + s.runs - 1) / s.runs, q = s.quantum;
+    return (max(1u, each) + q - 1) / q * q;
 }
 
 // ----------------------------------------------------------- small pieces
@@ -286,8 +281,7 @@ constexpr int order(int i) {
     return BITS == 8 ? o8[i] : o4[i];
 }
 
-// Largest magnitude among fp16 or bfloat16 words, as its bits; Inf and NaN are
-// the largest of all.
+using ss2 = Vec<short, 2>;
 __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
     using us2 = Vec<unsigned short, 2>;
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, a),
@@ -299,6 +293,8 @@ __device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
 // (halves_of_*); else the codes themselves.
 template <class T, int BITS, int D, int NB, bool RAW>
 struct Rows {
+    // (the short form for even scales is worth its code to many rows only)
+    static constexpr bool kShort = !RAW;
     static constexpr int kSteps = D / 32;                  // products over D
     static constexpr int kOTiles = D / 16;
     static constexpr float kOffset = BITS == 8 ? 128.f : 8.f;
@@ -336,25 +332,16 @@ struct Rows {
                 raw[rb][u] = *reinterpret_cast<const Vec<T, 8>*>(p + dim(u));
                 const u4 w = __builtin_bit_cast(u4, raw[rb][u]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top2 = pk_max(top2, w[i] & 0x7FFF7FFFu);
+                for (int i = 0; i < 4; ++i) {
+                    // magnitudes, 0 for Inf and NaN: their sum with 2^15 - Inf
+                    // is negative in 16 bits
+                    const uint32_t m = w[i] & 0x7FFF7FFFu;
+                    const ss2 bad = __builtin_bit_cast(ss2, m + (0x8000u - kInf) * 0x10001u) >> 15;
+                    top2 = pk_max(top2, m & ~__builtin_bit_cast(uint32_t, bad));
+                }
             }
         }
-        uint32_t bits = max(top2 & 0xFFFFu, top2 >> 16);
-        if (__any(bits >= kInf)) {
-            // the largest that is a number
-            bits = 0;
-#pragma unroll
-            for (int rb = 0; rb < NB; ++rb)
-#pragma unroll
-                for (int u = 0; u < kSteps; ++u) {
-                    const u4 w = __builtin_bit_cast(u4, raw[rb][u]);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t x = (w[i / 2] >> (16 * (i & 1))) & 0x7FFFu;
-                        bits = x < kInf ? max(bits, x) : bits;
-                    }
-                }
-        }
+        const uint32_t bits = max(top2 & 0xFFFFu, top2 >> 16);
         // One factor for the wave: exact down to 2^-27 of its largest element,
         // 2^-38 of that where fp16 is subnormal, so an error far below FP32's
         // in the largest row's scores is all that a small row can show.
@@ -402,11 +389,13 @@ struct Rows {
     __device__ __forceinline__ void weights(const f4 (&sc)[NB][4], float ks, float vs, bool there,
                                             int tile, int lane, h8 (&w)[NB][2]) {
         const int e = max((int)((__float_as_uint(vs) >> 23) & 0xFF) - 126, kLeastExp);
-        const int most = __builtin_amdgcn_readfirstlane((int)wave_max((float)e));
-        const bool even = tile < full && most < 128 && __all(there && e >= most - kEven);
+        const int most = kShort ? __builtin_amdgcn_readfirstlane((int)wave_max((float)e)) : 0;
+        const bool even = kShort && tile < full && most < 128 && __all(there && e >= most - kEven);
         const int by = even ? most : e;
         const float kf = ks * qscale, ef = (float)by, vf = __builtin_amdgcn_ldexpf(vs, -by);
         const float back = __builtin_amdgcn_ldexpf(1.f, -by);
+        float kfs[16];
+        sixteen([&](auto j) { kfs[j] = of_lane<j>(kf); });
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
             // keys of the lane's 16 that its row sees
@@ -415,12 +404,12 @@ struct Rows {
             if (even) {
                 const float t = ef - ref[rb];
                 sixteen([&](auto j) {
-                    x[j] = __builtin_fmaf(of_lane<j>(kf), sc[rb][j / 4][j % 4], t);
+                    x[j] = __builtin_fmaf(kfs[j], sc[rb][j / 4][j % 4], t);
                 });
             } else {
                 sixteen([&](auto j) {
                     const float t = of_lane<j>(ef) - ref[rb];
-                    x[j] = __builtin_fmaf(of_lane<j>(kf), sc[rb][j / 4][j % 4], t);
+                    x[j] = __builtin_fmaf(kfs[j], sc[rb][j / 4][j % 4], t);
                     x[j] = j < n ? x[j] : kNegInf;
                 });
             }
@@ -495,12 +484,12 @@ struct Rows {
 template <class Part>
 __device__ __forceinline__ void walk_run(const Source& s, int lane, Part&& part) {
     Entries at(s, 0, lane);
-    const int64_t total = all_steps(s, at, lane);
-    const int64_t per = run_length(s, total);
-    const int64_t pos = (int64_t)blockIdx.x * per;
-    const int64_t stop = min(pos + per, total * s.c.heads);
+    const uint32_t total = all_steps(s, at, lane);
+    const uint32_t per = run_length(s, total);
+    const uint32_t pos = blockIdx.x * per;
+    const uint32_t stop = min(pos + per, total * s.c.heads);
     if (pos >= stop) return;
-    int64_t before = 0;                 // steps of one head ahead of entry at.base
+    uint32_t before = 0;                // steps of one head ahead of entry at.base
     uint64_t past;
     while ((past = __ballot((before + at.upto) * s.c.heads > pos)) == 0) {
         before += at.all();
@@ -511,12 +500,12 @@ __device__ __forceinline__ void walk_run(const Source& s, int lane, Part&& part)
     int n = __builtin_amdgcn_readlane(at.tiles, slot_e);
     int steps = __builtin_amdgcn_readlane(at.steps, slot_e);
     before += (uint32_t)__builtin_amdgcn_readlane(at.upto, slot_e) - (uint32_t)steps;
-    const int64_t in_entry = pos - before * s.c.heads;
-    int h = __builtin_amdgcn_readfirstlane((int)quotient(in_entry, steps));
-    int tile = __builtin_amdgcn_readfirstlane((int)(in_entry - (int64_t)h * steps));
-    int64_t left = stop - pos;
+    const uint32_t in_entry = pos - before * s.c.heads;
+    int h = __builtin_amdgcn_readfirstlane(in_entry / (uint32_t)steps);
+    int tile = in_entry - h * steps;
+    int left = stop - pos;
     for (;;) {
-        const int take = __builtin_amdgcn_readfirstlane((int)min((int64_t)(steps - tile), left));
+        const int take = min(steps - tile, left);
         const int end = min(tile + take, n);
         const int e = at.base + slot_e;
         const int b = s.prefix ? 0 : s.row_groups == 1 ? e : e / s.row_groups;
@@ -545,42 +534,49 @@ __device__ __forceinline__ void walk_run(const Source& s, int lane, Part&& part)
 // is the whole unit, else a slot of the run.
 template <class T, int D>
 struct Sink {
-    const Source& s;
-    int b, h, row0;
-    bool whole, triple;
-    int64_t slot;
-    __device__ __forceinline__ Sink(const Source& src, int b_, int h_, int row0_, int tile, int end,
-                                    int n)
-        : s(src), b(b_), h(h_), row0(row0_), whole(tile == 0 && end == n),
-          triple(!whole || !src.finish),
-          slot(((int64_t)blockIdx.x * 2 + (tile > 0 ? 0 : 1)) * src.rows_per_unit) {}
-    __device__ __forceinline__ void put_ml(int r, float m, float l) const {
-        const int64_t to = whole ? RowAt(s, b, r, h).flat(s) : slot + r - row0;
-        float* ml = whole ? s.home_ml : s.broken_ml;
-        ml[2 * to] = m;
-        ml[2 * to + 1] = l;
-    }
-    __device__ __forceinline__ void put_o(int r, int dim, f4 v, float l) const {
-        if (!whole) {
-            *reinterpret_cast<f4*>(s.broken_o + (slot + r - row0) * D + dim) = v;
-            return;
-        }
-        const int64_t to = RowAt(s, b, r, h).flat(s) * D + dim;
-        if (s.finish) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            store4(static_cast<T*>(s.a.out) + to, l == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * inv);
+    T* out;            // null: a triple
+    float* o;
+    float* ml;
+    __device__ __forceinline__ Sink(const Source& s, int b, int h, int row0, bool whole,
+                                    bool behind, int r) {
+        out = nullptr;
+        if (whole) {
+            const int64_t to = RowAt(s, b, r, h).flat(s);
+            if (s.finish) out = static_cast<T*>(s.a.out) + to * D;
+            o = s.home_o + to * D;
+            ml = s.home_ml + to * 2;
         } else {
-            *reinterpret_cast<f4*>(s.home_o + to) = v;
+            const int64_t to =
+                ((int64_t)blockIdx.x * 2 + (behind ? 0 : 1)) * s.rows_per_unit + r - row0;
+            o = s.broken_o + to * D;
+            ml = s.broken_ml + to * 2;
         }
+    }
+    __device__ __forceinline__ void put(int dim, f4 v, float l) const {
+        if (out != nullptr)
+            store4(out + dim, l == 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.f / l));
+        else
+            *reinterpret_cast<f4*>(o + dim) = v;
+    }
+    __device__ __forceinline__ void put(float m, float l) const {
+        if (out == nullptr) *reinterpret_cast<Vec<float, 2>*>(ml) = Vec<float, 2>{m, l};
     }
 };
 
-// Table entry of 16 keys `sub` of a tile (any entry past the table), whether it
-// names a page, and which (0 for none).
-__device__ __forceinline__ uint32_t entry_at(const Source& s, const int32_t* table, int cols,
-                                             int tile, int sub) {
-    return (uint32_t)table[min((tile * kTile + sub * 16) >> s.page_shift, cols - 1)];
-}
+// The block table of a unit's keys: the entry of 16 keys `sub` of a tile (past
+// the table: its last).
+struct Table {
+    const int32_t* p;
+    int cols;
+    __device__ __forceinline__ Table(const Source& s, int b)
+        : p(s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride),
+          cols(s.prefix ? s.a.prefix_cols : s.a.table_cols) {}
+    __device__ __forceinline__ uint32_t of(const Source& s, int tile, int sub) const {
+        return (uint32_t)p[(uint32_t)min((tile * kTile + sub * 16) >> s.page_shift, cols - 1)];
+    }
+};
+
+// Whether an entry names a page, and which (0 for none).
 __device__ __forceinline__ bool is_page(const Source& s, uint32_t entry) {
     return entry < (uint32_t)s.c.pages;
 }
@@ -619,8 +615,8 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
         const int g = lane >> 4, r = lane & 15;
         const int in = (tile * kTile + (r >> 2) * 16) & (s.c.page_size - 1);
         const uint8_t* p = static_cast<const uint8_t*>(s.c.k) +
-                           head_of(s, page_or_0(s, entry), h, kRow) + (in + (r & 3)) * kRow +
-                           g * kChunk;
+                           head_of(s, page_or_0(s, entry), h, kRow) +
+                           (in + (r & 3)) * kRow + g * kChunk;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -632,8 +628,8 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
     __device__ __forceinline__ void load_v(const Source& s, uint32_t entry, int tile, int h,
                                            int lane) {
         const int g = lane >> 4, r = lane & 15;
-        there = is_page(s, entry);
         const uint32_t page = page_or_0(s, entry);
+        there = is_page(s, entry);
         const int in = (tile * kTile + g * 16) & (s.c.page_size - 1);
         const float* sc = s.c.scales + head_of(s, page, h, 2) + in + r;
         ks = sc[0];
@@ -723,28 +719,34 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
     // out before the queries are fetched.
     __device__ __forceinline__ void run(const Source& s, int b, int first_row, int h, int tile,
                                         int end, int stride, int lane) {
-        const int32_t* table = s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride;
-        const int cols = s.prefix ? s.a.prefix_cols : s.a.table_cols;
-        const int g = lane >> 4, ksub = (lane & 15) >> 2;
+        const int g = lane >> 4;
+        const int ksub = (lane & 15) >> 2;
+        const Table table(s, b);
+        // Loads go out unconditionally, the last tile's again behind it: under a
+        // condition they would be waited for with everything behind them.  (A
+        // second copy of the step, or of the loads, costs more in instruction
+        // fetches; scalar loads of the table doubled short calls.)
+        const int last = end - 1 - (end - 1 - tile) % stride;
+        auto next_of = [&](int t) { return t + stride < end ? t + stride : last; };
         uint32_t ke = 0, ve = 0;
         if (tile < end) {
-            ke = entry_at(s, table, cols, tile, ksub);
-            ve = entry_at(s, table, cols, tile, g);
-            load_k(s, ke, tile, h, lane);
-            load_v(s, ve, tile, h, lane);
+            const uint32_t k0 = table.of(s, tile, ksub), v0 = table.of(s, tile, g);
+            ke = table.of(s, next_of(tile), ksub);
+            ve = table.of(s, next_of(tile), g);
+            load_k(s, k0, tile, h, lane);
+            load_v(s, v0, tile, h, lane);
         }
         this->load(s, b, first_row, h, lane, [&](int u) {
             constexpr int per = kChunk / BITS;
             return ((u / per) * 4 * kChunk + g * kChunk) * 8 / BITS + (u % per) * 8;
         });
         for (; tile < end; tile += stride) {
-            const int next = tile + stride;
-            if (next < end) {
-                ke = entry_at(s, table, cols, next, ksub);
-                ve = entry_at(s, table, cols, next, g);
-            }
-            step(tile, lane, [&] { if (next < end) load_k(s, ke, next, h, lane); },
-                 [&] { if (next < end) load_v(s, ve, next, h, lane); });
+            const int next = next_of(tile), then = next_of(next);
+            const uint32_t k2 = table.of(s, then, ksub), v2 = table.of(s, then, g);
+            step(tile, lane, [&] { load_k(s, ke, next, h, lane); },
+                 [&] { load_v(s, ve, next, h, lane); });
+            ke = k2;
+            ve = v2;
         }
     }
 };
@@ -774,7 +776,6 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
                            [&](int dim, f4 x) { *reinterpret_cast<f4*>(&sm_o[wave][r][dim]) = x; });
         }
         __syncthreads();
-        const Sink<T, D> sink(s, b, h, row0, tile, end, n);
         const int rows = min(kRows, s.rows - row0);
         for (int i = threadIdx.x; i < rows * (D / 4); i += kBlock) {
             const int r = i / (D / 4), dim = i % (D / 4) * 4;
@@ -788,8 +789,9 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
                 sum += sm_l[v][r] * keep;
                 x += *reinterpret_cast<const f4*>(&sm_o[v][r][dim]) * keep;
             }
-            if (sink.triple && dim == 0) sink.put_ml(row0 + r, top, sum);
-            sink.put_o(row0 + r, dim, x, sum);
+            const Sink<T, D> sink(s, b, h, row0, tile == 0 && end == n, tile > 0, row0 + r);
+            if (dim == 0) sink.put(top, sum);
+            sink.put(dim, x, sum);
         }
         __syncthreads();
     });
@@ -817,19 +819,17 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
     u4 kq[kEach], vq[kEach];
 
     walk_run(s, lane, [&](int b, int h, int row0, int tile, int end, int n) {
-        const int32_t* table = s.prefix ? s.a.prefix_table : s.a.table + b * s.a.table_stride;
-        const int cols = s.prefix ? s.a.prefix_cols : s.a.table_cols;
+        const Table table(s, b);
         const int mine = row0 + 32 * wave;
         const bool live = mine < s.rows;
-        // pieces of a tile: K's by key and part, V's by 16 keys and row; their
-        // table entries are looked up a tile ahead
+        // pieces of a tile: K's by key and part, V's by 16 keys and row
         uint32_t ke[kEach], ve[kEach], se;
         auto look_up = [&](int t) {
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const int c = threadIdx.x + i * kThreads;
-                ke[i] = entry_at(s, table, cols, t, min(c / kParts, kTile - 1) >> 4);
-                ve[i] = entry_at(s, table, cols, t, min(c / kRow, 3));
+                ke[i] = table.of(s, t, c / kParts >> 4 & 3);
+                ve[i] = table.of(s, t, c / kRow & 3);
             }
         };
         auto fetch = [&](int t) {
@@ -901,65 +901,92 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
             ks = sc[0];
             vs = sc[s.c.page_size];
         };
+        // (loads go out unconditionally, past the end for the last tile again:
+        // under a condition they would be waited for with everything behind)
+        se = table.of(s, tile, g);
         look_up(tile);
-        se = entry_at(s, table, cols, tile, g);
-        fetch(tile);
         fetch_scales(tile);
-        if (tile + 1 < end) look_up(tile + 1);
+        fetch(tile);
+        look_up(min(tile + 1, end - 1));
         if (live) rows.load(s, b, mine, h, lane, [&](int u) { return u * 32 + g * 8; });
         spread(0);
-        if (tile + 1 < end) fetch(tile + 1);
+        fetch(min(tile + 1, end - 1));
         __syncthreads();
         for (int t = tile; t < end; ++t) {
-            const int buf = (t - tile) & 1;
-            if (t + 2 < end) look_up(t + 2);
-            if (t + 1 < end) se = entry_at(s, table, cols, t + 1, g);
+            const int buf = (t - tile) & 1, t1 = min(t + 1, end - 1), t2 = min(t + 2, end - 1);
+            se = table.of(s, t1, g);
+            look_up(t2);
+            h8 w[NB][2];
             if (live) {
                 f4 sc[NB][4];
+                h8 k[2][4];
+                // reads four at a time, a group ahead of their products
+                constexpr int kU = D / 32;
+                auto read_k = [&](int group) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = (4 * group + j) / kU, u = (4 * group + j) % kU;
+                        k[group & 1][j] = *reinterpret_cast<const h8*>(
+                            &sm_k[buf][16 * i + r16][u * 32 + g * 8]);
+                    }
+                };
+                read_k(0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int rb = 0; rb < NB; ++rb) sc[rb][i] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int u = 0; u < D / 32; ++u) {
-                        const h8 k = *reinterpret_cast<const h8*>(
-                            &sm_k[buf][16 * i + r16][u * 32 + g * 8]);
+                for (int group = 0; group < kU; ++group) {
+                    if (group < kU - 1) read_k(group + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = (4 * group + j) / kU, u = (4 * group + j) % kU;
 #pragma unroll
                         for (int rb = 0; rb < NB; ++rb)
                             sc[rb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                k, rows.q[rb][u], sc[rb][i], 0, 0, 0);
+                                k[group & 1][j], rows.q[rb][u], sc[rb][i], 0, 0, 0);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                h8 w[NB][2];
                 rows.weights(sc, ks, vs, there, t, lane, w);
-                if (t + 1 < end) fetch_scales(t + 1);
+            }
+            fetch_scales(t1);
+            if (live) {
+                h8 v[2][4];
+                auto read_v = [&](int i) {
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
+                    for (int j = 0; j < 4; ++j)
+                        v[i & 1][j] = *reinterpret_cast<const h8*>(
+                            &sm_v[buf][16 * (2 * i + j / 2) + r16][g * 16 + (j & 1) * 8]);
+                };
+                read_v(0);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const h8 v = *reinterpret_cast<const h8*>(
-                            &sm_v[buf][16 * i + r16][g * 16 + u * 8]);
+                for (int i = 0; i < D / 32; ++i) {
+                    if (i < D / 32 - 1) read_v(i + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int rb = 0; rb < NB; ++rb)
-                            rows.o[rb][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                v, w[rb][u], rows.o[rb][i], 0, 0, 0);
-                    }
+                            rows.o[rb][2 * i + j / 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                v[i & 1][j], w[rb][j & 1], rows.o[rb][2 * i + j / 2], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
-            if (t + 1 < end) {
-                spread(buf ^ 1);
-                if (t + 2 < end) fetch(t + 2);
-            }
+            spread(buf ^ 1);
+            fetch(t2);
             __syncthreads();
         }
         if (live) {
-            const Sink<T, D> sink(s, b, h, row0, tile, end, n);
 #pragma unroll
             for (int rb = 0; rb < NB; ++rb) {
                 const int r = mine + 16 * rb + r16;
                 const float l = quad_sum(rows.l[rb]);
                 if (r < s.rows) {
-                    if (sink.triple && lane < 16) sink.put_ml(r, rows.reference(rb), l);
-                    rows.each_four(rb, lane, [&](int dim, f4 v) { sink.put_o(r, dim, v, l); });
+                    const Sink<T, D> sink(s, b, h, row0, tile == 0 && end == n, tile > 0, r);
+                    if (lane < 16) sink.put(rows.reference(rb), l);
+                    rows.each_four(rb, lane, [&](int dim, f4 v) { sink.put(dim, v, l); });
                 }
             }
         }
@@ -983,18 +1010,18 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
     const int h = unit % own.c.heads, b = unit / own.c.heads;
     if (b >= a.batch) return;                       // uniform over the wave
 
-    // a source's triples of the row at `local` in its unit: in runs run,
-    // run + 1, ..., or in the row's home
+    // a source's triples of a row: the first, and from the second on rows a step
+    // apart; `home` if the row was finished in one run
     struct Parts {
         int count = 0;
         bool home = false;
-        int64_t run = 0;
+        uint32_t run = 0;
     };
     auto parts_of = [&](const Source& s, int entry) {
         Parts p;
         Entries at(s, 0, lane);
-        const int64_t per = run_length(s, all_steps(s, at, lane));
-        int64_t before = 0;
+        const uint32_t per = run_length(s, all_steps(s, at, lane));
+        uint32_t before = 0;
         while (at.base + 64 <= entry) {
             before += at.all();
             at = Entries(s, at.base + 64, lane);
@@ -1003,11 +1030,15 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
         if (n == 0) return p;
         const int steps = __builtin_amdgcn_readlane(at.steps, entry - at.base);
         before += (uint32_t)__builtin_amdgcn_readlane(at.upto, entry - at.base) - (uint32_t)steps;
-        const int64_t from = before * s.c.heads + (int64_t)h * steps;
-        p.run = quotient(from, per);
-        p.count = (int)(quotient(from + n - 1, per) - p.run) + 1;
+        const uint32_t from = before * s.c.heads + h * steps;
+        p.run = from / per;
+        p.count = (int)((from + n - 1) / per - p.run) + 1;
         p.home = p.count == 1;
         return p;
+    };
+    // rows, counted from the source's first triple, of a row's triple i
+    auto slot_of = [&](const Source& s, const Parts& p, int i, int local) {
+        return ((int64_t)(p.run + i) * 2 + (i == 0 ? 1 : 0)) * s.rows_per_unit + local;
     };
     const Parts mine = parts_of(own, b * own.row_groups + r0 / own.rows_per_unit);
     if (own.finish && mine.home) return;
@@ -1025,14 +1056,15 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
         }
         const int count = mine.count + pre.count;
         auto at = [&](int i, const float*& o, const float*& ml) {
-            const bool first = i < mine.count;
-            const Source& s = first ? own : ahead;
-            const Parts& p = first ? mine : pre;
-            if (!first) i -= mine.count;
-            const int64_t x = p.home ? row : ((p.run + i) * 2 + (i == 0 ? 1 : 0)) * s.rows_per_unit +
-                                                 (first ? own_local : pre_local);
-            o = (p.home ? s.home_o : s.broken_o) + x * D;
-            ml = (p.home ? s.home_ml : s.broken_ml) + x * 2;
+            const bool first = i < mine.count, home = first ? mine.home : pre.home;
+            const int64_t x = home ? row : first ? slot_of(own, mine, i, own_local)
+                                                 : slot_of(ahead, pre, i - mine.count, pre_local);
+            const float* os = home ? (first ? own.home_o : ahead.home_o)
+                                   : (first ? own.broken_o : ahead.broken_o);
+            const float* ms = home ? (first ? own.home_ml : ahead.home_ml)
+                                   : (first ? own.broken_ml : ahead.broken_ml);
+            o = os + x * D;
+            ml = ms + x * 2;
         };
         float ref = kNegInf, sum = 0.f;
         VE acc = {};
@@ -1113,6 +1145,7 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
     const int64_t entries = (int64_t)s.row_groups * (prefix ? 1 : a.batch);
     const __int128 steps = (__int128)((keys + kTile - 1) / kTile + s.quantum + s.cost) * entries *
                            c.heads;
+    s.fits = steps + (__int128)kCus * 8 * s.quantum < ((__int128)1 << 31);
     const int64_t room = (int64_t)kCus * shape->resident;
     const __int128 most = steps / s.quantum;
     s.runs = (uint32_t)(most < room ? (int64_t)most : room);
@@ -1179,6 +1212,7 @@ int64_t attention_workspace(const cq_kv_cache_t& c, const cq_attention_t& a) {
     Shape os{}, as{};
     Source own = source_of(c, a, false, &os), ahead{};
     if (a.prefix_len > 0) ahead = source_of(c, a, true, &as);
+    if (!own.fits || (ahead.rows > 0 && !ahead.fits)) return -1;
     return lay_out(c, a, &own, &ahead, nullptr);
 }
 

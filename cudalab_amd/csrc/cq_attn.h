@@ -31,6 +31,7 @@ hipError_t launch_kv_append(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int 
 hipError_t launch_kv_read(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int dtype,
                           void* k_out, void* v_out, hipStream_t stream);
 
+// Bytes, or -1 for a call whose tables span more tiles than 31 bits count.
 int64_t attention_workspace(const cq_kv_cache_t& c, const cq_attention_t& a);
 hipError_t launch_attention(const cq_kv_cache_t& c, const cq_attention_t& a,
                             hipStream_t stream);

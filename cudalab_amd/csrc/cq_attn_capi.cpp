@@ -269,6 +269,9 @@ int check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launch
     if (a.table_cols < 1) return invalid("table_cols must be >= 1");
     if (std::isnan(a.softmax_scale) || std::isinf(a.softmax_scale))
         return invalid("softmax_scale must be finite");
+    const int64_t need = cq::attention_workspace(c, a);
+    if (need < 0)
+        return invalid("the tables' tokens times batch, rows and heads are too many for one call");
     if (!launching) return CQ_OK;
     if ((st = check_table(a.table, a.table_stride, a.table_cols, a.batch)) != CQ_OK) return st;
     if (a.q == nullptr || a.out == nullptr || a.lengths == nullptr ||
@@ -280,7 +283,6 @@ int check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launch
     for (int64_t n : {a.q_batch_stride, a.q_token_stride, a.q_head_stride})
         if (n < 0 || n > (int64_t)1 << 40 || n % 8 != 0)
             return invalid("q's strides must be multiples of 8 in [0, 2^40]");
-    const int64_t need = cq::attention_workspace(c, a);
     if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need || !aligned(a.workspace, 16)))
         return cq::set_error(CQ_ERR_BUFFER_TOO_SMALL,
                              "the call needs " + std::to_string(need) +
