@@ -79,12 +79,40 @@ struct Source {
     uint32_t runs;         // workgroups
     int32_t fits;          // the deal's sums fit 31 bits
     int32_t finish;        // 1: units of one run write `out`; 0: their home
-    // workspace: triples of broken units, two per run, and of whole units
+    // workspace: which runs have a unit's triples (first run and how many; none
+    // for a unit without keys); triples of broken units, two per run, and of
+    // whole units
+    uint32_t* where;       // [entries * heads, 2]
     float* broken_o;       // [runs * 2 * rows_per_unit, D]
     float* broken_ml;      // [.., 2]
     float* home_o;         // [batch * tokens * q_heads, D]
     float* home_ml;
 };
+
+// ------------------------------------------------- over a wave
+// Maximum and sum over the four lanes l, l + 16, l + 32, l + 48, in each.
+template <class F>
+__device__ __forceinline__ float quad_fold(float v, F&& f) {
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const uint32_t y = __float_as_uint(v);
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_max(float v) {
+    return quad_fold(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    return quad_fold(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, row_dpp<0x128>(v));
+    v = fmaxf(v, row_dpp<0x124>(v));
+    v = fmaxf(v, row_dpp<0x122>(v));
+    v = fmaxf(v, row_dpp<0x121>(v));
+    return quad_max(v);
+}
 
 // -------------------------------------------------------------- the units
 __device__ __forceinline__ int new_tokens(const cq_attention_t& a, int b) {
@@ -145,20 +173,50 @@ struct Entries {
         steps = steps_of(s, tiles);
         upto = wave_scan(steps);
     }
+    __device__ __forceinline__ void count_units() {
+        steps = tiles > 0;
+        upto = wave_scan(steps);
+    }
     __device__ __forceinline__ uint32_t all() const { return __builtin_amdgcn_readlane(upto, 63); }
 };
 
-// Steps of all units of one head; `first` holds entries 0 .. 63.  (The host
-// sees to it that the steps of all heads stay below 2^31.)
-__device__ __forceinline__ uint32_t all_steps(const Source& s, const Entries& first, int lane) {
-    uint32_t total = first.all();
-    for (int base = 64; base < entries_of(s); base += 64) total += Entries(s, base, lane).all();
-    return total;
-}
+// How a source's units are dealt to the runs: in equal numbers of steps, or,
+// where that leaves hardly more to the longest run, in whole units: those need
+// no joining.  (The host sees to it that the steps of all heads stay below 2^31.)
+struct Deal {
+    bool whole;
+    uint32_t all;      // steps or units of all heads
+    uint32_t per;      // of a run
+};
 
-__device__ __forceinline__ uint32_t run_length(const Source& s, uint32_t total) {
-    const uint32_t each = (total * s.c.heads + s.runs - 1) / s.runs, q = s.quantum;
-    return (max(1u, each) + q - 1) / q * q;
+// `at`: entries 0 .. 63; afterwards counts units if those are dealt.
+__device__ __forceinline__ Deal deal(const Source& s, Entries& at, int lane) {
+    const uint32_t heads = s.c.heads;
+    uint32_t steps = 0, units = 0, most = 0;
+    for (int base = 0;;) {
+        const Entries e = base == 0 ? at : Entries(s, base, lane);
+        steps += e.all();
+        units += __builtin_popcountll(__ballot(e.tiles > 0));
+        most = max(most, (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_max((float)e.steps)));
+        // units without keys are no run's: any workgroup notes them
+        if (threadIdx.x < 64 && base + lane < entries_of(s) && e.tiles == 0 &&
+            (uint32_t)(base + lane) % s.runs == blockIdx.x)
+            for (uint32_t h = 0; h < heads; ++h) s.where[((base + lane) * heads + h) * 2 + 1] = 0;
+        base += 64;
+        if (base >= entries_of(s)) break;
+    }
+    Deal d;
+    const uint32_t q = s.quantum;
+    d.all = steps * heads;
+    d.per = (max(1u, (d.all + s.runs - 1) / s.runs) + q - 1) / q * q;
+    const uint32_t each = (units * heads + s.runs - 1) / s.runs;
+    d.whole = each * most <= d.per + d.per / 8;
+    if (d.whole) {
+        d.all = units * heads;
+        d.per = max(1u, each);
+        at.count_units();
+    }
+    return d;
 }
 
 // ----------------------------------------------------------- small pieces
@@ -193,30 +251,6 @@ __device__ __forceinline__ void codes_of_nibbles(uint32_t w, uint32_t (&p)[4]) {
     p[1] = less((w & 0x00F000F0u) ^ 0x54805480u, 72.f);
     p[2] = less((x & 0x000F000Fu) ^ 0x64086408u, 1032.f);
     p[3] = less((x & 0x00F000F0u) ^ 0x54805480u, 72.f);
-}
-
-// Maximum and sum over the four lanes l, l + 16, l + 32, l + 48, in each.
-template <class F>
-__device__ __forceinline__ float quad_fold(float v, F&& f) {
-    const uint32_t x = __float_as_uint(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const uint32_t y = __float_as_uint(v);
-    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
-    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float quad_max(float v) {
-    return quad_fold(v, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float quad_sum(float v) {
-    return quad_fold(v, [](float a, float b) { return a + b; });
-}
-__device__ __forceinline__ float wave_max(float v) {
-    v = fmaxf(v, row_dpp<0x128>(v));
-    v = fmaxf(v, row_dpp<0x124>(v));
-    v = fmaxf(v, row_dpp<0x122>(v));
-    v = fmaxf(v, row_dpp<0x121>(v));
-    return quad_max(v);
 }
 
 // What a triple's sums are multiplied with to stand at reference `top`.  One
@@ -484,42 +518,51 @@ struct Rows {
 template <class Part>
 __device__ __forceinline__ void walk_run(const Source& s, int lane, Part&& part) {
     Entries at(s, 0, lane);
-    const uint32_t total = all_steps(s, at, lane);
-    const uint32_t per = run_length(s, total);
-    const uint32_t pos = blockIdx.x * per;
-    const uint32_t stop = min(pos + per, total * s.c.heads);
+    const Deal d = deal(s, at, lane);
+    uint32_t pos = blockIdx.x * d.per;
+    const uint32_t stop = min(pos + d.per, d.all), heads = s.c.heads;
     if (pos >= stop) return;
+    auto next_entries = [&] {
+        at = Entries(s, at.base + 64, lane);
+        if (d.whole) at.count_units();
+    };
     uint32_t before = 0;                // steps of one head ahead of entry at.base
     uint64_t past;
-    while ((past = __ballot((before + at.upto) * s.c.heads > pos)) == 0) {
+    while ((past = __ballot((before + at.upto) * heads > pos)) == 0) {
         before += at.all();
         if (at.base + 64 >= entries_of(s)) return;
-        at = Entries(s, at.base + 64, lane);
+        next_entries();
     }
     int slot_e = __builtin_ctzll(past);
     int n = __builtin_amdgcn_readlane(at.tiles, slot_e);
     int steps = __builtin_amdgcn_readlane(at.steps, slot_e);
     before += (uint32_t)__builtin_amdgcn_readlane(at.upto, slot_e) - (uint32_t)steps;
-    const uint32_t in_entry = pos - before * s.c.heads;
+    const uint32_t in_entry = pos - before * heads;
     int h = __builtin_amdgcn_readfirstlane(in_entry / (uint32_t)steps);
     int tile = in_entry - h * steps;
-    int left = stop - pos;
     for (;;) {
-        const int take = min(steps - tile, left);
-        const int end = min(tile + take, n);
+        const int take = min(steps - tile, (int)(stop - pos));
+        const int end = d.whole ? n : min(tile + take, n);
         const int e = at.base + slot_e;
         const int b = s.prefix ? 0 : s.row_groups == 1 ? e : e / s.row_groups;
         // (a unit's cost alone may be what is left of it)
-        if (tile < end) part(b, h, (e - b * s.row_groups) * s.rows_per_unit, tile, end, n);
-        left -= take;
-        if (left <= 0) return;
+        if (tile < end) {
+            if (tile == 0 && threadIdx.x == 0) {
+                uint32_t* w = s.where + (e * heads + h) * 2;
+                w[0] = blockIdx.x;
+                w[1] = d.whole ? 1 : (pos + n - 1) / d.per - blockIdx.x + 1;
+            }
+            part(b, h, (e - b * s.row_groups) * s.rows_per_unit, tile, end, n);
+        }
+        pos += take;
+        if (pos >= stop) return;
         tile = 0;
         if (++h == s.c.heads) {
             h = 0;
             do {
                 if (++slot_e == 64) {
                     if (at.base + 64 >= entries_of(s)) return;
-                    at = Entries(s, at.base + 64, lane);
+                    next_entries();
                     slot_e = 0;
                 }
                 if (at.base + slot_e >= entries_of(s)) return;
@@ -996,7 +1039,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
 // Joins the triples of rows: those of their own keys' runs and, with a prefix,
 // those of the prefix's.  One wave per `each` rows of a unit.  Rows that a run
 // has finished are left alone; rows without any keys become zeros.
-constexpr int kJoin = 8;                // triples in flight
+constexpr int kJoin = 16;               // triples in flight
 template <class T, int D>
 __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, int each) {
     constexpr int E = D / 64;
@@ -1010,38 +1053,21 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
     const int h = unit % own.c.heads, b = unit / own.c.heads;
     if (b >= a.batch) return;                       // uniform over the wave
 
-    // a source's triples of a row: the first, and from the second on rows a step
-    // apart; `home` if the row was finished in one run
+    // the runs that have a unit's triples
     struct Parts {
-        int count = 0;
-        bool home = false;
         uint32_t run = 0;
+        int count = 0;
     };
     auto parts_of = [&](const Source& s, int entry) {
-        Parts p;
-        Entries at(s, 0, lane);
-        const uint32_t per = run_length(s, all_steps(s, at, lane));
-        uint32_t before = 0;
-        while (at.base + 64 <= entry) {
-            before += at.all();
-            at = Entries(s, at.base + 64, lane);
-        }
-        const int n = __builtin_amdgcn_readlane(at.tiles, entry - at.base);
-        if (n == 0) return p;
-        const int steps = __builtin_amdgcn_readlane(at.steps, entry - at.base);
-        before += (uint32_t)__builtin_amdgcn_readlane(at.upto, entry - at.base) - (uint32_t)steps;
-        const uint32_t from = before * s.c.heads + h * steps;
-        p.run = from / per;
-        p.count = (int)((from + n - 1) / per - p.run) + 1;
-        p.home = p.count == 1;
-        return p;
+        const uint32_t* w = s.where + (entry * (uint32_t)s.c.heads + h) * 2;
+        return Parts{w[0], (int)w[1]};
     };
     // rows, counted from the source's first triple, of a row's triple i
     auto slot_of = [&](const Source& s, const Parts& p, int i, int local) {
         return ((int64_t)(p.run + i) * 2 + (i == 0 ? 1 : 0)) * s.rows_per_unit + local;
     };
     const Parts mine = parts_of(own, b * own.row_groups + r0 / own.rows_per_unit);
-    if (own.finish && mine.home) return;
+    if (own.finish && mine.count == 1) return;
     for (int r = r0; r < min(r0 + each, own.rows); ++r) {
         const int t = r / own.group;
         const int64_t row = ((int64_t)b * a.tokens + t) * a.q_heads + h * own.group +
@@ -1056,7 +1082,7 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
         }
         const int count = mine.count + pre.count;
         auto at = [&](int i, const float*& o, const float*& ml) {
-            const bool first = i < mine.count, home = first ? mine.home : pre.home;
+            const bool first = i < mine.count, home = (first ? mine.count : pre.count) == 1;
             const int64_t x = home ? row : first ? slot_of(own, mine, i, own_local)
                                                  : slot_of(ahead, pre, i - mine.count, pre_local);
             const float* os = home ? (first ? own.home_o : ahead.home_o)
@@ -1156,6 +1182,7 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
 int64_t lay_out(const cq_kv_cache_t& c, const cq_attention_t& a, Source* own, Source* ahead,
                 char* base) {
     int64_t used = 0;
+    const int64_t heads = c.heads;
     auto take = [&](int64_t rows, float** o, float** ml) {
         *o = reinterpret_cast<float*>(base + used);
         used += rows * c.head_dim * 4;
@@ -1166,6 +1193,8 @@ int64_t lay_out(const cq_kv_cache_t& c, const cq_attention_t& a, Source* own, So
     for (Source* s : {own, ahead}) {
         if (s->rows == 0) continue;
         take((int64_t)s->runs * 2 * s->rows_per_unit, &s->broken_o, &s->broken_ml);
+        s->where = reinterpret_cast<uint32_t*>(base + used);
+        used += ((int64_t)s->row_groups * (s->prefix ? 1 : a.batch) * heads * 8 + 15) / 16 * 16;
         if (!s->finish) take(all, &s->home_o, &s->home_ml);
     }
     return used;
