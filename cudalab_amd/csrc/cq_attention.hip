@@ -83,10 +83,11 @@ struct Source {
     // for a unit without keys); triples of broken units, two per run, and of
     // whole units
     uint32_t* where;       // [entries * heads, 2]
-    float* broken_o;       // [runs * 2 * rows_per_unit, D]
-    float* broken_ml;      // [.., 2]
-    float* home_o;         // [batch * tokens * q_heads, D]
-    float* home_ml;
+    // runs * 2 * rows_per_unit of broken units from row `broken`, batch *
+    // tokens * q_heads of whole ones from row `home` of both arrays
+    float* o;              // [.., D]
+    float* ml;             // [.., 2]
+    int64_t broken, home;
 };
 
 // ------------------------------------------------- over a wave
@@ -583,17 +584,15 @@ struct Sink {
     __device__ __forceinline__ Sink(const Source& s, int b, int h, int row0, bool whole,
                                     bool behind, int r) {
         out = nullptr;
+        int64_t to = s.broken + ((int64_t)blockIdx.x * 2 + (behind ? 0 : 1)) * s.rows_per_unit +
+                     r - row0;
         if (whole) {
-            const int64_t to = RowAt(s, b, r, h).flat(s);
-            if (s.finish) out = static_cast<T*>(s.a.out) + to * D;
-            o = s.home_o + to * D;
-            ml = s.home_ml + to * 2;
-        } else {
-            const int64_t to =
-                ((int64_t)blockIdx.x * 2 + (behind ? 0 : 1)) * s.rows_per_unit + r - row0;
-            o = s.broken_o + to * D;
-            ml = s.broken_ml + to * 2;
+            const int64_t row = RowAt(s, b, r, h).flat(s);
+            if (s.finish) out = static_cast<T*>(s.a.out) + row * D;
+            to = s.home + row;
         }
+        o = s.o + to * D;
+        ml = s.ml + to * 2;
     }
     __device__ __forceinline__ void put(int dim, f4 v, float l) const {
         if (out != nullptr)
@@ -1037,21 +1036,25 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
 }
 
 // Joins the triples of rows: those of their own keys' runs and, with a prefix,
-// those of the prefix's.  One wave per `each` rows of a unit.  Rows that a run
-// has finished are left alone; rows without any keys become zeros.
-constexpr int kJoin = 16;               // triples in flight
-template <class T, int D>
+// those of the prefix's.  `W` waves per row, each its share of the triples, and
+// `each` rows of a unit in turn.  Rows that a run has finished are left alone;
+// rows without any keys become zeros.
+template <int D>
+constexpr int in_flight = D == 256 ? 8 : 16;       // triples
+template <class T, int D, int W>
 __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, int each) {
-    constexpr int E = D / 64;
+    constexpr int E = D / 64, J = in_flight<D>;
     using VE = Vec<float, E>;
+    __shared__ float part[W > 1 ? W : 1][W > 1 ? D + 2 : 1];
     const int lane = threadIdx.x & 63;
     const cq_attention_t& a = own.a;
     const uint32_t blocks = (own.rows + each - 1) / each;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-    const uint32_t unit = wave / blocks;
-    const int r0 = (wave - unit * blocks) * each;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t place = W == 1 ? blockIdx.x * kWaves + w : blockIdx.x;
+    const uint32_t unit = place / blocks;
+    const int r0 = (place - unit * blocks) * each;
     const int h = unit % own.c.heads, b = unit / own.c.heads;
-    if (b >= a.batch) return;                       // uniform over the wave
+    if (b >= a.batch) return;          // uniform over the wave (W = 1) or workgroup
 
     // the runs that have a unit's triples
     struct Parts {
@@ -1059,12 +1062,8 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
         int count = 0;
     };
     auto parts_of = [&](const Source& s, int entry) {
-        const uint32_t* w = s.where + (entry * (uint32_t)s.c.heads + h) * 2;
-        return Parts{w[0], (int)w[1]};
-    };
-    // rows, counted from the source's first triple, of a row's triple i
-    auto slot_of = [&](const Source& s, const Parts& p, int i, int local) {
-        return ((int64_t)(p.run + i) * 2 + (i == 0 ? 1 : 0)) * s.rows_per_unit + local;
+        const uint32_t* at = s.where + (entry * (uint32_t)s.c.heads + h) * 2;
+        return Parts{at[0], (int)at[1]};
     };
     const Parts mine = parts_of(own, b * own.row_groups + r0 / own.rows_per_unit);
     if (own.finish && mine.count == 1) return;
@@ -1072,54 +1071,81 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
         const int t = r / own.group;
         const int64_t row = ((int64_t)b * a.tokens + t) * a.q_heads + h * own.group +
                             (r - t * own.group);
-        const int own_local = r % own.rows_per_unit;
         Parts pre;
-        int pre_local = 0;
+        // where a source's triples start: one at home, or the first run's last
+        // row block and every next one's first
+        auto start_of = [&](const Source& s, const Parts& p, int local) {
+            return p.count == 1 ? s.home + row
+                                : s.broken + (int64_t)p.run * 2 * s.rows_per_unit + local;
+        };
+        const int64_t at_mine = start_of(own, mine, r % own.rows_per_unit);
+        int64_t at_pre = 0;
+        int pre_rows = 0;
         if (!own.finish) {
             const int pr = b * own.rows + r;
             pre = parts_of(ahead, pr / ahead.rows_per_unit);
-            pre_local = pr % ahead.rows_per_unit;
+            pre_rows = ahead.rows_per_unit;
+            at_pre = start_of(ahead, pre, pr % pre_rows);
         }
         const int count = mine.count + pre.count;
-        auto at = [&](int i, const float*& o, const float*& ml) {
-            const bool first = i < mine.count, home = (first ? mine.count : pre.count) == 1;
-            const int64_t x = home ? row : first ? slot_of(own, mine, i, own_local)
-                                                 : slot_of(ahead, pre, i - mine.count, pre_local);
-            const float* os = home ? (first ? own.home_o : ahead.home_o)
-                                   : (first ? own.broken_o : ahead.broken_o);
-            const float* ms = home ? (first ? own.home_ml : ahead.home_ml)
-                                   : (first ? own.broken_ml : ahead.broken_ml);
-            o = os + x * D;
-            ml = ms + x * 2;
+        auto triple = [&](int i) {
+            const bool first = i < mine.count;
+            const int j = first ? i : i - mine.count;
+            const int n = first ? mine.count : pre.count;
+            const int step = first ? own.rows_per_unit : pre_rows;
+            const int64_t from = first ? at_mine : at_pre;
+            return from + (n == 1 ? 0 : (j == 0 ? 1 : 2 * j) * step);
         };
         float ref = kNegInf, sum = 0.f;
         VE acc = {};
-        for (int base = 0; base < count; base += kJoin) {
-            VE v[kJoin];
-            float m[kJoin], l[kJoin];
-            float top = ref;
+        for (int base = W == 1 ? 0 : w * J; base < count; base += W * J) {
+            // a triple's reference and sum to a lane, its row over the wave
+            const Vec<float, 2> ml = *reinterpret_cast<const Vec<float, 2>*>(
+                own.ml + triple(min(base + min(lane, J - 1), count - 1)) * 2);
+            VE v[J];
 #pragma unroll
-            for (int i = 0; i < kJoin; ++i) {
-                const float *o, *ml;
-                at(min(base + i, count - 1), o, ml);
-                v[i] = *reinterpret_cast<const VE*>(o + lane * E);
-                m[i] = ml[0];
-                l[i] = ml[1];
-            }
-#pragma unroll
-            for (int i = 0; i < kJoin; ++i) top = fmaxf(top, m[i]);
+            for (int i = 0; i < J; ++i)
+                v[i] = *reinterpret_cast<const VE*>(
+                    own.o + triple(min(base + i, count - 1)) * D + lane * E);
+            const float top = fmaxf(ref, wave_max(ml[0]));
             const float keep = factor(ref, sum, top);
+            const float by = factor(ml[0], ml[1], top);
+            const float share = by * ml[1];
             sum *= keep;
 #pragma unroll
             for (int j = 0; j < E; ++j) acc[j] *= keep;
             ref = top;
 #pragma unroll
-            for (int i = 0; i < kJoin; ++i) {
-                if (base + i >= count) break;
-                const float by = factor(m[i], l[i], top);
-                sum += by * l[i];
+            for (int i = 0; i < J; ++i) {
+                const bool more = base + i < count;
+                const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), i));
+                const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), i));
+                sum += more ? g : 0.f;
 #pragma unroll
-                for (int j = 0; j < E; ++j) acc[j] += v[i][j] * by;
+                for (int j = 0; j < E; ++j) acc[j] += more ? v[i][j] * f : 0.f;
+            }
+        }
+        if constexpr (W > 1) {
+            if (r > r0) __syncthreads();
+#pragma unroll
+            for (int j = 0; j < E; ++j) part[w][lane * E + j] = acc[j];
+            if (lane == 0) {
+                part[w][D] = ref;
+                part[w][D + 1] = sum;
+            }
+            __syncthreads();
+            if (w > 0) continue;
+            float top = ref;
+#pragma unroll
+            for (int i = 1; i < W; ++i) top = fmaxf(top, part[i][D]);
+            sum = 0.f;
+            acc = VE{};
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float by = factor(part[i][D], part[i][D + 1], top);
+                sum += by * part[i][D + 1];
+#pragma unroll
+                for (int j = 0; j < E; ++j) acc[j] += by * part[i][lane * E + j];
             }
         }
         T* out = static_cast<T*>(a.out) + row * D + lane * E;
@@ -1181,21 +1207,23 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
 // Lays out the workspace from `base` (null: only sizes); returns its bytes.
 int64_t lay_out(const cq_kv_cache_t& c, const cq_attention_t& a, Source* own, Source* ahead,
                 char* base) {
-    int64_t used = 0;
-    const int64_t heads = c.heads;
-    auto take = [&](int64_t rows, float** o, float** ml) {
-        *o = reinterpret_cast<float*>(base + used);
-        used += rows * c.head_dim * 4;
-        *ml = reinterpret_cast<float*>(base + used);
-        used += (rows * 8 + 15) / 16 * 16;
-    };
     const int64_t all = (int64_t)a.batch * a.tokens * a.q_heads;
+    int64_t triples = 0;
     for (Source* s : {own, ahead}) {
         if (s->rows == 0) continue;
-        take((int64_t)s->runs * 2 * s->rows_per_unit, &s->broken_o, &s->broken_ml);
+        s->broken = triples;
+        triples += (int64_t)s->runs * 2 * s->rows_per_unit;
+        s->home = triples;
+        if (!s->finish) triples += all;
+    }
+    int64_t used = triples * (c.head_dim + 2) * 4;
+    used = (used + 15) / 16 * 16;
+    for (Source* s : {own, ahead}) {
+        if (s->rows == 0) continue;
+        s->o = reinterpret_cast<float*>(base);
+        s->ml = reinterpret_cast<float*>(base + triples * c.head_dim * 4);
         s->where = reinterpret_cast<uint32_t*>(base + used);
-        used += ((int64_t)s->row_groups * (s->prefix ? 1 : a.batch) * heads * 8 + 15) / 16 * 16;
-        if (!s->finish) take(all, &s->home_o, &s->home_ml);
+        used += ((int64_t)s->row_groups * (s->prefix ? 1 : a.batch) * c.heads * 8 + 15) / 16 * 16;
     }
     return used;
 }
@@ -1229,9 +1257,19 @@ hipError_t launch_typed(const Source& own, Shape os, const Source& ahead, Shape 
     // with eight); of few rows most have triples to join, one row a wave
     const int64_t all = (int64_t)own.rows * own.a.batch * own.c.heads;
     const int each = own.finish && os.nb == 0 && all >= 32 * kWaves * kCus ? 8 : 1;
-    const int64_t waves = (int64_t)((own.rows + each - 1) / each) * own.a.batch * own.c.heads;
-    join_kernel<T, D><<<dim3((unsigned)((waves + kWaves - 1) / kWaves)), dim3(kBlock), 0, stream>>>(
-        own, ahead, each);
+    const int64_t places = (int64_t)((own.rows + each - 1) / each) * own.a.batch * own.c.heads;
+    // units over more runs than a wave has loads for: four waves to a row, as
+    // long as the rows alone do not fill the device (64 rows of 150 runs: 8.9 us
+    // with one wave, 3.9 with four; 4096 of 18: 12.1 and 13.6)
+    const int64_t runs = own.runs / ((int64_t)own.row_groups * own.a.batch * own.c.heads) +
+                         (ahead.rows > 0 ? ahead.runs / ((int64_t)ahead.row_groups * own.c.heads)
+                                         : 0);
+    if (each == 1 && places <= 4 * kCus && runs > in_flight<D>)
+        join_kernel<T, D, kWaves><<<dim3((unsigned)places), dim3(kBlock), 0, stream>>>(own, ahead,
+                                                                                       each);
+    else
+        join_kernel<T, D, 1><<<dim3((unsigned)((places + kWaves - 1) / kWaves)), dim3(kBlock), 0,
+                               stream>>>(own, ahead, each);
     return hipGetLastError();
 }
 
