@@ -16,10 +16,16 @@ grouped-query attention; Llama-70B: H = 8192, I = 28672, KV = 1024):
                                                  own launch)
   gate, up  H -> I   from o                     (independent: one group)
   down      I -> H   from up                    (feeds the next layer)
-Norms, attention over a longer context, the residual adds and the SwiGLU
-product are outside the GEMV path and are not modelled; the data
-dependencies between projections follow the layer's order.  At 70B the
-down projection (K = 28672) runs the K-tiled kernel.
+The norms of the layer, the residual adds and the SwiGLU product are outside
+the GEMV path and are not modelled; the data dependencies between projections
+follow the layer's order.  At 70B the down projection (K = 28672) runs the
+K-tiled kernel.
+
+With a context of N tokens (--context N) every layer has a quantized paged
+cache that holds them, and between its q/k/v and o projections the step runs
+  norms     of each head of q and k, and their rotation, in place
+  append    of the token's k and v to the cache, at position N
+  attention of q over the cache's N + 1 tokens        (o's input)
 
 Weights are random-init: W ~ N(0, 1/K) in fp16 (so activations stay O(1)
 through all layers), quantized with the path's own quantizers on the
@@ -32,6 +38,7 @@ All three produce bit-identical outputs.
 Usage: python -m cudalab_amd.decode [--model 7b|70b] [--layers N]
        [--op int4gemv|qgemv] [--steps 20] [--warmup 3]
        [--modes sequential,grouped,graph]
+       [--context N] [--cache-bits 8|4]
        python -m cudalab_amd.decode --stress [--op int4gemv|qgemv] [--steps 20]
 
 --stress times the decode stress sequence instead, Llama-7B projection shapes
@@ -54,6 +61,8 @@ HIDDEN = 4096
 INTER = 11008
 LAYERS = 32
 HEAD_DIM = 128
+PAGE = 64                 # tokens of a cache page
+ROPE_BASE = 10000.0
 # Llama-shaped presets: hidden, intermediate, k/v width, layers
 MODELS = {"7b": dict(hidden=4096, inter=11008, kv=4096, layers=32),
           "70b": dict(hidden=8192, inter=28672, kv=1024, layers=80)}
@@ -90,6 +99,8 @@ def proj_bytes(op: str, N: int, K: int) -> int:
 class Layer:
     w: dict = field(default_factory=dict)      # name -> (W, scale)
     out: dict = field(default_factory=dict)    # name -> fp16 output buffer
+    norm: tuple = ()                           # weights of q's and k's head norms
+    cache: object = None                       # KVCache of the context
 
 
 class DecodeModel:
@@ -99,7 +110,11 @@ class DecodeModel:
     def __init__(self, op: str = "int4gemv", layers: int = LAYERS,
                  seed: int = 7, device: str = "cuda",
                  hidden: int = HIDDEN, inter: int = INTER,
-                 kv: int | None = None):
+                 kv: int | None = None, context: int = 0,
+                 cache_bits: int = 8, room: int = 1):
+        """`context` tokens of random keys and values come before the step's
+        own (0: a single-token context, no cache); the caches have pages for
+        `room` more."""
         self.op = op
         self.ext = build(op)
         self.variant = VARIANT[op]
@@ -120,13 +135,57 @@ class DecodeModel:
                 L.w[name] = _quantize(op, W)
                 L.out[name] = torch.empty(N, dtype=torch.float16, device=device)
                 del W
-            # o's input: v itself, or v repeated per query head group
-            L.out["o_in"] = (L.out["v"] if kv == hidden else
+            # o's input: v itself, or v repeated per query head group, or
+            # the attention over the context
+            L.out["o_in"] = (L.out["v"] if kv == hidden and not context else
                              torch.empty(hidden, dtype=torch.float16, device=device))
             self.layers.append(L)
         self.x0 = (torch.randn(hidden, generator=g, device=device)).half()
         self.bytes_per_step = layers * sum(proj_bytes(op, N, K)
                                            for _, N, K in self.proj)
+        self.context, self.cache_bits = context, cache_bits
+        if context:
+            self._fill_caches(context, room, device)
+
+    def _fill_caches(self, context: int, room: int, device: str) -> None:
+        from .kvcache import KVCache
+        self.att = build("attention")
+        heads, pages = self.kv // HEAD_DIM, -(-(context + room) // PAGE)
+        g = torch.Generator(device=device)
+        g.manual_seed(context)
+
+        def rand(*shape):
+            return torch.randn(*shape, generator=g, device=device).half()
+
+        self.table = torch.randperm(pages, generator=g, device=device).int()[None]
+        self.position = torch.full((1,), context, dtype=torch.int32, device=device)
+        self.length = self.position + 1
+        angle = (torch.arange(context + room, device=device)[:, None] * ROPE_BASE **
+                 (-torch.arange(0, HEAD_DIM, 2, device=device) / HEAD_DIM))
+        self.cos, self.sin = angle.cos(), angle.sin()
+        first = torch.zeros_like(self.position)
+        for L in self.layers:
+            L.norm = (1 + rand(HEAD_DIM) / 8, 1 + rand(HEAD_DIM) / 8)
+            L.cache = KVCache.empty(pages, heads, HEAD_DIM, PAGE, self.cache_bits, device)
+            k, v = (rand(1, context, heads, HEAD_DIM) for _ in range(2))
+            self.att.append(L.cache, k, v, self.table, first)
+        # what a step's attention reads: the codes and scales of its tokens
+        self.cache_bytes_per_step = (len(self.layers) * (context + 1) * heads * 2 *
+                                     (HEAD_DIM * self.cache_bits // 8 + 4))
+
+    def advance(self) -> None:
+        """On to the next token: later steps (replayed ones too) write to the
+        position behind, and see the token of the step before."""
+        self.position.add_(1)
+        self.length.add_(1)
+
+    def _attend(self, L: Layer) -> None:
+        """From the q, k, v projections' outputs to o's input."""
+        q, k, v = (L.out[n].view(1, -1, HEAD_DIM) for n in ("q", "k", "v"))
+        self.att.qk_norm_rope_into(q, k, q, k, *L.norm, self.cos, self.sin, self.position)
+        self.att.append(L.cache, k[None], v[None], self.table, self.position)
+        self.att.forward_into(q[None], L.cache, self.table, self.length,
+                              L.out["o_in"].view(1, 1, -1, HEAD_DIM))
 
     # -- one decode step over all layers ---------------------------------
     def _one(self, L: Layer, name: str, x: torch.Tensor):
@@ -135,7 +194,7 @@ class DecodeModel:
 
     def _group(self, L: Layer, names, x: torch.Tensor):
         problems = [(L.w[n][0], L.w[n][1], x, L.out[n]) for n in names]
-        if "v" in names and self.kv != self.hidden:
+        if "v" in names and self.kv != self.hidden and not self.context:
             # attention over a single-token context: each query head gets its
             # kv head's v
             self.ext.forward_grouped_repeat(self.variant, problems, names.index("v"),
@@ -148,10 +207,12 @@ class DecodeModel:
         for L in self.layers:
             for n in ("q", "k"):
                 self._one(L, n, x)
-            if self.kv == self.hidden:
+            if self.kv == self.hidden or self.context:
                 self._one(L, "v", x)
             else:
                 self._group(L, ("v",), x)
+            if self.context:
+                self._attend(L)
             self._one(L, "o", L.out["o_in"])
             for n in ("gate", "up"):
                 self._one(L, n, L.out["o"])
@@ -163,6 +224,8 @@ class DecodeModel:
         x = self.x0
         for L in self.layers:
             self._group(L, ("q", "k", "v"), x)
+            if self.context:
+                self._attend(L)
             self._one(L, "o", L.out["o_in"])
             self._group(L, ("gate", "up"), L.out["o"])
             self._one(L, "down", L.out["up"])
@@ -258,11 +321,12 @@ def stress(op: str = "int4gemv", replays: int = 20, warmup: int = 3,
 
 
 def run(op: str = "int4gemv", layers: int | None = None, steps: int = 20,
-        warmup: int = 3, modes=MODES, model: str = "7b") -> dict:
+        warmup: int = 3, modes=MODES, model: str = "7b", context: int = 0,
+        cache_bits: int = 8) -> dict:
     cfg = MODELS[model]
     layers = cfg["layers"] if layers is None else layers
     m = DecodeModel(op, layers, hidden=cfg["hidden"], inter=cfg["inter"],
-                    kv=cfg["kv"])
+                    kv=cfg["kv"], context=context, cache_bits=cache_bits)
     graph = m.capture() if "graph" in modes else None
     res = {"op": op, "variant": m.variant, "model": model, "layers": layers,
            "hidden": m.hidden, "inter": m.inter, "kv": m.kv,
@@ -272,6 +336,12 @@ def run(op: str = "int4gemv", layers: int | None = None, steps: int = 20,
                    "every call (forward_into and forward_grouped through "
                    "the checked-once fast path); graph replays the grouped "
                    "step's launches from one HIP graph"}
+    if context:
+        # norms, append and attention's two kernels between the projections
+        res["launches_per_layer"] = {n: c + 4 for n, c in res["launches_per_layer"].items()}
+        res.update(context=context, cache_bits=cache_bits,
+                   cache_bytes_per_step=m.cache_bytes_per_step)
+    nbytes = m.bytes_per_step + (m.cache_bytes_per_step if context else 0)
     fns = {"sequential": m.step_sequential, "grouped": m.step_grouped,
            "graph": graph.replay if graph is not None else None}
     for mode in modes:
@@ -279,8 +349,8 @@ def run(op: str = "int4gemv", layers: int | None = None, steps: int = 20,
         us = time_steps(fn, steps, warmup)
         res[mode] = {"us_per_step": round(us, 2),
                      "us_per_layer": round(us / layers, 3),
-                     "GBps": round(m.bytes_per_step / us / 1e3, 1),
-                     "frac_peak": round(m.bytes_per_step / us / 1e3 / 8000.0, 4)}
+                     "GBps": round(nbytes / us / 1e3, 1),
+                     "frac_peak": round(nbytes / us / 1e3 / 8000.0, 4)}
     return res
 
 
@@ -297,6 +367,10 @@ def main(argv=None) -> int:
     ap.add_argument("--stress", action="store_true",
                     help="time the decode stress sequence (11008x4096, 4096x11008, "
                          "4 x 4096x4096) over an HBM-cold pool instead of a model")
+    ap.add_argument("--context", type=int, default=0,
+                    help="tokens before the step's own, in a quantized cache that "
+                         "attention reads (default 0: attention is the identity on v)")
+    ap.add_argument("--cache-bits", type=int, choices=(8, 4), default=8)
     a = ap.parse_args(argv)
     from . import _capi
     print(f"library: {_capi.version()}", flush=True)   # the build that ran
@@ -313,10 +387,14 @@ def main(argv=None) -> int:
     if a.layers is not None and a.layers < 1:
         print("decode: --layers must be >= 1", file=sys.stderr)
         return 2
+    if a.context < 0:
+        print("decode: --context must be >= 0", file=sys.stderr)
+        return 2
     if not torch.cuda.is_available():
         print("decode: no GPU visible", file=sys.stderr)
         return 1
-    print(json.dumps(run(a.op, a.layers, a.steps, a.warmup, modes, a.model)), flush=True)
+    print(json.dumps(run(a.op, a.layers, a.steps, a.warmup, modes, a.model, a.context,
+                         a.cache_bits)), flush=True)
     return 0
 
 
