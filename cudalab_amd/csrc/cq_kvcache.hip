@@ -38,25 +38,47 @@ __device__ __forceinline__ void scale_of(uint32_t amax_bits, float& scale, float
     }
 }
 
-template <int BITS>
-__device__ __forceinline__ int code_of(float x, float inv) {
-    constexpr float top = BITS == 8 ? 127.0f : 7.0f;
-    // inv 0 stands for a vector of zeros, whose x may be NaN or Inf
-    const float r = inv == 0.f ? 0.f : rintf(x * inv);
-    return (int)fminf(fmaxf(r, -top), top);
-}
-
 // Largest |x| of the 16 lanes that share a token, as FP32 bits (NaN above
-// Inf above every number).
+// Inf above every number).  Magnitudes of 16 bits are compared as they are, two
+// at a time.
 template <class T, int E>
 __device__ __forceinline__ uint32_t amax16(const T (&x)[E]) {
+    auto over16 = [](uint32_t m, auto&& larger) {
+        m = larger(m, row_dpp<0x128>(m));
+        m = larger(m, row_dpp<0x124>(m));
+        m = larger(m, row_dpp<0x122>(m));
+        return larger(m, row_dpp<0x121>(m));
+    };
     uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
+        auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
 #pragma unroll
-    for (int i = 0; i < E; ++i) m = max(m, __float_as_uint((float)x[i]) & 0x7FFFFFFFu);
-    m = max(m, row_dpp<0x128>(m));
-    m = max(m, row_dpp<0x124>(m));
-    m = max(m, row_dpp<0x122>(m));
-    return max(m, row_dpp<0x121>(m));
+        for (int i = 0; i < E; ++i) m = larger(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        return over16(m, larger);
+    } else {
+        using u2 = Vec<unsigned short, 2>;
+        auto larger = [](uint32_t a, uint32_t b) {
+            return __builtin_bit_cast(uint32_t,
+                                      __builtin_elementwise_max(__builtin_bit_cast(u2, a),
+                                                                __builtin_bit_cast(u2, b)));
+        };
+#pragma unroll
+        for (int i = 0; i < E; i += 2)
+            m = larger(m, __builtin_bit_cast(uint32_t, Vec<T, 2>{x[i], x[i + 1]}) & 0x7FFF7FFFu);
+        m = over16(m, larger);
+        const unsigned short top = (unsigned short)max(m & 0xFFFFu, m >> 16);
+        return __float_as_uint((float)__builtin_bit_cast(T, top));
+    }
+}
+
+// Bytes are transposed among lanes l, l + 16, l + 32, l + 48: byte j of lane
+// l + 16 i becomes byte i of lane l + 16 j.
+__device__ __forceinline__ uint32_t turn_bytes(uint32_t x) {
+    const int q = (threadIdx.x >> 4) & 3;
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const uint32_t y = __builtin_amdgcn_perm(a[1], a[0], q & 1 ? 0x07030501u : 0x06020400u);
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return __builtin_amdgcn_perm(b[1], b[0], q & 2 ? 0x07060302u : 0x05040100u);
 }
 
 // E elements at p; `wide` when 16 bytes (or all E) may be loaded at once.
@@ -82,17 +104,34 @@ struct Codes {
     static constexpr int kBytes = BITS == 8 ? E : E / 2;
     static constexpr int kWords = (kBytes + 3) / 4;
     uint32_t w[kWords] = {};
+    // x * inv lies within qmax (1 + 2^-21), so rounding it needs no clamp.  Four
+    // codes make one number: bytes are the low bits of 1.5 * 2^23 and the code;
+    // nibbles are digits 8 above their code, all four below 2^16.
     template <class T>
     __device__ __forceinline__ void pack(const T (&x)[E], float inv) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const uint32_t c = (uint32_t)code_of<BITS>((float)x[i], inv);
-            if constexpr (BITS == 8) w[i / 4] |= (c & 0xFFu) << (8 * (i % 4));
-            else w[i / 8] |= (c & 0xFu) << (4 * (i % 8));
+        for (int i = 0; i < E; i += 4) {
+            uint32_t four;
+            if constexpr (BITS == 8) {
+                uint32_t c[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    c[j] = __float_as_uint((float)x[i + j] * inv + 0x1.8p23f);
+                four = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0C0C0400u),
+                                             __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u),
+                                             0x05040100u);
+            } else {
+                float sum = rintf((float)x[i + 3] * inv);
+#pragma unroll
+                for (int j = 2; j >= 0; --j)
+                    sum = __builtin_fmaf(sum, 16.f, rintf((float)x[i + j] * inv));
+                four = (__float_as_uint(sum + (0x1p23f + 0x8888)) & 0xFFFFu) ^ 0x8888u;
+            }
+            // inv 0 stands for a vector of zeros, whose x may be NaN or Inf
+            if (inv == 0.f) four = 0;
+            if constexpr (BITS == 8) w[i / 4] = four;
+            else w[i / 8] |= four << (4 * (i % 8));
         }
-    }
-    __device__ __forceinline__ uint8_t byte(int i) const {
-        return (uint8_t)(w[i / 4] >> (8 * (i % 4)));
     }
     __device__ __forceinline__ void store(uint8_t* p) const {
         if constexpr (kBytes == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
@@ -154,27 +193,31 @@ __global__ __launch_bounds__(kBlock) void append_kernel(cq_kv_cache_t c, cq_kv_s
     constexpr int E = D / 16;
     constexpr int R = BITS == 8 ? D : D / 2;       // bytes of a row
     using C = Codes<BITS, E>;
-    __shared__ __attribute__((aligned(16))) uint8_t turned[R][16];
+    // a lane's rows, and 16 bytes of padding
+    __shared__ __attribute__((aligned(16))) uint8_t turned[16][C::kBytes * 16 + 16];
     const int h = blockIdx.x % c.heads;
     const uint32_t bt = blockIdx.x / c.heads;
     const int b = bt / tiles;
     const Tile tile(c, s, b, bt % tiles);
     const int i = threadIdx.x >> 4, lane = threadIdx.x & 15;
     const int64_t t = tile.first + i;
-    const bool live = tile.page >= 0 && t >= 0 && t < tile.count;
     const int64_t lo = tile.first < 0 ? 0 : tile.first;
-    if (tile.page < 0 || lo >= tile.count) return;     // uniform over the workgroup
-    const int64_t ph = tile.page * c.heads + h;
-    C kc, vc;
+    if (lo >= tile.count) return;                      // uniform over the workgroup
+    const bool live = t >= 0 && t < tile.count;
+    T x[E] = {}, y[E] = {};
     if (live) {
-        T x[E], y[E];
         load_row(x, k + b * ks.batch + t * ks.token + h * ks.head + lane * E, wide);
         load_row(y, v + b * vs.batch + t * vs.token + h * vs.head + lane * E, wide);
-        float kscale, vscale, kinv, vinv;
-        scale_of<BITS>(amax16(x), kscale, kinv);
-        scale_of<BITS>(amax16(y), vscale, vinv);
-        kc.pack(x, kinv);
-        vc.pack(y, vinv);
+    }
+    if (tile.page < 0) return;
+    const int64_t ph = tile.page * c.heads + h;
+    C kc, vc;
+    float kscale, vscale, kinv, vinv;
+    scale_of<BITS>(amax16(x), kscale, kinv);
+    scale_of<BITS>(amax16(y), vscale, vinv);
+    kc.pack(x, kinv);
+    vc.pack(y, vinv);
+    if (live) {
         const int64_t at = ph * c.page_size + tile.in_page + i;
         kc.store(static_cast<uint8_t*>(c.k) + at * R + lane * C::kBytes);
         if (lane == 0) {
@@ -182,20 +225,26 @@ __global__ __launch_bounds__(kBlock) void append_kernel(cq_kv_cache_t c, cq_kv_s
             sc[0] = kscale;
             sc[c.page_size] = vscale;
         }
+    }
+    // four tokens of a row to a word
 #pragma unroll
-        for (int j = 0; j < C::kBytes; ++j) turned[lane * C::kBytes + j][i] = vc.byte(j);
+    for (int m = 0; m < C::kWords; ++m) {
+        const uint32_t word = turn_bytes(vc.w[m]);
+        const int r = 4 * m + (i & 3);
+        if (r < C::kBytes) *reinterpret_cast<uint32_t*>(turned[lane] + r * 16 + (i & ~3)) = word;
     }
     __syncthreads();
     uint8_t* vd = static_cast<uint8_t*>(c.v) +
                   (ph * (c.page_size / 16) + tile.in_page / 16) * R * 16;
     if ((int)threadIdx.x < R) {
         const int r = threadIdx.x;
+        const uint8_t* row = turned[r / C::kBytes] + r % C::kBytes * 16;
         const int from = (int)(lo - tile.first);
         const int to = (int)min((int64_t)16, tile.count - tile.first);
         if (from == 0 && to == 16)
-            *reinterpret_cast<uint4*>(vd + r * 16) = *reinterpret_cast<const uint4*>(turned[r]);
+            *reinterpret_cast<uint4*>(vd + r * 16) = *reinterpret_cast<const uint4*>(row);
         else
-            for (int j = from; j < to; ++j) vd[r * 16 + j] = turned[r][j];
+            for (int j = from; j < to; ++j) vd[r * 16 + j] = row[j];
     }
 }
 
@@ -205,8 +254,7 @@ __global__ __launch_bounds__(kBlock) void read_kernel(cq_kv_cache_t c, cq_kv_slo
     constexpr int E = D / 16;
     constexpr int R = BITS == 8 ? D : D / 2;
     using C = Codes<BITS, E>;
-    // 16 bytes of padding a token: the turned bytes of the 16 tokens start in
-    // different banks
+    // 16 bytes of padding a token: four tokens' words lie in different banks
     __shared__ __attribute__((aligned(16))) uint8_t turned[16][R + 16];
     const int h = blockIdx.x % c.heads;
     const uint32_t bt = blockIdx.x / c.heads;
@@ -217,14 +265,21 @@ __global__ __launch_bounds__(kBlock) void read_kernel(cq_kv_cache_t c, cq_kv_slo
     const bool there = tile.page >= 0;                 // uniform over the workgroup
     if (tile.first + 15 < 0 || tile.first >= s.tokens) return;
     const int64_t ph = there ? tile.page * c.heads + h : 0;
-    if (there && (int)threadIdx.x < R) {
-        const int r = threadIdx.x;
-        const uint4 q = *reinterpret_cast<const uint4*>(
-            static_cast<const uint8_t*>(c.v) +
-            ((ph * (c.page_size / 16) + tile.in_page / 16) * R + r) * 16);
+    const int wave = threadIdx.x >> 6;
+    if (there && wave * 64 < R) {                      // uniform over the wave
+        const int r = wave * 64 + 4 * lane + (i & 3);
+        uint4 q = {};
+        if (r < R)
+            q = *reinterpret_cast<const uint4*>(
+                static_cast<const uint8_t*>(c.v) +
+                ((ph * (c.page_size / 16) + tile.in_page / 16) * R + r) * 16);
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int j = 0; j < 16; ++j) turned[j][r] = (uint8_t)(w[j / 4] >> (8 * (j % 4)));
+        for (int j = 0; j < 4; ++j) {                  // four rows of a token to a word
+            const uint32_t word = turn_bytes(w[j]);
+            if (r < R)
+                *reinterpret_cast<uint32_t*>(turned[4 * j + (i & 3)] + wave * 64 + 4 * lane) = word;
+        }
     }
     __syncthreads();
     if (t < 0 || t >= s.tokens) return;
