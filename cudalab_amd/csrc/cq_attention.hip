@@ -652,6 +652,8 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
     bool there;                          // the lane group's 16 keys have a page
 
     // K's rows in the order that gives lane group g keys 16 g .. 16 g + 15.
+    // Codes are read once, past the caches (64 sequences of up to 16384 keys:
+    // 213 us with ordinary loads, 197 with non-temporal ones).
     __device__ __forceinline__ void load_k(const Source& s, uint32_t entry, int tile, int h,
                                            int lane) {
         const int g = lane >> 4, r = lane & 15;
@@ -663,8 +665,9 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int c = 0; c < kChunks; ++c)
-                kq[t][c] = *reinterpret_cast<const Vec<uint32_t, kWords>*>(
-                    p + t * 4 * kRow + c * 4 * kChunk);
+                kq[t][c] =
+                    __builtin_nontemporal_load(reinterpret_cast<const Vec<uint32_t, kWords>*>(
+                        p + t * 4 * kRow + c * 4 * kChunk));
     }
 
     __device__ __forceinline__ void load_v(const Source& s, uint32_t entry, int tile, int h,
@@ -679,7 +682,8 @@ struct Tiles : Rows<T, BITS, D, NB, true> {
         const uint8_t* p = static_cast<const uint8_t*>(s.c.v) + head_of(s, page, h, kRow) +
                            in * kRow + r * 16;
 #pragma unroll
-        for (int i = 0; i < kVTiles; ++i) vq[i] = *reinterpret_cast<const u4*>(p + i * 256);
+        for (int i = 0; i < kVTiles; ++i)
+            vq[i] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p + i * 256));
     }
 
     static __device__ __forceinline__ h8 unpack_k(const Vec<uint32_t, kWords> (&row)[kChunks],
