@@ -23,8 +23,10 @@ __device__ __forceinline__ float row_dpp(float v) {
 // them; rows of 16 by rotations, wider groups by lane exchanges.
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
-    if constexpr (LANES == 2 || LANES == 4 || LANES == 8) {
-        for (int off = LANES / 2; off > 0; off >>= 1) v += __shfl_xor(v, off);
+    if constexpr (LANES == 4 || LANES == 8) {
+        v += row_dpp<0xB1>(v);                      // quad_perm 1 0 3 2
+        v += row_dpp<0x4E>(v);                      // quad_perm 2 3 0 1
+        if (LANES == 8) v += row_dpp<0x141>(v);     // the row's halves mirrored
     } else if constexpr (LANES >= 16) {
         v += row_dpp<0x128>(v);
         v += row_dpp<0x124>(v);

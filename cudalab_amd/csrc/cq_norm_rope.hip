@@ -8,12 +8,11 @@
 // the rotation, as a chain of separate calls would, is left out: one rounding
 // is closer to the formula.
 //
-// Bound by memory: each element is read and written once, and the tables'
-// rows of a token serve all its heads.  LANES lanes take a head, eight
-// elements each: the lane that holds a holds its b too, so the rotation needs
-// no exchange, and the only one is the sum of squares.
-
-#include <algorithm>
+// Bound by memory: each element is read and written once, past the caches, and
+// the tables' rows of a token serve all its heads; by the launch at one token.
+// LANES lanes take a head, C elements of each end of its pairs each: the lane
+// that holds a holds its b too, so the rotation needs no exchange, and the only
+// one is the sum of squares.
 
 #include "cq_attn.h"
 #include "cq_elem.h"
@@ -22,7 +21,7 @@ namespace cq {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int64_t kManyHeads = 256 * 8 * 4 * 8;   // 256 CUs of eight waves of four groups, times 8
+constexpr int64_t kManyHeads = 1 << 16;       // 256 CUs of four waves of eight groups of eight
 
 __device__ __forceinline__ float load_weight(const void* p, int dtype, int i) {
     if (dtype == CQ_DTYPE_F16) return (float)static_cast<const _Float16*>(p)[i];
@@ -30,22 +29,22 @@ __device__ __forceinline__ float load_weight(const void* p, int dtype, int i) {
     return static_cast<const float*>(p)[i];
 }
 
-// Four weights from i, a multiple of four (all at once where `wide`).
+// C weights from i, a multiple of C (all at once where `wide`).
+template <int C>
 __device__ __forceinline__ void load_weights(const void* p, int dtype, int i, bool wide,
-                                             float (&w)[4]) {
-    if (wide && dtype == CQ_DTYPE_F16) {
-        const Vec<_Float16, 4> v = *reinterpret_cast<const Vec<_Float16, 4>*>(
-            static_cast<const _Float16*>(p) + i);
+                                             float (&w)[C]) {
+    if (wide && dtype != CQ_DTYPE_F32) {
+        const Vec<uint16_t, C> v =
+            *reinterpret_cast<const Vec<uint16_t, C>*>(static_cast<const uint16_t*>(p) + i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = (float)v[j];
-    } else if (wide && dtype == CQ_DTYPE_BF16) {
-        const Vec<__bf16, 4> v = *reinterpret_cast<const Vec<__bf16, 4>*>(
-            static_cast<const __bf16*>(p) + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = (float)v[j];
+        for (int j = 0; j < C; ++j) {
+            const uint16_t bits = v[j];      // (a cast of v[j] itself takes v[0])
+            w[j] = dtype == CQ_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, bits)
+                                         : __uint_as_float((uint32_t)bits << 16);
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = load_weight(p, dtype, i + j);
+        for (int j = 0; j < C; ++j) w[j] = load_weight(p, dtype, i + j);
     }
 }
 
@@ -77,15 +76,15 @@ struct Head {
     }
 };
 
-// Vector kernel: head_dim and rot_dim multiples of 8, head_dim <= 8 * LANES,
-// rows and weights aligned to four elements, tables to 16 bytes.  A group of
-// LANES lanes takes heads part, part + parts, ... of one token, BATCH loads in
-// flight; lane l holds elements e0..e0+3 and e1..e1+3, in the half style the
-// two ends of pairs 4l..4l+3, else eight neighbours.
-template <class T, bool PAIRS, int LANES, int BATCH>
+// Vector kernel: head_dim and rot_dim multiples of 2 C, head_dim <= 2 C * LANES,
+// rows aligned to C elements, tables to 16 bytes.  A group of LANES lanes takes
+// heads part, part + parts, ... of one token, BATCH loads of each end in
+// flight; lane l holds elements e0..e0+C-1 and e1..e1+C-1, in the half style
+// the two ends of pairs Cl..Cl+C-1, else 2 C neighbours.
+template <class T, bool PAIRS, int C, int LANES, int BATCH>
 __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uint32_t parts,
                                                            uint32_t iters, bool wide) {
-    using V = Vec<T, 4>;
+    using V = Vec<T, C>;
     const int lane = threadIdx.x % LANES;
     const uint32_t group = blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
     const int heads = a.q_heads + a.k_heads;
@@ -93,11 +92,11 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
     const bool live = group / parts < a.tokens;
     const int64_t token = live ? group / parts : a.tokens - 1;
     const uint32_t part = group % parts;
-    const bool active = 8 * lane < a.head_dim;
-    const bool turn = a.cos_table != nullptr && 8 * lane < a.rot_dim;
+    const bool active = 2 * C * lane < a.head_dim;
+    const bool turn = a.cos_table != nullptr && 2 * C * lane < a.rot_dim;
     const bool halves = turn && !PAIRS;
-    const int e0 = !active ? 0 : halves ? 4 * lane : 8 * lane;
-    const int e1 = !active ? 4 : halves ? a.rot_dim / 2 + 4 * lane : 8 * lane + 4;
+    const int e0 = !active ? 0 : halves ? C * lane : 2 * C * lane;
+    const int e1 = !active ? C : halves ? a.rot_dim / 2 + C * lane : 2 * C * lane + C;
 
     V x0[BATCH], x1[BATCH];
     auto load = [&](uint32_t it) {
@@ -110,29 +109,36 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
         }
     };
     load(0);
-    float w[2][2][4];           // of q and k, at e0 and e1
+    float w[2][2][C];           // of q and k, at e0 and e1
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const void* p = i == 0 ? a.q_weight : a.k_weight;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[i][0][j] = w[i][1][j] = 1.f;
+        for (int j = 0; j < C; ++j) w[i][0][j] = w[i][1][j] = 1.f;
         if (p != nullptr) {
             load_weights(p, a.weight_dtype, e0, wide, w[i][0]);
             load_weights(p, a.weight_dtype, e1, wide, w[i][1]);
         }
     }
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+    float c[C], s[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) c[i] = 1.f, s[i] = 0.f;
     if (turn) {
         const int64_t row = table_row(a, token);
         if (row >= 0) {
-            const int64_t at = row * (a.rot_dim / 2) + 4 * lane;
-            const Vec<float, 4> cv = *reinterpret_cast<const Vec<float, 4>*>(a.cos_table + at);
-            const Vec<float, 4> sv = *reinterpret_cast<const Vec<float, 4>*>(a.sin_table + at);
+            const int64_t at = row * (a.rot_dim / 2) + C * lane;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = cv[i], s[i] = sv[i];
+            for (int i = 0; i < C; i += 4) {
+                const Vec<float, 4> cv =
+                    *reinterpret_cast<const Vec<float, 4>*>(a.cos_table + at + i);
+                const Vec<float, 4> sv =
+                    *reinterpret_cast<const Vec<float, 4>*>(a.sin_table + at + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[i + j] = cv[j], s[i + j] = sv[j];
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = s[i] = __builtin_nanf("");
+            for (int i = 0; i < C; ++i) c[i] = s[i] = __builtin_nanf("");
         }
     }
     const bool norm = a.q_weight != nullptr || a.k_weight != nullptr;
@@ -143,25 +149,25 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
         for (int u = 0; u < BATCH; ++u) {
             const uint32_t h = part + (it + u) * parts;
             const Head<T> head(a, token, (int)min(h, (uint32_t)heads - 1));
-            float f[8];
+            float f[2 * C];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = (float)x0[u][i], f[4 + i] = (float)x1[u][i];
+            for (int i = 0; i < C; ++i) f[i] = (float)x0[u][i], f[C + i] = (float)x1[u][i];
             if (norm) {
                 float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
+                for (int i = 0; i < 2 * C; ++i) ss = __builtin_fmaf(f[i], f[i], ss);
                 ss = lanes_sum<LANES>(active ? ss : 0.f);
                 const bool has = head.is_q ? a.q_weight != nullptr : a.k_weight != nullptr;
                 const float r = has ? 1.f / sqrtf(ss * mean + a.eps) : 1.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    f[i] = f[i] * r * (head.is_q ? w[0][i / 4][i % 4] : w[1][i / 4][i % 4]);
+                for (int i = 0; i < 2 * C; ++i)
+                    f[i] = f[i] * r * (head.is_q ? w[0][i / C][i % C] : w[1][i / C][i % C]);
             }
             if (turn) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < C; ++i) {
                     float& p = f[PAIRS ? 2 * i : i];
-                    float& q = f[PAIRS ? 2 * i + 1 : 4 + i];
+                    float& q = f[PAIRS ? 2 * i + 1 : C + i];
                     const float t = p * c[i] - q * s[i];
                     q = q * c[i] + p * s[i];
                     p = t;
@@ -169,7 +175,7 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
             }
             V y0, y1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y0[i] = (T)f[i], y1[i] = (T)f[4 + i];
+            for (int i = 0; i < C; ++i) y0[i] = (T)f[i], y1[i] = (T)f[C + i];
             if (live && active && h < (uint32_t)heads) {
                 __builtin_nontemporal_store(y0, reinterpret_cast<V*>(head.dst + e0));
                 __builtin_nontemporal_store(y1, reinterpret_cast<V*>(head.dst + e1));
@@ -243,15 +249,17 @@ __global__ __launch_bounds__(kBlock) void norm_rope_any_kernel(cq_norm_rope_t a)
 
 bool multiple(int64_t v, int64_t m) { return v % m == 0; }
 
-// Whether the vector kernel may run: everything it reads or writes as four
-// elements starts at a multiple of them.
-bool vector_ok(const cq_norm_rope_t& a, int64_t elem) {
+// Whether the vector kernel may run with C elements at a time: everything it
+// reads or writes so starts at a multiple of them.
+bool vector_ok(const cq_norm_rope_t& a, int64_t elem, int c) {
+    const int64_t bytes = c * elem;
     auto rows_ok = [&](const void* p, int64_t ts, int64_t hs) {
-        return multiple((int64_t)(uintptr_t)p, 4 * elem) && multiple(ts, 4) && multiple(hs, 4);
+        return multiple((int64_t)(uintptr_t)p, bytes) && multiple(ts * elem, bytes) &&
+               multiple(hs * elem, bytes);
     };
-    if (a.head_dim % 8 != 0 || a.head_dim > 512) return false;
+    if (a.head_dim % (2 * c) != 0 || a.head_dim > 512) return false;
     if (a.cos_table != nullptr &&
-        (a.rot_dim % 8 != 0 || !multiple((int64_t)(uintptr_t)a.cos_table, 16) ||
+        (a.rot_dim % (2 * c) != 0 || !multiple((int64_t)(uintptr_t)a.cos_table, 16) ||
          !multiple((int64_t)(uintptr_t)a.sin_table, 16)))
         return false;
     if (a.q_heads > 0 && !(rows_ok(a.q, a.q_token_stride, a.q_head_stride) &&
@@ -264,35 +272,45 @@ bool vector_ok(const cq_norm_rope_t& a, int64_t elem) {
 template <class T, bool PAIRS>
 hipError_t launch_typed(const cq_norm_rope_t& a, hipStream_t stream) {
     const int64_t heads = (int64_t)a.q_heads + a.k_heads;
-    if (!vector_ok(a, sizeof(T))) {
+    if (!vector_ok(a, sizeof(T), 4)) {
         const int64_t units = a.tokens * heads, grid = (units + kBlock / 64 - 1) / (kBlock / 64);
         if (grid > kMaxGrid) return hipErrorInvalidValue;
         norm_rope_any_kernel<T><<<dim3((unsigned)grid), dim3(kBlock), 0, stream>>>(a);
         return hipGetLastError();
     }
-    const int lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : a.head_dim <= 256 ? 32 : 64;
-    const int64_t per = kBlock / lanes;
-    auto weight_wide = [&](const void* p) {
-        return a.weight_dtype == CQ_DTYPE_F32 || (uintptr_t)p % 8 == 0;
-    };
-    const bool wide = weight_wide(a.q_weight) && weight_wide(a.k_weight);
-    auto go = [&](auto* kernel, int64_t iters) {
+    auto go = [&](auto* kernel, int c, int lanes, int64_t iters) {
+        const int64_t per = kBlock / lanes;
         const int64_t parts = (heads + iters - 1) / iters, groups = a.tokens * parts;
         if (groups + per > kMaxGrid) return hipErrorInvalidValue;
+        auto weight_wide = [&](const void* p) {
+            return a.weight_dtype == CQ_DTYPE_F32 || (uintptr_t)p % (2 * c) == 0;
+        };
         kernel<<<dim3((unsigned)((groups + per - 1) / per)), dim3(kBlock), 0, stream>>>(
-            a, (uint32_t)parts, (uint32_t)iters, wide);
+            a, (uint32_t)parts, (uint32_t)iters,
+            weight_wide(a.q_weight) && weight_wide(a.k_weight));
         return hipGetLastError();
     };
     // Few heads in all: one to a group, so that each wave has as little to wait
-    // for as can be.  Many: eight, four loads of each end in flight, and the
-    // weights and tables are fetched once for them.
+    // for as can be.  Many: eight, whose weights and tables are fetched once,
+    // with 16 bytes of each end in flight for two heads (8192 tokens of 64 heads
+    // of 128: 52 us; one head 55, four 58; one head to a group 77; pieces of 8
+    // bytes, four heads in flight, 70).
+    constexpr int kHeads = 8;
     const bool many = a.tokens * heads > kManyHeads;
-#define CQ_GO(L)                                                       \
-    (many ? go(&norm_rope_kernel<T, PAIRS, L, 4>, 8)                   \
-          : go(&norm_rope_kernel<T, PAIRS, L, 1>, 1))
-    if (lanes == 8) return CQ_GO(8);
-    if (lanes == 16) return CQ_GO(16);
-    if (lanes == 32) return CQ_GO(32);
+    if (many && vector_ok(a, sizeof(T), 8)) {
+#define CQ_GO(L) go(&norm_rope_kernel<T, PAIRS, 8, L, 2>, 8, L, kHeads)
+        if (a.head_dim <= 64) return CQ_GO(4);
+        if (a.head_dim <= 128) return CQ_GO(8);
+        if (a.head_dim <= 256) return CQ_GO(16);
+        return CQ_GO(32);
+#undef CQ_GO
+    }
+#define CQ_GO(L)                                                            \
+    (many ? go(&norm_rope_kernel<T, PAIRS, 4, L, 4>, 4, L, kHeads)           \
+          : go(&norm_rope_kernel<T, PAIRS, 4, L, 1>, 4, L, 1))
+    if (a.head_dim <= 64) return CQ_GO(8);
+    if (a.head_dim <= 128) return CQ_GO(16);
+    if (a.head_dim <= 256) return CQ_GO(32);
     return CQ_GO(64);
 #undef CQ_GO
 }

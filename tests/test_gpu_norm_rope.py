@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from attention_oracle import assert_close, norm_rope, norm_rope_tolerance
+from attention_oracle import UNIT, assert_close, norm_rope, norm_rope_tolerance
 from conftest import announce
 
 pytestmark = pytest.mark.gpu
@@ -168,3 +168,38 @@ def test_refusals(att):
         att.qk_norm_rope_into(q, q.clone(), o, o, *rest)
     with pytest.raises(RuntimeError):
         att.qk_norm_rope_into(q, k, q[:2], k, *rest)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("d,rot,shift", [(64, 64, 0), (128, 32, 0), (128, 128, 4), (256, 256, 0),
+                                         (40, 24, 0), (512, 480, 0), (96, 96, 0), (160, 144, 0)])
+def test_many_heads(att, dtype, inter, d, rot, shift):
+    """Heads enough for groups of them, at odd counts, rows off 16 bytes too;
+    every head as in a call of few, but for roundings (of FP32 16 each, of sums of
+    two normed values, below 16 in all)."""
+    g = torch.Generator(device="cuda").manual_seed(d)
+    tokens, hq, hkv = 2117, 23, 8
+    dt = DT[dtype]
+
+    def rand(h):
+        row = torch.randn(tokens, h * d + 8, generator=g, device="cuda").to(dt)
+        return row[:, shift:shift + h * d].unflatten(1, (h, d))
+    q, k = rand(hq), rand(hkv)
+    qw, kw = ((1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(dt) for _ in range(2))
+    cos, sin = (t.cuda() for t in _tables(50, rot))
+    pos = torch.randint(0, 50, (tokens,), generator=g, dtype=torch.int32, device="cuda")
+    announce(f"norm_rope many heads {dtype} inter={inter} d={d} rot={rot} shift={shift}")
+    gq, gk = att.qk_norm_rope(q, k, qw, kw, cos, sin, pos, interleaved=inter)
+    some = [0, 1, 777, tokens - 2, tokens - 1]
+    for got, x, w, name in ((gq, q, qw, "q"), (gk, k, kw, "k")):
+        _check(got[some], x[some].cpu(), w.cpu(), cos.cpu(), sin.cpu(), pos[some].cpu(), inter,
+               name)
+    few = 900                   # of few heads in all: one to a group
+    for at in (0, tokens - few):
+        part = slice(at, at + few)
+        sq, sk = att.qk_norm_rope(q[part], k[part], qw, kw, cos, sin, pos[part],
+                                  interleaved=inter)
+        for a, b in ((gq[part], sq), (gk[part], sk)):
+            assert bool(((a.double() - b.double()).abs()
+                         <= 2 * UNIT[dt] * b.double().abs() + 2 * 16 * 2.0 ** -24 * 16).all())
