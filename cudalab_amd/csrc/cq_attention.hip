@@ -39,6 +39,24 @@
 // that lies in one run is finished there; a longer one leaves a triple per run
 // in the workspace, which join_kernel joins.  Equal runs keep every workgroup
 // busy to the end for any mix of lengths, and the grid never depends on them.
+// Where whole units to a run are as even, they are dealt whole: 1024 new tokens
+// of 64 heads over 8700 keys then leave nothing to join (373 us, whole 337).
+//
+// Three kernels:
+//   tile_kernel   few rows (shape_of): a wave takes whole tiles, four waves
+//                 every fourth, joined in LDS.  Bound by memory: 64 sequences
+//                 of up to 16384 keys of 8 heads (int8, 1.14 GB) 196 us, 5.8
+//                 TB/s.  A short call is bound by waits that follow one another
+//                 (lengths, table, codes, the join).
+//   block_kernel  more rows: four or eight waves of 32 rows share tiles that
+//                 the workgroup unpacks into LDS once.  Bound by the matrix
+//                 units and the softmax between their products: 1024 new tokens
+//                 of 64 heads over 8700 keys (int4) 334 us, 822 TFLOP/s; a
+//                 prefix of 16384 keys for 64 sequences of 64 heads 86 us, of
+//                 which 40 are tiles (2.5 us each of 64 keys and 256 rows), 8
+//                 the join of 16 triples to a row, the rest the sequences' own
+//                 keys and starts and ends of units.
+//   join_kernel   joins triples; one token over 4096 keys of 8 heads 3.9 us.
 
 #include <algorithm>
 #include <utility>
@@ -77,7 +95,7 @@ struct Source {
     int32_t quantum;       // a run's length is a multiple of it
     int32_t cost;          // of a unit besides its tiles, in tiles
     uint32_t runs;         // workgroups
-    int32_t fits;          // the deal's sums fit 31 bits
+    int32_t fits;          // the deal's sums, keys and rows fit 31 bits
     int32_t finish;        // 1: units of one run write `out`; 0: their home
     // workspace: which runs have a unit's triples (first run and how many; none
     // for a unit without keys); triples of broken units, two per run, and of
@@ -1170,9 +1188,23 @@ struct Shape {
     int resident;    // workgroups that a CU holds
 };
 
-Shape shape_of(int64_t rows, int d) {
-    if (rows <= 16) return {1, kWaves, 16, waves_of(d, 1)};
-    if (rows <= 32 && d <= 128) return {2, kWaves, 32, waves_of(d, 2)};
+// The tile kernel unpacks every code once per row group; the block kernel once
+// for up to 256 rows, but has a unit's start and end to pay for.  So with few
+// units of many keys (as the table has room for) the tile kernel is ahead for
+// longer.
+// Measured on 8 heads over 4096 keys, us, tile and block kernel:
+//   heads of 128, 16 sequences: 32 rows 44, 55; 64 rows 57, 71; 80 rows 105, 80
+//                 64 sequences of 1000 keys: 40 rows 89, 60
+//                 2 sequences of 700 keys: 64 rows 18.2, 17.5
+//   heads of 64, 16 sequences: 64 rows 48, 58; 96 rows 72, 66
+//                 7 sequences of up to 1501 keys, 4 heads: 35 rows 15.8, 14.4
+//   heads of 256 (groups of 16), 16 sequences: 32 rows 84, 139; 48 rows 158, 146
+//                 64 sequences of 600 keys: 32 rows 108, 94
+// and of the block kernel four waves or eight: 128 rows 88, 93; 160 rows 135, 122.
+Shape shape_of(int64_t rows, int64_t units, int64_t keys, int d) {
+    const bool few = units <= kCus;
+    if (rows <= (d == 256 && few ? 32 : 16)) return {1, kWaves, 16, waves_of(d, 1)};
+    if (d <= 128 && rows <= (few && keys >= 2048 ? 64 : 32)) return {2, kWaves, 32, waves_of(d, 2)};
     if (d == 256) return {0, 4, 128, 1};
     if (rows <= 128) return {0, 4, 128, 2};
     return {0, 8, 256, 1};
@@ -1187,7 +1219,8 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
     s.page_shift = __builtin_ctz((unsigned)c.page_size);
     const int64_t rows = (int64_t)a.tokens * s.group * (prefix ? a.batch : 1);
     s.rows = (int32_t)rows;
-    *shape = shape_of(rows, c.head_dim);
+    const int64_t keys = prefix ? a.prefix_len : (int64_t)a.table_cols * c.page_size;
+    *shape = shape_of(rows, (int64_t)c.heads * (prefix ? 1 : a.batch), keys, c.head_dim);
     s.rows_per_unit = shape->rows;
     s.row_groups = (int32_t)((rows + s.rows_per_unit - 1) / s.rows_per_unit);
     // a workgroup of the tile kernel takes four tiles at a time; a unit's start
@@ -1197,11 +1230,11 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
     s.cost = shape->nb > 0 ? 2 * kWaves : 2;
     s.finish = a.prefix_len == 0;
     // no more runs than quanta, as far as the tables' sizes tell
-    const int64_t keys = prefix ? a.prefix_len : (int64_t)a.table_cols * c.page_size;
     const int64_t entries = (int64_t)s.row_groups * (prefix ? 1 : a.batch);
     const __int128 steps = (__int128)((keys + kTile - 1) / kTile + s.quantum + s.cost) * entries *
                            c.heads;
-    s.fits = steps + (__int128)kCus * 8 * s.quantum < ((__int128)1 << 31);
+    s.fits = steps + (__int128)kCus * 8 * s.quantum < ((__int128)1 << 31) &&
+             keys <= 0x7FFFFFFF - kTile && rows <= 0x7FFFFFFF;
     const int64_t room = (int64_t)kCus * shape->resident;
     const __int128 most = steps / s.quantum;
     s.runs = (uint32_t)(most < room ? (int64_t)most : room);

@@ -211,3 +211,15 @@ def test_oracle_rotation_turns():
         assert not torch.allclose(x[..., :32], y[..., :32]) and torch.equal(x[..., 32:], y[..., 32:])
         z, _ = norm_rope(y, None, ang.cos(), -ang.sin(), pos, 1e-6, inter)
         assert torch.allclose(x, z, atol=1e-6)
+
+
+def test_attention_refuses_more_keys_than_ints_count():
+    """Tables whose positions, or whose tiles over all units, pass 31 bits."""
+    bad = _capi.CQ_ERR_INVALID_ARG
+    one = dict(batch=1, q_heads=_cache().heads, prefix_len=0)
+    page = _cache().page_size
+    assert _attention(workspace=True, table_cols=2 ** 30 // page, **one) >= 0
+    for change in (dict(table_cols=2 ** 31 // page), dict(table_cols=2 ** 30),
+                   dict(table_cols=2 ** 30 // page, batch=2 ** 10)):
+        assert _attention(**{**one, **change}) == bad, change
+        assert _attention(workspace=True, **{**one, **change}) == -bad, change

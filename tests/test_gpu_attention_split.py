@@ -81,3 +81,17 @@ def test_table_too_long_for_the_deal(att):                        # noqa: F811
     announce("attention table too long")
     with pytest.raises(RuntimeError):
         att.forward(q, c, table, _ints([1] * 32))
+
+
+@pytest.mark.parametrize("bits,dtype", [(8, "bf16"), (4, "fp16")])
+@pytest.mark.parametrize("dim,tokens,group,lens", [
+    (128, 8, 8, [2500, 60]), (128, 11, 3, [2100]), (64, 5, 13, [2300, 0, 700]),
+    (256, 4, 8, [500, 33]), (256, 19, 1, [700])])
+def test_few_units_of_several_row_groups(att, bits, dtype, dim, tokens, group, lens):  # noqa: F811
+    """Rows of two groups of 16 or 32, over sequences that runs break."""
+    pages, table, _ = _setup(lens, 2, dim, 64, bits, seed=dim * tokens)
+    announce(f"attention {tokens} tokens x {group}, d={dim}, {bits} bits, few units")
+    counts = [tokens, tokens - 2, 1][:len(lens)]
+    q = _q(len(lens), tokens, 2 * group, dim, dtype)
+    _run(att, pages, table, lens, q, "few units")
+    _run(att, pages, table, lens, q, "few units, ragged", counts)
