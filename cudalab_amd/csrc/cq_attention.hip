@@ -1257,9 +1257,11 @@ int64_t lay_out(const cq_kv_cache_t& c, const cq_attention_t& a, Source* own, So
     used = (used + 15) / 16 * 16;
     for (Source* s : {own, ahead}) {
         if (s->rows == 0) continue;
-        s->o = reinterpret_cast<float*>(base);
-        s->ml = reinterpret_cast<float*>(base + triples * c.head_dim * 4);
-        s->where = reinterpret_cast<uint32_t*>(base + used);
+        if (base != nullptr) {
+            s->o = reinterpret_cast<float*>(base);
+            s->ml = reinterpret_cast<float*>(base + triples * c.head_dim * 4);
+            s->where = reinterpret_cast<uint32_t*>(base + used);
+        }
         used += ((int64_t)s->row_groups * (s->prefix ? 1 : a.batch) * c.heads * 8 + 15) / 16 * 16;
     }
     return used;
