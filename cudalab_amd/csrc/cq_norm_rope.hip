@@ -21,7 +21,6 @@ namespace cq {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int64_t kManyHeads = 1 << 16;       // 256 CUs of four waves of eight groups of eight
 
 __device__ __forceinline__ float load_weight(const void* p, int dtype, int i) {
     if (dtype == CQ_DTYPE_F16) return (float)static_cast<const _Float16*>(p)[i];
@@ -290,28 +289,34 @@ hipError_t launch_typed(const cq_norm_rope_t& a, hipStream_t stream) {
             weight_wide(a.q_weight) && weight_wide(a.k_weight));
         return hipGetLastError();
     };
-    // Few heads in all: one to a group, so that each wave has as little to wait
-    // for as can be.  Many: eight, whose weights and tables are fetched once,
-    // with 16 bytes of each end in flight for two heads (8192 tokens of 64 heads
-    // of 128: 52 us; one head 55, four 58; one head to a group 77; pieces of 8
-    // bytes, four heads in flight, 70).
-    constexpr int kHeads = 8;
-    const bool many = a.tokens * heads > kManyHeads;
-    if (many && vector_ok(a, sizeof(T), 8)) {
-#define CQ_GO(L) go(&norm_rope_kernel<T, PAIRS, 8, L, 2>, 8, L, kHeads)
-        if (a.head_dim <= 64) return CQ_GO(4);
-        if (a.head_dim <= 128) return CQ_GO(8);
-        if (a.head_dim <= 256) return CQ_GO(16);
-        return CQ_GO(32);
-#undef CQ_GO
+    // Pieces of 16 bytes of each end, two heads in flight and weights and tables
+    // fetched once for several heads, as long as waves enough are left: by how
+    // many there are with one head to a group.  Few: one, in pieces of four
+    // elements, so that each wave has as little to wait for as can be.  fp16 heads
+    // of 128, us with one head to a group in pieces of 8 and 16 bytes, then with
+    // two, four and eight:
+    //   16384 heads (2048 waves)   5.8  5.4  5.9  7.6 11.5
+    //   65536       (8192)        14.0 12.9  9.8 11.4 14.2
+    //   169696      (21212)       33.9 29.5 23.8 23.1 23.1
+    //   524288      (65536)       95.9 83.8 68.2 59.5 57.4
+    // (FP32 in pieces of 32 bytes is slower: 262144 heads 65 us, of 16 bytes 58.)
+    const int lanes = a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : a.head_dim <= 256 ? 32 : 64;
+    const bool wide_ok = sizeof(T) == 2 && vector_ok(a, sizeof(T), 8);
+    const int64_t waves = a.tokens * heads * (wide_ok ? lanes / 2 : lanes) / 64;
+    const int64_t each = waves < 4096 ? 1 : waves <= 8192 ? 2 : waves < 32768 ? 4 : 8;
+#define CQ_GO(C, L, B) go(&norm_rope_kernel<T, PAIRS, C, L, B>, C, L, each)
+    if constexpr (sizeof(T) == 2) {
+        if (wide_ok && each > 1) {
+            if (a.head_dim <= 64) return CQ_GO(8, 4, 2);
+            if (a.head_dim <= 128) return CQ_GO(8, 8, 2);
+            if (a.head_dim <= 256) return CQ_GO(8, 16, 2);
+            return CQ_GO(8, 32, 2);
+        }
     }
-#define CQ_GO(L)                                                            \
-    (many ? go(&norm_rope_kernel<T, PAIRS, 4, L, 4>, 4, L, kHeads)           \
-          : go(&norm_rope_kernel<T, PAIRS, 4, L, 1>, 4, L, 1))
-    if (a.head_dim <= 64) return CQ_GO(8);
-    if (a.head_dim <= 128) return CQ_GO(16);
-    if (a.head_dim <= 256) return CQ_GO(32);
-    return CQ_GO(64);
+    if (lanes == 8) return each > 1 ? CQ_GO(4, 8, 2) : CQ_GO(4, 8, 1);
+    if (lanes == 16) return each > 1 ? CQ_GO(4, 16, 2) : CQ_GO(4, 16, 1);
+    if (lanes == 32) return each > 1 ? CQ_GO(4, 32, 2) : CQ_GO(4, 32, 1);
+    return each > 1 ? CQ_GO(4, 64, 2) : CQ_GO(4, 64, 1);
 #undef CQ_GO
 }
 

@@ -203,3 +203,23 @@ def test_many_heads(att, dtype, inter, d, rot, shift):
         for a, b in ((gq[part], sq), (gk[part], sk)):
             assert bool(((a.double() - b.double()).abs()
                          <= 2 * UNIT[dt] * b.double().abs() + 2 * 16 * 2.0 ** -24 * 16).all())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("tokens,hq,hkv,d,rot", [(2500, 13, 2, 128, 64), (901, 64, 9, 128, 128),
+                                                 (5003, 7, 1, 256, 256), (20011, 3, 1, 64, 64),
+                                                 (1501, 21, 3, 512, 512)])
+def test_two_and_four_heads_to_a_group(att, dtype, tokens, hq, hkv, d, rot):
+    """Between one head to a group and eight, at counts that leave groups short."""
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    dt = DT[dtype]
+    q, k = (torch.randn(tokens, h, d, generator=g, device="cuda").to(dt) for h in (hq, hkv))
+    qw, kw = ((1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(dt) for _ in range(2))
+    cos, sin = (t.cuda() for t in _tables(50, rot))
+    pos = torch.randint(0, 50, (tokens,), generator=g, dtype=torch.int32, device="cuda")
+    announce(f"norm_rope some heads {dtype} {tokens}x({hq}+{hkv})x{d} rot={rot}")
+    gq, gk = att.qk_norm_rope(q, k, qw, kw, cos, sin, pos)
+    some = torch.linspace(0, tokens - 1, 24).long()
+    for got, x, w, name in ((gq, q, qw, "q"), (gk, k, kw, "k")):
+        _check(got[some], x[some].cpu(), w.cpu(), cos.cpu(), sin.cpu(), pos[some].cpu(), False,
+               name)
