@@ -20,7 +20,9 @@
 // score is the same for every key of a row, so the score sums start at minus
 // that.  V's codes go in as they are: there a common offset would cost digits
 // where a key of large weight has small codes.  q is brought to fp16 times a
-// power of two that puts the wave's largest finite element into [2^13, 2^14).
+// power of two, the row's own, that puts its largest finite element into
+// [2^13, 2^14): rows share waves with other heads, tokens and sequences, and
+// with rows past the counts, whose numbers may be any.
 //
 // Matrix form, 64 keys at a time (v_mfma_f32_16x16x32_f16, FP32 sums):
 //   S^T [keys x rows] = K [keys x D] Q^T [D x rows]
@@ -352,11 +354,14 @@ struct Rows {
     static constexpr int kOTiles = D / 16;
     static constexpr float kOffset = BITS == 8 ? 128.f : 8.f;
     static constexpr float kUnit = 0x1p-24f;
+    // 1 / kUnit, half of it in K's scale and half in q's: neither leaves FP32's
+    // range by it
+    static constexpr float kHalfUnit = RAW ? 0x1p12f : 1.f;
     static constexpr uint32_t kInf = std::is_same_v<T, _Float16> ? 0x7C00u : 0x7F80u;
 
     h8 q[NB][kSteps];
     float start[NB];                     // what the score sums start at
-    float qscale;                        // of a score sum: scale log2(e), units, q's factor
+    float qscale[NB];                    // of a score sum: scale log2(e), units, q's factor
     int limit[NB];                       // keys that the lane's row sees
     int full;                            // tiles of which every row sees all
     f4 o[NB][kOTiles];
@@ -368,7 +373,7 @@ struct Rows {
                                          Dim&& dim) {
         int least = 0x7FFFFFFF;
         Vec<T, 8> raw[NB][kSteps];
-        uint32_t top2 = 0;
+        uint32_t top2[NB] = {};
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
             // rows past the last repeat it (nobody stores them)
@@ -390,20 +395,19 @@ struct Rows {
                     // is negative in 16 bits
                     const uint32_t m = w[i] & 0x7FFF7FFFu;
                     const ss2 bad = __builtin_bit_cast(ss2, m + (0x8000u - kInf) * 0x10001u) >> 15;
-                    top2 = pk_max(top2, m & ~__builtin_bit_cast(uint32_t, bad));
+                    top2[rb] = pk_max(top2[rb], m & ~__builtin_bit_cast(uint32_t, bad));
                 }
             }
         }
-        const uint32_t bits = max(top2 & 0xFFFFu, top2 >> 16);
-        // One factor for the wave: exact down to 2^-27 of its largest element,
-        // 2^-38 of that where fp16 is subnormal, so an error far below FP32's
-        // in the largest row's scores is all that a small row can show.
-        const float top =
-            wave_max((float)__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
-        const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
-        qscale = ldexpf(s.a.softmax_scale * kLog2e * (RAW ? 1.f / kUnit : 1.f), e);
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
+            // exact down to 2^-27 of the row's largest element, to 2^-38 of it
+            // where fp16 is subnormal: far below the scores' own rounding
+            const uint32_t bits = max(top2[rb] & 0xFFFFu, top2[rb] >> 16);
+            const float top =
+                quad_max((float)__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
+            const int e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 14 : 0;
+            qscale[rb] = ldexpf(s.a.softmax_scale * kLog2e * kHalfUnit, e);
             float sum = 0.f;
 #pragma unroll
             for (int u = 0; u < kSteps; ++u)
@@ -432,8 +436,7 @@ struct Rows {
     // adding to l.  sc[.][t][i] is the lane's row against key 16 g + 4 t + i of
     // the tile (lane group g = lane / 16); ks, vs are the scales of key `lane`,
     // `there` whether the group's keys have a page.  Each lane prepares one key
-    // for the 16 lanes of its row, whose keys these are: K's scale with all that
-    // a score takes, V's as f 2^e.
+    // for the 16 lanes of its row, whose keys these are: K's scale, V's as f 2^e.
     //
     // Where every row sees every key and V's scales lie within 2^kEven of the
     // largest, e is the tile's largest instead: the weight of the key with the
@@ -445,12 +448,12 @@ struct Rows {
         const int most = kShort ? __builtin_amdgcn_readfirstlane((int)wave_max((float)e)) : 0;
         const bool even = kShort && tile < full && most < 128 && __all(there && e >= most - kEven);
         const int by = even ? most : e;
-        const float kf = ks * qscale, ef = (float)by, vf = __builtin_amdgcn_ldexpf(vs, -by);
+        const float kf = ks * kHalfUnit, ef = (float)by, vf = __builtin_amdgcn_ldexpf(vs, -by);
         const float back = __builtin_amdgcn_ldexpf(1.f, -by);
-        float kfs[16];
-        sixteen([&](auto j) { kfs[j] = of_lane<j>(kf); });
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
+            float kfs[16];
+            sixteen([&](auto j) { kfs[j] = of_lane<j>(kf) * qscale[rb]; });
             // keys of the lane's 16 that its row sees
             const int n = there ? limit[rb] - tile * kTile - (lane & 48) : 0;
             float x[16];
