@@ -10,9 +10,17 @@
 // and raises M (scaling l and o down) when an exponent passes kRaise; triples
 // (M, l, o) of disjoint keys join the same way.  Folding V's exponent into
 // that of the softmax keeps w_j, which the matrix instructions take as fp16,
-// in range for any scales: the largest w of a row lies in [2^-5, 2^kRaise), and
-// what fp16 then rounds off is 2^-11 of each weight, or 2^-25 of 1.
-// Scores, statistics and sums are FP32.
+// in range: the largest w of a row lies in [2^-5, 2^kRaise), and what fp16 then
+// rounds off is 2^-11 of each weight, or 2^-25 of 1.  Scores, statistics and
+// sums are FP32.
+//
+// A key counts in l whatever its V scale, so l's term 2^(s_j log2(e) - M) is
+// 2^-e_j times the exponential that w_j takes, and that must stay inside FP32's
+// exponents.  So e_j is taken no lower than kSpan below the largest that the wave
+// has met (a scale of zero has no exponent of its own, and smaller ones only a
+// smaller f): keys down to 2^-56 of the row's largest probability are counted, and
+// scales down to 2^-80 of the largest seen keep their digits.  l itself, a raise
+// or a join may move by more than one exponential holds; it is scaled in two.
 //
 // A code of K goes into the matrix units as the fp16 subnormal
 // (code + 2^(bits-1)) 2^-24, which is the code's bits with the sign bit turned
@@ -75,7 +83,9 @@ constexpr int kTile = 64;               // keys of a tile
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 8.f;
-constexpr int kLeastExp = -100;         // a V scale below 2^-100 counts as 0
+constexpr int kSpan = 70;               // of the exponents of V's scales
+constexpr int kLeastExp = -96;          // 2^23 terms of l of 2^(96 + kRaise) fit FP32
+constexpr int kMostExp = 122;           // of the largest numbers' scales; also Inf's, NaN's
 constexpr int kEven = 4;
 
 using h8 = Vec<_Float16, 8>;
@@ -126,6 +136,26 @@ __device__ __forceinline__ float quad_max(float v) {
 }
 __device__ __forceinline__ float quad_sum(float v) {
     return quad_fold(v, [](float a, float b) { return a + b; });
+}
+// f over the 16 lanes of a row, in each.
+template <class F>
+__device__ __forceinline__ int row_fold(int v, F&& f) {
+    v = f(v, (int)row_dpp<0x128>((uint32_t)v));
+    v = f(v, (int)row_dpp<0x124>((uint32_t)v));
+    v = f(v, (int)row_dpp<0x122>((uint32_t)v));
+    return f(v, (int)row_dpp<0x121>((uint32_t)v));
+}
+__device__ __forceinline__ int row_min(int v) {
+    return row_fold(v, [](int a, int b) { return min(a, b); });
+}
+__device__ __forceinline__ int row_max(int v) {
+    return row_fold(v, [](int a, int b) { return max(a, b); });
+}
+// Maximum over the wave, for the scalar unit.
+__device__ __forceinline__ int wave_most(int v) {
+    v = row_max(v);
+    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, row_dpp<0x128>(v));
@@ -274,11 +304,12 @@ __device__ __forceinline__ void codes_of_nibbles(uint32_t w, uint32_t (&p)[4]) {
     p[3] = less((x & 0x00F000F0u) ^ 0x54805480u, 72.f);
 }
 
-// What a triple's sums are multiplied with to stand at reference `top`.  One
-// that has seen no number has M = -Inf and sums of 0, or of NaN where it saw
-// only NaN: l itself then.
-__device__ __forceinline__ float factor(float m, float l, float top) {
-    return m == kNegInf ? l : __builtin_amdgcn_exp2f(m - top);
+// The root of what a triple's sums are multiplied with to stand at reference
+// `top`: l is large where V's scales are small, so it may be in range there
+// though 2^(m - top) is not.  One that has seen no number has M = -Inf and sums
+// of 0, or of NaN where it saw only NaN: l itself then.
+__device__ __forceinline__ float root(float m, float l, float top) {
+    return m == kNegInf ? l : __builtin_amdgcn_exp2f(0.5f * (m - top));
 }
 
 template <class T>
@@ -364,6 +395,8 @@ struct Rows {
     float qscale[NB];                    // of a score sum: scale log2(e), units, q's factor
     int limit[NB];                       // keys that the lane's row sees
     int full;                            // tiles of which every row sees all
+    int reach;                           // keys that some row sees
+    int largest;                         // exponent of V's scales met so far
     f4 o[NB][kOTiles];
     float l[NB], ref[NB], raise[NB];
 
@@ -371,7 +404,7 @@ struct Rows {
     template <class Dim>
     __device__ __forceinline__ void load(const Source& s, int b, int first_row, int h, int lane,
                                          Dim&& dim) {
-        int least = 0x7FFFFFFF;
+        int least = 0x7FFFFFFF, most = 0;
         Vec<T, 8> raw[NB][kSteps];
         uint32_t top2[NB] = {};
 #pragma unroll
@@ -383,6 +416,7 @@ struct Rows {
             limit[rb] = s.prefix ? (at.t < count ? s.a.prefix_len : 0)
                                  : own_limit(s, s.a.lengths[at.b], count, at.t);
             least = min(least, limit[rb]);
+            most = max(most, limit[rb]);
             const T* p = static_cast<const T*>(s.a.q) + at.b * s.a.q_batch_stride +
                          at.t * s.a.q_token_stride + at.hq * s.a.q_head_stride;
 #pragma unroll
@@ -420,9 +454,9 @@ struct Rows {
                 }
             start[rb] = RAW ? -kOffset * kUnit * quad_sum(sum) : 0.f;
         }
-#pragma unroll
-        for (int off = 1; off < 16; off <<= 1) least = min(least, __shfl_xor(least, off));
-        full = __builtin_amdgcn_readfirstlane(least) / kTile;
+        full = __builtin_amdgcn_readfirstlane(row_min(least)) / kTile;
+        reach = __builtin_amdgcn_readfirstlane(row_max(most));
+        largest = kLeastExp;
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
             l[rb] = ref[rb] = 0.f;
@@ -444,12 +478,17 @@ struct Rows {
     // one addition for 16 keys instead of two operations for each.
     __device__ __forceinline__ void weights(const f4 (&sc)[NB][4], float ks, float vs, bool there,
                                             int tile, int lane, h8 (&w)[NB][2]) {
-        const int e = max((int)((__float_as_uint(vs) >> 23) & 0xFF) - 126, kLeastExp);
-        const int most = kShort ? __builtin_amdgcn_readfirstlane((int)wave_max((float)e)) : 0;
-        const bool even = kShort && tile < full && most < 128 && __all(there && e >= most - kEven);
-        const int by = even ? most : e;
-        const float kf = ks * kHalfUnit, ef = (float)by, vf = __builtin_amdgcn_ldexpf(vs, -by);
-        const float back = __builtin_amdgcn_ldexpf(1.f, -by);
+        // (a branch around the maximum costs the products their schedule: 1024
+        // new tokens 351 us with it, 341 without)
+        const int own = (int)((__float_as_uint(vs) >> 23) & 0xFF) - 126;
+        const bool met = there && tile * kTile + lane < reach && own <= kMostExp;
+        const int most = wave_most(met ? own : kLeastExp);
+        largest = max(largest, most);
+        const int least = max(largest - kSpan, kLeastExp);
+        const bool even = kShort && tile < full && __all(met && own >= most - kEven);
+        const int e = even ? max(most, least) : min(max(own, least), kMostExp);
+        const float kf = ks * kHalfUnit, ef = (float)e, vf = __builtin_amdgcn_ldexpf(vs, -e);
+        const float back = __builtin_amdgcn_ldexpf(1.f, -e);
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
             float kfs[16];
@@ -476,10 +515,11 @@ struct Rows {
                 top = quad_max(top);
                 const bool first = raise[rb] == kNegInf;
                 if (top > (first ? kNegInf : 0.f)) {
-                    const float keep = first ? 1.f : __builtin_amdgcn_exp2f(-top);
+                    const float half = first ? 1.f : __builtin_amdgcn_exp2f(-0.5f * top);
+                    const float keep = half * half;
                     ref[rb] += top;
                     raise[rb] = kRaise;
-                    l[rb] *= keep;
+                    l[rb] = l[rb] * half * half;
 #pragma unroll
                     for (int i = 0; i < kOTiles; ++i) o[rb][i] *= keep;
 #pragma unroll
@@ -852,9 +892,9 @@ __global__ __launch_bounds__(kBlock, waves_of(D, NB)) void tile_kernel(Source s)
             f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int v = 0; v < kWaves; ++v) {
-                const float keep = factor(sm_m[v][r], sm_l[v][r], top);
-                sum += sm_l[v][r] * keep;
-                x += *reinterpret_cast<const f4*>(&sm_o[v][r][dim]) * keep;
+                const float by = root(sm_m[v][r], sm_l[v][r], top);
+                sum += sm_l[v][r] * by * by;
+                x += *reinterpret_cast<const f4*>(&sm_o[v][r][dim]) * (by * by);
             }
             const Sink<T, D> sink(s, b, h, row0, tile == 0 && end == n, tile > 0, row0 + r);
             if (dim == 0) sink.put(top, sum);
@@ -1133,12 +1173,12 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
                 v[i] = *reinterpret_cast<const VE*>(
                     own.o + triple(min(base + i, count - 1)) * D + lane * E);
             const float top = fmaxf(ref, wave_max(ml[0]));
-            const float keep = factor(ref, sum, top);
-            const float by = factor(ml[0], ml[1], top);
-            const float share = by * ml[1];
-            sum *= keep;
+            const float keep = root(ref, sum, top);
+            const float half = root(ml[0], ml[1], top);
+            const float by = half * half, share = ml[1] * half * half;
+            sum = sum * keep * keep;
 #pragma unroll
-            for (int j = 0; j < E; ++j) acc[j] *= keep;
+            for (int j = 0; j < E; ++j) acc[j] *= keep * keep;
             ref = top;
 #pragma unroll
             for (int i = 0; i < J; ++i) {
@@ -1167,10 +1207,10 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
             acc = VE{};
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                const float by = factor(part[i][D], part[i][D + 1], top);
-                sum += by * part[i][D + 1];
+                const float by = root(part[i][D], part[i][D + 1], top);
+                sum += part[i][D + 1] * by * by;
 #pragma unroll
-                for (int j = 0; j < E; ++j) acc[j] += by * part[i][lane * E + j];
+                for (int j = 0; j < E; ++j) acc[j] += by * by * part[i][lane * E + j];
             }
         }
         T* out = static_cast<T*>(a.out) + row * D + lane * E;
