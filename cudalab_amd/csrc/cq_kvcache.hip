@@ -314,6 +314,12 @@ __global__ __launch_bounds__(kBlock) void read_kernel(cq_kv_cache_t c, cq_kv_slo
 // Tiles that the tokens of a sequence may touch, wherever they start.
 int64_t tiles_of(const cq_kv_slots_t& s) { return ((int64_t)s.tokens + 15 + 15) / 16; }
 
+// Workgroups of a call; kMaxGrid + 1 for more (the product may pass 64 bits).
+int64_t workgroups(const cq_kv_cache_t& c, const cq_kv_slots_t& s) {
+    const __int128 n = (__int128)s.batch * tiles_of(s) * c.heads;
+    return n <= kMaxGrid ? (int64_t)n : kMaxGrid + 1;
+}
+
 template <class F>
 hipError_t by_form(const cq_kv_cache_t& c, F&& go) {
     if (c.bits == 8)
@@ -328,7 +334,7 @@ hipError_t by_form(const cq_kv_cache_t& c, F&& go) {
 template <class T>
 hipError_t append_typed(const cq_kv_cache_t& c, const cq_kv_slots_t& s, const void* k,
                         KvStrides ks, const void* v, KvStrides vs, hipStream_t stream) {
-    const int64_t tiles = tiles_of(s), grid = (int64_t)s.batch * tiles * c.heads;
+    const int64_t tiles = tiles_of(s), grid = workgroups(c, s);
     if (grid > kMaxGrid) return hipErrorInvalidValue;
     return by_form(c, [&](auto bits, auto dim) {
         constexpr int E = decltype(dim)::value / 16;
@@ -348,7 +354,7 @@ hipError_t append_typed(const cq_kv_cache_t& c, const cq_kv_slots_t& s, const vo
 template <class T>
 hipError_t read_typed(const cq_kv_cache_t& c, const cq_kv_slots_t& s, void* k, void* v,
                       hipStream_t stream) {
-    const int64_t tiles = tiles_of(s), grid = (int64_t)s.batch * tiles * c.heads;
+    const int64_t tiles = tiles_of(s), grid = workgroups(c, s);
     if (grid > kMaxGrid) return hipErrorInvalidValue;
     return by_form(c, [&](auto bits, auto dim) {
         read_kernel<T, decltype(bits)::value, decltype(dim)::value>
