@@ -1102,12 +1102,13 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
 
 // Joins the triples of rows: those of their own keys' runs and, with a prefix,
 // those of the prefix's.  `W` waves per row, each its share of the triples, and
-// `each` rows of a unit in turn.  Rows that a run has finished are left alone;
-// rows without any keys become zeros.
+// `each` rows of a unit in turn, from the launch's first workgroup on.  Rows
+// that a run has finished are left alone; rows without any keys become zeros.
 template <int D>
 constexpr int in_flight = D == 256 ? 8 : 16;       // triples
 template <class T, int D, int W>
-__global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, int each) {
+__global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, int each,
+                                                      uint32_t first_block) {
     constexpr int E = D / 64, J = in_flight<D>;
     using VE = Vec<float, E>;
     __shared__ float part[W > 1 ? W : 1][W > 1 ? D + 2 : 1];
@@ -1115,7 +1116,8 @@ __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, 
     const cq_attention_t& a = own.a;
     const uint32_t blocks = (own.rows + each - 1) / each;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t place = W == 1 ? blockIdx.x * kWaves + w : blockIdx.x;
+    const uint32_t block = first_block + blockIdx.x;
+    const uint32_t place = W == 1 ? block * kWaves + w : block;
     const uint32_t unit = place / blocks;
     const int r0 = (place - unit * blocks) * each;
     const int h = unit % own.c.heads, b = unit / own.c.heads;
@@ -1346,13 +1348,14 @@ hipError_t launch_typed(const Source& own, Shape os, const Source& ahead, Shape 
     const int64_t runs = own.runs / ((int64_t)own.row_groups * own.a.batch * own.c.heads) +
                          (ahead.rows > 0 ? ahead.runs / ((int64_t)ahead.row_groups * own.c.heads)
                                          : 0);
-    if (each == 1 && places <= 4 * kCus && runs > in_flight<D>)
-        join_kernel<T, D, kWaves><<<dim3((unsigned)places), dim3(kBlock), 0, stream>>>(own, ahead,
-                                                                                       each);
-    else
-        join_kernel<T, D, 1><<<dim3((unsigned)((places + kWaves - 1) / kWaves)), dim3(kBlock), 0,
-                               stream>>>(own, ahead, each);
-    return hipGetLastError();
+    const bool four = each == 1 && places <= 4 * kCus && runs > in_flight<D>;
+    const int64_t grid = four ? places : (places + kWaves - 1) / kWaves;
+    return launch_parts(grid, [&](dim3 blocks, uint32_t first) {
+        if (four)
+            join_kernel<T, D, kWaves><<<blocks, dim3(kBlock), 0, stream>>>(own, ahead, each, first);
+        else
+            join_kernel<T, D, 1><<<blocks, dim3(kBlock), 0, stream>>>(own, ahead, each, first);
+    });
 }
 
 }  // namespace

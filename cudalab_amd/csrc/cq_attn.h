@@ -4,6 +4,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -15,8 +16,21 @@ namespace cq {
 // (cq_capi.cpp).
 int set_error(int code, const std::string& msg);
 
-// Workgroups a launch may have (the grid's x dimension).
+// Workgroups of all of a call's launches (31 bits in the kernels), and those of
+// 256 threads that one launch may have: HIP counts a launch's threads in 32 bits.
 constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+constexpr int64_t kMaxLaunch = 0xFFFFFFFF / 256;
+
+// go(workgroups, first) for each launch of a call of `grid` workgroups.
+template <class Go>
+hipError_t launch_parts(int64_t grid, Go&& go) {
+    hipError_t e = hipSuccess;
+    for (int64_t first = 0; first < grid && e == hipSuccess; first += kMaxLaunch) {
+        go(dim3((unsigned)std::min(grid - first, kMaxLaunch)), (uint32_t)first);
+        e = hipGetLastError();
+    }
+    return e;
+}
 
 // Launchers: arguments are checked, sizes are positive.  A launcher that
 // finds its grid beyond kMaxGrid returns hipErrorInvalidValue unlaunched.

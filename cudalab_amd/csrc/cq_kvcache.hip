@@ -188,18 +188,20 @@ struct Tile {
 };
 
 // One workgroup per (sequence, tile, head), heads side by side: neighbouring
-// workgroups read neighbouring rows.
+// workgroups read neighbouring rows.  `first` is the launch's first workgroup.
 template <class T, int BITS, int D>
 __global__ __launch_bounds__(kBlock) void append_kernel(cq_kv_cache_t c, cq_kv_slots_t s,
                                                         uint32_t tiles, const T* k, KvStrides ks,
-                                                        const T* v, KvStrides vs, bool wide) {
+                                                        const T* v, KvStrides vs, bool wide,
+                                                        uint32_t first) {
     constexpr int E = D / 16;
     constexpr int R = BITS == 8 ? D : D / 2;       // bytes of a row
     using C = Codes<BITS, E>;
     // a lane's rows, and 16 bytes of padding
     __shared__ __attribute__((aligned(16))) uint8_t turned[16][C::kBytes * 16 + 16];
-    const int h = blockIdx.x % c.heads;
-    const uint32_t bt = blockIdx.x / c.heads;
+    const uint32_t block = first + blockIdx.x;
+    const int h = block % c.heads;
+    const uint32_t bt = block / c.heads;
     const int b = bt / tiles;
     const Tile tile(c, s, b, bt % tiles);
     const int i = threadIdx.x >> 4, lane = threadIdx.x & 15;
@@ -253,14 +255,16 @@ __global__ __launch_bounds__(kBlock) void append_kernel(cq_kv_cache_t c, cq_kv_s
 
 template <class T, int BITS, int D>
 __global__ __launch_bounds__(kBlock) void read_kernel(cq_kv_cache_t c, cq_kv_slots_t s,
-                                                      uint32_t tiles, T* k, T* v) {
+                                                      uint32_t tiles, T* k, T* v,
+                                                      uint32_t first) {
     constexpr int E = D / 16;
     constexpr int R = BITS == 8 ? D : D / 2;
     using C = Codes<BITS, E>;
     // 16 bytes of padding a token: four tokens' words lie in different banks
     __shared__ __attribute__((aligned(16))) uint8_t turned[16][R + 16];
-    const int h = blockIdx.x % c.heads;
-    const uint32_t bt = blockIdx.x / c.heads;
+    const uint32_t block = first + blockIdx.x;
+    const int h = block % c.heads;
+    const uint32_t bt = block / c.heads;
     const int b = bt / tiles;
     const Tile tile(c, s, b, bt % tiles);
     const int i = threadIdx.x >> 4, lane = threadIdx.x & 15;
@@ -343,11 +347,12 @@ hipError_t append_typed(const cq_kv_cache_t& c, const cq_kv_slots_t& s, const vo
         for (const KvStrides& st : {ks, vs})
             wide = wide && st.batch % N == 0 && st.token % N == 0 && st.head % N == 0;
         wide = wide && (uintptr_t)k % (N * sizeof(T)) == 0 && (uintptr_t)v % (N * sizeof(T)) == 0;
-        append_kernel<T, decltype(bits)::value, decltype(dim)::value>
-            <<<dim3((unsigned)grid), dim3(kBlock), 0, stream>>>(
-                c, s, (uint32_t)tiles, static_cast<const T*>(k), ks, static_cast<const T*>(v), vs,
-                wide);
-        return hipGetLastError();
+        return launch_parts(grid, [&](dim3 blocks, uint32_t first) {
+            append_kernel<T, decltype(bits)::value, decltype(dim)::value>
+                <<<blocks, dim3(kBlock), 0, stream>>>(c, s, (uint32_t)tiles,
+                                                      static_cast<const T*>(k), ks,
+                                                      static_cast<const T*>(v), vs, wide, first);
+        });
     });
 }
 
@@ -357,10 +362,11 @@ hipError_t read_typed(const cq_kv_cache_t& c, const cq_kv_slots_t& s, void* k, v
     const int64_t tiles = tiles_of(s), grid = workgroups(c, s);
     if (grid > kMaxGrid) return hipErrorInvalidValue;
     return by_form(c, [&](auto bits, auto dim) {
-        read_kernel<T, decltype(bits)::value, decltype(dim)::value>
-            <<<dim3((unsigned)grid), dim3(kBlock), 0, stream>>>(
-                c, s, (uint32_t)tiles, static_cast<T*>(k), static_cast<T*>(v));
-        return hipGetLastError();
+        return launch_parts(grid, [&](dim3 blocks, uint32_t first) {
+            read_kernel<T, decltype(bits)::value, decltype(dim)::value>
+                <<<blocks, dim3(kBlock), 0, stream>>>(c, s, (uint32_t)tiles, static_cast<T*>(k),
+                                                      static_cast<T*>(v), first);
+        });
     });
 }
 

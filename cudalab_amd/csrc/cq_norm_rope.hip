@@ -79,13 +79,15 @@ struct Head {
 // rows aligned to C elements, tables to 16 bytes.  A group of LANES lanes takes
 // heads part, part + parts, ... of one token, BATCH loads of each end in
 // flight; lane l holds elements e0..e0+C-1 and e1..e1+C-1, in the half style
-// the two ends of pairs Cl..Cl+C-1, else 2 C neighbours.
+// the two ends of pairs Cl..Cl+C-1, else 2 C neighbours.  `first` is the
+// launch's first workgroup.
 template <class T, bool PAIRS, int C, int LANES, int BATCH>
 __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uint32_t parts,
-                                                           uint32_t iters, bool wide) {
+                                                           uint32_t iters, bool wide,
+                                                           uint32_t first) {
     using V = Vec<T, C>;
     const int lane = threadIdx.x % LANES;
-    const uint32_t group = blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+    const uint32_t group = (first + blockIdx.x) * (kBlock / LANES) + threadIdx.x / LANES;
     const int heads = a.q_heads + a.k_heads;
     // groups past the last token repeat it and store nothing
     const bool live = group / parts < a.tokens;
@@ -191,9 +193,10 @@ __global__ __launch_bounds__(kBlock) void norm_rope_kernel(cq_norm_rope_t a, uin
 constexpr int kMaxPairs = 8;      // head_dim <= 1024
 
 template <class T>
-__global__ __launch_bounds__(kBlock) void norm_rope_any_kernel(cq_norm_rope_t a) {
+__global__ __launch_bounds__(kBlock) void norm_rope_any_kernel(cq_norm_rope_t a,
+                                                               uint32_t first) {
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
+    const int64_t unit = (int64_t)(first + blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
     const int heads = a.q_heads + a.k_heads;
     const int64_t token = unit / heads;
     if (token >= a.tokens) return;                 // uniform over the wave
@@ -274,8 +277,9 @@ hipError_t launch_typed(const cq_norm_rope_t& a, hipStream_t stream) {
     if (!vector_ok(a, sizeof(T), 4)) {
         const int64_t units = a.tokens * heads, grid = (units + kBlock / 64 - 1) / (kBlock / 64);
         if (grid > kMaxGrid) return hipErrorInvalidValue;
-        norm_rope_any_kernel<T><<<dim3((unsigned)grid), dim3(kBlock), 0, stream>>>(a);
-        return hipGetLastError();
+        return launch_parts(grid, [&](dim3 blocks, uint32_t first) {
+            norm_rope_any_kernel<T><<<blocks, dim3(kBlock), 0, stream>>>(a, first);
+        });
     }
     auto go = [&](auto* kernel, int c, int lanes, int64_t iters) {
         const int64_t per = kBlock / lanes;
@@ -284,10 +288,11 @@ hipError_t launch_typed(const cq_norm_rope_t& a, hipStream_t stream) {
         auto weight_wide = [&](const void* p) {
             return a.weight_dtype == CQ_DTYPE_F32 || (uintptr_t)p % (2 * c) == 0;
         };
-        kernel<<<dim3((unsigned)((groups + per - 1) / per)), dim3(kBlock), 0, stream>>>(
-            a, (uint32_t)parts, (uint32_t)iters,
-            weight_wide(a.q_weight) && weight_wide(a.k_weight));
-        return hipGetLastError();
+        const bool wide = weight_wide(a.q_weight) && weight_wide(a.k_weight);
+        return launch_parts((groups + per - 1) / per, [&](dim3 blocks, uint32_t first) {
+            kernel<<<blocks, dim3(kBlock), 0, stream>>>(a, (uint32_t)parts, (uint32_t)iters, wide,
+                                                        first);
+        });
     };
     // Pieces of 16 bytes of each end, two heads in flight and weights and tables
     // fetched once for several heads, as long as waves enough are left: by how
