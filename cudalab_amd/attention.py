@@ -366,7 +366,9 @@ class AttentionExt:
         if batch == 0 or tokens == 0:
             return
         if q.data_ptr() % 16 or any(s % 8 for s in q.stride()[:3]):
-            q = q.contiguous()      # the kernels read 16 bytes of a head at once
+            # the kernels read 16 bytes of a head at once; a q that is contiguous
+            # may still start, or have a dimension of one, off them
+            q = torch.empty(q.shape, dtype=q.dtype, device=dev).copy_(q)
         a.q, a.out = q.data_ptr(), out.data_ptr()
         a.q_batch_stride, a.q_token_stride, a.q_head_stride = q.stride()[:3]
         a.table, a.lengths = block_table.data_ptr(), lengths.data_ptr()
