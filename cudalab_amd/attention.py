@@ -83,6 +83,21 @@ def _table(name: str, t: torch.Tensor, batch: int, device: torch.device) -> None
         _fail(f"the rows of {name} must be contiguous")
 
 
+def _number(name: str, x) -> float:
+    try:
+        if hasattr(x, "__float__"):
+            return float(x)
+    except (TypeError, ValueError, OverflowError):
+        pass
+    _fail(f"{name} must be a number that a float holds, got {type(x).__name__}")
+
+
+def _pair(prefix) -> tuple:
+    if not isinstance(prefix, (tuple, list)) or len(prefix) != 2:
+        _fail(f"prefix must be a pair (pages, length), got {type(prefix).__name__}")
+    return prefix
+
+
 class AttentionExt:
     """Norms with rotation, the quantized cache and attention over it."""
 
@@ -105,6 +120,7 @@ class AttentionExt:
         """RMS norm of each head of q (tokens, Hq, D) and k (tokens, Hkv, D),
         then the rotation of its first R dims, into new contiguous tensors.
         See qk_norm_rope_into."""
+        eps, interleaved = _number("eps", eps), bool(interleaved)
         if self._fast is not None:
             got = self._fast.norm_rope(q, k, None, None, q_weight, k_weight, cos, sin,
                                        positions, eps, interleaved)
@@ -132,6 +148,7 @@ class AttentionExt:
         row positions[token] (int32 or int64).  Tokens and heads may have any
         stride; a position outside the tables turns the token's rotated dims
         into NaN."""
+        eps, interleaved = _number("eps", eps), bool(interleaved)
         if self._fast is not None and q_out is not None and k_out is not None \
                 and self._fast.norm_rope(q, k, q_out, k_out, q_weight, k_weight, cos, sin,
                                          positions, eps, interleaved) is not None:
@@ -203,7 +220,7 @@ class AttentionExt:
         a.tokens, a.q_heads, a.k_heads, a.head_dim = tokens, q.size(1), k.size(1), D
         a.dtype = _DTYPES[q.dtype]
         a.weight_dtype = _DTYPES[wdt or torch.float32]
-        a.interleaved, a.eps = bool(interleaved), eps
+        a.interleaved, a.eps = interleaved, eps
         _check(_on_device(dev, lambda s: self._lib.cq_qk_norm_rope(ctypes.byref(a), s)),
                "qk_norm_rope")
 
@@ -286,6 +303,8 @@ class AttentionExt:
                 scale: Optional[float] = None) -> torch.Tensor:
         """Attention of q (batch, tokens, Hq, D), float16 or bfloat16, over the
         cache, into a new tensor of q's shape and type.  See forward_into."""
+        if scale is not None:
+            scale = _number("scale", scale)
         got = self._fast_forward(q, cache, block_table, lengths, None, counts, prefix, scale)
         if got is not None:
             return got
@@ -311,6 +330,8 @@ class AttentionExt:
         and `lengths` does not count them.  `scale` multiplies the scores
         (default D ** -0.5).  FP32 scores, statistics and sums, one rounding; a
         query that sees nothing, or lies past counts[b], gives zeros."""
+        if scale is not None:
+            scale = _number("scale", scale)
         if out is not None and self._fast_forward(q, cache, block_table, lengths, out, counts,
                                                   prefix, scale) is not None:
             return
@@ -321,13 +342,11 @@ class AttentionExt:
             return None
         pages, n = None, 0
         if prefix is not None:
-            pages, n = prefix
+            pages, n = _pair(prefix)
             if type(n) is not int or not 0 <= n < 2 ** 31 or pages is None:
                 return None
         if scale is None:
             scale = cache.head_dim ** -0.5
-        elif not isinstance(scale, (int, float)):
-            return None
         return self._fast.forward(cache.fast, q, block_table, lengths, counts, out, pages, n,
                                   scale)
 
@@ -352,7 +371,7 @@ class AttentionExt:
             _ints("counts", counts, (batch,), dev)
         a = _capi.CqAttention()
         if prefix is not None:
-            pages, n = prefix
+            pages, n = _pair(prefix)
             _gpu("the prefix's pages", pages, dev)
             if pages.dtype != torch.int32 or pages.dim() != 1 or not pages.is_contiguous():
                 _fail(f"the prefix's pages must be contiguous int32 (n,), got {pages.dtype} "
