@@ -328,8 +328,11 @@ class AttentionExt:
         (pages int32 (n,), length) names tokens that every query of every
         sequence sees before its own: they are read once for the whole batch,
         and `lengths` does not count them.  `scale` multiplies the scores
-        (default D ** -0.5).  FP32 scores, statistics and sums, one rounding; a
-        query that sees nothing, or lies past counts[b], gives zeros."""
+        (default D ** -0.5).  Scores, statistics and sums are FP32, from q held
+        in FP16 times a power of two of its row; each probability times its V
+        scale is rounded to FP16 before it multiplies V's codes, the result once
+        to q's type.  A query that sees nothing, or lies past counts[b], gives
+        zeros, whatever it holds."""
         if scale is not None:
             scale = _number("scale", scale)
         if out is not None and self._fast_forward(q, cache, block_table, lengths, out, counts,

@@ -12,7 +12,8 @@
 // that of the softmax keeps w_j, which the matrix instructions take as fp16,
 // in range: the largest w of a row lies in [2^-5, 2^kRaise), and what fp16 then
 // rounds off is 2^-11 of each weight, or 2^-25 of 1.  Scores, statistics and
-// sums are FP32.
+// sums are FP32; the weights' rounding is the one beside the result's (q's,
+// below, is far under both).
 //
 // A key counts in l whatever its V scale, so l's term 2^(s_j log2(e) - M) is
 // 2^-e_j times the exponential that w_j takes, and that must stay inside FP32's
@@ -50,7 +51,7 @@
 // in the workspace, which join_kernel joins.  Equal runs keep every workgroup
 // busy to the end for any mix of lengths, and the grid never depends on them.
 // Where whole units to a run are as even, they are dealt whole: 1024 new tokens
-// of 64 heads over 8700 keys then leave nothing to join (373 us, whole 337).
+// of 64 heads over 8700 keys then leave nothing to join (399 us, whole 348).
 //
 // Three kernels:
 //   tile_kernel   few rows (shape_of): a wave takes whole tiles, four waves
@@ -61,8 +62,8 @@
 //   block_kernel  more rows: four or eight waves of 32 rows share tiles that
 //                 the workgroup unpacks into LDS once.  Bound by the matrix
 //                 units and the softmax between their products: 1024 new tokens
-//                 of 64 heads over 8700 keys (int4) 334 us, 822 TFLOP/s; a
-//                 prefix of 16384 keys for 64 sequences of 64 heads 86 us, of
+//                 of 64 heads over 8700 keys (int4) 341 us, 805 TFLOP/s; a
+//                 prefix of 16384 keys for 64 sequences of 64 heads 87 us, of
 //                 which 40 are tiles (2.5 us each of 64 keys and 256 rows), 8
 //                 the join of 16 triples to a row, the rest the sequences' own
 //                 keys and starts and ends of units.
@@ -92,7 +93,6 @@ using h8 = Vec<_Float16, 8>;
 using h2 = Vec<_Float16, 2>;
 using f4 = Vec<float, 4>;
 using u4 = Vec<uint32_t, 4>;
-using u2 = Vec<uint32_t, 2>;
 
 // One launch over one source of keys (the sequences' own, or the prefix).
 struct Source {
@@ -435,8 +435,8 @@ struct Rows {
         }
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
-            // exact down to 2^-27 of the row's largest element, to 2^-38 of it
-            // where fp16 is subnormal: far below the scores' own rounding
+            // exact down to 2^-23 of the row's largest element, to 2^-34 of it
+            // below (2^4 more without the nibbles' 16): less than FP32 rounds off
             const uint32_t bits = max(top2[rb] & 0xFFFFu, top2[rb] >> 16);
             const float top =
                 quad_max((float)__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
@@ -1238,14 +1238,14 @@ struct Shape {
 // units of many keys (as the table has room for) the tile kernel is ahead for
 // longer.
 // Measured on 8 heads over 4096 keys, us, tile and block kernel:
-//   heads of 128, 16 sequences: 32 rows 44, 55; 64 rows 57, 71; 80 rows 105, 80
-//                 64 sequences of 1000 keys: 40 rows 89, 60
-//                 2 sequences of 700 keys: 64 rows 18.2, 17.5
-//   heads of 64, 16 sequences: 64 rows 48, 58; 96 rows 72, 66
-//                 7 sequences of up to 1501 keys, 4 heads: 35 rows 15.8, 14.4
-//   heads of 256 (groups of 16), 16 sequences: 32 rows 84, 139; 48 rows 158, 146
-//                 64 sequences of 600 keys: 32 rows 108, 94
-// and of the block kernel four waves or eight: 128 rows 88, 93; 160 rows 135, 122.
+//   heads of 128, 16 sequences: 32 rows 48, 61; 64 rows 61, 77; 80 rows 105, 79
+//                 64 sequences of 1000 keys: 40 rows 101, 63
+//                 2 sequences of 700 keys: 64 rows 18.1, 17.7
+//   heads of 64, 16 sequences: 64 rows 51, 59; 96 rows 71, 64
+//                 7 sequences of up to 1501 keys, 4 heads: 35 rows 16.7, 15.0
+//   heads of 256 (groups of 16), 16 sequences: 32 rows 82, 142; 48 rows 154, 151
+//                 64 sequences of 600 keys: 32 rows 106, 97
+// and of the block kernel four waves or eight: 128 rows 94, 100; 160 rows 135, 124.
 Shape shape_of(int64_t rows, int64_t units, int64_t keys, int d) {
     const bool few = units <= kCus;
     if (rows <= (d == 256 && few ? 32 : 16)) return {1, kWaves, 16, waves_of(d, 1)};
@@ -1337,14 +1337,16 @@ hipError_t launch_typed(const Source& own, Shape os, const Source& ahead, Shape 
     e = wide ? launch_tiles<T, 8, D>(own, os, stream) : launch_tiles<T, 4, D>(own, os, stream);
     if (e != hipSuccess) return e;
     // a wave finds out for eight rows at once that they are finished, as most
-    // are where rows are many (1024 tokens x 64 heads: 62 us with one row, 35
-    // with eight); of few rows most have triples to join, one row a wave
+    // are where rows are many (1024 tokens of 64 heads over 8700 keys: the call 357
+    // us with one row, 348 with eight; of four sequences 1376 and 1336); of few
+    // rows most have triples to join, one row a wave
     const int64_t all = (int64_t)own.rows * own.a.batch * own.c.heads;
     const int each = own.finish && os.nb == 0 && all >= 32 * kWaves * kCus ? 8 : 1;
     const int64_t places = (int64_t)((own.rows + each - 1) / each) * own.a.batch * own.c.heads;
     // units over more runs than a wave has loads for: four waves to a row, as
-    // long as the rows alone do not fill the device (64 rows of 150 runs: 8.9 us
-    // with one wave, 3.9 with four; 4096 of 18: 12.1 and 13.6)
+    // long as the rows alone do not fill the device (calls of 64 rows, us with one
+    // wave and with four: of 19 runs 13.6 13.7, of 64 22.0 20.7, of 256 22.8 18.8;
+    // the join of 4096 rows of 18: 12.1 13.6)
     const int64_t runs = own.runs / ((int64_t)own.row_groups * own.a.batch * own.c.heads) +
                          (ahead.rows > 0 ? ahead.runs / ((int64_t)ahead.row_groups * own.c.heads)
                                          : 0);

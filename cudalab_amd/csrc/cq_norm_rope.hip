@@ -297,10 +297,15 @@ hipError_t launch_typed(const cq_norm_rope_t& a, hipStream_t stream) {
     // Pieces of 16 bytes of each end, two heads in flight and weights and tables
     // fetched once for several heads, as long as waves enough are left: by how
     // many there are with one head to a group.  Few: one, in pieces of four
-    // elements, so that each wave has as little to wait for as can be.  fp16 heads
-    // of 128, us with one head to a group in pieces of 8 and 16 bytes, then with
-    // two, four and eight:
-    //   16384 heads (2048 waves)   5.8  5.4  5.9  7.6 11.5
+    // elements, which is ahead where a call is hardly more than its launch and
+    // level then.  fp16 heads of 128, us with one head to a group in pieces of 8 and
+    // 16 bytes, then (from where it matters) with two, four and eight:
+    //   72 heads     (9 waves)     3.03 3.31
+    //   2304         (288)         3.64 3.87
+    //   4000         (500)         3.69 3.93
+    //   9216         (1152)        4.62 4.53
+    //   20480        (2560)        5.79 5.76
+    //   16384        (2048)         -    -   5.9  7.6 11.5
     //   65536       (8192)        14.0 12.9  9.8 11.4 14.2
     //   169696      (21212)       33.9 29.5 23.8 23.1 23.1
     //   524288      (65536)       95.9 83.8 68.2 59.5 57.4

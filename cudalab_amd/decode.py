@@ -175,7 +175,8 @@ class DecodeModel:
 
     def advance(self) -> None:
         """On to the next token: later steps (replayed ones too) write to the
-        position behind, and see the token of the step before."""
+        position behind, and see the token of the step before.  Past `room`
+        tokens the rotation's tables end, and q and k turn NaN."""
         self.position.add_(1)
         self.length.add_(1)
 

@@ -531,9 +531,13 @@ int cq_kv_read(const cq_kv_cache_t* cache, const cq_kv_slots_t* slots, int dtype
  * t is at position p = lengths[b] - count + t and sees the sequence's positions
  * 0..p and all prefix_len tokens of the prefix, whose pages are
  * prefix_table[0 .. prefix_cols).  Positions without a page in range are not
- * seen.  out = sum_j softmax_j(softmax_scale * q . k_j) v_j, FP32 scores,
- * statistics and sums, rounded once to `dtype` (F16 or BF16); 0 for a row that
- * sees nothing and for rows t >= count. */
+ * seen.  out = sum_j softmax_j(softmax_scale * q . k_j) v_j with FP32 scores,
+ * statistics and sums.  What has fewer bits: q is held in fp16 times a power of
+ * two of its row (exact to 2^-23 of the row's largest element), each weight
+ * softmax_j * (v_j's scale) is rounded to fp16 (2^-11 of it, or 2^-20 of the
+ * row's largest weight), and the result once to `dtype` (F16 or BF16).  V scales
+ * keep their digits down to 2^-80 of the largest in the cache's pages seen.  0 for
+ * a row that sees nothing and for rows t >= count, whatever q holds there. */
 typedef struct cq_attention {
     const void* q;             /* 16-byte aligned; strides multiples of 8 */
     void* out;                 /* contiguous, 16-byte aligned */
