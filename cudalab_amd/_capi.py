@@ -126,6 +126,15 @@ class CqAttention(ctypes.Structure):
                             "q_heads", "dtype")] + [("softmax_scale", ctypes.c_float)]
 
 
+class CqPlace(ctypes.Structure):
+    """cq_place_t"""
+    _fields_ = [(n, _vp) for n in ("starts", "counts", "free_pages", "taken_in", "table",
+                                   "slots", "positions", "offsets", "lengths",
+                                   "taken_out")] + [
+        (n, _i64) for n in ("table_stride", "tokens", "free_count")] + [
+        (n, _i32) for n in ("table_cols", "batch", "page_size")]
+
+
 _cstr = ctypes.c_char_p
 
 # name -> (restype, argtypes); must match include/cdnaqgemv.h
@@ -194,6 +203,10 @@ SIGNATURES = {
                                     ctypes.POINTER(CqAttention), _vp]),
     "cq_attention_workspace": (_i64, [ctypes.POINTER(CqKvCache),
                                       ctypes.POINTER(CqAttention)]),
+    "cq_place": (ctypes.c_int, [ctypes.POINTER(CqPlace), _vp]),
+    "cq_kv_append_rows": (ctypes.c_int, [
+        ctypes.POINTER(CqKvCache), ctypes.c_int, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
+        _vp]),
     "cq_last_error": (ctypes.c_char_p, []),
     "cq_version": (ctypes.c_char_p, []),
 }

@@ -7,6 +7,12 @@ counterpart in the reference, whose path ends at the projections.
     att.append(cache, k, v, block_table, lengths_before)
     out = att.forward(q, cache, block_table, lengths_after)
 
+and, for prompts whose tokens lie end to end ("packed"),
+
+    p = att.place(block_table, starts, counts, tokens, page_size, free_pages)
+    q, k = att.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, p.positions)
+    att.append_rows(cache, k, v, p.slots)
+
 Every check that needs only shapes, types and devices runs on the host before
 anything is launched and raises RuntimeError.  Lengths, positions and page
 numbers live on the device and are never read by the host: the kernels check
@@ -22,13 +28,13 @@ here then runs and raises.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _capi
 from .ext import _on_device, fast_module_or_none
-from .kvcache import KVCache
+from .kvcache import PAGE_SIZES, KVCache
 
 _DTYPES = {torch.float16: _capi.CQ_DTYPE_F16, torch.float32: _capi.CQ_DTYPE_F32,
            torch.bfloat16: _capi.CQ_DTYPE_BF16}
@@ -83,6 +89,12 @@ def _table(name: str, t: torch.Tensor, batch: int, device: torch.device) -> None
         _fail(f"the rows of {name} must be contiguous")
 
 
+def _count(name: str, n) -> int:
+    if isinstance(n, bool) or not isinstance(n, int) or not 0 <= n < 2 ** 31:
+        _fail(f"{name} must be an int in [0, 2^31), got {n!r}")
+    return n
+
+
 def _number(name: str, x) -> float:
     try:
         if hasattr(x, "__float__"):
@@ -98,6 +110,15 @@ def _pair(prefix) -> tuple:
     return prefix
 
 
+class Placed(NamedTuple):
+    """Where a packed batch's tokens go (AttentionExt.place)."""
+    slots: torch.Tensor        # int64 (tokens,): page * page_size + offset, or -1
+    positions: torch.Tensor    # int32 (tokens,)
+    offsets: torch.Tensor      # int32 (batch + 1,): rows before each sequence
+    lengths: torch.Tensor      # int32 (batch,): tokens with the added ones
+    taken: torch.Tensor        # int32 (1,): entries of the free list that are gone
+
+
 class AttentionExt:
     """Norms with rotation, the quantized cache and attention over it."""
 
@@ -107,6 +128,8 @@ class AttentionExt:
         self._fast = mod and mod.AttentionCalls(*(_capi.entry_address(n) for n in (
             "cq_qk_norm_rope", "cq_kv_append", "cq_kv_read", "cq_attention",
             "cq_attention_workspace", "cq_last_error")))
+        self._step = mod and mod.StepCalls(*(_capi.entry_address(n) for n in (
+            "cq_place", "cq_kv_append_rows", "cq_last_error")))
 
     # ---- norms and rotation ----
     def qk_norm_rope(self, q: torch.Tensor, k: torch.Tensor,
@@ -295,6 +318,96 @@ class AttentionExt:
                 ctypes.byref(cache.c), ctypes.byref(slots), _DTYPES[dtype], k.data_ptr(),
                 v.data_ptr(), s)), "read")
         return k, v
+
+    # ---- packed batches ----
+    def place(self, block_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor,
+              tokens: int, page_size: int, free_pages: torch.Tensor,
+              taken: Optional[torch.Tensor] = None) -> Placed:
+        """Pages, positions and slots for a packed batch of `tokens` rows in
+        which sequence b adds counts[b] tokens to the starts[b] that it has.
+
+        Sequence b holds the first ceil(starts[b] / page_size) entries of its
+        row of block_table int32 (batch, pages); the pages that it needs beyond
+        come from free_pages int32 (n,), in the sequences' order, from entry
+        taken[0] (int32 (1,), 0 if None) on, and are written into the table (-1
+        where the list has ended).  The result's `taken` says how many entries
+        are gone then: above n the list did not suffice.  It may be the next
+        call's `taken`.  A token without a page, or past the table, has slot -1,
+        and so have rows behind the last sequence.  Tokens that do not fit
+        `tokens` rows are not placed, and `lengths` does not count them.
+        Negative starts and counts are zero."""
+        if self._step is not None:
+            got = self._step.place(block_table, starts, counts, tokens, page_size, free_pages,
+                                   taken)
+            if got is not None:
+                return Placed(*got)
+        if not isinstance(block_table, torch.Tensor):
+            _fail(f"block_table must be a tensor, got {type(block_table).__name__}")
+        dev = block_table.device
+        batch = block_table.size(0) if block_table.dim() == 2 else 0
+        _table("block_table", block_table, batch, dev)
+        _ints("starts", starts, (batch,), dev)
+        _ints("counts", counts, (batch,), dev)
+        _count("tokens", tokens)
+        if isinstance(page_size, bool) or page_size not in PAGE_SIZES:
+            _fail(f"the page size must be one of {PAGE_SIZES}, got {page_size!r}")
+        _gpu("free_pages", free_pages, dev)
+        _ints("free_pages", free_pages, (free_pages.numel(),), dev)
+        if taken is not None:
+            _ints("taken", taken, (1,), dev)
+
+        def ints(n, dtype=torch.int32):
+            return torch.empty(n, dtype=dtype, device=dev)
+
+        p = Placed(ints(tokens, torch.int64), ints(tokens), ints(batch + 1), ints(batch),
+                   ints(1))
+        if batch == 0:
+            p.slots.fill_(-1)
+            p.positions.zero_()
+            p.offsets.zero_()
+            p.taken.zero_()
+            return p if taken is None else p._replace(taken=taken.clamp(min=0))
+        a = _capi.CqPlace(
+            starts.data_ptr(), counts.data_ptr(), free_pages.data_ptr() or None,
+            None if taken is None else taken.data_ptr(), block_table.data_ptr(),
+            p.slots.data_ptr() or None, p.positions.data_ptr() or None, p.offsets.data_ptr(),
+            p.lengths.data_ptr(), p.taken.data_ptr(), block_table.stride(0), tokens,
+            free_pages.numel(), block_table.size(1), batch, page_size)
+        _check(_on_device(dev, lambda s: self._lib.cq_place(ctypes.byref(a), s)), "place")
+        return p
+
+    def append_rows(self, cache: KVCache, k: torch.Tensor, v: torch.Tensor,
+                    slots: torch.Tensor) -> None:
+        """Quantizes packed k and v (tokens, heads, D) into the cache: row t
+        goes to slots[t] = page * page_size + offset (int64 (tokens,)), as `place`
+        gives them.  A row with a slot outside the cache (-1) is not written; no
+        two rows have one slot.  Accepted drafts are closed up this way: their
+        rows again, to the slots behind one another, the others' -1."""
+        if not isinstance(cache, KVCache):
+            _fail(f"cache must be a KVCache, got {type(cache).__name__}")
+        if self._step is not None and cache.fast is not None \
+                and self._step.append_rows(cache.fast, k, v, slots):
+            return
+        for name, t in (("k", k), ("v", v)):
+            _heads(name, t, 3, cache.device)
+            if t.dtype != k.dtype or t.shape != k.shape:
+                _fail(f"k and v must share type and shape, got {k.dtype} {tuple(k.shape)} "
+                      f"and {t.dtype} {tuple(t.shape)}")
+        tokens = k.size(0)
+        if k.size(1) != cache.heads or k.size(2) != cache.head_dim:
+            _fail(f"k and v must be (tokens, {cache.heads}, {cache.head_dim}), got "
+                  f"{tuple(k.shape)}")
+        _gpu("slots", slots, cache.device)
+        if slots.dtype != torch.int64 or tuple(slots.shape) != (tokens,) \
+                or not slots.is_contiguous():
+            _fail(f"slots must be contiguous int64 ({tokens},), got {slots.dtype} "
+                  f"{tuple(slots.shape)}")
+        if tokens == 0:
+            return
+        ks, vs = k.stride(), v.stride()
+        _check(_on_device(cache.device, lambda s: self._lib.cq_kv_append_rows(
+            ctypes.byref(cache.c), _DTYPES[k.dtype], tokens, slots.data_ptr(), k.data_ptr(),
+            ks[0], ks[1], v.data_ptr(), vs[0], vs[1], s)), "append_rows")
 
     # ---- attention ----
     def forward(self, q: torch.Tensor, cache: KVCache, block_table: torch.Tensor,

@@ -4,66 +4,14 @@
 
 #include <climits>
 #include <cmath>
-#include <initializer_list>
 #include <string>
 
-#include "cdnaqgemv.h"
 #include "cq_attn.h"
+#include "cq_checks.h"
+
+using namespace cq::checks;
 
 namespace {
-
-using U = unsigned __int128;
-
-int invalid(const char* what) { return cq::set_error(CQ_ERR_INVALID_ARG, what); }
-
-int hip_status(hipError_t e, const char* what) {
-    if (e == hipSuccess) return CQ_OK;
-    if (e == hipErrorInvalidValue)
-        return cq::set_error(CQ_ERR_INVALID_ARG,
-                             std::string(what) + ": the call needs more workgroups than a launch holds");
-    return cq::set_error(CQ_ERR_HIP, std::string(what) + ": " + hipGetErrorName(e) + " (" +
-                                         hipGetErrorString(e) + ")");
-}
-
-// Runs an entry point's body; nothing may be thrown through the C interface
-// (std::string allocates).
-template <class F>
-auto guarded(F&& body, decltype(body()) thrown = CQ_ERR_HIP) noexcept -> decltype(body()) {
-    try {
-        return body();
-    } catch (...) {
-        return thrown;
-    }
-}
-
-int64_t elem_bytes(int dtype) { return dtype == CQ_DTYPE_F32 ? 4 : 2; }
-
-bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
-
-// Bytes [lo, hi) of an operand; empty where there is none.
-struct Span {
-    U lo = 0, hi = 0;
-    Span() = default;
-    Span(const void* p, U bytes) : lo(reinterpret_cast<uintptr_t>(p)), hi(lo + bytes) {
-        if (p == nullptr) lo = hi = 0;
-    }
-};
-
-bool overlap(const Span& a, const Span& b) {
-    return a.lo < a.hi && b.lo < b.hi && a.lo < b.hi && b.lo < a.hi;
-}
-
-// An operand of `rows` x `cols` x ... innermost runs: extents and strides in
-// elements, strides not negative.
-Span strided(const void* p, std::initializer_list<std::pair<int64_t, int64_t>> dims,
-             int64_t run, int64_t elem) {
-    U last = 0;
-    for (const auto& [n, stride] : dims) {
-        if (n <= 0) return {};
-        last += static_cast<U>(n - 1) * static_cast<U>(stride);
-    }
-    return Span(p, (last + static_cast<U>(run)) * static_cast<U>(elem));
-}
 
 int check_norm_rope(const cq_norm_rope_t& a) {
     if (a.tokens < 1 || a.tokens > INT_MAX) return invalid("tokens must be in [1, 2^31-1]");
@@ -155,47 +103,6 @@ int check_norm_rope(const cq_norm_rope_t& a) {
     return CQ_OK;
 }
 
-int check_cache(const cq_kv_cache_t& c) {
-    if (c.k == nullptr || c.v == nullptr || c.scales == nullptr) return invalid("null pointer: cache");
-    if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.scales, 16))
-        return invalid("the cache's tensors must be 16-byte aligned");
-    if (c.pages < 1 || c.pages > INT_MAX) return invalid("pages must be in [1, 2^31-1]");
-    if (c.heads < 1 || c.heads > 65535) return invalid("heads must be in [1, 65535]");
-    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
-        return invalid("the cache's head_dim must be 64, 128 or 256");
-    if (c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1)) != 0)
-        return invalid("page_size must be 16, 32, 64, 128 or 256");
-    if (c.bits != 4 && c.bits != 8) return invalid("bits must be 4 or 8");
-    return CQ_OK;
-}
-
-struct CacheSpans {
-    Span k, v, scales;
-    explicit CacheSpans(const cq_kv_cache_t& c) {
-        const U tokens = static_cast<U>(c.pages) * static_cast<U>(c.heads) *
-                         static_cast<U>(c.page_size);
-        const U row = static_cast<U>(c.head_dim * c.bits / 8);
-        k = Span(c.k, tokens * row);
-        v = Span(c.v, tokens * row);
-        scales = Span(c.scales, tokens * 8);
-    }
-    bool meet(const Span& s) const {
-        return overlap(k, s) || overlap(v, s) || overlap(scales, s);
-    }
-    bool meet_themselves() const {
-        return overlap(k, v) || overlap(k, scales) || overlap(v, scales);
-    }
-};
-
-int check_table(const int32_t* table, int64_t stride, int32_t cols, int32_t batch) {
-    if (table == nullptr) return invalid("null pointer: table");
-    if (!aligned(table, 4)) return invalid("table must be 4-byte aligned");
-    if (cols < 1) return invalid("table_cols must be >= 1");
-    if (batch > 1 && (stride < cols || stride > (int64_t)1 << 40))
-        return invalid("table_stride must be at least table_cols");
-    return CQ_OK;
-}
-
 int check_slots(const cq_kv_slots_t& s) {
     if (s.batch < 1 || s.tokens < 1) return invalid("batch and tokens must be >= 1");
     if (s.starts == nullptr) return invalid("null pointer: starts");
@@ -203,12 +110,6 @@ int check_slots(const cq_kv_slots_t& s) {
         return invalid("starts and counts must be 4-byte aligned");
     return check_table(s.table, s.table_stride, s.table_cols, s.batch);
 }
-
-Span table_span(const int32_t* table, int64_t stride, int32_t cols, int32_t batch) {
-    return strided(table, {{batch, stride}}, cols, 4);
-}
-
-bool known_dtype(int d) { return d == CQ_DTYPE_F16 || d == CQ_DTYPE_F32 || d == CQ_DTYPE_BF16; }
 
 int check_append(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int dtype, const void* k,
                  cq::KvStrides ks, const void* v, cq::KvStrides vs) {
@@ -253,7 +154,9 @@ int check_read(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int dtype, const 
     return CQ_OK;
 }
 
-int check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launching) {
+}  // namespace
+
+int cq::check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launching) {
     int st = check_cache(c);
     if (st != CQ_OK) return st;
     if (a.batch < 1 || a.tokens < 1) return invalid("batch and tokens must be >= 1");
@@ -307,8 +210,6 @@ int check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launch
     return CQ_OK;
 }
 
-}  // namespace
-
 extern "C" {
 
 int cq_qk_norm_rope(const cq_norm_rope_t* args, void* stream) {
@@ -352,7 +253,7 @@ int cq_kv_read(const cq_kv_cache_t* cache, const cq_kv_slots_t* slots, int dtype
 int cq_attention(const cq_kv_cache_t* cache, const cq_attention_t* args, void* stream) {
     return guarded([&]() -> int {
         if (cache == nullptr || args == nullptr) return invalid("null pointer: cache or args");
-        const int st = check_attention(*cache, *args, true);
+        const int st = cq::check_attention(*cache, *args, true);
         if (st != CQ_OK) return st;
         return hip_status(cq::launch_attention(*cache, *args, static_cast<hipStream_t>(stream)),
                           "cq_attention");
@@ -362,7 +263,7 @@ int cq_attention(const cq_kv_cache_t* cache, const cq_attention_t* args, void* s
 int64_t cq_attention_workspace(const cq_kv_cache_t* cache, const cq_attention_t* args) {
     return guarded([&]() -> int64_t {
         if (cache == nullptr || args == nullptr) return -invalid("null pointer: cache or args");
-        const int st = check_attention(*cache, *args, false);
+        const int st = cq::check_attention(*cache, *args, false);
         if (st != CQ_OK) return -st;
         return cq::attention_workspace(*cache, *args);
     }, -CQ_ERR_HIP);

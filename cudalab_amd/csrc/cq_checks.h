@@ -1,0 +1,115 @@
+// What the C entry points check with: spans of memory that must not meet, the
+// cache's and the tables' arguments, statuses.  Host code only.
+#pragma once
+
+#include <climits>
+#include <initializer_list>
+#include <string>
+#include <utility>
+
+#include "cdnaqgemv.h"
+#include "cq_attn.h"
+
+namespace cq::checks {
+
+using U = unsigned __int128;
+
+inline int invalid(const char* what) { return cq::set_error(CQ_ERR_INVALID_ARG, what); }
+
+inline int hip_status(hipError_t e, const char* what) {
+    if (e == hipSuccess) return CQ_OK;
+    if (e == hipErrorInvalidValue)
+        return cq::set_error(CQ_ERR_INVALID_ARG,
+                             std::string(what) + ": the call needs more workgroups than a launch holds");
+    return cq::set_error(CQ_ERR_HIP, std::string(what) + ": " + hipGetErrorName(e) + " (" +
+                                         hipGetErrorString(e) + ")");
+}
+
+// Runs an entry point's body; nothing may be thrown through the C interface
+// (std::string allocates).
+template <class F>
+auto guarded(F&& body, decltype(body()) thrown = CQ_ERR_HIP) noexcept -> decltype(body()) {
+    try {
+        return body();
+    } catch (...) {
+        return thrown;
+    }
+}
+
+inline int64_t elem_bytes(int dtype) { return dtype == CQ_DTYPE_F32 ? 4 : 2; }
+
+inline bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// Bytes [lo, hi) of an operand; empty where there is none.
+struct Span {
+    U lo = 0, hi = 0;
+    Span() = default;
+    Span(const void* p, U bytes) : lo(reinterpret_cast<uintptr_t>(p)), hi(lo + bytes) {
+        if (p == nullptr) lo = hi = 0;
+    }
+};
+
+inline bool overlap(const Span& a, const Span& b) {
+    return a.lo < a.hi && b.lo < b.hi && a.lo < b.hi && b.lo < a.hi;
+}
+
+// An operand of `rows` x `cols` x ... innermost runs: extents and strides in
+// elements, strides not negative.
+inline Span strided(const void* p, std::initializer_list<std::pair<int64_t, int64_t>> dims,
+                    int64_t run, int64_t elem) {
+    U last = 0;
+    for (const auto& [n, stride] : dims) {
+        if (n <= 0) return {};
+        last += static_cast<U>(n - 1) * static_cast<U>(stride);
+    }
+    return Span(p, (last + static_cast<U>(run)) * static_cast<U>(elem));
+}
+
+inline int check_cache(const cq_kv_cache_t& c) {
+    if (c.k == nullptr || c.v == nullptr || c.scales == nullptr) return invalid("null pointer: cache");
+    if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.scales, 16))
+        return invalid("the cache's tensors must be 16-byte aligned");
+    if (c.pages < 1 || c.pages > INT_MAX) return invalid("pages must be in [1, 2^31-1]");
+    if (c.heads < 1 || c.heads > 65535) return invalid("heads must be in [1, 65535]");
+    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
+        return invalid("the cache's head_dim must be 64, 128 or 256");
+    if (c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1)) != 0)
+        return invalid("page_size must be 16, 32, 64, 128 or 256");
+    if (c.bits != 4 && c.bits != 8) return invalid("bits must be 4 or 8");
+    return CQ_OK;
+}
+
+struct CacheSpans {
+    Span k, v, scales;
+    explicit CacheSpans(const cq_kv_cache_t& c) {
+        const U tokens = static_cast<U>(c.pages) * static_cast<U>(c.heads) *
+                         static_cast<U>(c.page_size);
+        const U row = static_cast<U>(c.head_dim * c.bits / 8);
+        k = Span(c.k, tokens * row);
+        v = Span(c.v, tokens * row);
+        scales = Span(c.scales, tokens * 8);
+    }
+    bool meet(const Span& s) const {
+        return overlap(k, s) || overlap(v, s) || overlap(scales, s);
+    }
+    bool meet_themselves() const {
+        return overlap(k, v) || overlap(k, scales) || overlap(v, scales);
+    }
+};
+
+inline int check_table(const int32_t* table, int64_t stride, int32_t cols, int32_t batch) {
+    if (table == nullptr) return invalid("null pointer: table");
+    if (!aligned(table, 4)) return invalid("table must be 4-byte aligned");
+    if (cols < 1) return invalid("table_cols must be >= 1");
+    if (batch > 1 && (stride < cols || stride > (int64_t)1 << 40))
+        return invalid("table_stride must be at least table_cols");
+    return CQ_OK;
+}
+
+inline Span table_span(const int32_t* table, int64_t stride, int32_t cols, int32_t batch) {
+    return strided(table, {{batch, stride}}, cols, 4);
+}
+
+inline bool known_dtype(int d) { return d == CQ_DTYPE_F16 || d == CQ_DTYPE_F32 || d == CQ_DTYPE_BF16; }
+
+}  // namespace cq::checks

@@ -17,8 +17,8 @@
 // is read or written once goes past the caches (non-temporal): reading 54009
 // tokens of 8 heads of 128 back took 59 us with ordinary stores, 40 with these.
 
-#include "cq_attn.h"
 #include "cq_elem.h"
+#include "cq_step.h"
 
 namespace cq {
 namespace {
@@ -253,6 +253,104 @@ __global__ __launch_bounds__(kBlock) void append_kernel(cq_kv_cache_t c, cq_kv_s
     }
 }
 
+// Packed rows to their slots (page * page_size + offset): row t of k and v goes
+// to slots[t].  Rows whose slots follow one another inside 16 aligned places
+// form a group, which is what a tile of the cache is; a workgroup takes the
+// groups that begin in its 16 rows (and so up to 31 rows, 16 at a time), one
+// head.  A whole group leaves as whole words of V, anything else byte by byte.
+// With every group broken (64 sequences of 5 tokens, three of them kept, 8 heads
+// of 128) the stores of single bytes still hide behind the launch.
+template <class T, int BITS, int D>
+__global__ __launch_bounds__(kBlock) void append_rows_kernel(cq_kv_cache_t c, uint32_t tokens,
+                                                             const int64_t* slots, const T* k,
+                                                             KvStrides ks, const T* v,
+                                                             KvStrides vs, bool wide,
+                                                             uint32_t first) {
+    constexpr int E = D / 16;
+    constexpr int R = BITS == 8 ? D : D / 2;       // bytes of a row
+    using C = Codes<BITS, E>;
+    __shared__ __attribute__((aligned(16))) uint8_t turned[16][C::kBytes * 16 + 16];
+    const uint32_t block = first + blockIdx.x;
+    const int h = block % c.heads;
+    const uint32_t t0 = block / c.heads * 16;
+    const int i = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    // lane j of a wave: the slot of row t0 - 1 + j, -1 for none
+    const int j = threadIdx.x & 63;
+    const int64_t at = (int64_t)t0 - 1 + j;
+    const int64_t mine = at >= 0 && at < tokens ? slots[at] : -1;
+    const int64_t ahead = __shfl_up(mine, 1);
+    const bool starts = at >= tokens || (uint64_t)mine != (uint64_t)ahead + 1 || mine % 16 == 0 ||
+                        at == 0;
+    const uint64_t begins = __ballot(j > 0 && starts) >> 1;     // of rows t0 .. t0 + 62
+    if ((begins & 0xFFFF) == 0) return;            // uniform over the workgroup
+    const int from = __builtin_ctzll(begins);
+    const int to = 16 + __builtin_ctzll(begins >> 16);          // row t0 + 31 is in reach
+    const int64_t places = c.pages * c.page_size;
+    const int shift = __builtin_ctz(c.page_size);
+    for (int base = from; base < to; base += 16) {
+        const int r = base + i;
+        const uint32_t t = t0 + r;
+        const int64_t its = __shfl(mine, r + 1);   // (r is below 47)
+        const int64_t slot = r < to ? its : -1;
+        const bool live = slot >= 0 && slot < places;
+        T x[E] = {}, y[E] = {};
+        if (live) {
+            load_row(x, k + t * ks.token + h * ks.head + lane * E, wide);
+            load_row(y, v + t * vs.token + h * vs.head + lane * E, wide);
+        }
+        C kc, vc;
+        float kscale, vscale, kinv, vinv;
+        scale_of<BITS>(amax16(x), kscale, kinv);
+        scale_of<BITS>(amax16(y), vscale, vinv);
+        kc.pack(x, kinv);
+        vc.pack(y, vinv);
+        if (live) {
+            const int64_t ph = (slot >> shift) * c.heads + h;
+            const int64_t in = slot & (c.page_size - 1);
+            kc.store(static_cast<uint8_t*>(c.k) + (ph * c.page_size + in) * R + lane * C::kBytes);
+            if (lane == 0) {
+                float* sc = c.scales + ph * 2 * c.page_size + in;
+                sc[0] = kscale;
+                sc[c.page_size] = vscale;
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < C::kWords; ++m) {
+            const uint32_t word = turn_bytes(vc.w[m]);
+            const int row = 4 * m + (i & 3);
+            if (row < C::kBytes)
+                *reinterpret_cast<uint32_t*>(turned[lane] + row * 16 + (i & ~3)) = word;
+        }
+        __syncthreads();
+        auto v_at = [&](int64_t s) {               // dim 0 of a slot
+            const int64_t in = s & (c.page_size - 1);
+            return static_cast<uint8_t*>(c.v) +
+                   (((s >> shift) * c.heads + h) * (c.page_size / 16) + in / 16) * R * 16 + in % 16;
+        };
+        // the slots of the 16 rows, the same in every wave
+        const int64_t slot0 = __shfl(mine, base + 1);
+        const bool whole = base + 16 <= to && slot0 >= 0 && slot0 < places && slot0 % 16 == 0 &&
+                           ((begins >> base) & 0xFFFF) == 1;
+        if (whole) {
+            if ((int)threadIdx.x < R) {
+                const int row = threadIdx.x;
+                *reinterpret_cast<uint4*>(v_at(slot0) + row * 16) =
+                    *reinterpret_cast<const uint4*>(turned[row / C::kBytes] + row % C::kBytes * 16);
+            }
+        } else {
+            for (int n = 0; n < 16 && base + n < to; ++n) {
+                const int64_t s = __shfl(mine, base + n + 1);
+                if (s < 0 || s >= places) continue;
+                if ((int)threadIdx.x < R) {
+                    const int row = threadIdx.x;
+                    v_at(s)[row * 16] = turned[row / C::kBytes][row % C::kBytes * 16 + n];
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 template <class T, int BITS, int D>
 __global__ __launch_bounds__(kBlock) void read_kernel(cq_kv_cache_t c, cq_kv_slots_t s,
                                                       uint32_t tiles, T* k, T* v,
@@ -357,6 +455,27 @@ hipError_t append_typed(const cq_kv_cache_t& c, const cq_kv_slots_t& s, const vo
 }
 
 template <class T>
+hipError_t append_rows_typed(const cq_kv_cache_t& c, int64_t tokens, const int64_t* slots,
+                             const void* k, KvStrides ks, const void* v, KvStrides vs,
+                             hipStream_t stream) {
+    const __int128 grid = (__int128)((tokens + 15) / 16) * c.heads;
+    if (grid > kMaxGrid) return hipErrorInvalidValue;
+    return by_form(c, [&](auto bits, auto dim) {
+        constexpr int E = decltype(dim)::value / 16;
+        constexpr int N = E * sizeof(T) > 16 ? 16 / sizeof(T) : E;
+        bool wide = (uintptr_t)k % (N * sizeof(T)) == 0 && (uintptr_t)v % (N * sizeof(T)) == 0;
+        for (const KvStrides& st : {ks, vs})
+            wide = wide && st.token % N == 0 && st.head % N == 0;
+        return launch_parts((int64_t)grid, [&](dim3 blocks, uint32_t first) {
+            append_rows_kernel<T, decltype(bits)::value, decltype(dim)::value>
+                <<<blocks, dim3(kBlock), 0, stream>>>(c, (uint32_t)tokens, slots,
+                                                      static_cast<const T*>(k), ks,
+                                                      static_cast<const T*>(v), vs, wide, first);
+        });
+    });
+}
+
+template <class T>
 hipError_t read_typed(const cq_kv_cache_t& c, const cq_kv_slots_t& s, void* k, void* v,
                       hipStream_t stream) {
     const int64_t tiles = tiles_of(s), grid = workgroups(c, s);
@@ -378,6 +497,16 @@ hipError_t launch_kv_append(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int 
     if (dtype == CQ_DTYPE_F16) return append_typed<_Float16>(c, s, k, ks, v, vs, stream);
     if (dtype == CQ_DTYPE_BF16) return append_typed<__bf16>(c, s, k, ks, v, vs, stream);
     return append_typed<float>(c, s, k, ks, v, vs, stream);
+}
+
+hipError_t launch_kv_append_rows(const cq_kv_cache_t& c, int dtype, int64_t tokens,
+                                 const int64_t* slots, const void* k, KvStrides ks, const void* v,
+                                 KvStrides vs, hipStream_t stream) {
+    if (dtype == CQ_DTYPE_F16)
+        return append_rows_typed<_Float16>(c, tokens, slots, k, ks, v, vs, stream);
+    if (dtype == CQ_DTYPE_BF16)
+        return append_rows_typed<__bf16>(c, tokens, slots, k, ks, v, vs, stream);
+    return append_rows_typed<float>(c, tokens, slots, k, ks, v, vs, stream);
 }
 
 hipError_t launch_kv_read(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int dtype,

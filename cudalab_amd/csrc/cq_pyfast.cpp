@@ -39,7 +39,7 @@
 #include <vector>
 
 #include "cdnaqgemv.h"
-#include "cq_pyattn.h"
+#include "cq_pystep.h"
 
 namespace py = pybind11;
 
@@ -399,4 +399,5 @@ PYBIND11_MODULE(_cqfast, m) {
         .def("cached", &Launcher::cached)
         .def("clear", &Launcher::clear);
     cqattn::bind(m);
+    cqstep::bind(m);
 }

@@ -1,0 +1,22 @@
+// Internal interface of the operators of a step of many tokens: the C entry
+// points (cq_step_capi.cpp) check a call's arguments and hand them on unchanged
+// to the launchers.
+#pragma once
+
+#include "cq_attn.h"
+
+namespace cq {
+
+// Launchers: arguments are checked, sizes are positive.  A launcher that
+// finds its grid beyond kMaxGrid returns hipErrorInvalidValue unlaunched.
+
+// cq_place.hip
+hipError_t launch_place(const cq_place_t& a, hipStream_t stream);
+
+// cq_kvcache.hip.  Element strides of k or v [tokens, heads, head_dim] (of
+// KvStrides `batch` is not used).
+hipError_t launch_kv_append_rows(const cq_kv_cache_t& c, int dtype, int64_t tokens,
+                                 const int64_t* slots, const void* k, KvStrides ks, const void* v,
+                                 KvStrides vs, hipStream_t stream);
+
+}  // namespace cq

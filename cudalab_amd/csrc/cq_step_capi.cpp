@@ -1,0 +1,114 @@
+// C entry points of the operators of a step of many tokens (declared in
+// include/cdnaqgemv.h): the checks that a safe launch needs.  What lies on the
+// device (lengths, offsets, slots) the kernels check themselves.
+
+#include <climits>
+#include <string>
+
+#include "cq_checks.h"
+#include "cq_step.h"
+
+using namespace cq::checks;
+
+namespace {
+
+// Whether a span written meets another operand of the call.
+template <int N, int M>
+bool meet(const Span (&out)[N], const Span (&in)[M]) {
+    for (int i = 0; i < N; ++i) {
+        for (int j = i + 1; j < N; ++j)
+            if (overlap(out[i], out[j])) return true;
+        for (const Span& x : in)
+            if (overlap(out[i], x)) return true;
+    }
+    return false;
+}
+
+int check_place(const cq_place_t& a) {
+    if (a.batch < 1 || a.batch == INT_MAX) return invalid("batch must be in [1, 2^31-2]");
+    if (a.tokens < 0 || a.tokens > INT_MAX) return invalid("tokens must be in [0, 2^31-1]");
+    if (a.page_size < 16 || a.page_size > 256 || (a.page_size & (a.page_size - 1)) != 0)
+        return invalid("page_size must be 16, 32, 64, 128 or 256");
+    if (a.free_count < 0 || a.free_count > (int64_t)1 << 40)
+        return invalid("free_count must be in [0, 2^40]");
+    int st = check_table(a.table, a.table_stride, a.table_cols, a.batch);
+    if (st != CQ_OK) return st;
+    if ((int64_t)a.table_cols * a.page_size > INT_MAX)
+        return invalid("table_cols * page_size must be below 2^31");
+    if (a.starts == nullptr || a.counts == nullptr || a.offsets == nullptr ||
+        a.lengths == nullptr || a.taken_out == nullptr ||
+        (a.free_count > 0 && a.free_pages == nullptr) ||
+        (a.tokens > 0 && (a.slots == nullptr || a.positions == nullptr)))
+        return invalid("null pointer argument");
+    for (const void* p : {(const void*)a.starts, (const void*)a.counts, (const void*)a.free_pages,
+                          (const void*)a.taken_in, (const void*)a.positions,
+                          (const void*)a.offsets, (const void*)a.lengths,
+                          (const void*)a.taken_out})
+        if (!aligned(p, 4)) return invalid("a pointer is not aligned to its element size");
+    if (!aligned(a.slots, 8)) return invalid("a pointer is not aligned to its element size");
+    const U batch = static_cast<U>(a.batch), tokens = static_cast<U>(a.tokens);
+    const Span out[] = {table_span(a.table, a.table_stride, a.table_cols, a.batch),
+                        Span(a.slots, tokens * 8),
+                        Span(a.positions, tokens * 4),
+                        Span(a.offsets, (batch + 1) * 4),
+                        Span(a.lengths, batch * 4),
+                        Span(a.taken_out, 4)};
+    const Span in[] = {Span(a.starts, batch * 4), Span(a.counts, batch * 4),
+                       Span(a.free_pages, static_cast<U>(a.free_count) * 4), Span(a.taken_in, 4)};
+    if (meet(out, in)) return invalid("an output overlaps another operand");
+    return CQ_OK;
+}
+
+bool stride_ok(int64_t n) { return n >= 0 && n <= (int64_t)1 << 40; }
+
+int check_append_rows(const cq_kv_cache_t& c, int dtype, int64_t tokens, const int64_t* slots,
+                      const void* k, cq::KvStrides ks, const void* v, cq::KvStrides vs) {
+    const int st = check_cache(c);
+    if (st != CQ_OK) return st;
+    if (!known_dtype(dtype)) return invalid("unknown dtype");
+    if (tokens < 1 || tokens > INT_MAX) return invalid("tokens must be in [1, 2^31-1]");
+    if (k == nullptr || v == nullptr || slots == nullptr) return invalid("null pointer argument");
+    const int64_t es = elem_bytes(dtype);
+    if (!aligned(k, es) || !aligned(v, es) || !aligned(slots, 8))
+        return invalid("a pointer is not aligned to its element size");
+    for (int64_t n : {ks.token, ks.head, vs.token, vs.head})
+        if (!stride_ok(n)) return invalid("strides must be in [0, 2^40]");
+    const CacheSpans cs(c);
+    for (const Span& in : {strided(k, {{tokens, ks.token}, {c.heads, ks.head}}, c.head_dim, es),
+                           strided(v, {{tokens, vs.token}, {c.heads, vs.head}}, c.head_dim, es),
+                           Span(slots, static_cast<U>(tokens) * 8)})
+        if (cs.meet(in)) return invalid("an input overlaps the cache");
+    if (cs.meet_themselves()) return invalid("the cache's tensors overlap");
+    return CQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cq_place(const cq_place_t* args, void* stream) {
+    return guarded([&]() -> int {
+        if (args == nullptr) return invalid("null pointer: args");
+        const int st = check_place(*args);
+        if (st != CQ_OK) return st;
+        return hip_status(cq::launch_place(*args, static_cast<hipStream_t>(stream)), "cq_place");
+    });
+}
+
+int cq_kv_append_rows(const cq_kv_cache_t* cache, int dtype, int64_t tokens,
+                      const int64_t* slots, const void* k, int64_t k_token_stride,
+                      int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                      int64_t v_head_stride, void* stream) {
+    return guarded([&]() -> int {
+        if (cache == nullptr) return invalid("null pointer: cache");
+        const cq::KvStrides ks{0, k_token_stride, k_head_stride};
+        const cq::KvStrides vs{0, v_token_stride, v_head_stride};
+        const int st = check_append_rows(*cache, dtype, tokens, slots, k, ks, v, vs);
+        if (st != CQ_OK) return st;
+        return hip_status(cq::launch_kv_append_rows(*cache, dtype, tokens, slots, k, ks, v, vs,
+                                                    static_cast<hipStream_t>(stream)),
+                          "cq_kv_append_rows");
+    });
+}
+
+}  // extern "C"

@@ -559,6 +559,57 @@ int cq_attention(const cq_kv_cache_t* cache, const cq_attention_t* args, void* s
 int64_t cq_attention_workspace(const cq_kv_cache_t* cache, const cq_attention_t* args);
 
 /*
+ * The operators of a step that takes many tokens: requests' tokens laid end to
+ * end ("packed"), sequence b's in rows offsets[b] .. offsets[b + 1].  The same
+ * conventions as above.
+ */
+
+/* From the requests' lengths, the pages that they need and where their tokens
+ * go.  Sequence b holds max(0, starts[b]) tokens in the first ceil(that / page_size)
+ * entries of its row of `table` and adds max(0, counts[b]), as far as all before
+ * it and they fit `tokens` rows; what does not fit is not placed.  New pages come
+ * from free_pages in the sequences' order, from entry *taken_in (0 if NULL) on,
+ * and are written into the table behind the held ones (-1 where the list has
+ * ended); the rest of the table stays as it is.  Written besides:
+ *   offsets   [batch + 1] rows before each sequence
+ *   lengths   [batch]     tokens with the added ones
+ *   taken_out [1]         entries of the free list that are gone (more than
+ *                         free_count: it did not suffice)
+ *   positions [tokens]    of each packed token in its sequence
+ *   slots     [tokens]    page * page_size + offset, or -1 for a token without
+ *                         a page or past the table's columns
+ * Rows behind the last sequence have position 0 and slot -1.  Nothing written
+ * shares a byte with anything else of the call. */
+typedef struct cq_place {
+    const int32_t* starts;     /* [batch] */
+    const int32_t* counts;     /* [batch] */
+    const int32_t* free_pages; /* [free_count]; NULL if that is 0 */
+    const int32_t* taken_in;   /* [1] or NULL */
+    int32_t* table;            /* [batch, table_cols], rows table_stride apart */
+    int64_t* slots;
+    int32_t* positions;
+    int32_t* offsets;
+    int32_t* lengths;
+    int32_t* taken_out;
+    int64_t table_stride;
+    int64_t tokens;            /* 0..2^31-1 */
+    int64_t free_count;
+    int32_t table_cols;        /* table_cols * page_size below 2^31 */
+    int32_t batch;             /* 1..2^31-2 */
+    int32_t page_size;         /* 16, 32, 64, 128 or 256 */
+} cq_place_t;
+int cq_place(const cq_place_t* args, void* stream);
+
+/* cq_kv_append for packed rows of known slots: row t of k and v [tokens, heads,
+ * head_dim] is quantized into slot slots[t] = page * page_size + offset of every
+ * head.  A row whose slot is negative or past the last page is not written.  No
+ * two rows have one slot. */
+int cq_kv_append_rows(const cq_kv_cache_t* cache, int dtype, int64_t tokens,
+                      const int64_t* slots, const void* k, int64_t k_token_stride,
+                      int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                      int64_t v_head_stride, void* stream);
+
+/*
  * Message of the last failed call on this thread ("" if none).  Replaces
  * the TORCH_CHECK error text that the reference's pybind layer raised.
  */
