@@ -135,6 +135,16 @@ class CqPlace(ctypes.Structure):
         (n, _i32) for n in ("table_cols", "batch", "page_size")]
 
 
+class CqPrompt(ctypes.Structure):
+    """cq_prompt_t"""
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "out")] + [
+        (n, _i64) for n in ("q_token_stride", "q_head_stride", "k_token_stride",
+                            "k_head_stride", "v_token_stride", "v_head_stride")] + [
+        ("q_offsets", _vp), ("k_offsets", _vp), ("q_tokens", _i64), ("k_tokens", _i64)] + [
+        (n, _i32) for n in ("batch", "q_heads", "k_heads", "head_dim", "dtype",
+                            "causal")] + [("softmax_scale", ctypes.c_float)]
+
+
 _cstr = ctypes.c_char_p
 
 # name -> (restype, argtypes); must match include/cdnaqgemv.h
@@ -207,6 +217,7 @@ SIGNATURES = {
     "cq_kv_append_rows": (ctypes.c_int, [
         ctypes.POINTER(CqKvCache), ctypes.c_int, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
         _vp]),
+    "cq_prompt_attention": (ctypes.c_int, [ctypes.POINTER(CqPrompt), _vp]),
     "cq_last_error": (ctypes.c_char_p, []),
     "cq_version": (ctypes.c_char_p, []),
 }

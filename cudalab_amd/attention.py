@@ -12,6 +12,7 @@ and, for prompts whose tokens lie end to end ("packed"),
     p = att.place(block_table, starts, counts, tokens, page_size, free_pages)
     q, k = att.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, p.positions)
     att.append_rows(cache, k, v, p.slots)
+    out = att.prompt(q, k, v, p.offsets)
 
 Every check that needs only shapes, types and devices runs on the host before
 anything is launched and raises RuntimeError.  Lengths, positions and page
@@ -34,7 +35,7 @@ import torch
 
 from . import _capi
 from .ext import _on_device, fast_module_or_none
-from .kvcache import PAGE_SIZES, KVCache
+from .kvcache import HEAD_DIMS, PAGE_SIZES, KVCache
 
 _DTYPES = {torch.float16: _capi.CQ_DTYPE_F16, torch.float32: _capi.CQ_DTYPE_F32,
            torch.bfloat16: _capi.CQ_DTYPE_BF16}
@@ -129,7 +130,7 @@ class AttentionExt:
             "cq_qk_norm_rope", "cq_kv_append", "cq_kv_read", "cq_attention",
             "cq_attention_workspace", "cq_last_error")))
         self._step = mod and mod.StepCalls(*(_capi.entry_address(n) for n in (
-            "cq_place", "cq_kv_append_rows", "cq_last_error")))
+            "cq_place", "cq_kv_append_rows", "cq_prompt_attention", "cq_last_error")))
 
     # ---- norms and rotation ----
     def qk_norm_rope(self, q: torch.Tensor, k: torch.Tensor,
@@ -408,6 +409,96 @@ class AttentionExt:
         _check(_on_device(cache.device, lambda s: self._lib.cq_kv_append_rows(
             ctypes.byref(cache.c), _DTYPES[k.dtype], tokens, slots.data_ptr(), k.data_ptr(),
             ks[0], ks[1], v.data_ptr(), vs[0], vs[1], s)), "append_rows")
+
+    def prompt(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               offsets: torch.Tensor, *, k_offsets: Optional[torch.Tensor] = None,
+               causal: bool = True, scale: Optional[float] = None) -> torch.Tensor:
+        """Attention of packed sequences over keys and values that lie beside
+        them, into a new tensor of q's shape and type.  See prompt_into."""
+        return self._prompt(q, k, v, offsets, None, k_offsets, causal, scale)
+
+    def prompt_into(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    offsets: torch.Tensor, out: torch.Tensor, *,
+                    k_offsets: Optional[torch.Tensor] = None, causal: bool = True,
+                    scale: Optional[float] = None) -> None:
+        """Attention of packed sequences into a given contiguous `out`.
+
+        q (tokens, Hq, D), k and v (keys, H, D), float16 or bfloat16, as they are
+        before they enter a cache: nothing is quantized.  Sequence b's n queries
+        are the rows offsets[b] .. offsets[b + 1] (int32 (batch + 1,), ascending
+        from 0), its m keys the rows k_offsets[b] .. k_offsets[b + 1] of k and v
+        (offsets, if None; with more keys than queries the earlier ones are of
+        earlier chunks).  Query t sees the keys up to m - n + t, or all m without
+        `causal`; query head h reads key head h // (Hq // H).  `scale` multiplies
+        the scores (default D ** -0.5).  Scores, statistics and sums are FP32;
+        each weight is rounded to the type before it multiplies v, the result
+        once.  A key that a query does not see leaves no trace, whatever it
+        holds.  Queries that see nothing and rows of no sequence give zeros."""
+        if out is None:
+            _fail("out must be a tensor, got NoneType")
+        self._prompt(q, k, v, offsets, out, k_offsets, causal, scale)
+
+    def _prompt(self, q, k, v, offsets, out, k_offsets, causal, scale):
+        causal = bool(causal)
+        if scale is not None:
+            scale = _number("scale", scale)
+        if self._step is not None:
+            got = self._step.prompt(q, k, v, offsets, out, k_offsets, causal, scale)
+            if got is not None:
+                return got
+        if not isinstance(q, torch.Tensor):
+            _fail(f"q must be a tensor, got {type(q).__name__}")
+        dev = q.device
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            _heads(name, t, 3, dev)
+            if t.dtype != q.dtype or t.dtype == torch.float32:
+                _fail(f"q, k and v must share float16 or bfloat16, got {q.dtype} and {t.dtype}")
+        tokens, hq, D = q.shape
+        keys, heads = k.size(0), k.size(1)
+        if v.shape != k.shape or k.size(2) != D:
+            _fail(f"k and v must be (keys, heads, {D}), got {tuple(k.shape)} and "
+                  f"{tuple(v.shape)}")
+        if D not in HEAD_DIMS:
+            _fail(f"the head size must be one of {HEAD_DIMS}, got {D}")
+        if heads < 1 or hq < 1 or hq % heads:
+            _fail(f"q's heads must be a multiple of k's, got {hq} and {heads}")
+        _gpu("offsets", offsets, dev)
+        if offsets.dim() != 1 or offsets.numel() < 1:
+            _fail(f"offsets must be (batch + 1,), got {tuple(offsets.shape)}")
+        batch = offsets.numel() - 1
+        _ints("offsets", offsets, (batch + 1,), dev)
+        if k_offsets is not None:
+            _ints("k_offsets", k_offsets, (batch + 1,), dev)
+        elif keys != tokens:
+            _fail(f"without k_offsets k and v have q's {tokens} rows, got {keys}")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        _gpu("out", out, dev)
+        if out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
+            _fail(f"out must be contiguous {q.dtype} {tuple(q.shape)}, got {out.dtype} "
+                  f"{tuple(out.shape)}")
+        if tokens == 0:
+            return out
+        if batch == 0:
+            return out.zero_()
+
+        def aligned(t, most):
+            # the kernels read 16 bytes of a head at once
+            if t.numel() == 0 or not (t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:2])
+                                      or t.stride(0) > most):
+                return t
+            return torch.empty(t.shape, dtype=t.dtype, device=dev).copy_(t)
+
+        q, k, v = aligned(q, 2 ** 40), aligned(k, 2 ** 24), aligned(v, 2 ** 24)
+        a = _capi.CqPrompt(
+            q.data_ptr(), k.data_ptr() or None, v.data_ptr() or None, out.data_ptr(),
+            q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            offsets.data_ptr(), None if k_offsets is None else k_offsets.data_ptr(), tokens,
+            keys, batch, hq, heads, D, _DTYPES[q.dtype], causal,
+            D ** -0.5 if scale is None else scale)
+        _check(_on_device(dev, lambda s: self._lib.cq_prompt_attention(ctypes.byref(a), s)),
+               "prompt")
+        return out
 
     # ---- attention ----
     def forward(self, q: torch.Tensor, cache: KVCache, block_table: torch.Tensor,

@@ -37,6 +37,15 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+// 16 bytes a lane from base + at (0 where that passes `bytes`; both the wave's)
+// straight to LDS, lane after lane from `to` (the wave's, 16-byte aligned).
+__device__ __forceinline__ void load_to_lds(void* to, const void* base, int bytes, int at) {
+    const __amdgpu_buffer_rsrc_t from =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        from, (__attribute__((address_space(3))) void*)to, 16, at, 0, 0, 0);
+}
+
 // Page of a table entry, or -1 for one outside the cache.
 __device__ __forceinline__ int64_t page_in(int32_t entry, int64_t pages) {
     return entry >= 0 && entry < pages ? (int64_t)entry : -1;

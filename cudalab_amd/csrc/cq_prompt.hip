@@ -1,0 +1,451 @@
+// Attention of packed sequences over their own keys and values (gfx950): whole
+// prompts, or chunks of them with the keys of earlier chunks ahead.
+//
+//   o_t = sum_j softmax_j(scale * q_t . k_j) v_j over the keys j that token t
+//   sees: all m of its sequence, or (causal) those up to m - n + t, of n tokens
+//
+// One pass over the keys with a running reference M and sum l of the softmax, in
+// matrix form, 64 keys at a time (v_mfma_f32_32x32x16, FP32 sums):
+//   S^T [keys x rows] = K [keys x D] Q^T [D x rows]
+//   O^T [D x rows]   += V^T [D x keys] P^T [keys x rows]
+// with p = 2^(s scale log2(e) - M), M raised when an exponent passes kRaise, so
+// that the sums are seldom rescaled.  A wave takes 32 rows of one query head and
+// keeps their queries, scores and sums in registers.  S comes out with a row's
+// keys in the two lanes row and row + 32, four keys of each eight in a lane,
+// which is how P goes in again if V is read in that order: nothing crosses lanes
+// but a raise of M and the last sums.  K's rows are read from LDS as they lie, V
+// by the transposing read, which gives a lane four keys of one dim.
+//
+// The waves of a workgroup share the tiles of keys, which go from memory straight
+// to LDS, two tiles in turn: the next one is on its way while one is computed
+// with.  Pieces of 16 bytes are stored at places turned by the row, so that
+// neither read meets its own banks.
+//
+// Rounded to fewer than 32 bits: p to V's type before it multiplies (2^-11 of
+// each weight in fp16, 2^-8 in bf16; l is summed from the unrounded), and the
+// result.
+//
+// A key that a row does not see has p = 0; so that an Inf or NaN in its V stays
+// out of the sums, tiles that some row sees only part of are looked through for
+// such values, and where there are any these enter by themselves, for the rows
+// that see them.
+//
+// Rows and keys lie wherever the offsets on the device say, so every workgroup
+// finds its tile of rows by itself: tiles in the order of their depth in their
+// sequence, the deepest first (they see the most keys), by bisection over the
+// number of tiles that lie as deep or deeper.
+
+#include <algorithm>
+
+#include "cq_elem.h"
+#include "cq_step.h"
+
+namespace cq {
+namespace {
+
+constexpr int kKeys = 64;                      // of a tile
+constexpr int kRows = 32;                      // of a wave
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kRaise = 8.f;
+
+template <class T> struct Typed;
+template <> struct Typed<_Float16> {
+    using v8 = Vec<_Float16, 8>;
+    static constexpr uint32_t kInf = 0x7C00;
+    static __device__ __forceinline__ Vec<float, 16> mfma(v8 a, v8 b, Vec<float, 16> c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Typed<__bf16> {
+    using v8 = Vec<__bf16, 8>;
+    static constexpr uint32_t kInf = 0x7F80;
+    static __device__ __forceinline__ Vec<float, 16> mfma(v8 a, v8 b, Vec<float, 16> c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+using u4 = Vec<uint32_t, 4>;
+using f16v = Vec<float, 16>;
+using s2 = Vec<short, 2>;
+using s4 = Vec<short, 4>;
+
+struct Args {
+    cq_prompt_t a;
+    int32_t group;        // query heads per key head
+    int32_t heads_apart;  // 1: neighbouring workgroups take heads of one run each
+};
+
+// f over a lane and its other half, in both.
+template <class F>
+__device__ __forceinline__ float half_fold(float v, F&& f) {
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+__device__ __forceinline__ int wave_sum(int v) {
+    v += (int)row_dpp<0x128>((uint32_t)v);
+    v += (int)row_dpp<0x124>((uint32_t)v);
+    v += (int)row_dpp<0x122>((uint32_t)v);
+    v += (int)row_dpp<0x121>((uint32_t)v);
+    return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
+           (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+
+// Rows of sequence b (of its queries or keys), within the tensor's.
+struct Span {
+    int first, count;
+    __device__ __forceinline__ Span(const int32_t* offsets, int b, int64_t rows) {
+        const int most = (int)rows;
+        first = max(0, min(offsets[b], most));
+        count = max(0, max(0, min(offsets[b + 1], most)) - first);
+    }
+};
+
+// The `index`th tile of `rows` rows: its sequence and place there (or, behind
+// the sequences' tiles, rows that belong to none: sequence -1).
+struct Tile {
+    int b, row0, rows, first;          // b = -2: none
+    __device__ __forceinline__ Tile(const cq_prompt_t& a, int tile_rows, int index, int lane) {
+        auto tiles_at = [&](int b) {
+            return b < a.batch ? (Span(a.q_offsets, b, a.q_tokens).count + tile_rows - 1) / tile_rows
+                               : 0;
+        };
+        const int near = tiles_at(lane);
+        auto tiles = [&](int base) { return base == 0 ? near : tiles_at(base + lane); };
+        // tiles at depth `level` and below
+        auto from = [&](int level) {
+            int n = 0;
+            for (int base = 0; base < a.batch; base += 64) n += wave_sum(max(0, tiles(base) - level));
+            return n;
+        };
+        const int all = from(0);
+        b = -2;
+        if (index >= all) {
+            // rows ahead of the first sequence, then those behind the last
+            const int most = (int)a.q_tokens;
+            const int ahead = max(0, min(a.q_offsets[0], most));
+            const int last = max(0, min(a.q_offsets[a.batch], most));
+            index -= all;
+            const int n = (ahead + tile_rows - 1) / tile_rows;
+            first = index < n ? 0 : last;
+            const int end = index < n ? ahead : most;
+            row0 = (index < n ? index : index - n) * tile_rows;
+            rows = min(tile_rows, end - first - row0);
+            if (rows > 0) b = -1;
+            return;
+        }
+        // the level with from(level + 1) <= index < from(level)
+        int level = 0, end = ((int)a.q_tokens + tile_rows - 1) / tile_rows, deeper = 0;
+        while (end - level > 1) {
+            const int mid = level + (end - level) / 2;
+            const int n = from(mid);
+            if (n > index) {
+                level = mid;
+            } else {
+                end = mid;
+                deeper = n;
+            }
+        }
+        int rank = index - deeper;     // among the sequences that go so deep
+        for (int base = 0; base < a.batch; base += 64) {
+            uint64_t some = __ballot(tiles(base) > level);
+            const int n = __builtin_popcountll(some);
+            if (rank < n) {
+                for (; rank > 0; --rank) some &= some - 1;
+                b = base + __builtin_ctzll(some);
+                break;
+            }
+            rank -= n;
+        }
+        if (b < 0) return;
+        const Span q(a.q_offsets, b, a.q_tokens);
+        first = q.first;
+        row0 = level * tile_rows;
+        rows = min(tile_rows, q.count - row0);
+    }
+};
+
+template <class T, int D, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s,
+                                                                        uint32_t first_block) {
+    using Ty = Typed<T>;
+    using v8 = typename Ty::v8;
+    constexpr int kSteps = D / 16;             // products over D
+    constexpr int kDims = D / 32;              // dim tiles of O
+    constexpr int kBytes = D * 2;              // of a row
+    constexpr int kPieces = kBytes / 16;       // 16 bytes of a row
+    constexpr int kLoadRows = 64 / kPieces;    // rows of a wave's load
+    constexpr int kLoads = kKeys / kLoadRows / W;      // of a wave, for K (and for V)
+    constexpr int kTileBytes = kKeys * kBytes;
+    static_assert(kLoads * kLoadRows * W == kKeys, "whole loads");
+    __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * kTileBytes];     // K, V; twice
+    const cq_prompt_t& a = s.a;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t block = first_block + blockIdx.x;
+    const uint32_t place = block % (uint32_t)a.q_heads;
+    const int h = s.heads_apart ? (int)(place % 8 * (a.q_heads / 8) + place / 8) : (int)place;
+    const Tile tile(a, kRows * W, (int)(block / (uint32_t)a.q_heads), lane);
+    if (tile.b == -2) return;
+    const int row0 = kRows * wave;             // of the tile
+    T* out = static_cast<T*>(a.out) + ((int64_t)(tile.first + tile.row0) * a.q_heads + h) * D;
+    const int64_t out_row = (int64_t)a.q_heads * D;
+    const Span keys = tile.b >= 0 ? Span(a.k_offsets != nullptr ? a.k_offsets : a.q_offsets, tile.b,
+                                         a.k_tokens)
+                                  : Span(a.q_offsets, 0, 0);
+    const int tokens = tile.b >= 0 ? Span(a.q_offsets, tile.b, a.q_tokens).count : 0;
+    // keys that row r of the tile sees
+    auto limit_of = [&](int r) {
+        if (!a.causal) return keys.count;
+        const int64_t n = (int64_t)keys.count - tokens + tile.row0 + r + 1;
+        return (int)max((int64_t)0, min(n, (int64_t)keys.count));
+    };
+    const int reach = tile.b >= 0 ? limit_of(tile.rows - 1) : 0;        // of the workgroup
+    if (reach == 0) {                          // no keys: zeros
+        for (int i = threadIdx.x; i < tile.rows * kPieces; i += 64 * W)
+            *reinterpret_cast<u4*>(out + i / kPieces * out_row + i % kPieces * 8) = u4{0, 0, 0, 0};
+        return;
+    }
+    const bool live = row0 < tile.rows;
+    const int r = min(row0 + col, tile.rows - 1);      // rows past the last repeat it
+    const int limit = limit_of(r);
+    const int full = limit_of(min(row0, tile.rows - 1));               // every row of the wave sees
+    const int wave_reach = live ? limit_of(min(row0 + kRows, tile.rows) - 1) : 0;
+
+    // the tiles of keys
+    const int64_t k_row = a.k_token_stride * 2, v_row = a.v_token_stride * 2;      // bytes
+    const uint8_t* kp = static_cast<const uint8_t*>(a.k) + keys.first * k_row +
+                        (int64_t)(h / s.group) * a.k_head_stride * 2;
+    const uint8_t* vp = static_cast<const uint8_t*>(a.v) + keys.first * v_row +
+                        (int64_t)(h / s.group) * a.v_head_stride * 2;
+    // where a row's pieces are turned to: K's reads take one piece of 16 rows, V's
+    // four pieces of four rows
+    auto k_turn = [](int row) { return D == 64 ? row >> 1 & 7 : row & 15; };
+    auto v_turn = [](int row) { return D == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; };
+    int k_at[kLoads], v_at[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int row = (wave + W * i) * kLoadRows + lane / kPieces, piece = lane % kPieces;
+        k_at[i] = row * (int)k_row + (piece ^ k_turn(row)) * 16;
+        v_at[i] = row * (int)v_row + (piece ^ v_turn(row)) * 16;
+    }
+    auto fetch = [&](int t, int buf) {
+        const int rows = min(kKeys, reach - t * kKeys);        // past them zeros come
+        const uint8_t* kt = kp + t * (kKeys * k_row);
+        const uint8_t* vt = vp + t * (kKeys * v_row);
+        const int k_bytes = (int)((rows - 1) * k_row) + kBytes;
+        const int v_bytes = (int)((rows - 1) * v_row) + kBytes;
+        uint8_t* to = sm + buf * 2 * kTileBytes;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            load_to_lds(to + (wave + W * i) * 1024, kt, k_bytes, k_at[i]);
+            load_to_lds(to + kTileBytes + (wave + W * i) * 1024, vt, v_bytes, v_at[i]);
+        }
+    };
+    fetch(0, 0);
+
+    // the queries; a negative scale goes into their signs
+    v8 q[kSteps];
+    {
+        const T* p = static_cast<const T*>(a.q) +
+                     (int64_t)(tile.first + tile.row0 + r) * a.q_token_stride +
+                     (int64_t)h * a.q_head_stride + half * 8;
+        const uint32_t turn = a.softmax_scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u) {
+            u4 w = *reinterpret_cast<const u4*>(p + u * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] ^= turn;
+            q[u] = __builtin_bit_cast(v8, w);
+        }
+    }
+    const float by = fabsf(a.softmax_scale) * 1.4426950408889634f;
+    f16v o[kDims];
+#pragma unroll
+    for (int i = 0; i < kDims; ++i) o[i] = f16v{};
+    float ref = 0.f, sum = 0.f, raise = kNegInf;       // ref: M
+
+    const int tiles = (reach + kKeys - 1) / kKeys;
+    for (int t = 0; t < tiles; ++t) {
+        __syncthreads();                       // tile t has come, t - 1 is done with
+        if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
+        const int key0 = t * kKeys;
+        if (key0 >= wave_reach) continue;
+        const uint8_t* ks = sm + (t & 1) * 2 * kTileBytes;
+        const uint8_t* vs = ks + kTileBytes;
+        const bool part = key0 + kKeys > full;         // some row does not see all
+        f16v x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[i] = f16v{};
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u) {
+                const int row = i * 32 + col;
+                const v8 k = *reinterpret_cast<const v8*>(
+                    ks + row * kBytes + ((u * 2 + half) ^ k_turn(row)) * 16);
+                x[i] = Ty::mfma(k, q[u], x[i]);
+            }
+        }
+        // key of x[i][j]: key0 + 32 i + 8 (j / 4) + 4 half + j % 4
+        const int mine = limit - key0 - 4 * half;
+        if (part) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    x[i][j] = 32 * i + 8 * (j / 4) + j % 4 < mine ? x[i][j] : kNegInf;
+        }
+        float top = kNegInf;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, x[i][j]);
+        if (__any(__builtin_fmaf(top, by, -ref) > raise)) {
+            top = half_fold(top, [](float m, float n) { return fmaxf(m, n); }) * by;
+            const bool first = raise == kNegInf;
+            if (top - ref > (first ? kNegInf : 0.f)) {
+                const float keep = first ? 1.f : __builtin_amdgcn_exp2f(ref - top);
+                ref = top;
+                raise = kRaise;
+                sum *= keep;
+#pragma unroll
+                for (int i = 0; i < kDims; ++i) o[i] *= keep;
+            }
+        }
+        v8 p[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], by, -ref));
+                if (part) e = 32 * i + 8 * (j / 4) + j % 4 < mine ? e : 0.f;
+                x[i][j] = e;
+                sum += e;
+                p[2 * i + j / 8][j % 8] = (T)e;
+            }
+        // V's part of step s and dim tile d: keys 16 s + 4 half + 0..3 and 8 more
+        auto read_v = [&](int s, int d) {
+            const int row = 16 * s + 4 * half + (lane >> 2 & 3);
+            const int piece = 4 * d + 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+            const uint8_t* at = vs + row * kBytes + (piece ^ v_turn(row)) * 16 + (lane & 1) * 8;
+            auto read = [&](const uint8_t* from) {
+                return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s4*)from);
+            };
+            const s4 lo = read(at), hi = read(at + 8 * kBytes);      // (the same turn)
+            return __builtin_bit_cast(u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        // whether a masked key's V may spoil the sums
+        bool spoilt = false;
+        constexpr uint32_t kOver = (0x8000u - Ty::kInf) * 0x10001u;
+        if (part) {
+            uint32_t over = 0;
+            for (int i = lane; i < kTileBytes / 16; i += 64) {
+                const u4 w = *reinterpret_cast<const u4*>(vs + i * 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) over |= (w[j] & 0x7FFF7FFFu) + kOver;
+            }
+            spoilt = __any((over & 0x80008000u) != 0);
+        }
+        if (!spoilt) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+                    o[d] = Ty::mfma(__builtin_bit_cast(v8, read_v(s, d)), p[s], o[d]);
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int d = 0; d < kDims; ++d) {
+                    u4 w = read_v(s, d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const s2 bad = __builtin_bit_cast(s2, (w[i] & 0x7FFF7FFFu) + kOver) >> 15;
+                        w[i] &= ~__builtin_bit_cast(uint32_t, bad);
+                    }
+                    o[d] = Ty::mfma(__builtin_bit_cast(v8, w), p[s], o[d]);
+                }
+            // Inf and NaN, key by key
+            for (int key = 0; key < kKeys; ++key) {
+                float e = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        e = 32 * i + 8 * (j / 4) + 4 * half + j % 4 == key ? x[i][j] : e;
+                e = half_fold(e, [](float m, float n) { return m + n; });
+                const bool sees = key < limit - key0;
+#pragma unroll
+                for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const int dim = 32 * d + 2 * j + 4 * half;
+                        const Vec<uint32_t, 2> w = *reinterpret_cast<const Vec<uint32_t, 2>*>(
+                            vs + key * kBytes + ((dim / 8) ^ v_turn(key)) * 16 + half * 8);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint16_t bits = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+                            const float v = (float)__builtin_bit_cast(T, bits);
+                            if (sees && (bits & 0x7FFF) >= Ty::kInf) o[d][j + i] += e * v;
+                        }
+                    }
+            }
+        }
+    }
+    if (!live) return;
+    sum = half_fold(sum, [](float m, float n) { return m + n; });
+    const float share = sum == 0.f ? 0.f : 1.f / sum;
+    if (row0 + col < tile.rows) {
+        T* to = out + (row0 + col) * out_row + 4 * half;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                Vec<T, 4> v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (T)(sum == 0.f ? 0.f : o[d][j + i] * share);
+                *reinterpret_cast<Vec<T, 4>*>(to + 32 * d + 2 * j) = v;
+            }
+    }
+}
+
+// ------------------------------------------------------------------- host
+template <class T, int D, int W>
+hipError_t launch_shaped(const Args& s, hipStream_t stream) {
+    const cq_prompt_t& a = s.a;
+    // every sequence's last tile may be a part of one, and so those of the rows
+    // that belong to none
+    const int64_t tiles = a.q_tokens / (kRows * W) + a.batch + 2;
+    const __int128 grid = (__int128)tiles * a.q_heads;
+    if (grid > kMaxGrid) return hipErrorInvalidValue;
+    return launch_parts((int64_t)grid, [&](dim3 blocks, uint32_t first) {
+        prompt_kernel<T, D, W><<<blocks, dim3(64 * W), 0, stream>>>(s, first);
+    }, 64 * W);
+}
+
+template <class T>
+hipError_t launch_typed(const Args& s, hipStream_t stream) {
+    const cq_prompt_t& a = s.a;
+    const int64_t rows = a.q_tokens / a.batch;
+    const bool eight = rows >= 512 && a.q_tokens / 256 * a.q_heads >= 512;
+    if (a.head_dim == 64)
+        return eight ? launch_shaped<T, 64, 8>(s, stream) : launch_shaped<T, 64, 4>(s, stream);
+    if (a.head_dim == 128)
+        return eight ? launch_shaped<T, 128, 8>(s, stream) : launch_shaped<T, 128, 4>(s, stream);
+    return launch_shaped<T, 256, 4>(s, stream);
+}
+
+}  // namespace
+
+hipError_t launch_prompt(const cq_prompt_t& a, hipStream_t stream) {
+    Args s{};
+    s.a = a;
+    s.group = a.q_heads / a.k_heads;
+    s.heads_apart = a.q_heads % 8 == 0;
+    return a.dtype == CQ_DTYPE_F16 ? launch_typed<_Float16>(s, stream)
+                                   : launch_typed<__bf16>(s, stream);
+}
+
+}  // namespace cq

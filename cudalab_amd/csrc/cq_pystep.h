@@ -28,9 +28,10 @@ int64_t count(py::handle o) {
 
 class Calls {
 public:
-    Calls(uintptr_t place, uintptr_t append_rows, uintptr_t last_error)
+    Calls(uintptr_t place, uintptr_t append_rows, uintptr_t prompt, uintptr_t last_error)
         : place_(reinterpret_cast<decltype(place_)>(place)),
           append_rows_(reinterpret_cast<decltype(append_rows_)>(append_rows)),
+          prompt_(reinterpret_cast<decltype(prompt_)>(prompt)),
           last_error_(reinterpret_cast<decltype(last_error_)>(last_error)) {}
 
     // (slots, positions, offsets, lengths, taken), or None.
@@ -94,6 +95,60 @@ public:
                     "append_rows");
     }
 
+    // out (a new one for None), or None.
+    py::object prompt(py::handle q_, py::handle k_, py::handle v_, py::handle offsets_,
+                      py::handle out_, py::handle k_offsets_, bool causal, py::handle scale) const {
+        bool ok = true;
+        const at::Tensor *q = tensor(q_, false, ok), *k = tensor(k_, false, ok);
+        const at::Tensor *v = tensor(v_, false, ok), *offsets = tensor(offsets_, false, ok);
+        const at::Tensor *out = tensor(out_, true, ok), *koff = tensor(k_offsets_, true, ok);
+        if (!ok || q->dim() != 3 || k->dim() != 3 || v->sizes() != k->sizes() || !on_current(*q) ||
+            offsets->dim() != 1)
+            return py::none();
+        const c10::Device dev = q->device();
+        const at::ScalarType type = q->scalar_type();
+        const int64_t tokens = q->size(0), heads = q->size(1), D = q->size(2);
+        const int64_t keys = k->size(0), batch = offsets->size(0) - 1;
+        if ((type != at::kHalf && type != at::kBFloat16) || tokens < 1 || batch < 1 ||
+            batch >= INT32_MAX || heads < 1 || heads > 65535 || k->size(1) < 1 ||
+            heads % k->size(1) != 0 || k->size(2) != D || D > 256 || (koff == nullptr && keys != tokens))
+            return py::none();
+        for (const at::Tensor* t : {q, k, v})
+            if (t->scalar_type() != type || t->device() != dev || !last_contiguous(*t) ||
+                t->stride(0) % 8 != 0 || t->stride(1) % 8 != 0 ||
+                reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 != 0)
+                return py::none();
+        if (!ints(*offsets, batch + 1, dev) || (koff != nullptr && !ints(*koff, batch + 1, dev)))
+            return py::none();
+        at::Tensor made;
+        if (out == nullptr) {
+            made = at::empty(q->sizes(), q->options());
+            out = &made;
+        }
+        if (out->scalar_type() != type || out->device() != dev || out->sizes() != q->sizes() ||
+            !out->is_contiguous())
+            return py::none();
+        cq_prompt_t a{};
+        a.q = q->data_ptr(), a.k = k->data_ptr(), a.v = v->data_ptr(), a.out = out->data_ptr();
+        a.q_token_stride = q->stride(0), a.q_head_stride = q->stride(1);
+        a.k_token_stride = k->stride(0), a.k_head_stride = k->stride(1);
+        a.v_token_stride = v->stride(0), a.v_head_stride = v->stride(1);
+        a.q_offsets = static_cast<const int32_t*>(offsets->data_ptr());
+        a.k_offsets = koff != nullptr ? static_cast<const int32_t*>(koff->data_ptr()) : nullptr;
+        a.q_tokens = tokens;
+        a.k_tokens = keys;
+        a.batch = static_cast<int32_t>(batch);
+        a.q_heads = static_cast<int32_t>(heads);
+        a.k_heads = static_cast<int32_t>(k->size(1));
+        a.head_dim = static_cast<int32_t>(D);
+        a.dtype = dtype_code(type);
+        a.causal = causal;
+        a.softmax_scale = scale.is_none() ? static_cast<float>(1.0 / std::sqrt(static_cast<double>(D)))
+                                          : static_cast<float>(PyFloat_AsDouble(scale.ptr()));
+        if (!done(prompt_(&a, stream_of(*q)), "prompt")) return py::none();
+        return py::cast(*out);
+    }
+
 private:
     bool done(int status, const char* what) const {
         if (status == CQ_ERR_HIP)
@@ -105,12 +160,14 @@ private:
     int (*place_)(const cq_place_t*, void*);
     int (*append_rows_)(const cq_kv_cache_t*, int, int64_t, const int64_t*, const void*, int64_t,
                         int64_t, const void*, int64_t, int64_t, void*);
+    int (*prompt_)(const cq_prompt_t*, void*);
     const char* (*last_error_)();
 };
 
 void bind(py::module_& m) {
     py::class_<Calls>(m, "StepCalls")
-        .def(py::init<uintptr_t, uintptr_t, uintptr_t>())
+        .def(py::init<uintptr_t, uintptr_t, uintptr_t, uintptr_t>())
+        .def("prompt", &Calls::prompt)
         .def("place", &Calls::place)
         .def("append_rows", &Calls::append_rows);
 }

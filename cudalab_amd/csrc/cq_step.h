@@ -19,4 +19,7 @@ hipError_t launch_kv_append_rows(const cq_kv_cache_t& c, int dtype, int64_t toke
                                  const int64_t* slots, const void* k, KvStrides ks, const void* v,
                                  KvStrides vs, hipStream_t stream);
 
+// cq_prompt.hip
+hipError_t launch_prompt(const cq_prompt_t& a, hipStream_t stream);
+
 }  // namespace cq

@@ -3,6 +3,7 @@
 // device (lengths, offsets, slots) the kernels check themselves.
 
 #include <climits>
+#include <cmath>
 #include <string>
 
 #include "cq_checks.h"
@@ -82,9 +83,56 @@ int check_append_rows(const cq_kv_cache_t& c, int dtype, int64_t tokens, const i
     return CQ_OK;
 }
 
+int check_prompt(const cq_prompt_t& a) {
+    constexpr int64_t kMostRows = INT_MAX - 511;      // a tile's rows behind them fit an int
+    if (a.batch < 1 || a.batch == INT_MAX) return invalid("batch must be in [1, 2^31-2]");
+    if (a.q_tokens < 1 || a.q_tokens > kMostRows || a.k_tokens < 0 || a.k_tokens > kMostRows)
+        return invalid("q_tokens must be in [1, 2^31-512], k_tokens in [0, 2^31-512]");
+    if (a.k_heads < 1 || a.q_heads < 1 || a.q_heads > 65535 || a.q_heads % a.k_heads != 0)
+        return invalid("q_heads must be a multiple of k_heads, at most 65535");
+    if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256)
+        return invalid("head_dim must be 64, 128 or 256");
+    if (a.dtype != CQ_DTYPE_F16 && a.dtype != CQ_DTYPE_BF16)
+        return invalid("dtype must be CQ_DTYPE_F16 or CQ_DTYPE_BF16");
+    if (std::isnan(a.softmax_scale) || std::isinf(a.softmax_scale))
+        return invalid("softmax_scale must be finite");
+    if (a.q == nullptr || a.out == nullptr || a.q_offsets == nullptr ||
+        (a.k_tokens > 0 && (a.k == nullptr || a.v == nullptr)))
+        return invalid("null pointer argument");
+    if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16))
+        return invalid("q, k, v and out must be 16-byte aligned");
+    if (!aligned(a.q_offsets, 4) || !aligned(a.k_offsets, 4))
+        return invalid("the offsets must be 4-byte aligned");
+    for (int64_t n : {a.q_token_stride, a.q_head_stride, a.k_token_stride, a.k_head_stride,
+                      a.v_token_stride, a.v_head_stride})
+        if (!stride_ok(n) || n % 8 != 0) return invalid("strides must be multiples of 8 in [0, 2^40]");
+    if (a.k_token_stride > 1 << 24 || a.v_token_stride > 1 << 24)
+        return invalid("the token strides of k and v must be at most 2^24");
+    const Span out[] = {strided(a.out, {{a.q_tokens, (int64_t)a.q_heads * a.head_dim}},
+                                (int64_t)a.q_heads * a.head_dim, 2)};
+    const Span in[] = {
+        strided(a.q, {{a.q_tokens, a.q_token_stride}, {a.q_heads, a.q_head_stride}}, a.head_dim, 2),
+        strided(a.k, {{a.k_tokens, a.k_token_stride}, {a.k_heads, a.k_head_stride}}, a.head_dim, 2),
+        strided(a.v, {{a.k_tokens, a.v_token_stride}, {a.k_heads, a.v_head_stride}}, a.head_dim, 2),
+        Span(a.q_offsets, (static_cast<U>(a.batch) + 1) * 4),
+        Span(a.k_offsets, (static_cast<U>(a.batch) + 1) * 4)};
+    if (meet(out, in)) return invalid("out overlaps an input");
+    return CQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int cq_prompt_attention(const cq_prompt_t* args, void* stream) {
+    return guarded([&]() -> int {
+        if (args == nullptr) return invalid("null pointer: args");
+        const int st = check_prompt(*args);
+        if (st != CQ_OK) return st;
+        return hip_status(cq::launch_prompt(*args, static_cast<hipStream_t>(stream)),
+                          "cq_prompt_attention");
+    });
+}
 
 int cq_place(const cq_place_t* args, void* stream) {
     return guarded([&]() -> int {

@@ -609,6 +609,37 @@ int cq_kv_append_rows(const cq_kv_cache_t* cache, int dtype, int64_t tokens,
                       int64_t k_head_stride, const void* v, int64_t v_token_stride,
                       int64_t v_head_stride, void* stream);
 
+/* Attention of packed sequences over keys and values that lie beside them,
+ * q [q_tokens, q_heads, head_dim], k and v [k_tokens, k_heads, head_dim], q head h
+ * on key head h / (q_heads / k_heads): sequence b's n queries are the rows
+ * q_offsets[b] .. q_offsets[b + 1], its m keys the rows k_offsets[b] ..
+ * k_offsets[b + 1] (q_offsets, if NULL).  Query t sees all m keys, or, if causal,
+ * those up to m - n + t.  out = sum_j softmax_j(softmax_scale * q . k_j) v_j with
+ * FP32 scores, statistics and sums; each weight is rounded to `dtype` (F16 or BF16)
+ * before it multiplies v, the result once.  Keys that a row does not see leave no
+ * trace in it, whatever they hold.  0 for a row that sees nothing and for rows of
+ * no sequence.  Offsets ascend; they are cut to the tensors' rows. */
+typedef struct cq_prompt {
+    const void* q;             /* pointers 16-byte aligned, */
+    const void* k;             /* strides multiples of 8, those of k's and v's */
+    const void* v;             /* tokens at most 2^24 */
+    void* out;                 /* contiguous [q_tokens, q_heads, head_dim] */
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride;
+    const int32_t* q_offsets;  /* [batch + 1] */
+    const int32_t* k_offsets;  /* [batch + 1] or NULL */
+    int64_t q_tokens;          /* 1..2^31-512 */
+    int64_t k_tokens;          /* 0..2^31-512 */
+    int32_t batch;             /* 1..2^31-2 */
+    int32_t q_heads, k_heads;
+    int32_t head_dim;          /* 64, 128 or 256 */
+    int32_t dtype;
+    int32_t causal;
+    float softmax_scale;
+} cq_prompt_t;
+int cq_prompt_attention(const cq_prompt_t* args, void* stream);
+
 /*
  * Message of the last failed call on this thread ("" if none).  Replaces
  * the TORCH_CHECK error text that the reference's pybind layer raised.
