@@ -145,6 +145,13 @@ class CqPrompt(ctypes.Structure):
                             "causal")] + [("softmax_scale", ctypes.c_float)]
 
 
+class CqQgemm(ctypes.Structure):
+    """cq_qgemm_t"""
+    _fields_ = [(n, _vp) for n in ("x", "x_scale", "w", "w_scale", "out")] + [
+        (n, _i64) for n in ("x_stride", "tokens", "n", "k")] + [
+        ("workspace", _vp), ("workspace_bytes", _i64), ("dtype", _i32)]
+
+
 _cstr = ctypes.c_char_p
 
 # name -> (restype, argtypes); must match include/cdnaqgemv.h
@@ -218,6 +225,9 @@ SIGNATURES = {
         ctypes.POINTER(CqKvCache), ctypes.c_int, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
         _vp]),
     "cq_prompt_attention": (ctypes.c_int, [ctypes.POINTER(CqPrompt), _vp]),
+    "cq_quantize_tokens": (ctypes.c_int, [ctypes.c_int, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "cq_qgemm": (ctypes.c_int, [ctypes.POINTER(CqQgemm), _vp]),
+    "cq_qgemm_workspace": (_i64, [ctypes.POINTER(CqQgemm)]),
     "cq_last_error": (ctypes.c_char_p, []),
     "cq_version": (ctypes.c_char_p, []),
 }

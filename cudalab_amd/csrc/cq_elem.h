@@ -37,6 +37,22 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+// Scale of a vector and the reciprocal that its codes are rounded with, from the
+// bits of its largest |x|: 0 for a vector of tiny numbers (the scale or its
+// reciprocal would leave FP32's normal range), NaN for one with NaN or Inf.
+template <int BITS>
+__device__ __forceinline__ void scale_of(uint32_t amax_bits, float& scale, float& inv) {
+    constexpr float rcp = 1.0f / (BITS == 8 ? 127.0f : 7.0f);
+    const float amax = __uint_as_float(amax_bits);
+    scale = amax * rcp;
+    inv = 1.0f / scale;
+    if (amax < 0x1p-100f) scale = inv = 0.f;
+    if (amax_bits >= 0x7F800000u) {
+        scale = __builtin_nanf("");
+        inv = 0.f;
+    }
+}
+
 // 16 bytes a lane from base + at (0 where that passes `bytes`; both the wave's)
 // straight to LDS, lane after lane from `to` (the wave's, 16-byte aligned).
 __device__ __forceinline__ void load_to_lds(void* to, const void* base, int bytes, int at) {

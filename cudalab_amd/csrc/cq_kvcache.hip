@@ -24,21 +24,6 @@ namespace cq {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr float kTiny = 0x1p-100f;
-
-// Scale of a vector and the reciprocal that its codes are rounded with.
-template <int BITS>
-__device__ __forceinline__ void scale_of(uint32_t amax_bits, float& scale, float& inv) {
-    constexpr float rcp = 1.0f / (BITS == 8 ? 127.0f : 7.0f);
-    const float amax = __uint_as_float(amax_bits);
-    scale = amax * rcp;
-    inv = 1.0f / scale;
-    if (amax < kTiny) scale = inv = 0.f;
-    if (amax_bits >= 0x7F800000u) {
-        scale = __builtin_nanf("");
-        inv = 0.f;
-    }
-}
 
 // Largest |x| of the 16 lanes that share a token, as FP32 bits (NaN above
 // Inf above every number).  Magnitudes of 16 bits are compared as they are, two

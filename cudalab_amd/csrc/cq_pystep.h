@@ -164,7 +164,104 @@ private:
     const char* (*last_error_)();
 };
 
+class Qgemm {
+public:
+    Qgemm(uintptr_t quantize, uintptr_t gemm, uintptr_t workspace, uintptr_t last_error)
+        : quantize_(reinterpret_cast<decltype(quantize_)>(quantize)),
+          gemm_(reinterpret_cast<decltype(gemm_)>(gemm)),
+          workspace_(reinterpret_cast<decltype(workspace_)>(workspace)),
+          last_error_(reinterpret_cast<decltype(last_error_)>(last_error)) {}
+
+    // (codes, scales), or None.
+    py::object quantize(py::handle x_) const {
+        bool ok = true;
+        const at::Tensor* x = tensor(x_, false, ok);
+        if (!ok || x->dim() != 2 || !on_current(*x) || !last_contiguous(*x)) return py::none();
+        const int dt = dtype_code(x->scalar_type());
+        const int64_t tokens = x->size(0), k = x->size(1);
+        if (dt < 0 || tokens < 1 || k < 1) return py::none();
+        at::Tensor codes = at::empty({tokens, k}, x->options().dtype(at::kChar));
+        at::Tensor scales = at::empty({tokens}, x->options().dtype(at::kFloat));
+        if (!done(quantize_(dt, x->data_ptr(), x->stride(0), tokens, k,
+                            static_cast<int8_t*>(codes.data_ptr()),
+                            static_cast<float*>(scales.data_ptr()), stream_of(*x)),
+                  "quantize_tokens"))
+            return py::none();
+        return py::make_tuple(codes, scales);
+    }
+
+    // out (a new one of `dtype` for None), or None.
+    py::object forward(py::handle codes_, py::handle scales_, py::handle w_, py::handle scale_,
+                       py::handle out_, py::handle dtype) const {
+        bool ok = true;
+        const at::Tensor *x = tensor(codes_, false, ok), *xs = tensor(scales_, false, ok);
+        const at::Tensor *w = tensor(w_, false, ok), *ws = tensor(scale_, false, ok);
+        const at::Tensor* out = tensor(out_, true, ok);
+        if (!ok || x->dim() != 2 || w->dim() != 2 || x->scalar_type() != at::kChar ||
+            w->scalar_type() != at::kChar || !on_current(*w) || x->device() != w->device())
+            return py::none();
+        const c10::Device dev = w->device();
+        const int64_t tokens = x->size(0), n = w->size(0), k = w->size(1);
+        if (tokens < 1 || n < 1 || k < 1 || x->size(1) != k || !w->is_contiguous() ||
+            !last_contiguous(*x) || (tokens > 1 && x->stride(0) < k) || !scales_ok(*ws, n, dev) ||
+            !scales_ok(*xs, tokens, dev))
+            return py::none();
+        at::Tensor made;
+        if (out == nullptr) {
+            if (!THPDtype_Check(dtype.ptr())) return py::none();
+            const at::ScalarType type = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+            if (dtype_code(type) < 0) return py::none();
+            made = at::empty({tokens, n}, w->options().dtype(type));
+            out = &made;
+        }
+        cq_qgemm_t a{};
+        a.dtype = dtype_code(out->scalar_type());
+        if (a.dtype < 0 || out->dim() != 2 || out->size(0) != tokens || out->size(1) != n ||
+            !out->is_contiguous() || out->device() != dev)
+            return py::none();
+        a.x = static_cast<const int8_t*>(x->data_ptr());
+        a.x_scale = static_cast<const float*>(xs->data_ptr());
+        a.w = static_cast<const int8_t*>(w->data_ptr());
+        a.w_scale = static_cast<const float*>(ws->data_ptr());
+        a.out = out->data_ptr();
+        a.x_stride = x->stride(0) < k ? k : x->stride(0);
+        a.tokens = tokens, a.n = n, a.k = k;
+        const int64_t need = workspace_(&a);
+        if (need < 0) return py::none();
+        at::Tensor space;      // given back at the end: work queued behind on this stream follows
+        if (need > 0) {
+            space = at::empty({need}, w->options().dtype(at::kByte));
+            a.workspace = space.data_ptr();
+            a.workspace_bytes = need;
+        }
+        if (!done(gemm_(&a, stream_of(*w)), "forward")) return py::none();
+        return py::cast(*out);
+    }
+
+private:
+    static bool scales_ok(const at::Tensor& t, int64_t n, const c10::Device& d) {
+        return t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n &&
+               t.is_contiguous() && t.device() == d;
+    }
+
+    bool done(int status, const char* what) const {
+        if (status == CQ_ERR_HIP)
+            throw std::runtime_error(std::string(what) + " failed (status " +
+                                     std::to_string(status) + "): " + last_error_());
+        return status == CQ_OK;
+    }
+
+    int (*quantize_)(int, const void*, int64_t, int64_t, int64_t, int8_t*, float*, void*);
+    int (*gemm_)(const cq_qgemm_t*, void*);
+    int64_t (*workspace_)(const cq_qgemm_t*);
+    const char* (*last_error_)();
+};
+
 void bind(py::module_& m) {
+    py::class_<Qgemm>(m, "QgemmCalls")
+        .def(py::init<uintptr_t, uintptr_t, uintptr_t, uintptr_t>())
+        .def("quantize", &Qgemm::quantize)
+        .def("forward", &Qgemm::forward);
     py::class_<Calls>(m, "StepCalls")
         .def(py::init<uintptr_t, uintptr_t, uintptr_t, uintptr_t>())
         .def("prompt", &Calls::prompt)

@@ -22,4 +22,10 @@ hipError_t launch_kv_append_rows(const cq_kv_cache_t& c, int dtype, int64_t toke
 // cq_prompt.hip
 hipError_t launch_prompt(const cq_prompt_t& a, hipStream_t stream);
 
+// cq_qgemm.hip
+hipError_t launch_quantize_tokens(int dtype, const void* x, int64_t x_stride, int64_t tokens,
+                                  int64_t k, int8_t* codes, float* scales, hipStream_t stream);
+int64_t qgemm_workspace(const cq_qgemm_t& a);
+hipError_t launch_qgemm(const cq_qgemm_t& a, hipStream_t stream);
+
 }  // namespace cq

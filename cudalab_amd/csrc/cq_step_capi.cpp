@@ -83,8 +83,9 @@ int check_append_rows(const cq_kv_cache_t& c, int dtype, int64_t tokens, const i
     return CQ_OK;
 }
 
+constexpr int64_t kMostRows = INT_MAX - 511;      // a tile's rows behind them fit an int
+
 int check_prompt(const cq_prompt_t& a) {
-    constexpr int64_t kMostRows = INT_MAX - 511;      // a tile's rows behind them fit an int
     if (a.batch < 1 || a.batch == INT_MAX) return invalid("batch must be in [1, 2^31-2]");
     if (a.q_tokens < 1 || a.q_tokens > kMostRows || a.k_tokens < 0 || a.k_tokens > kMostRows)
         return invalid("q_tokens must be in [1, 2^31-512], k_tokens in [0, 2^31-512]");
@@ -120,9 +121,86 @@ int check_prompt(const cq_prompt_t& a) {
     return CQ_OK;
 }
 
+constexpr int64_t kMostK = 131071;                // of products of 2^14 a sum in 32 bits
+
+int check_quantize(int dtype, const void* x, int64_t x_stride, int64_t tokens, int64_t k,
+                   const int8_t* codes, const float* scales) {
+    if (!known_dtype(dtype)) return invalid("unknown dtype");
+    if (tokens < 1 || tokens > kMostRows) return invalid("tokens must be in [1, 2^31-512]");
+    if (k < 1 || k > INT_MAX) return invalid("k must be in [1, 2^31-1]");
+    if (x == nullptr || codes == nullptr || scales == nullptr) return invalid("null pointer argument");
+    const int64_t es = elem_bytes(dtype);
+    if (!aligned(x, es) || !aligned(scales, 4))
+        return invalid("a pointer is not aligned to its element size");
+    if (!stride_ok(x_stride)) return invalid("strides must be in [0, 2^40]");
+    const Span out[] = {Span(codes, static_cast<U>(tokens) * static_cast<U>(k)),
+                        Span(scales, static_cast<U>(tokens) * 4)};
+    const Span in[] = {strided(x, {{tokens, x_stride}}, k, es)};
+    if (meet(out, in)) return invalid("an output overlaps another operand");
+    return CQ_OK;
+}
+
+int check_qgemm(const cq_qgemm_t& a, bool launching) {
+    if (!known_dtype(a.dtype)) return invalid("unknown dtype");
+    if (a.tokens < 1 || a.tokens > kMostRows || a.n < 1 || a.n > kMostRows)
+        return invalid("tokens and n must be in [1, 2^31-512]");
+    if (a.k < 1 || a.k > kMostK) return invalid("k must be in [1, 131071]");
+    if (a.x_stride < a.k || a.x_stride > (int64_t)1 << 40)
+        return invalid("x_stride must be in [k, 2^40]");
+    if (!launching) return CQ_OK;
+    if (a.x == nullptr || a.x_scale == nullptr || a.w == nullptr || a.w_scale == nullptr ||
+        a.out == nullptr)
+        return invalid("null pointer argument");
+    if (!aligned(a.x_scale, 4) || !aligned(a.w_scale, 4) || !aligned(a.out, 16))
+        return invalid("out must be 16-byte aligned, the scales 4-byte aligned");
+    const int64_t need = cq::qgemm_workspace(a);
+    if (need > 0 && (a.workspace == nullptr || a.workspace_bytes < need || !aligned(a.workspace, 16)))
+        return cq::set_error(CQ_ERR_BUFFER_TOO_SMALL,
+                             "the call needs " + std::to_string(need) +
+                                 " bytes of 16-byte aligned workspace, got " +
+                                 std::to_string(a.workspace_bytes));
+    const U n = static_cast<U>(a.n), tokens = static_cast<U>(a.tokens);
+    const Span out[] = {Span(a.out, tokens * n * static_cast<U>(elem_bytes(a.dtype))),
+                        Span(need > 0 ? a.workspace : nullptr, static_cast<U>(need > 0 ? need : 0))};
+    const Span in[] = {strided(a.x, {{a.tokens, a.x_stride}}, a.k, 1),
+                       Span(a.w, n * static_cast<U>(a.k)), Span(a.x_scale, tokens * 4),
+                       Span(a.w_scale, n * 4)};
+    if (meet(out, in)) return invalid("out or the workspace overlaps an input");
+    return CQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+int cq_quantize_tokens(int dtype, const void* x, int64_t x_stride, int64_t tokens, int64_t k,
+                       int8_t* codes, float* scales, void* stream) {
+    return guarded([&]() -> int {
+        const int st = check_quantize(dtype, x, x_stride, tokens, k, codes, scales);
+        if (st != CQ_OK) return st;
+        return hip_status(cq::launch_quantize_tokens(dtype, x, x_stride, tokens, k, codes, scales,
+                                                     static_cast<hipStream_t>(stream)),
+                          "cq_quantize_tokens");
+    });
+}
+
+int cq_qgemm(const cq_qgemm_t* args, void* stream) {
+    return guarded([&]() -> int {
+        if (args == nullptr) return invalid("null pointer: args");
+        const int st = check_qgemm(*args, true);
+        if (st != CQ_OK) return st;
+        return hip_status(cq::launch_qgemm(*args, static_cast<hipStream_t>(stream)), "cq_qgemm");
+    });
+}
+
+int64_t cq_qgemm_workspace(const cq_qgemm_t* args) {
+    return guarded([&]() -> int64_t {
+        if (args == nullptr) return -invalid("null pointer: args");
+        const int st = check_qgemm(*args, false);
+        if (st != CQ_OK) return -st;
+        return cq::qgemm_workspace(*args);
+    }, -CQ_ERR_HIP);
+}
 
 int cq_prompt_attention(const cq_prompt_t* args, void* stream) {
     return guarded([&]() -> int {

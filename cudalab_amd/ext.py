@@ -684,11 +684,14 @@ _EXT_TYPES = {"int4gemv": Int4gemvExt, "qgemv": QgemvExt, "gemv": GemvExt}
 
 
 def get_ext(op: str):
-    """Singleton extension object for "int4gemv", "qgemv", "gemv" or
-    "attention"."""
+    """Singleton extension object for "int4gemv", "qgemv", "gemv",
+    "attention" or "qgemm"."""
     if op == "attention":
         from .attention import get_attention
         return get_attention()
+    if op == "qgemm":
+        from .qgemm import get_qgemm
+        return get_qgemm()
     if op not in _EXT_TYPES:
         raise KeyError(f"no extension for operator {op!r}")
     e = _EXTS.get(op)

@@ -641,6 +641,39 @@ typedef struct cq_prompt {
 int cq_prompt_attention(const cq_prompt_t* args, void* stream);
 
 /*
+ * INT8 products of many tokens: the weights of cq_qgemv (int8 [n, k] with an FP32
+ * scale a row), activations quantized with a scale a token.
+ */
+
+/* codes int8 [tokens, k] and scales [tokens] of x [tokens, k] (CQ_DTYPE_*, rows
+ * x_stride elements apart), every operation rounded to FP32:
+ *   scale = amax * fl(1 / 127), code = clamp(rint(x * fl(1 / scale)), +-127)
+ * An amax below 2^-100 gives scale 0 and codes 0, one that is not finite scale
+ * NaN and codes 0. */
+int cq_quantize_tokens(int dtype, const void* x, int64_t x_stride, int64_t tokens, int64_t k,
+                       int8_t* codes, float* scales, void* stream);
+
+/* out[t, n] = (sum_k x[t, k] w[n, k]) * x_scale[t] * w_scale[n]: the sum a whole
+ * number, the products (in this order) FP32, rounded once to `dtype`.  out
+ * [tokens, n] is contiguous and shares no byte with an input. */
+typedef struct cq_qgemm {
+    const int8_t* x;           /* [tokens, k], rows x_stride apart */
+    const float* x_scale;      /* [tokens] */
+    const int8_t* w;           /* [n, k] */
+    const float* w_scale;      /* [n] */
+    void* out;                 /* 16-byte aligned */
+    int64_t x_stride;          /* at least k, at most 2^40 */
+    int64_t tokens, n;         /* 1..2^31-512 */
+    int64_t k;                 /* 1..131071: sums of that many fit 32 bits */
+    void* workspace;           /* cq_qgemm_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int32_t dtype;             /* CQ_DTYPE_F16, _F32 or _BF16 */
+} cq_qgemm_t;
+int cq_qgemm(const cq_qgemm_t* args, void* stream);
+/* Bytes of workspace that the call needs (0 or more), or a negative CQ_* status. */
+int64_t cq_qgemm_workspace(const cq_qgemm_t* args);
+
+/*
  * Message of the last failed call on this thread ("" if none).  Replaces
  * the TORCH_CHECK error text that the reference's pybind layer raised.
  */

@@ -70,3 +70,70 @@ def test_place_by_hand():
     assert got[1] == [15, 16, 17, *range(18), 0, 0]
     assert got[2:5] == ([0, 3, 21], [18, 18], 3)
     assert got[5] == [[4, 7, 9], [5, -1, 9]]
+
+
+def _quantize(dtype=0, x=P[0], stride=64, tokens=5, k=64, codes=P[1], scales=P[2]):
+    return _capi.load().cq_quantize_tokens(dtype, x, stride, tokens, k, codes, scales, None)
+
+
+def _qgemm(workspace=False, **change):
+    a = _capi.CqQgemm(x=P[0], x_scale=P[1], w=P[2], w_scale=P[3], out=P[4], x_stride=64,
+                      tokens=5, n=7, k=64, workspace=P[5], workspace_bytes=1 << 31, dtype=0)
+    for n, v in change.items():
+        setattr(a, n, v)
+    lib = _capi.load()
+    return (lib.cq_qgemm_workspace(ctypes.byref(a)) if workspace
+            else lib.cq_qgemm(ctypes.byref(a), None))
+
+
+def test_qgemm_refuses():
+    for change in (dict(dtype=3), dict(x=None), dict(codes=None), dict(scales=None), dict(x=P[0] + 1),
+                   dict(scales=P[2] + 2), dict(stride=-1), dict(stride=2 ** 41), dict(tokens=0),
+                   dict(tokens=2 ** 31 - 1), dict(k=0), dict(k=2 ** 31), dict(codes=P[0] + 8),
+                   dict(scales=P[0]), dict(scales=P[1] + 4)):
+        assert _quantize(**change) == BAD, change
+    sizes = (dict(dtype=-1), dict(tokens=0), dict(tokens=2 ** 31 - 1), dict(n=0), dict(n=2 ** 31),
+             dict(k=0), dict(k=131072, x_stride=131072), dict(x_stride=63),
+             dict(x_stride=2 ** 41))
+    for change in sizes:
+        assert _qgemm(**change) == BAD, change
+        assert _qgemm(True, **change) == -BAD, change
+    for change in (*(dict([(n, None)]) for n in ("x", "x_scale", "w", "w_scale", "out")),
+                   dict(x_scale=P[1] + 2), dict(w_scale=P[3] + 1), dict(out=P[4] + 8),
+                   dict(out=P[0]), dict(out=P[2] + 432), dict(out=P[1]), dict(out=P[3] + 16)):
+        assert _qgemm(**change) == BAD, change
+    # more workgroups than a launch holds
+    assert _qgemm(tokens=2 ** 31 - 512, n=2 ** 31 - 512) == BAD
+    assert _capi.load().cq_qgemm(None, None) == BAD
+    assert _capi.load().cq_qgemm_workspace(None) == -BAD
+
+
+def _prompt(**change):
+    a = _capi.CqPrompt(
+        q=P[0], k=P[1], v=P[2], out=P[3], q_token_stride=512, q_head_stride=128,
+        k_token_stride=256, k_head_stride=128, v_token_stride=256, v_head_stride=128,
+        q_offsets=P[4], k_offsets=P[5], q_tokens=9, k_tokens=11, batch=2, q_heads=4, k_heads=2,
+        head_dim=128, dtype=0, causal=1, softmax_scale=0.1)
+    for n, v in change.items():
+        setattr(a, n, v)
+    return _capi.load().cq_prompt_attention(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("change", [
+    *(dict([(n, None)]) for n in ("q", "k", "v", "out", "q_offsets")),
+    *(dict([(n, P[12] + 8)]) for n in ("q", "k", "v", "out")), dict(q_offsets=P[4] + 2),
+    dict(k_offsets=P[5] + 1), dict(batch=0), dict(batch=2 ** 31 - 1), dict(q_tokens=0),
+    dict(q_tokens=2 ** 31 - 511), dict(k_tokens=-1), dict(k_tokens=2 ** 31 - 1), dict(q_heads=0),
+    dict(q_heads=3), dict(k_heads=0), dict(q_heads=131072), dict(head_dim=96), dict(dtype=1),
+    dict(dtype=3), dict(softmax_scale=float("nan")), dict(softmax_scale=float("inf")),
+    dict(q_token_stride=-8), dict(q_head_stride=4), dict(k_token_stride=2 ** 24 + 8),
+    dict(v_token_stride=2 ** 25), dict(v_head_stride=2 ** 41), dict(out=P[0]),
+    dict(out=P[1] + 2048), dict(out=P[2] - 64), dict(out=P[4]), dict(out=P[5] - 9216 + 16)])
+def test_prompt_refuses(change):
+    assert _prompt(**change) == BAD
+    assert _capi.last_error()
+    assert _capi.load().cq_prompt_attention(None, None) == BAD
+
+
+def test_prompt_refuses_too_many_workgroups():
+    assert _prompt(batch=2 ** 30, q_heads=65534) == BAD
