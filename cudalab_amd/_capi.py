@@ -228,6 +228,8 @@ SIGNATURES = {
     "cq_quantize_tokens": (ctypes.c_int, [ctypes.c_int, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
     "cq_qgemm": (ctypes.c_int, [ctypes.POINTER(CqQgemm), _vp]),
     "cq_qgemm_workspace": (_i64, [ctypes.POINTER(CqQgemm)]),
+    "cq_attention_tree": (ctypes.c_int, [ctypes.POINTER(CqKvCache),
+                                         ctypes.POINTER(CqAttention), _vp, _vp]),
     "cq_last_error": (ctypes.c_char_p, []),
     "cq_version": (ctypes.c_char_p, []),
 }

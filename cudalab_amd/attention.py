@@ -128,7 +128,7 @@ class AttentionExt:
         mod = fast_module_or_none()
         self._fast = mod and mod.AttentionCalls(*(_capi.entry_address(n) for n in (
             "cq_qk_norm_rope", "cq_kv_append", "cq_kv_read", "cq_attention",
-            "cq_attention_workspace", "cq_last_error")))
+            "cq_attention_workspace", "cq_attention_tree", "cq_last_error")))
         self._step = mod and mod.StepCalls(*(_capi.entry_address(n) for n in (
             "cq_place", "cq_kv_append_rows", "cq_prompt_attention", "cq_last_error")))
 
@@ -504,25 +504,28 @@ class AttentionExt:
     def forward(self, q: torch.Tensor, cache: KVCache, block_table: torch.Tensor,
                 lengths: torch.Tensor, counts: Optional[torch.Tensor] = None, *,
                 prefix: Optional[tuple[torch.Tensor, int]] = None,
-                scale: Optional[float] = None) -> torch.Tensor:
+                scale: Optional[float] = None,
+                tree: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of q (batch, tokens, Hq, D), float16 or bfloat16, over the
         cache, into a new tensor of q's shape and type.  See forward_into."""
         if scale is not None:
             scale = _number("scale", scale)
-        got = self._fast_forward(q, cache, block_table, lengths, None, counts, prefix, scale)
+        got = self._fast_forward(q, cache, block_table, lengths, None, counts, prefix, scale,
+                                 tree)
         if got is not None:
             return got
         if not isinstance(q, torch.Tensor):
             _fail(f"q must be a tensor, got {type(q).__name__}")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        self._forward(q, cache, block_table, lengths, out, counts, prefix, scale)
+        self._forward(q, cache, block_table, lengths, out, counts, prefix, scale, tree)
         return out
 
     def forward_into(self, q: torch.Tensor, cache: KVCache, block_table: torch.Tensor,
                      lengths: torch.Tensor, out: torch.Tensor,
                      counts: Optional[torch.Tensor] = None, *,
                      prefix: Optional[tuple[torch.Tensor, int]] = None,
-                     scale: Optional[float] = None) -> None:
+                     scale: Optional[float] = None,
+                     tree: Optional[torch.Tensor] = None) -> None:
         """Attention into a given contiguous `out`.
 
         Sequence b holds lengths[b] tokens in the pages block_table[b]; the
@@ -532,7 +535,14 @@ class AttentionExt:
         (pages int32 (n,), length) names tokens that every query of every
         sequence sees before its own: they are read once for the whole batch,
         and `lengths` does not count them.  `scale` multiplies the scores
-        (default D ** -0.5).  Scores, statistics and sums are FP32, from q held
+        (default D ** -0.5).
+
+        `tree` int64 (batch, tokens, ceil(tokens / 64)) says which of the call's
+        tokens each of them sees, in the place of those up to itself: query t sees
+        token j if bit j % 64 of tree[b, t, j // 64] is set (a drafted token's own
+        bit and its ancestors'), and everything ahead of the call's tokens.
+
+        Scores, statistics and sums are FP32, from q held
         in FP16 times a power of two of its row; each probability times its V
         scale is rounded to FP16 before it multiplies V's codes, the result once
         to q's type.  A query that sees nothing, or lies past counts[b], gives
@@ -540,11 +550,11 @@ class AttentionExt:
         if scale is not None:
             scale = _number("scale", scale)
         if out is not None and self._fast_forward(q, cache, block_table, lengths, out, counts,
-                                                  prefix, scale) is not None:
+                                                  prefix, scale, tree) is not None:
             return
-        self._forward(q, cache, block_table, lengths, out, counts, prefix, scale)
+        self._forward(q, cache, block_table, lengths, out, counts, prefix, scale, tree)
 
-    def _fast_forward(self, q, cache, block_table, lengths, out, counts, prefix, scale):
+    def _fast_forward(self, q, cache, block_table, lengths, out, counts, prefix, scale, tree):
         if self._fast is None or not isinstance(cache, KVCache) or cache.fast is None:
             return None
         pages, n = None, 0
@@ -555,9 +565,9 @@ class AttentionExt:
         if scale is None:
             scale = cache.head_dim ** -0.5
         return self._fast.forward(cache.fast, q, block_table, lengths, counts, out, pages, n,
-                                  scale)
+                                  scale, tree)
 
-    def _forward(self, q, cache, block_table, lengths, out, counts, prefix, scale) -> None:
+    def _forward(self, q, cache, block_table, lengths, out, counts, prefix, scale, tree) -> None:
         if not isinstance(cache, KVCache):
             _fail(f"cache must be a KVCache, got {type(cache).__name__}")
         dev = cache.device
@@ -576,6 +586,13 @@ class AttentionExt:
         _ints("lengths", lengths, (batch,), dev)
         if counts is not None:
             _ints("counts", counts, (batch,), dev)
+        if tree is not None:
+            _gpu("tree", tree, dev)
+            shape = (batch, tokens, (tokens + 63) // 64)
+            if tree.dtype != torch.int64 or tuple(tree.shape) != shape \
+                    or not tree.is_contiguous():
+                _fail(f"tree must be contiguous int64 {shape}, got {tree.dtype} "
+                      f"{tuple(tree.shape)}")
         a = _capi.CqAttention()
         if prefix is not None:
             pages, n = _pair(prefix)
@@ -609,8 +626,12 @@ class AttentionExt:
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        _check(_on_device(dev, lambda s: self._lib.cq_attention(
-            ctypes.byref(cache.c), ctypes.byref(a), s)), "forward")
+        if tree is None:
+            _check(_on_device(dev, lambda s: self._lib.cq_attention(
+                ctypes.byref(cache.c), ctypes.byref(a), s)), "forward")
+        else:
+            _check(_on_device(dev, lambda s: self._lib.cq_attention_tree(
+                ctypes.byref(cache.c), ctypes.byref(a), tree.data_ptr(), s)), "forward")
 
 
 _ATTENTION: Optional[AttentionExt] = None

@@ -92,12 +92,13 @@ struct Cache {
 class Calls {
 public:
     Calls(uintptr_t norm_rope, uintptr_t append, uintptr_t read, uintptr_t attention,
-          uintptr_t workspace, uintptr_t last_error)
+          uintptr_t workspace, uintptr_t tree, uintptr_t last_error)
         : norm_rope_(reinterpret_cast<decltype(norm_rope_)>(norm_rope)),
           append_(reinterpret_cast<decltype(append_)>(append)),
           read_(reinterpret_cast<decltype(read_)>(read)),
           attention_(reinterpret_cast<decltype(attention_)>(attention)),
           workspace_(reinterpret_cast<decltype(workspace_)>(workspace)),
+          tree_(reinterpret_cast<decltype(tree_)>(tree)),
           last_error_(reinterpret_cast<decltype(last_error_)>(last_error)) {}
 
     // (q_out, k_out), or None; outputs None: new ones.
@@ -221,11 +222,12 @@ public:
     // out (a new one for None), or None.
     py::object forward(const Cache& c, py::handle q_, py::handle table_, py::handle lengths_,
                        py::handle counts_, py::handle out_, py::handle pages_,
-                       int64_t prefix_len, double scale) const {
+                       int64_t prefix_len, double scale, py::handle seen_) const {
         bool ok = true;
         const at::Tensor *q = tensor(q_, false, ok), *out = tensor(out_, true, ok);
         const at::Tensor *table = tensor(table_, false, ok), *len = tensor(lengths_, false, ok);
         const at::Tensor *counts = tensor(counts_, true, ok), *pages = tensor(pages_, true, ok);
+        const at::Tensor* seen = tensor(seen_, true, ok);
         if (!ok || q->dim() != 4 || q->device() != c.device || !on_current(*q) ||
             !last_contiguous(*q))
             return py::none();
@@ -237,6 +239,11 @@ public:
             return py::none();
         if (!table_ok(*table, batch, c.device) || !ints(*len, batch, c.device) ||
             (counts != nullptr && !ints(*counts, batch, c.device)))
+            return py::none();
+        if (seen != nullptr &&
+            (seen->scalar_type() != at::kLong || seen->dim() != 3 || seen->size(0) != batch ||
+             seen->size(1) != tokens || seen->size(2) != (tokens + 63) / 64 ||
+             !seen->is_contiguous() || seen->device() != c.device))
             return py::none();
         cq_attention_t a{};
         if (pages != nullptr) {
@@ -281,7 +288,11 @@ public:
             a.workspace = ws.data_ptr();
             a.workspace_bytes = need;
         }
-        if (!done(attention_(&c.c, &a, stream_of(*q)), "forward")) return py::none();
+        void* const stream = stream_of(*q);
+        const int status = seen == nullptr
+                               ? attention_(&c.c, &a, stream)
+                               : tree_(&c.c, &a, static_cast<const int64_t*>(seen->data_ptr()), stream);
+        if (!done(status, "forward")) return py::none();
         return py::cast(*out);
     }
 
@@ -324,6 +335,7 @@ private:
     int (*read_)(const cq_kv_cache_t*, const cq_kv_slots_t*, int, void*, void*, void*);
     int (*attention_)(const cq_kv_cache_t*, const cq_attention_t*, void*);
     int64_t (*workspace_)(const cq_kv_cache_t*, const cq_attention_t*);
+    int (*tree_)(const cq_kv_cache_t*, const cq_attention_t*, const int64_t*, void*);
     const char* (*last_error_)();
 };
 
@@ -331,7 +343,8 @@ void bind(py::module_& m) {
     py::class_<Cache>(m, "Cache")
         .def(py::init<py::handle, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>());
     py::class_<Calls>(m, "AttentionCalls")
-        .def(py::init<uintptr_t, uintptr_t, uintptr_t, uintptr_t, uintptr_t, uintptr_t>())
+        .def(py::init<uintptr_t, uintptr_t, uintptr_t, uintptr_t, uintptr_t, uintptr_t,
+                      uintptr_t>())
         .def("norm_rope", &Calls::norm_rope)
         .def("append", &Calls::append)
         .def("read", &Calls::read)

@@ -22,6 +22,15 @@ hipError_t launch_kv_append_rows(const cq_kv_cache_t& c, int dtype, int64_t toke
 // cq_prompt.hip
 hipError_t launch_prompt(const cq_prompt_t& a, hipStream_t stream);
 
+// cq_attention.hip: the prefix's part of a call, and the join of its parts
+hipError_t launch_attention_ahead(const cq_kv_cache_t& c, const cq_attention_t& a,
+                                  hipStream_t stream);
+hipError_t launch_attention_join(const cq_kv_cache_t& c, const cq_attention_t& a,
+                                 hipStream_t stream);
+// cq_attention_tree.hip
+hipError_t launch_attention_tree(const cq_kv_cache_t& c, const cq_attention_t& a,
+                                 const int64_t* seen, hipStream_t stream);
+
 // cq_qgemm.hip
 hipError_t launch_quantize_tokens(int dtype, const void* x, int64_t x_stride, int64_t tokens,
                                   int64_t k, int8_t* codes, float* scales, hipStream_t stream);

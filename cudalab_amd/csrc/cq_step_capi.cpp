@@ -173,6 +173,30 @@ int check_qgemm(const cq_qgemm_t& a, bool launching) {
 
 extern "C" {
 
+int cq_attention_tree(const cq_kv_cache_t* cache, const cq_attention_t* args,
+                      const int64_t* seen, void* stream) {
+    return guarded([&]() -> int {
+        if (cache == nullptr || args == nullptr || seen == nullptr)
+            return invalid("null pointer: cache, args or seen");
+        const int st = cq::check_attention(*cache, *args, true);
+        if (st != CQ_OK) return st;
+        if (!aligned(seen, 8)) return invalid("seen must be 8-byte aligned");
+        const cq_attention_t& a = *args;
+        const Span bits(seen, static_cast<U>(a.batch) * static_cast<U>(a.tokens) *
+                                  static_cast<U>((a.tokens + (int64_t)63) / 64) * 8);
+        const Span out(a.out, static_cast<U>(a.batch) * static_cast<U>(a.tokens) *
+                                  static_cast<U>(a.q_heads) *
+                                  static_cast<U>(cache->head_dim * elem_bytes(a.dtype)));
+        const int64_t need = cq::attention_workspace(*cache, a);
+        if (overlap(out, bits) ||
+            overlap(Span(need > 0 ? a.workspace : nullptr, static_cast<U>(need > 0 ? need : 0)), bits))
+            return invalid("out or the workspace overlaps an input");
+        return hip_status(cq::launch_attention_tree(*cache, a, seen,
+                                                    static_cast<hipStream_t>(stream)),
+                          "cq_attention_tree");
+    });
+}
+
 int cq_quantize_tokens(int dtype, const void* x, int64_t x_stride, int64_t tokens, int64_t k,
                        int8_t* codes, float* scales, void* stream) {
     return guarded([&]() -> int {

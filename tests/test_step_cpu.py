@@ -137,3 +137,24 @@ def test_prompt_refuses(change):
 
 def test_prompt_refuses_too_many_workgroups():
     assert _prompt(batch=2 ** 30, q_heads=65534) == BAD
+
+
+def test_tree_refuses():
+    a = _capi.CqAttention(
+        q=P[6], out=P[7], q_batch_stride=5120, q_token_stride=1024, q_head_stride=128,
+        table=P[3], lengths=P[4], counts=None, prefix_table=None, table_stride=5,
+        workspace=P[9], workspace_bytes=1 << 31, table_cols=5, prefix_cols=0, prefix_len=0,
+        batch=2, tokens=5, q_heads=8, dtype=0, softmax_scale=0.1)
+    c, lib = _cache(), _capi.load()
+
+    def call(seen=P[10], cache=c, args=a):
+        return lib.cq_attention_tree(cache and ctypes.byref(cache), args and ctypes.byref(args),
+                                     seen, None)
+
+    for bad in (dict(seen=None), dict(seen=P[10] + 4), dict(seen=P[7] + 64), dict(seen=P[9]),
+                dict(cache=None), dict(args=None), dict(cache=_cache(head_dim=96))):
+        assert call(**bad) == BAD, bad
+    a.q = P[6] + 8
+    assert call() == BAD
+    a.q, a.workspace_bytes = P[6], 16
+    assert call() == _capi.CQ_ERR_BUFFER_TOO_SMALL
