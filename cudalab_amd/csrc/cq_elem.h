@@ -53,13 +53,22 @@ __device__ __forceinline__ void scale_of(uint32_t amax_bits, float& scale, float
     }
 }
 
+// `bytes` from base on as a buffer: a load past them gives 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);
+}
+
 // 16 bytes a lane from base + at (0 where that passes `bytes`; both the wave's)
 // straight to LDS, lane after lane from `to` (the wave's, 16-byte aligned).
 __device__ __forceinline__ void load_to_lds(void* to, const void* base, int bytes, int at) {
-    const __amdgpu_buffer_rsrc_t from =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        from, (__attribute__((address_space(3))) void*)to, 16, at, 0, 0, 0);
+        buffer_of(base, bytes), (__attribute__((address_space(3))) void*)to, 16, at, 0, 0, 0);
+}
+
+// 16 bytes of a buffer, to registers.
+__device__ __forceinline__ Vec<int, 4> load16(__amdgpu_buffer_rsrc_t from, int at) {
+    using i4 = Vec<int, 4>;
+    return __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
 }
 
 // Page of a table entry, or -1 for one outside the cache.

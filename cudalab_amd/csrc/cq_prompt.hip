@@ -36,6 +36,7 @@
 // number of tiles that lie as deep or deeper.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cq_elem.h"
 #include "cq_step.h"
@@ -65,6 +66,7 @@ template <> struct Typed<__bf16> {
 };
 
 using u4 = Vec<uint32_t, 4>;
+using f4 = Vec<float, 4>;
 using f16v = Vec<float, 16>;
 using s2 = Vec<short, 2>;
 using s4 = Vec<short, 4>;
@@ -210,7 +212,6 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     const bool live = row0 < tile.rows;
     const int r = min(row0 + col, tile.rows - 1);      // rows past the last repeat it
     const int limit = limit_of(r);
-    const int full = limit_of(min(row0, tile.rows - 1));               // every row of the wave sees
     const int wave_reach = live ? limit_of(min(row0 + kRows, tile.rows) - 1) : 0;
 
     // the tiles of keys
@@ -264,43 +265,36 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     f16v o[kDims];
 #pragma unroll
     for (int i = 0; i < kDims; ++i) o[i] = f16v{};
-    float ref = 0.f, sum = 0.f, raise = kNegInf;       // ref: M
+    float ref = 0.f, raise = kNegInf;                  // ref: M
+    f4 sums = {0.f, 0.f, 0.f, 0.f};
 
-    const int tiles = (reach + kKeys - 1) / kKeys;
-    for (int t = 0; t < tiles; ++t) {
-        __syncthreads();                       // tile t has come, t - 1 is done with
-        if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
+    // A tile of keys.  MASKED: rows may see a part of it, or nothing.
+    auto advance = [&](int t, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
         const int key0 = t * kKeys;
-        if (key0 >= wave_reach) continue;
         const uint8_t* ks = sm + (t & 1) * 2 * kTileBytes;
         const uint8_t* vs = ks + kTileBytes;
-        const bool part = key0 + kKeys > full;         // some row does not see all
-        f16v x[2];
+        f16v x[2] = {f16v{}, f16v{}};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            x[i] = f16v{};
+        for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-            for (int u = 0; u < kSteps; ++u) {
+            for (int i = 0; i < 2; ++i) {
                 const int row = i * 32 + col;
                 const v8 k = *reinterpret_cast<const v8*>(
                     ks + row * kBytes + ((u * 2 + half) ^ k_turn(row)) * 16);
                 x[i] = Ty::mfma(k, q[u], x[i]);
             }
-        }
         // key of x[i][j]: key0 + 32 i + 8 (j / 4) + 4 half + j % 4
         const int mine = limit - key0 - 4 * half;
-        if (part) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    x[i][j] = 32 * i + 8 * (j / 4) + j % 4 < mine ? x[i][j] : kNegInf;
-        }
+        auto sees = [&](int i, int j) { return 32 * i + 8 * (j / 4) + j % 4 < mine; };
         float top = kNegInf;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) top = fmaxf(top, x[i][j]);
+            for (int j = 0; j < 16; ++j) {
+                if (MASKED && !sees(i, j)) x[i][j] = kNegInf;
+                top = fmaxf(top, x[i][j]);
+            }
         if (__any(__builtin_fmaf(top, by, -ref) > raise)) {
             top = half_fold(top, [](float m, float n) { return fmaxf(m, n); }) * by;
             const bool first = raise == kNegInf;
@@ -308,7 +302,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
                 const float keep = first ? 1.f : __builtin_amdgcn_exp2f(ref - top);
                 ref = top;
                 raise = kRaise;
-                sum *= keep;
+                sums *= keep;
 #pragma unroll
                 for (int i = 0; i < kDims; ++i) o[i] *= keep;
             }
@@ -319,9 +313,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], by, -ref));
-                if (part) e = 32 * i + 8 * (j / 4) + j % 4 < mine ? e : 0.f;
+                if (MASKED && !sees(i, j)) e = 0.f;
                 x[i][j] = e;
-                sum += e;
+                sums[j % 4] += e;
                 p[2 * i + j / 8][j % 8] = (T)e;
             }
         // V's part of step s and dim tile d: keys 16 s + 4 half + 0..3 and 8 more
@@ -339,7 +333,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
         // whether a masked key's V may spoil the sums
         bool spoilt = false;
         constexpr uint32_t kOver = (0x8000u - Ty::kInf) * 0x10001u;
-        if (part) {
+        if constexpr (MASKED) {
             uint32_t over = 0;
             for (int i = lane; i < kTileBytes / 16; i += 64) {
                 const u4 w = *reinterpret_cast<const u4*>(vs + i * 16);
@@ -348,27 +342,26 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
             }
             spoilt = __any((over & 0x80008000u) != 0);
         }
-        if (!spoilt) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int d = 0; d < kDims; ++d)
-                    o[d] = Ty::mfma(__builtin_bit_cast(v8, read_v(s, d)), p[s], o[d]);
-        } else {
+            for (int d = 0; d < kDims; ++d) {
+                u4 w = read_v(s, d);
+                if constexpr (MASKED) {
+                    if (spoilt) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int d = 0; d < kDims; ++d) {
-                    u4 w = read_v(s, d);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const s2 bad = __builtin_bit_cast(s2, (w[i] & 0x7FFF7FFFu) + kOver) >> 15;
-                        w[i] &= ~__builtin_bit_cast(uint32_t, bad);
+                        for (int i = 0; i < 4; ++i) {
+                            const s2 bad =
+                                __builtin_bit_cast(s2, (w[i] & 0x7FFF7FFFu) + kOver) >> 15;
+                            w[i] &= ~__builtin_bit_cast(uint32_t, bad);
+                        }
                     }
-                    o[d] = Ty::mfma(__builtin_bit_cast(v8, w), p[s], o[d]);
                 }
+                o[d] = Ty::mfma(__builtin_bit_cast(v8, w), p[s], o[d]);
+            }
+        if constexpr (MASKED) {
             // Inf and NaN, key by key
-            for (int key = 0; key < kKeys; ++key) {
+            for (int key = 0; spoilt && key < kKeys; ++key) {
                 float e = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -376,7 +369,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
                     for (int j = 0; j < 16; ++j)
                         e = 32 * i + 8 * (j / 4) + 4 * half + j % 4 == key ? x[i][j] : e;
                 e = half_fold(e, [](float m, float n) { return m + n; });
-                const bool sees = key < limit - key0;
+                const bool seen = key < limit - key0;
 #pragma unroll
                 for (int d = 0; d < kDims; ++d)
 #pragma unroll
@@ -388,14 +381,30 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
                         for (int i = 0; i < 4; ++i) {
                             const uint16_t bits = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
                             const float v = (float)__builtin_bit_cast(T, bits);
-                            if (sees && (bits & 0x7FFF) >= Ty::kInf) o[d][j + i] += e * v;
+                            if (seen && (bits & 0x7FFF) >= Ty::kInf) o[d][j + i] += e * v;
                         }
                     }
             }
         }
+    };
+    // tiles that every row of the workgroup sees all of, then the others
+    const int tiles = (reach + kKeys - 1) / kKeys, whole = limit_of(0) / kKeys;
+    auto next = [&](int t) {
+        __syncthreads();                       // tile t has come, t - 1 is done with
+        if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
+    };
+    int t = 0;
+    for (; t < whole; ++t) {
+        next(t);
+        advance(t, std::false_type{});
+    }
+    for (; t < tiles; ++t) {
+        next(t);
+        if (t * kKeys < wave_reach) advance(t, std::true_type{});
     }
     if (!live) return;
-    sum = half_fold(sum, [](float m, float n) { return m + n; });
+    const float sum = half_fold((sums[0] + sums[1]) + (sums[2] + sums[3]),
+                                [](float m, float n) { return m + n; });
     const float share = sum == 0.f ? 0.f : 1.f / sum;
     if (row0 + col < tile.rows) {
         T* to = out + (row0 + col) * out_row + 4 * half;

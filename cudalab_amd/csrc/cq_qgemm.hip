@@ -20,6 +20,7 @@ namespace {
 using i4 = Vec<int, 4>;
 using i16v = Vec<int, 16>;
 using u4 = Vec<uint32_t, 4>;
+using f4 = Vec<float, 4>;
 
 // -------------------------------------------------------------- activations
 constexpr int kBlock = 256;
@@ -30,12 +31,16 @@ __device__ __forceinline__ uint32_t magnitude(T x) {
     return __float_as_uint((float)x) & 0x7FFFFFFFu;
 }
 
+// How rows of x lie: elements by element, pieces of 16 bytes at 16 bytes, or at words
+// (a row a whole number of them).
+enum { kElements, kPieces, kWords };
+
 // One workgroup to a token; what it holds of the row (HOLD pieces of 8 elements a
 // thread) is read once, the rest again.  Codes need no clamp: x * inv lies within
 // 127 (1 + 2^-21).
 template <class T, int HOLD>
 __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t stride, int64_t k,
-                                                          int8_t* codes, float* scales, bool wide,
+                                                          int8_t* codes, float* scales, int form,
                                                           uint32_t first) {
     __shared__ uint32_t most[kBlock / 64];
     const int64_t row = (int64_t)first + blockIdx.x;
@@ -44,9 +49,21 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t st
     constexpr int N = 8;
     Vec<T, N> held[HOLD];
     uint32_t m = 0;
+    const auto words = buffer_of(p, form == kWords ? (int)(k * sizeof(T)) : 0);
     auto get = [&](int64_t at) {
         Vec<T, N> v = {};
-        if (wide && at + N <= k) {
+        if (form == kWords) {
+            // (at most 2^31 bytes; past the row zeros come)
+            if constexpr (sizeof(T) == 4) {
+                using V = Vec<T, 4>;
+                const V a = __builtin_bit_cast(V, load16(words, (int)(at * 4)));
+                const V b = __builtin_bit_cast(V, load16(words, (int)(at * 4) + 16));
+                v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+            } else {
+                using V = Vec<T, N>;
+                v = __builtin_bit_cast(V, load16(words, (int)(at * 2)));
+            }
+        } else if (form == kPieces && at + N <= k) {
             if constexpr (sizeof(T) == 4) {
                 const Vec<T, 4> a = *reinterpret_cast<const Vec<T, 4>*>(p + at);
                 const Vec<T, 4> b = *reinterpret_cast<const Vec<T, 4>*>(p + at + 4);
@@ -84,7 +101,7 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t st
     float scale, inv;
     scale_of<8>(m, scale, inv);
     if (threadIdx.x == 0) scales[row] = scale;
-    const bool whole = (reinterpret_cast<uintptr_t>(to) & 7) == 0;
+    const bool whole = (reinterpret_cast<uintptr_t>(to) & 3) == 0;
     auto put = [&](int64_t at, const Vec<T, N>& v) {
         if (at >= k) return;
         uint32_t w[2];
@@ -101,7 +118,8 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t st
             if (inv == 0.f) w[i] = 0;
         }
         if (whole && at + N <= k) {
-            *reinterpret_cast<Vec<uint32_t, 2>*>(to + at) = Vec<uint32_t, 2>{w[0], w[1]};
+            reinterpret_cast<uint32_t*>(to + at)[0] = w[0];
+            reinterpret_cast<uint32_t*>(to + at)[1] = w[1];
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -114,35 +132,53 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t st
 }
 
 // ------------------------------------------------------------------ products
-// 16 bytes of a row of codes from byte `at` on, where the row is not aligned to
-// words: the words around them that hold any, shifted.  `end` bytes belong to
-// the operand; what lies behind comes as 0.
-__device__ __forceinline__ u4 unaligned16(const int8_t* base, int64_t at, int64_t end) {
-    const uintptr_t p = reinterpret_cast<uintptr_t>(base) + at;
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(p & ~(uintptr_t)3);
-    const uint32_t shift = p & 3;
-    uint32_t w[5];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = at + 4 * i - (int64_t)shift < end ? words[i] : 0;
-    u4 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_alignbyte(w[i + 1], w[i], shift);
-    return r;
-}
+// A product whose rows start at words, with their distances.
+struct Product {
+    const int8_t* x;
+    const int8_t* w;
+    const float* x_scale;
+    const float* w_scale;
+    void* out;
+    int64_t tokens, n;
+    int32_t k, x_stride, w_stride;
+};
 
 // The bytes of 16 from `at` on that lie below k, the others 0.
-__device__ __forceinline__ u4 below(u4 v, int64_t at, int64_t k) {
+__device__ __forceinline__ u4 below(u4 v, int at, int k) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t left = k - at - 4 * i;
+        const int left = k - at - 4 * i;
         if (left < 4) v[i] &= left <= 0 ? 0u : (1u << (8 * left)) - 1;
     }
     return v;
 }
 
+// Rows that start at any byte, to rows of whole pieces of 16 (zeros behind their
+// ends).  A piece comes from the words around it that hold any of the row's bytes,
+// shifted: nothing else is read.  5003 rows of 4099: 13 us; a product with shifts
+// in its loads took 185 us of 777 tokens, this and the product of rows at words 60.
+__global__ __launch_bounds__(kBlock) void pack_kernel(const int8_t* from, int64_t stride,
+                                                      int64_t rows, int k, int8_t* to, int pieces,
+                                                      uint32_t first) {
+    const int64_t i = ((int64_t)first + blockIdx.x) * kBlock + threadIdx.x;
+    const int64_t row = i / pieces;
+    if (row >= rows) return;
+    const int at = (int)(i - row * pieces) * 16;
+    const uintptr_t p = reinterpret_cast<uintptr_t>(from) + row * stride + at;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(p & ~(uintptr_t)3);
+    const int shift = p & 3;
+    uint32_t w[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = at + 4 * j - shift < k ? words[j] : 0;
+    u4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __builtin_amdgcn_alignbyte(w[j + 1], w[j], shift);
+    *reinterpret_cast<u4*>(to + i * 16) = below(r, at, k);
+}
+
 template <class T, int N>
-__device__ __forceinline__ void store_scaled(T* p, const int* sums, float xs, const float* ws,
-                                             int n, bool whole) {
+__device__ __forceinline__ void store_scaled(T* p, const int* sums, float xs,
+                                             const Vec<float, N>& ws, int n, bool whole) {
     Vec<T, N> v;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -160,25 +196,28 @@ __device__ __forceinline__ void store_scaled(T* p, const int* sums, float xs, co
     }
 }
 
-constexpr int kDeep = 128;             // bytes of k of a tile
-
-// A workgroup computes BN channels of BM tokens; its WM x WN waves share tiles of
-// 128 codes of their rows, two in turn: the next comes from memory straight to
-// LDS while one is multiplied.  Pieces of 16 bytes lie at places turned by the
-// row, so that 16 rows' same piece meets every bank once.
-// WORDS: rows start at words and the loads need no shifting.
-template <class T, int BM, int BN, int WM, int WN, bool WORDS>
-__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(cq_qgemm_t a, uint32_t m_tiles,
-                                                            uint32_t n_tiles) {
-    constexpr int W = WM * WN;
+// A workgroup computes BN channels of BM tokens.  Its waves share tiles of BK codes
+// of their rows, STAGES in turn: the next come from memory straight to LDS while
+// one is multiplied.  WM x WN of them share the channels and tokens, and KS such
+// sets the codes of a tile; the sets' sums are added in LDS at the end.  Pieces of
+// 16 bytes lie at places turned by the row, so that 16 rows' same piece meets every
+// bank once.
+template <class T, int BM, int BN, int WM, int WN, int KS, int BK, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN * KS, WM * WN * KS * STAGES > 8 ? 1 : 2) void tile_kernel(
+    Product a, uint32_t m_tiles, uint32_t n_tiles) {
+    constexpr int W = WM * WN * KS;
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
-    constexpr int kTileBytes = (BM + BN) * kDeep;
-    constexpr int kXLoads = BM / 8 / W, kWLoads = BN / 8 / W;       // 8 rows each
-    static_assert(kXLoads * 8 * W == BM && kWLoads * 8 * W == BN, "whole loads");
-    __shared__ __attribute__((aligned(1024))) uint8_t sm[2 * kTileBytes];
+    constexpr int kTileBytes = (BM + BN) * BK;
+    constexpr int kRowPieces = BK / 16, kLoadRows = 64 / kRowPieces;      // rows of a wave's load
+    constexpr int kXLoads = BM / kLoadRows / W, kWLoads = BN / kLoadRows / W;
+    constexpr int kUnits = BK / 32 / KS;           // products over k of a wave and tile
+    static_assert(kXLoads * kLoadRows * W == BM && kWLoads * kLoadRows * W == BN, "whole loads");
+    constexpr int kSums = (KS - 1) * BM * BN * 4;
+    constexpr int kSpace = std::max(STAGES * kTileBytes, kSums);
+    __shared__ __attribute__((aligned(1024))) uint8_t sm[kSpace + (BM + BN) * 4];
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave % WM, wn = wave / WM;
+    const int wm = wave % WM, wn = wave / WM % WN, wk = wave / (WM * WN);
 
     // neighbours on an XCD take neighbouring tiles, four rows of tiles at a time
     const uint32_t all = m_tiles * n_tiles, xcd = blockIdx.x % 8, each = all / 8, over = all % 8;
@@ -189,65 +228,75 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(cq_qgemm_t a, uin
     const int64_t m0 = (int64_t)(first + in % high) * BM, n0 = (int64_t)(in / high) * BN;
 
     const int8_t* xp = a.x + m0 * a.x_stride;
-    const int8_t* wp = a.w + n0 * a.k;
-    const int64_t x_end = (std::min<int64_t>(a.tokens - m0, BM) - 1) * a.x_stride + a.k;
-    const int64_t w_end = std::min<int64_t>(a.n - n0, BN) * a.k;
-    auto turn = [](int row) { return row >> 1 & 7; };
-    const int piece = lane & 7;
-    auto row_of = [&](int i) { return (wave + W * i) * 8 + (lane >> 3); };
-    const int k = (int)a.k, steps = (k + kDeep - 1) / kDeep;
-    auto fetch = [&](int step, int buf) {
-        uint8_t* to = sm + buf * kTileBytes;
-        auto load = [&](uint8_t* dst, const int8_t* base, int64_t end, int64_t stride, int i) {
-            const int row = row_of(i), at = (piece ^ turn(row)) * 16;
-            if constexpr (WORDS) {
-                // past the row's end nothing is loaded: zeros come
-                const int64_t from = row * stride + step * kDeep + at;
-                const bool some = step * kDeep + at < k && row * stride < end;
-                load_to_lds(dst + (wave + W * i) * 1024, base, (int)end,
-                            some ? (int)from : 0x7FFFFFFF);
-            } else {
-                const int64_t from = row * stride + step * kDeep + at;
-                u4 v = {};
-                if (step * kDeep + at < k && row * stride < end)
-                    v = below(unaligned16(base, from, end), step * kDeep + at, k);
-                *reinterpret_cast<u4*>(dst + (wave + W * i) * 1024 + lane * 16) = v;
-            }
-        };
+    const int8_t* wp = a.w + n0 * a.w_stride;
+    const int k = a.k, steps = (k + BK - 1) / BK;
+    // (whole words: rows of a k that is none have been packed, with zeros behind)
+    const int row = (k + 3) & ~3;
+    const int x_end = ((int)std::min<int64_t>(a.tokens - m0, BM) - 1) * a.x_stride + row;
+    const int w_end = ((int)std::min<int64_t>(a.n - n0, BN) - 1) * a.w_stride + row;
+    // (a row's pieces, as many rows as fill the banks)
+    auto turn = [](int row) { return BK == 256 ? row & 15 : row / (256 / BK) & (kRowPieces - 1); };
+    const int piece = lane % kRowPieces;
+    auto row_of = [&](int i) { return (wave + W * i) * kLoadRows + lane / kRowPieces; };
+    // of a lane's loads: the place in the operand's rows (of rows that are not
+    // there it lies past the end, and zeros come), and in a row's tile
+    int x_at[kXLoads], w_at[kWLoads];
+    auto in_tile = [&](int i) { return (piece ^ turn(row_of(i))) * 16; };
 #pragma unroll
-        for (int i = 0; i < kXLoads; ++i) load(to, xp, x_end, a.x_stride, i);
+    for (int i = 0; i < kXLoads; ++i) x_at[i] = row_of(i) * a.x_stride + in_tile(i);
 #pragma unroll
-        for (int i = 0; i < kWLoads; ++i) load(to + BM * kDeep, wp, w_end, a.k, i);
+    for (int i = 0; i < kWLoads; ++i) w_at[i] = row_of(i) * a.w_stride + in_tile(i);
+    auto fetch = [&](int step) {
+        uint8_t* to = sm + step % STAGES * kTileBytes + wave * 1024;
+        const int from = step * BK;
+        const bool whole = from + BK <= k;
+        // nor is anything loaded past the row's end
+        auto place = [&](int at, int i) { return whole || from + in_tile(i) < k ? at + from : 0x7FFFFFFF; };
+#pragma unroll
+        for (int i = 0; i < kXLoads; ++i) load_to_lds(to + W * i * 1024, xp, x_end, place(x_at[i], i));
+#pragma unroll
+        for (int i = 0; i < kWLoads; ++i)
+            load_to_lds(to + BM * BK + W * i * 1024, wp, w_end, place(w_at[i], i));
     };
     i16v acc[TN][TM];
 #pragma unroll
     for (int n = 0; n < TN; ++n)
 #pragma unroll
         for (int m = 0; m < TM; ++m) acc[n][m] = i16v{};
-    fetch(0, 0);
-    for (int step = 0; step < steps; ++step) {
-        __syncthreads();
-        uint8_t* buf = sm + (step & 1) * kTileBytes;
-        if (WORDS && step == steps - 1 && k % 16 != 0) {
-            // a last piece that is a row's in part: the rest of x is made 0
-            if ((int)threadIdx.x < BM) {
-                const int row = threadIdx.x, p = k % kDeep / 16;
-                u4* at = reinterpret_cast<u4*>(buf + row * kDeep + (p ^ turn(row)) * 16);
-                *at = below(*at, p * 16, k % kDeep);
-            }
-            __syncthreads();
-        }
-        if (step + 1 < steps) fetch(step + 1, (step + 1) & 1);
-        const uint8_t* xs = buf + (wm * TM * 32 + col) * kDeep;
-        const uint8_t* ws = buf + BM * kDeep + (wn * TN * 32 + col) * kDeep;
+    // the scales, for the end
+    float* const sm_x = reinterpret_cast<float*>(sm + kSpace);
+    float* const sm_w = sm_x + BM;
+    for (int i = threadIdx.x; i < BM; i += 64 * W)
+        sm_x[i] = m0 + i < a.tokens ? a.x_scale[m0 + i] : 0.f;
+    for (int i = threadIdx.x; i < BN; i += 64 * W)
+        sm_w[i] = n0 + i < a.n ? a.w_scale[n0 + i] : 0.f;
 #pragma unroll
-        for (int u = 0; u < kDeep / 32; ++u) {
-            const int at = ((2 * u + half) ^ turn(col)) * 16;
+    for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+    for (int step = 0; step < steps; ++step) {
+        // the wave's loads of this step have come (those of the STAGES - 2 behind
+        // it may be on their way), then everybody's
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 2) * (kXLoads + kWLoads))
+                     : "memory");
+        const uint8_t* buf = sm + step % STAGES * kTileBytes;
+        fetch(step + STAGES - 1);        // (zeros behind the last step: the count of loads stays)
+        const uint8_t* xs = buf + (wm * TM * 32 + col) * BK;
+        const uint8_t* ws = buf + BM * BK + (wn * TN * 32 + col) * BK;
+        const bool cut = step == steps - 1 && k % 16 != 0;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const int p = 2 * (wk * kUnits + u) + half, at = (p ^ turn(col)) * 16;
             i4 x[TM], w[TN];
 #pragma unroll
-            for (int m = 0; m < TM; ++m) x[m] = *reinterpret_cast<const i4*>(xs + m * 32 * kDeep + at);
+            for (int m = 0; m < TM; ++m) x[m] = *reinterpret_cast<const i4*>(xs + m * 32 * BK + at);
 #pragma unroll
-            for (int n = 0; n < TN; ++n) w[n] = *reinterpret_cast<const i4*>(ws + n * 32 * kDeep + at);
+            for (int n = 0; n < TN; ++n) w[n] = *reinterpret_cast<const i4*>(ws + n * 32 * BK + at);
+            if (cut) {
+                // a last piece that is a row's in part: the rest of x counts as 0
+#pragma unroll
+                for (int m = 0; m < TM; ++m)
+                    x[m] = __builtin_bit_cast(
+                        i4, below(__builtin_bit_cast(u4, x[m]), step * BK + p * 16, k));
+            }
 #pragma unroll
             for (int n = 0; n < TN; ++n)
 #pragma unroll
@@ -255,65 +304,121 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(cq_qgemm_t a, uin
                     acc[n][m] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[n], x[m], acc[n][m], 0, 0, 0);
         }
     }
+    if constexpr (KS > 1) {
+        // (loads past the last step have come too: nothing but the sums is written)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        int* sums = reinterpret_cast<int*>(sm) + (wn * WM + wm) * TN * TM * 1024 + lane * 4;
+        constexpr int kSet = BM * BN;
+        if (wk > 0) {
+#pragma unroll
+            for (int n = 0; n < TN; ++n)
+#pragma unroll
+                for (int m = 0; m < TM; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<i4*>(sums + (wk - 1) * kSet + ((n * TM + m) * 4 + j) * 256) =
+                            i4{acc[n][m][4 * j], acc[n][m][4 * j + 1], acc[n][m][4 * j + 2],
+                               acc[n][m][4 * j + 3]};
+        }
+        __syncthreads();
+        if (wk > 0) return;
+#pragma unroll
+        for (int set = 0; set < KS - 1; ++set)
+#pragma unroll
+            for (int n = 0; n < TN; ++n)
+#pragma unroll
+                for (int m = 0; m < TM; ++m)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const i4 v = *reinterpret_cast<const i4*>(
+                            sums + set * kSet + ((n * TM + m) * 4 + j) * 256);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[n][m][4 * j + i] += v[i];
+                    }
+    }
     // acc[n][m][j]: token 32 m + col, channel 32 n + 8 (j / 4) + 4 half + j % 4
     T* out = static_cast<T*>(a.out);
     const bool even = a.n % 4 == 0;
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
-        const int64_t t = m0 + (wm * TM + m) * 32 + col;
-        if (t >= a.tokens) continue;
-        const float xscale = a.x_scale[t];
+        const int row = (wm * TM + m) * 32 + col;
+        if (m0 + row >= a.tokens) continue;
+        const float xscale = sm_x[row];
+        T* to = out + (m0 + row) * a.n + n0;
 #pragma unroll
         for (int n = 0; n < TN; ++n)
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
-                const int64_t c = n0 + (wn * TN + n) * 32 + 2 * j + 4 * half;
-                if (c >= a.n) continue;
-                const int left = (int)std::min<int64_t>(4, a.n - c);
-                float wscale[4];
+                const int c = (wn * TN + n) * 32 + 2 * j + 4 * half;
+                const int64_t left = a.n - n0 - c;
+                if (left <= 0) continue;
                 int sums[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    wscale[i] = a.w_scale[c + std::min(i, left - 1)];
-                    sums[i] = acc[n][m][j + i];
-                }
-                store_scaled<T, 4>(out + t * a.n + c, sums, xscale, wscale, left, even);
+                for (int i = 0; i < 4; ++i) sums[i] = acc[n][m][j + i];
+                store_scaled<T, 4>(to + c, sums, xscale, *reinterpret_cast<const f4*>(sm_w + c),
+                                   (int)std::min<int64_t>(4, left), even);
             }
     }
 }
 
 // ------------------------------------------------------------------- host
-template <class T, int BM, int BN, int WM, int WN>
-hipError_t launch_tiles(const cq_qgemm_t& a, hipStream_t stream) {
+template <class T, int BM, int BN, int WM, int WN, int KS, int BK, int STAGES>
+hipError_t launch_tiles(const Product& a, hipStream_t stream) {
     const int64_t m = (a.tokens + BM - 1) / BM, n = (a.n + BN - 1) / BN;
-    if ((__int128)m * n > kMaxLaunch / 4) return hipErrorInvalidValue;
-    const bool words = a.k % 4 == 0 && a.x_stride % 4 == 0 && (uintptr_t)a.x % 4 == 0 &&
-                       (uintptr_t)a.w % 4 == 0;
-    const dim3 grid((unsigned)(m * n)), block(64 * WM * WN);
-    // offsets inside a tile of rows fit 31 bits
-    if (words && a.x_stride <= (1 << 22))
-        tile_kernel<T, BM, BN, WM, WN, true><<<grid, block, 0, stream>>>(a, (uint32_t)m, (uint32_t)n);
-    else
-        tile_kernel<T, BM, BN, WM, WN, false><<<grid, block, 0, stream>>>(a, (uint32_t)m, (uint32_t)n);
+    constexpr int kThreads = 64 * WM * WN * KS;
+    if ((__int128)m * n > kMaxLaunch * 256 / kThreads) return hipErrorInvalidValue;
+    tile_kernel<T, BM, BN, WM, WN, KS, BK, STAGES>
+        <<<dim3((unsigned)(m * n)), dim3(kThreads), 0, stream>>>(a, (uint32_t)m, (uint32_t)n);
     return hipGetLastError();
 }
 
+// Which tile.  Small ones leave more workgroups, large ones read less: the
+// smallest that does not give the 256 CUs more than one workgroup each.  (us, the
+// tiles in the order below, fp16 out, weights from memory:
+//   35 tokens, 8192 x 8192:    16.8   22.0   26     35     55    94
+//   256 tokens, 4096 x 4096:   15.8   12.3   15.6   19.7   23    53
+//   256 tokens, 8192 x 8192:   62     46     31.9   40     58   105
+//   512 tokens, 8192 x 8192:  121     85     62     43     59   106)
+// Where that is too many, two workgroups of 128 x 128 to a CU, or one of 256 x 256:
+// per 128 codes a CU's pair takes 1.34 us (a workgroup alone 0.8), the large one
+// 2.07 us, in as many rounds as they need.  (2048 tokens, 4096 x 4096: 42.8, 63; 4096
+// tokens, 28672 x 8192: 1022, 936.)
 template <class T>
-hipError_t launch_typed(const cq_qgemm_t& a, hipStream_t stream) {
-    const int64_t large = ((a.tokens + 255) / 256) * ((a.n + 255) / 256);
-    if (a.tokens > 128 && large >= 192) return launch_tiles<T, 256, 256, 2, 4>(a, stream);
-    return launch_tiles<T, 128, 128, 2, 2>(a, stream);
+hipError_t launch_typed(const Product& a, hipStream_t stream) {
+    auto tiles = [&](int64_t m, int64_t n) {
+        return ((a.tokens + m - 1) / m) * ((a.n + n - 1) / n);
+    };
+    constexpr int kCus = 256;
+    // (few tokens are bound by memory: two workgroups to a CU do no harm)
+    if (a.tokens <= 64 && tiles(64, 32) <= 2 * kCus)
+        return launch_tiles<T, 64, 32, 1, 1, 4, 256, 4>(a, stream);
+    if (tiles(64, 64) <= kCus) return launch_tiles<T, 64, 64, 1, 1, 4, 256, 3>(a, stream);
+    if (tiles(128, 64) <= kCus) return launch_tiles<T, 128, 64, 2, 1, 4, 256, 3>(a, stream);
+    const int64_t middle = tiles(128, 128), large = tiles(256, 256);
+    if (middle <= kCus) return launch_tiles<T, 128, 128, 2, 2, 2, 128, 3>(a, stream);
+    const int64_t over = middle % (2 * kCus);
+    const double pairs = 1.34 * (double)(middle / (2 * kCus)) +
+                         (over == 0 ? 0. : over <= kCus ? 0.8 : 1.34);
+    if (2.07 * (double)((large + kCus - 1) / kCus) < pairs)
+        return launch_tiles<T, 256, 256, 2, 4, 1, 64, 3>(a, stream);
+    return launch_tiles<T, 128, 128, 2, 2, 1, 128, 2>(a, stream);
 }
 
 template <class T>
 hipError_t quantize_typed(const void* x, int64_t stride, int64_t tokens, int64_t k, int8_t* codes,
                           float* scales, hipStream_t stream) {
     const T* p = static_cast<const T*>(x);
-    const bool wide = (uintptr_t)x % 16 == 0 && stride % (16 / sizeof(T)) == 0;
+    const int64_t es = sizeof(T);
+    const int form = (uintptr_t)x % 16 == 0 && stride * es % 16 == 0 ? kPieces
+                     : (uintptr_t)x % 4 == 0 && stride * es % 4 == 0 && k * es % 4 == 0 &&
+                             k < (1 << 28)
+                         ? kWords
+                         : kElements;
     return launch_parts(tokens, [&](dim3 blocks, uint32_t first) {
         auto go = [&](auto hold) {
             quantize_kernel<T, decltype(hold)::value>
-                <<<blocks, dim3(kBlock), 0, stream>>>(p, stride, k, codes, scales, wide, first);
+                <<<blocks, dim3(kBlock), 0, stream>>>(p, stride, k, codes, scales, form, first);
         };
         if (k <= 2 * kBlock * 8) go(std::integral_constant<int, 2>{});
         else if (k <= 4 * kBlock * 8) go(std::integral_constant<int, 4>{});
@@ -332,12 +437,55 @@ hipError_t launch_quantize_tokens(int dtype, const void* x, int64_t x_stride, in
     return quantize_typed<float>(x, x_stride, tokens, k, codes, scales, stream);
 }
 
-int64_t qgemm_workspace(const cq_qgemm_t&) { return 0; }
+namespace {
+// Which operands need their rows moved to words (or nearer: a tile's offsets fit 31
+// bits), and the bytes that takes.
+struct Packing {
+    bool x, w;
+    int64_t row, x_bytes, w_bytes;
+    explicit Packing(const cq_qgemm_t& a)
+        : x(a.k % 4 != 0 || a.x_stride % 4 != 0 || (uintptr_t)a.x % 4 != 0 ||
+            a.x_stride > (1 << 22)),
+          w(a.k % 4 != 0 || (uintptr_t)a.w % 4 != 0), row((a.k + 15) / 16 * 16),
+          x_bytes(x ? a.tokens * row : 0), w_bytes(w ? a.n * row : 0) {}
+};
+
+hipError_t pack(const int8_t* from, int64_t stride, int64_t rows, int64_t k, int8_t* to,
+                int64_t row, hipStream_t stream) {
+    const int64_t grid = (rows * (row / 16) + kBlock - 1) / kBlock;
+    if (grid > kMaxGrid) return hipErrorInvalidValue;
+    return launch_parts(grid, [&](dim3 blocks, uint32_t first) {
+        pack_kernel<<<blocks, dim3(kBlock), 0, stream>>>(from, stride, rows, (int)k, to,
+                                                         (int)(row / 16), first);
+    });
+}
+}  // namespace
+
+int64_t qgemm_workspace(const cq_qgemm_t& a) {
+    const Packing p(a);
+    return p.x_bytes + p.w_bytes;
+}
 
 hipError_t launch_qgemm(const cq_qgemm_t& a, hipStream_t stream) {
-    if (a.dtype == CQ_DTYPE_F16) return launch_typed<_Float16>(a, stream);
-    if (a.dtype == CQ_DTYPE_BF16) return launch_typed<__bf16>(a, stream);
-    return launch_typed<float>(a, stream);
+    const Packing p(a);
+    Product s{a.x, a.w, a.x_scale, a.w_scale, a.out, a.tokens, a.n, (int32_t)a.k,
+              (int32_t)a.x_stride, (int32_t)a.k};
+    int8_t* space = static_cast<int8_t*>(a.workspace);
+    hipError_t e = hipSuccess;
+    if (p.x) {
+        e = pack(a.x, a.x_stride, a.tokens, a.k, space, p.row, stream);
+        s.x = space;
+        s.x_stride = (int32_t)p.row;
+    }
+    if (p.w && e == hipSuccess) {
+        e = pack(a.w, a.k, a.n, a.k, space + p.x_bytes, p.row, stream);
+        s.w = space + p.x_bytes;
+        s.w_stride = (int32_t)p.row;
+    }
+    if (e != hipSuccess) return e;
+    if (a.dtype == CQ_DTYPE_F16) return launch_typed<_Float16>(s, stream);
+    if (a.dtype == CQ_DTYPE_BF16) return launch_typed<__bf16>(s, stream);
+    return launch_typed<float>(s, stream);
 }
 
 }  // namespace cq

@@ -678,7 +678,9 @@ typedef struct cq_qgemm {
     int32_t dtype;             /* CQ_DTYPE_F16, _F32 or _BF16 */
 } cq_qgemm_t;
 int cq_qgemm(const cq_qgemm_t* args, void* stream);
-/* Bytes of workspace that the call needs (0 or more), or a negative CQ_* status. */
+/* Bytes of workspace that the call needs, or a negative CQ_* status: 0 where rows
+ * start at words (k, x_stride, x and w divisible by 4, x_stride at most 2^22), else
+ * room for the rows that do not, moved to such places first. */
 int64_t cq_qgemm_workspace(const cq_qgemm_t* args);
 
 /*
