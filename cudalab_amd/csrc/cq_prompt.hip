@@ -31,9 +31,9 @@
 // that see them.
 //
 // Rows and keys lie wherever the offsets on the device say, so every workgroup
-// finds its tile of rows by itself: tiles in the order of their depth in their
-// sequence, the deepest first (they see the most keys), by bisection over the
-// number of tiles that lie as deep or deeper.
+// finds its tile of rows by itself: the longest sequence's tiles first, from its
+// last to its first, by bisection over the number of tiles of longer sequences.
+// Tiles that see the same keys then run side by side, and short ones end the call.
 
 #include <algorithm>
 #include <type_traits>
@@ -105,7 +105,9 @@ struct Span {
 };
 
 // The `index`th tile of `rows` rows: its sequence and place there (or, behind
-// the sequences' tiles, rows that belong to none: sequence -1).
+// the sequences' tiles, rows that belong to none: sequence -1).  Sequences come in
+// the order of their tiles, the most first, each with its last tile (which sees the
+// most keys) first.
 struct Tile {
     int b, row0, rows, first;          // b = -2: none
     __device__ __forceinline__ Tile(const cq_prompt_t& a, int tile_rows, int index, int lane) {
@@ -115,13 +117,16 @@ struct Tile {
         };
         const int near = tiles_at(lane);
         auto tiles = [&](int base) { return base == 0 ? near : tiles_at(base + lane); };
-        // tiles at depth `level` and below
-        auto from = [&](int level) {
+        // tiles of the sequences that have more than `least`
+        auto above = [&](int least) {
             int n = 0;
-            for (int base = 0; base < a.batch; base += 64) n += wave_sum(max(0, tiles(base) - level));
+            for (int base = 0; base < a.batch; base += 64) {
+                const int some = tiles(base);
+                n += wave_sum(some > least ? some : 0);
+            }
             return n;
         };
-        const int all = from(0);
+        const int all = above(0);
         b = -2;
         if (index >= all) {
             // rows ahead of the first sequence, then those behind the last
@@ -137,21 +142,22 @@ struct Tile {
             if (rows > 0) b = -1;
             return;
         }
-        // the level with from(level + 1) <= index < from(level)
-        int level = 0, end = ((int)a.q_tokens + tile_rows - 1) / tile_rows, deeper = 0;
-        while (end - level > 1) {
-            const int mid = level + (end - level) / 2;
-            const int n = from(mid);
+        // the size with above(size) <= index < above(size - 1)
+        int low = 0, size = ((int)a.q_tokens + tile_rows - 1) / tile_rows, before = 0;
+        while (size - low > 1) {
+            const int mid = low + (size - low) / 2;
+            const int n = above(mid);
             if (n > index) {
-                level = mid;
+                low = mid;
             } else {
-                end = mid;
-                deeper = n;
+                size = mid;
+                before = n;
             }
         }
-        int rank = index - deeper;     // among the sequences that go so deep
+        int rank = (index - before) / size;            // among the sequences of that size
+        const int level = size - 1 - (index - before) % size;
         for (int base = 0; base < a.batch; base += 64) {
-            uint64_t some = __ballot(tiles(base) > level);
+            uint64_t some = __ballot(tiles(base) == size);
             const int n = __builtin_popcountll(some);
             if (rank < n) {
                 for (; rank > 0; --rank) some &= some - 1;
@@ -212,6 +218,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     const bool live = row0 < tile.rows;
     const int r = min(row0 + col, tile.rows - 1);      // rows past the last repeat it
     const int limit = limit_of(r);
+    const int full = limit_of(min(row0, tile.rows - 1));       // every row of the wave sees
     const int wave_reach = live ? limit_of(min(row0 + kRows, tile.rows) - 1) : 0;
 
     // the tiles of keys
@@ -246,7 +253,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     };
     fetch(0, 0);
 
-    // the queries; a negative scale goes into their signs
+    // the queries; a negative scale goes into their signs, one of 0 into them whole
     v8 q[kSteps];
     {
         const T* p = static_cast<const T*>(a.q) +
@@ -259,15 +266,18 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] ^= turn;
             q[u] = __builtin_bit_cast(v8, w);
+            if (a.softmax_scale == 0.f) q[u] *= (T)0.f;
         }
     }
-    const float by = fabsf(a.softmax_scale) * 1.4426950408889634f;
+    const float by =
+        a.softmax_scale == 0.f ? 1.f : fabsf(a.softmax_scale) * 1.4426950408889634f;
     f16v o[kDims];
 #pragma unroll
     for (int i = 0; i < kDims; ++i) o[i] = f16v{};
     float ref = 0.f, raise = kNegInf;                  // ref: M
     f4 sums = {0.f, 0.f, 0.f, 0.f};
 
+    constexpr uint32_t kOver = (0x8000u - Ty::kInf) * 0x10001u;
     // A tile of keys.  MASKED: rows may see a part of it, or nothing.
     auto advance = [&](int t, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
@@ -312,8 +322,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], by, -ref));
-                if (MASKED && !sees(i, j)) e = 0.f;
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], by, -ref));
                 x[i][j] = e;
                 sums[j % 4] += e;
                 p[2 * i + j / 8][j % 8] = (T)e;
@@ -332,7 +341,6 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
         };
         // whether a masked key's V may spoil the sums
         bool spoilt = false;
-        constexpr uint32_t kOver = (0x8000u - Ty::kInf) * 0x10001u;
         if constexpr (MASKED) {
             uint32_t over = 0;
             for (int i = lane; i < kTileBytes / 16; i += 64) {
@@ -400,7 +408,11 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     }
     for (; t < tiles; ++t) {
         next(t);
-        if (t * kKeys < wave_reach) advance(t, std::true_type{});
+        // (heads of 256 have no registers for a third form)
+        if (D < 256 && t * kKeys + kKeys <= full)
+            advance(t, std::false_type{});
+        else if (t * kKeys < wave_reach)
+            advance(t, std::true_type{});
     }
     if (!live) return;
     const float sum = half_fold((sums[0] + sums[1]) + (sums[2] + sums[3]),
@@ -434,15 +446,14 @@ hipError_t launch_shaped(const Args& s, hipStream_t stream) {
     }, 64 * W);
 }
 
+// Four waves of 32 rows: two workgroups of 128 rows on a CU wait for their tiles and
+// barriers apart.  (Eight waves read half as many tiles, and lose at the diagonal,
+// where rows see half a tile; us, 4 and 8 waves: one sequence of 8192 tokens, 64/8
+// heads of 128, causal 1090 1113, all keys 1949 1925; 16 of up to 2048, 64/8: 518 598.)
 template <class T>
 hipError_t launch_typed(const Args& s, hipStream_t stream) {
-    const cq_prompt_t& a = s.a;
-    const int64_t rows = a.q_tokens / a.batch;
-    const bool eight = rows >= 512 && a.q_tokens / 256 * a.q_heads >= 512;
-    if (a.head_dim == 64)
-        return eight ? launch_shaped<T, 64, 8>(s, stream) : launch_shaped<T, 64, 4>(s, stream);
-    if (a.head_dim == 128)
-        return eight ? launch_shaped<T, 128, 8>(s, stream) : launch_shaped<T, 128, 4>(s, stream);
+    if (s.a.head_dim == 64) return launch_shaped<T, 64, 4>(s, stream);
+    if (s.a.head_dim == 128) return launch_shaped<T, 128, 4>(s, stream);
     return launch_shaped<T, 256, 4>(s, stream);
 }
 
