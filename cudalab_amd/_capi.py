@@ -230,6 +230,8 @@ SIGNATURES = {
     "cq_qgemm_workspace": (_i64, [ctypes.POINTER(CqQgemm)]),
     "cq_attention_tree": (ctypes.c_int, [ctypes.POINTER(CqKvCache),
                                          ctypes.POINTER(CqAttention), _vp, _vp]),
+    "cq_attention_tree_workspace": (_i64, [ctypes.POINTER(CqKvCache),
+                                           ctypes.POINTER(CqAttention)]),
     "cq_last_error": (ctypes.c_char_p, []),
     "cq_version": (ctypes.c_char_p, []),
 }

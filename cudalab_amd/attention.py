@@ -128,7 +128,8 @@ class AttentionExt:
         mod = fast_module_or_none()
         self._fast = mod and mod.AttentionCalls(*(_capi.entry_address(n) for n in (
             "cq_qk_norm_rope", "cq_kv_append", "cq_kv_read", "cq_attention",
-            "cq_attention_workspace", "cq_attention_tree", "cq_last_error")))
+            "cq_attention_workspace", "cq_attention_tree", "cq_attention_tree_workspace",
+            "cq_last_error")))
         self._step = mod and mod.StepCalls(*(_capi.entry_address(n) for n in (
             "cq_place", "cq_kv_append_rows", "cq_prompt_attention", "cq_last_error")))
 
@@ -619,7 +620,9 @@ class AttentionExt:
         a.table_stride, a.table_cols = block_table.stride(0), block_table.size(1)
         a.batch, a.tokens, a.q_heads, a.dtype = batch, tokens, hq, _DTYPES[q.dtype]
         a.softmax_scale = D ** -0.5 if scale is None else scale
-        need = self._lib.cq_attention_workspace(ctypes.byref(cache.c), ctypes.byref(a))
+        sizes = (self._lib.cq_attention_workspace if tree is None
+                 else self._lib.cq_attention_tree_workspace)
+        need = sizes(ctypes.byref(cache.c), ctypes.byref(a))
         if need < 0:
             _check(-need, "forward")
         ws = None

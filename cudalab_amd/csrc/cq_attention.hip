@@ -34,36 +34,54 @@ hipError_t join(const Source& own, Shape os, const Source& ahead, hipStream_t st
     });
 }
 
-}  // namespace
-
-int64_t attention_workspace(const cq_kv_cache_t& c, const cq_attention_t& a) {
+// Bytes that a call's sources take, or -1 where their tables are too long.
+int64_t workspace_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool tree) {
     Shape os{}, as{};
-    Source own = source_of(c, a, false, &os), ahead{};
+    Source own = source_of(c, a, false, &os, tree), ahead{};
     if (a.prefix_len > 0) ahead = source_of(c, a, true, &as);
     if (!own.fits || (ahead.rows > 0 && !ahead.fits)) return -1;
     return lay_out(c, a, &own, &ahead, nullptr);
 }
 
+}  // namespace
+
+int64_t attention_workspace(const cq_kv_cache_t& c, const cq_attention_t& a) {
+    return workspace_of(c, a, false);
+}
+
+int64_t attention_tree_workspace(const cq_kv_cache_t& c, const cq_attention_t& a) {
+    return workspace_of(c, a, true);
+}
+
 hipError_t launch_attention_ahead(const cq_kv_cache_t& c, const cq_attention_t& a,
                                   hipStream_t stream) {
     if (a.prefix_len == 0) return hipSuccess;
-    const Sources s(c, a);
+    const Sources s(c, a, true);
     return by_head(c, a, [&](auto elem, auto dim) {
         return launch_source<decltype(elem), decltype(dim)::value, false>(s.ahead, s.as, stream);
     });
 }
 
-hipError_t launch_attention_join(const cq_kv_cache_t& c, const cq_attention_t& a,
-                                 hipStream_t stream) {
-    const Sources s(c, a);
+// A tree's rows are many, and most of their units lie in two runs or three: a wave to
+// a row, four triples in flight (49152 rows, us: eight rows to a wave and 16 in flight
+// as `join` has it for other calls 50, this 28).
+hipError_t launch_attention_tree_join(const cq_kv_cache_t& c, const cq_attention_t& a,
+                                      hipStream_t stream) {
+    const Sources s(c, a, true);
     return by_head(c, a, [&](auto elem, auto dim) {
-        return join<decltype(elem), decltype(dim)::value>(s.own, s.os, s.ahead, stream);
+        using T = decltype(elem);
+        constexpr int D = decltype(dim)::value;
+        const int64_t rows = (int64_t)s.own.rows * a.batch * c.heads;
+        if (rows < 4 * kWaves * kCus) return join<T, D>(s.own, s.os, s.ahead, stream);
+        return launch_parts((rows + kWaves - 1) / kWaves, [&](dim3 blocks, uint32_t first) {
+            join_kernel<T, D, 1, 4><<<blocks, dim3(kBlock), 0, stream>>>(s.own, s.ahead, 1, first);
+        });
     });
 }
 
 hipError_t launch_attention(const cq_kv_cache_t& c, const cq_attention_t& a,
                             hipStream_t stream) {
-    const Sources s(c, a);
+    const Sources s(c, a, false);
     return by_head(c, a, [&](auto elem, auto dim) {
         using T = decltype(elem);
         constexpr int D = decltype(dim)::value;

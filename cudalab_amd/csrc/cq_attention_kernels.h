@@ -1157,10 +1157,10 @@ __global__ __launch_bounds__(64 * W, W == 8 || D == 256 ? 1 : 2) void block_kern
 // that a run has finished are left alone; rows without any keys become zeros.
 template <int D>
 constexpr int in_flight = D == 256 ? 8 : 16;       // triples
-template <class T, int D, int W>
+template <class T, int D, int W, int J = in_flight<D>>
 __global__ __launch_bounds__(kBlock) void join_kernel(Source own, Source ahead, int each,
                                                       uint32_t first_block) {
-    constexpr int E = D / 64, J = in_flight<D>;
+    constexpr int E = D / 64;
     using VE = Vec<float, E>;
     __shared__ float part[W > 1 ? W : 1][W > 1 ? D + 2 : 1];
     const int lane = threadIdx.x & 63;
@@ -1306,7 +1306,16 @@ Shape shape_of(int64_t rows, int64_t units, int64_t keys, int d) {
     return {0, 8, 256, 1};
 }
 
-Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, Shape* shape) {
+// A tree's tokens are many rows of one sequence: where units of 256 rows would leave
+// half of the last one empty, units of 128 (16 sequences of up to 8000 keys, 48 tokens,
+// 64/8 heads of 128, INT8: 384 rows, us: 230 and 190).
+Shape tree_shape_of(int64_t rows, int64_t units, int64_t keys, int d) {
+    const Shape s = shape_of(rows, units, keys, d);
+    return s.waves == 8 && (rows + 127) / 128 % 2 != 0 ? Shape{0, 4, 128, 2} : s;
+}
+
+Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, Shape* shape,
+                 bool tree = false) {
     Source s{};
     s.c = c;
     s.a = a;
@@ -1316,7 +1325,8 @@ Source source_of(const cq_kv_cache_t& c, const cq_attention_t& a, bool prefix, S
     const int64_t rows = (int64_t)a.tokens * s.group * (prefix ? a.batch : 1);
     s.rows = (int32_t)rows;
     const int64_t keys = prefix ? a.prefix_len : (int64_t)a.table_cols * c.page_size;
-    *shape = shape_of(rows, (int64_t)c.heads * (prefix ? 1 : a.batch), keys, c.head_dim);
+    *shape = (tree ? tree_shape_of : shape_of)(rows, (int64_t)c.heads * (prefix ? 1 : a.batch),
+                                               keys, c.head_dim);
     s.rows_per_unit = shape->rows;
     s.row_groups = (int32_t)((rows + s.rows_per_unit - 1) / s.rows_per_unit);
     // a workgroup of the tile kernel takes four tiles at a time; a unit's start
@@ -1388,7 +1398,8 @@ hipError_t launch_source(const Source& s, Shape shape, hipStream_t stream) {
 struct Sources {
     Shape os{}, as{};
     Source own, ahead{};
-    Sources(const cq_kv_cache_t& c, const cq_attention_t& a) : own(source_of(c, a, false, &os)) {
+    Sources(const cq_kv_cache_t& c, const cq_attention_t& a, bool tree)
+        : own(source_of(c, a, false, &os, tree)) {
         if (a.prefix_len > 0) ahead = source_of(c, a, true, &as);
         lay_out(c, a, &own, &ahead, static_cast<char*>(a.workspace));
     }

@@ -12,7 +12,7 @@ namespace cq {
 
 hipError_t launch_attention_tree(const cq_kv_cache_t& c, const cq_attention_t& a,
                                  const int64_t* seen, hipStream_t stream) {
-    Sources s(c, a);
+    Sources s(c, a, true);
     s.own.seen = reinterpret_cast<const uint32_t*>(seen);
     s.own.words = (a.tokens + 63) / 64 * 2;
     hipError_t e = launch_attention_ahead(c, a, stream);
@@ -20,7 +20,7 @@ hipError_t launch_attention_tree(const cq_kv_cache_t& c, const cq_attention_t& a
         e = by_head(c, a, [&](auto elem, auto dim) {
             return launch_source<decltype(elem), decltype(dim)::value, true>(s.own, s.os, stream);
         });
-    return e == hipSuccess ? launch_attention_join(c, a, stream) : e;
+    return e == hipSuccess ? launch_attention_tree_join(c, a, stream) : e;
 }
 
 }  // namespace cq

@@ -47,9 +47,10 @@ hipError_t launch_kv_append(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int 
 hipError_t launch_kv_read(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int dtype,
                           void* k_out, void* v_out, hipStream_t stream);
 
-// The checks of an attention call (cq_attn_capi.cpp); `launching`: those of its
-// addresses too.
-int check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launching);
+// The checks of an attention call (cq_attn_capi.cpp) whose workspace is that many
+// bytes (-1: its tables are too long); `launching`: those of its addresses too.
+int check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launching,
+                    int64_t (*workspace)(const cq_kv_cache_t&, const cq_attention_t&));
 
 // Bytes, or -1 for a call whose tables span more tiles than 31 bits count.
 int64_t attention_workspace(const cq_kv_cache_t& c, const cq_attention_t& a);

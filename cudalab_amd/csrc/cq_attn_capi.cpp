@@ -156,7 +156,8 @@ int check_read(const cq_kv_cache_t& c, const cq_kv_slots_t& s, int dtype, const 
 
 }  // namespace
 
-int cq::check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launching) {
+int cq::check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool launching,
+                        int64_t (*workspace)(const cq_kv_cache_t&, const cq_attention_t&)) {
     int st = check_cache(c);
     if (st != CQ_OK) return st;
     if (a.batch < 1 || a.tokens < 1) return invalid("batch and tokens must be >= 1");
@@ -172,7 +173,7 @@ int cq::check_attention(const cq_kv_cache_t& c, const cq_attention_t& a, bool la
     if (a.table_cols < 1) return invalid("table_cols must be >= 1");
     if (std::isnan(a.softmax_scale) || std::isinf(a.softmax_scale))
         return invalid("softmax_scale must be finite");
-    const int64_t need = cq::attention_workspace(c, a);
+    const int64_t need = workspace(c, a);
     if (need < 0)
         return invalid("the tables' tokens times batch, rows and heads are too many for one call");
     if (!launching) return CQ_OK;
@@ -253,7 +254,7 @@ int cq_kv_read(const cq_kv_cache_t* cache, const cq_kv_slots_t* slots, int dtype
 int cq_attention(const cq_kv_cache_t* cache, const cq_attention_t* args, void* stream) {
     return guarded([&]() -> int {
         if (cache == nullptr || args == nullptr) return invalid("null pointer: cache or args");
-        const int st = cq::check_attention(*cache, *args, true);
+        const int st = cq::check_attention(*cache, *args, true, cq::attention_workspace);
         if (st != CQ_OK) return st;
         return hip_status(cq::launch_attention(*cache, *args, static_cast<hipStream_t>(stream)),
                           "cq_attention");
@@ -263,7 +264,7 @@ int cq_attention(const cq_kv_cache_t* cache, const cq_attention_t* args, void* s
 int64_t cq_attention_workspace(const cq_kv_cache_t* cache, const cq_attention_t* args) {
     return guarded([&]() -> int64_t {
         if (cache == nullptr || args == nullptr) return -invalid("null pointer: cache or args");
-        const int st = cq::check_attention(*cache, *args, false);
+        const int st = cq::check_attention(*cache, *args, false, cq::attention_workspace);
         if (st != CQ_OK) return -st;
         return cq::attention_workspace(*cache, *args);
     }, -CQ_ERR_HIP);

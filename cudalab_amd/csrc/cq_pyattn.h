@@ -92,13 +92,14 @@ struct Cache {
 class Calls {
 public:
     Calls(uintptr_t norm_rope, uintptr_t append, uintptr_t read, uintptr_t attention,
-          uintptr_t workspace, uintptr_t tree, uintptr_t last_error)
+          uintptr_t workspace, uintptr_t tree, uintptr_t tree_workspace, uintptr_t last_error)
         : norm_rope_(reinterpret_cast<decltype(norm_rope_)>(norm_rope)),
           append_(reinterpret_cast<decltype(append_)>(append)),
           read_(reinterpret_cast<decltype(read_)>(read)),
           attention_(reinterpret_cast<decltype(attention_)>(attention)),
           workspace_(reinterpret_cast<decltype(workspace_)>(workspace)),
           tree_(reinterpret_cast<decltype(tree_)>(tree)),
+          tree_workspace_(reinterpret_cast<decltype(tree_workspace_)>(tree_workspace)),
           last_error_(reinterpret_cast<decltype(last_error_)>(last_error)) {}
 
     // (q_out, k_out), or None; outputs None: new ones.
@@ -280,7 +281,7 @@ public:
         a.q_heads = static_cast<int32_t>(heads);
         a.dtype = dtype_code(type);
         a.softmax_scale = static_cast<float>(scale);
-        const int64_t need = workspace_(&c.c, &a);
+        const int64_t need = (seen == nullptr ? workspace_ : tree_workspace_)(&c.c, &a);
         if (need < 0) return py::none();
         at::Tensor ws;      // given back at the end: work queued behind on this stream follows
         if (need > 0) {
@@ -336,6 +337,7 @@ private:
     int (*attention_)(const cq_kv_cache_t*, const cq_attention_t*, void*);
     int64_t (*workspace_)(const cq_kv_cache_t*, const cq_attention_t*);
     int (*tree_)(const cq_kv_cache_t*, const cq_attention_t*, const int64_t*, void*);
+    int64_t (*tree_workspace_)(const cq_kv_cache_t*, const cq_attention_t*);
     const char* (*last_error_)();
 };
 
@@ -344,7 +346,7 @@ void bind(py::module_& m) {
         .def(py::init<py::handle, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t>());
     py::class_<Calls>(m, "AttentionCalls")
         .def(py::init<uintptr_t, uintptr_t, uintptr_t, uintptr_t, uintptr_t, uintptr_t,
-                      uintptr_t>())
+                      uintptr_t, uintptr_t>())
         .def("norm_rope", &Calls::norm_rope)
         .def("append", &Calls::append)
         .def("read", &Calls::read)

@@ -374,16 +374,20 @@ hipError_t launch_tiles(const Product& a, hipStream_t stream) {
 }
 
 // Which tile.  Small ones leave more workgroups, large ones read less: the
-// smallest that does not give the 256 CUs more than one workgroup each.  (us, the
-// tiles in the order below, fp16 out, weights from memory:
-//   35 tokens, 8192 x 8192:    16.8   22.0   26     35     55    94
-//   256 tokens, 4096 x 4096:   15.8   12.3   15.6   19.7   23    53
-//   256 tokens, 8192 x 8192:   62     46     31.9   40     58   105
-//   512 tokens, 8192 x 8192:  121     85     62     43     59   106)
-// Where that is too many, two workgroups of 128 x 128 to a CU, or one of 256 x 256:
-// per 128 codes a CU's pair takes 1.34 us (a workgroup alone 0.8), the large one
-// 2.07 us, in as many rounds as they need.  (2048 tokens, 4096 x 4096: 42.8, 63; 4096
-// tokens, 28672 x 8192: 1022, 936.)
+// smallest that does not give the 256 CUs more than one workgroup each.  (us, with
+// weights from memory, fp16 out:
+//   tile                      64x32 64x64 128x64 128x128 128x160 128x192 128x256 256x256
+//   35 tokens, 8192 x 8192     16.8  22.0   26     35                      55      94
+//   256 tokens, 4096 x 4096    15.8  12.3   15.6   19.7                    30      53
+//   256 tokens, 8192 x 8192    62    46     31.9   40                      58     105
+//   512 tokens, 8192 x 8192   121    85     62     43                      66     106
+//   777 tokens, 5003 x 4100    75    64     57     60      39.6    42.5    49      73
+//   512 tokens, 11008 x 4096                       49      49      33.3    37      59
+//   1500 tokens, 5000 x 4096                       56      50      56      39      60)
+// Where even the largest of these is too many, two workgroups of 128 x 128 to a CU, or
+// one of 256 x 256: per 128 codes a CU's pair takes 1.34 us (a workgroup alone 0.8),
+// the large one 2.07 us, in as many rounds as they need.  (4096 tokens, us: 11008 x 4096
+// 237, 211; 28672 x 8192 1022, 936.)
 template <class T>
 hipError_t launch_typed(const Product& a, hipStream_t stream) {
     auto tiles = [&](int64_t m, int64_t n) {
@@ -397,6 +401,9 @@ hipError_t launch_typed(const Product& a, hipStream_t stream) {
     if (tiles(128, 64) <= kCus) return launch_tiles<T, 128, 64, 2, 1, 4, 256, 3>(a, stream);
     const int64_t middle = tiles(128, 128), large = tiles(256, 256);
     if (middle <= kCus) return launch_tiles<T, 128, 128, 2, 2, 2, 128, 3>(a, stream);
+    if (tiles(128, 160) <= kCus) return launch_tiles<T, 128, 160, 4, 1, 2, 256, 2>(a, stream);
+    if (tiles(128, 192) <= kCus) return launch_tiles<T, 128, 192, 2, 2, 2, 128, 3>(a, stream);
+    if (tiles(128, 256) <= kCus) return launch_tiles<T, 128, 256, 2, 4, 1, 128, 3>(a, stream);
     const int64_t over = middle % (2 * kCus);
     const double pairs = 1.34 * (double)(middle / (2 * kCus)) +
                          (over == 0 ? 0. : over <= kCus ? 0.8 : 1.34);

@@ -22,11 +22,13 @@ hipError_t launch_kv_append_rows(const cq_kv_cache_t& c, int dtype, int64_t toke
 // cq_prompt.hip
 hipError_t launch_prompt(const cq_prompt_t& a, hipStream_t stream);
 
-// cq_attention.hip: the prefix's part of a call, and the join of its parts
+// cq_attention.hip: of a tree's call the workspace (-1 as attention_workspace), the
+// prefix's part, and the join of the parts
+int64_t attention_tree_workspace(const cq_kv_cache_t& c, const cq_attention_t& a);
 hipError_t launch_attention_ahead(const cq_kv_cache_t& c, const cq_attention_t& a,
                                   hipStream_t stream);
-hipError_t launch_attention_join(const cq_kv_cache_t& c, const cq_attention_t& a,
-                                 hipStream_t stream);
+hipError_t launch_attention_tree_join(const cq_kv_cache_t& c, const cq_attention_t& a,
+                                      hipStream_t stream);
 // cq_attention_tree.hip
 hipError_t launch_attention_tree(const cq_kv_cache_t& c, const cq_attention_t& a,
                                  const int64_t* seen, hipStream_t stream);

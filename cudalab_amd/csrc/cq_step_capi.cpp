@@ -178,7 +178,8 @@ int cq_attention_tree(const cq_kv_cache_t* cache, const cq_attention_t* args,
     return guarded([&]() -> int {
         if (cache == nullptr || args == nullptr || seen == nullptr)
             return invalid("null pointer: cache, args or seen");
-        const int st = cq::check_attention(*cache, *args, true);
+        const int st =
+            cq::check_attention(*cache, *args, true, cq::attention_tree_workspace);
         if (st != CQ_OK) return st;
         if (!aligned(seen, 8)) return invalid("seen must be 8-byte aligned");
         const cq_attention_t& a = *args;
@@ -187,7 +188,7 @@ int cq_attention_tree(const cq_kv_cache_t* cache, const cq_attention_t* args,
         const Span out(a.out, static_cast<U>(a.batch) * static_cast<U>(a.tokens) *
                                   static_cast<U>(a.q_heads) *
                                   static_cast<U>(cache->head_dim * elem_bytes(a.dtype)));
-        const int64_t need = cq::attention_workspace(*cache, a);
+        const int64_t need = cq::attention_tree_workspace(*cache, a);
         if (overlap(out, bits) ||
             overlap(Span(need > 0 ? a.workspace : nullptr, static_cast<U>(need > 0 ? need : 0)), bits))
             return invalid("out or the workspace overlaps an input");
@@ -195,6 +196,15 @@ int cq_attention_tree(const cq_kv_cache_t* cache, const cq_attention_t* args,
                                                     static_cast<hipStream_t>(stream)),
                           "cq_attention_tree");
     });
+}
+
+int64_t cq_attention_tree_workspace(const cq_kv_cache_t* cache, const cq_attention_t* args) {
+    return guarded([&]() -> int64_t {
+        if (cache == nullptr || args == nullptr) return -invalid("null pointer: cache or args");
+        const int st = cq::check_attention(*cache, *args, false, cq::attention_tree_workspace);
+        if (st != CQ_OK) return -st;
+        return cq::attention_tree_workspace(*cache, *args);
+    }, -CQ_ERR_HIP);
 }
 
 int cq_quantize_tokens(int dtype, const void* x, int64_t x_stride, int64_t tokens, int64_t k,

@@ -612,10 +612,12 @@ int cq_kv_append_rows(const cq_kv_cache_t* cache, int dtype, int64_t tokens,
 /* cq_attention for tokens that form a tree, as several drafts of one text do: query
  * t of sequence b sees all positions ahead of the call's tokens, and of these the
  * token j < count for which bit j % 64 of seen[(b * tokens + t) * words + j / 64]
- * is set, words = ceil(tokens / 64); not even itself without its bit.  All else,
- * the prefix and the workspace too, as there.  seen is 8-byte aligned. */
+ * is set, words = ceil(tokens / 64); not even itself without its bit.  All else as
+ * there, but that the workspace is cq_attention_tree_workspace bytes.  seen is
+ * 8-byte aligned. */
 int cq_attention_tree(const cq_kv_cache_t* cache, const cq_attention_t* args,
                       const int64_t* seen, void* stream);
+int64_t cq_attention_tree_workspace(const cq_kv_cache_t* cache, const cq_attention_t* args);
 
 /* Attention of packed sequences over keys and values that lie beside them,
  * q [q_tokens, q_heads, head_dim], k and v [k_tokens, k_heads, head_dim], q head h

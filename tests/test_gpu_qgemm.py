@@ -72,6 +72,15 @@ def test_large(gemm, m, n, k, dtype):
     _check(gemm, m, n, k, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(120, 8000, 256), (250, 8100, 516), (500, 8190, 132),
+                                   (777, 5003, 1028), (500, 11008, 260), (1500, 5001, 388),
+                                   (1300, 8201, 320), (2000, 9000, 4)])
+def test_every_tile(gemm, m, n, k, dtype):
+    """Sizes that take each of the tiles, with edges in both directions."""
+    _check(gemm, m, n, k, dtype)
+
+
 def test_longest_rows(gemm):
     """The largest sums that 32 bits hold, and one more k is refused."""
     k = 131071
