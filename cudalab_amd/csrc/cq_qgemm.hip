@@ -31,17 +31,12 @@ __device__ __forceinline__ uint32_t magnitude(T x) {
     return __float_as_uint((float)x) & 0x7FFFFFFFu;
 }
 
-// How rows of x lie: elements by element, pieces of 16 bytes at 16 bytes, or at words
-// (a row a whole number of them).
-enum { kElements, kPieces, kWords };
-
 // One workgroup to a token; what it holds of the row (HOLD pieces of 8 elements a
 // thread) is read once, the rest again.  Codes need no clamp: x * inv lies within
 // 127 (1 + 2^-21).
 template <class T, int HOLD>
 __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t stride, int64_t k,
-                                                          int8_t* codes, float* scales, int form,
-                                                          uint32_t first) {
+                                                          int8_t* codes, float* scales, uint32_t first) {
     __shared__ uint32_t most[kBlock / 64];
     const int64_t row = (int64_t)first + blockIdx.x;
     const T* p = x + row * stride;
@@ -49,28 +44,11 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t st
     constexpr int N = 8;
     Vec<T, N> held[HOLD];
     uint32_t m = 0;
-    const auto words = buffer_of(p, form == kWords ? (int)(k * sizeof(T)) : 0);
+    // (loads and stores of pieces need no alignment but an element's)
     auto get = [&](int64_t at) {
         Vec<T, N> v = {};
-        if (form == kWords) {
-            // (at most 2^31 bytes; past the row zeros come)
-            if constexpr (sizeof(T) == 4) {
-                using V = Vec<T, 4>;
-                const V a = __builtin_bit_cast(V, load16(words, (int)(at * 4)));
-                const V b = __builtin_bit_cast(V, load16(words, (int)(at * 4) + 16));
-                v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-            } else {
-                using V = Vec<T, N>;
-                v = __builtin_bit_cast(V, load16(words, (int)(at * 2)));
-            }
-        } else if (form == kPieces && at + N <= k) {
-            if constexpr (sizeof(T) == 4) {
-                const Vec<T, 4> a = *reinterpret_cast<const Vec<T, 4>*>(p + at);
-                const Vec<T, 4> b = *reinterpret_cast<const Vec<T, 4>*>(p + at + 4);
-                v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-            } else {
-                v = *reinterpret_cast<const Vec<T, N>*>(p + at);
-            }
+        if (at + N <= k) {
+            __builtin_memcpy(&v, p + at, sizeof v);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -101,7 +79,6 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t st
     float scale, inv;
     scale_of<8>(m, scale, inv);
     if (threadIdx.x == 0) scales[row] = scale;
-    const bool whole = (reinterpret_cast<uintptr_t>(to) & 3) == 0;
     auto put = [&](int64_t at, const Vec<T, N>& v) {
         if (at >= k) return;
         uint32_t w[2];
@@ -117,9 +94,8 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t st
             // inv 0 stands for a row of zeros, whose x may be NaN or Inf
             if (inv == 0.f) w[i] = 0;
         }
-        if (whole && at + N <= k) {
-            reinterpret_cast<uint32_t*>(to + at)[0] = w[0];
-            reinterpret_cast<uint32_t*>(to + at)[1] = w[1];
+        if (at + N <= k) {
+            __builtin_memcpy(to + at, w, sizeof w);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -176,9 +152,10 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(const int8_t* from, int64_
     *reinterpret_cast<u4*>(to + i * 16) = below(r, at, k);
 }
 
+// The scaled sums of `n` of N channels of a token.
 template <class T, int N>
 __device__ __forceinline__ void store_scaled(T* p, const int* sums, float xs,
-                                             const Vec<float, N>& ws, int n, bool whole) {
+                                             const Vec<float, N>& ws, int64_t n) {
     Vec<T, N> v;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -187,8 +164,8 @@ __device__ __forceinline__ void store_scaled(T* p, const int* sums, float xs,
         asm("" : "+v"(y));
         v[i] = (T)y;
     }
-    if (whole) {
-        *reinterpret_cast<Vec<T, N>*>(p) = v;
+    if (n >= N) {
+        __builtin_memcpy(p, &v, sizeof v);         // (at any element)
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -339,7 +316,6 @@ __global__ __launch_bounds__(64 * WM * WN * KS, WM * WN * KS * STAGES > 8 ? 1 : 
     }
     // acc[n][m][j]: token 32 m + col, channel 32 n + 8 (j / 4) + 4 half + j % 4
     T* out = static_cast<T*>(a.out);
-    const bool even = a.n % 4 == 0;
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
         const int row = (wm * TM + m) * 32 + col;
@@ -357,7 +333,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, WM * WN * KS * STAGES > 8 ? 1 : 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sums[i] = acc[n][m][j + i];
                 store_scaled<T, 4>(to + c, sums, xscale, *reinterpret_cast<const f4*>(sm_w + c),
-                                   (int)std::min<int64_t>(4, left), even);
+                                   left);
             }
     }
 }
@@ -416,16 +392,10 @@ template <class T>
 hipError_t quantize_typed(const void* x, int64_t stride, int64_t tokens, int64_t k, int8_t* codes,
                           float* scales, hipStream_t stream) {
     const T* p = static_cast<const T*>(x);
-    const int64_t es = sizeof(T);
-    const int form = (uintptr_t)x % 16 == 0 && stride * es % 16 == 0 ? kPieces
-                     : (uintptr_t)x % 4 == 0 && stride * es % 4 == 0 && k * es % 4 == 0 &&
-                             k < (1 << 28)
-                         ? kWords
-                         : kElements;
     return launch_parts(tokens, [&](dim3 blocks, uint32_t first) {
         auto go = [&](auto hold) {
             quantize_kernel<T, decltype(hold)::value>
-                <<<blocks, dim3(kBlock), 0, stream>>>(p, stride, k, codes, scales, form, first);
+                <<<blocks, dim3(kBlock), 0, stream>>>(p, stride, k, codes, scales, first);
         };
         if (k <= 2 * kBlock * 8) go(std::integral_constant<int, 2>{});
         else if (k <= 4 * kBlock * 8) go(std::integral_constant<int, 4>{});
