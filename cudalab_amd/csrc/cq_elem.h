@@ -53,6 +53,13 @@ __device__ __forceinline__ void scale_of(uint32_t amax_bits, float& scale, float
     }
 }
 
+// The upper half of the wave's a changes places with the lower half of its b.
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+
 // `bytes` from base on as a buffer: a load past them gives 0.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);

@@ -418,18 +418,28 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     const float sum = half_fold((sums[0] + sums[1]) + (sums[2] + sums[3]),
                                 [](float m, float n) { return m + n; });
     const float share = sum == 0.f ? 0.f : 1.f / sum;
-    if (row0 + col < tile.rows) {
-        T* to = out + (row0 + col) * out_row + 4 * half;
+    // the halves of the wave change fours of dims, so that a lane has eight side by side
+    T* to = out + (int64_t)(row0 + col) * out_row + 8 * half;
+    const bool there = row0 + col < tile.rows;
 #pragma unroll
-        for (int d = 0; d < kDims; ++d)
+    for (int d = 0; d < kDims; ++d)
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                Vec<T, 4> v;
+        for (int j = 0; j < 16; j += 8) {
+            using u2 = Vec<uint32_t, 2>;
+            Vec<T, 4> v[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = (T)(sum == 0.f ? 0.f : o[d][j + i] * share);
-                *reinterpret_cast<Vec<T, 4>*>(to + 32 * d + 2 * j) = v;
+            for (int i = 0; i < 8; ++i)
+                v[i / 4][i % 4] = (T)(sum == 0.f ? 0.f : o[d][j + i] * share);
+            u2 x = __builtin_bit_cast(u2, v[0]), y = __builtin_bit_cast(u2, v[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t p = x[i], q = y[i];
+                swap_halves(p, q);
+                x[i] = p;
+                y[i] = q;
             }
-    }
+            if (there) *reinterpret_cast<u4*>(to + 32 * d + 2 * j) = u4{x[0], x[1], y[0], y[1]};
+        }
 }
 
 // ------------------------------------------------------------------- host
