@@ -323,14 +323,20 @@ __global__ __launch_bounds__(kBlock) void append_rows_kernel(cq_kv_cache_t c, ui
                     *reinterpret_cast<const uint4*>(turned[row / C::kBytes] + row % C::kBytes * 16);
             }
         } else {
-            for (int n = 0; n < 16 && base + n < to; ++n) {
-                const int64_t s = __shfl(mine, base + n + 1);
-                if (s < 0 || s >= places) continue;
-                if ((int)threadIdx.x < R) {
-                    const int row = threadIdx.x;
-                    v_at(s)[row * 16] = turned[row / C::kBytes][row % C::kBytes * 16 + n];
-                }
+            // a dim (or two) of as many rows to a thread as fill the workgroup
+            constexpr int kEach = 16 * R / kBlock > 0 ? 16 * R / kBlock : 1;
+            const int dim = threadIdx.x % R, n0 = threadIdx.x / R * kEach;
+            int64_t s[kEach];
+            uint8_t code[kEach];
+#pragma unroll
+            for (int n = 0; n < kEach; ++n) {
+                s[n] = __shfl(mine, min(base + n0 + n + 1, 63));
+                if (base + n0 + n >= to) s[n] = -1;
+                code[n] = turned[dim / C::kBytes][dim % C::kBytes * 16 + n0 + n];
             }
+#pragma unroll
+            for (int n = 0; n < kEach; ++n)
+                if (s[n] >= 0 && s[n] < places) v_at(s[n])[dim * 16] = code[n];
         }
         __syncthreads();
     }
