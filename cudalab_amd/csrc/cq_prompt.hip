@@ -44,6 +44,11 @@ namespace {
 
 constexpr int kKeys = 64;                      // of a tile
 constexpr int kRows = 32;                      // of a wave
+// Two workgroups of four waves on a CU wait for their tiles and barriers apart.  (Eight
+// waves read half as many tiles, and lose at the diagonal, where rows see half a tile;
+// us, 4 and 8 waves: one sequence of 8192 tokens, 64/8 heads of 128, causal 1090 1113,
+// all keys 1949 1925; 16 of up to 2048, 64/8: 518 598.)
+constexpr int kWaves = 4;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kRaise = 8.f;
 
@@ -72,6 +77,7 @@ using s4 = Vec<short, 4>;
 struct Args {
     cq_prompt_t a;
     int32_t group;        // query heads per key head
+    int32_t heads;        // of a workgroup
     int32_t heads_apart;  // 1: neighbouring workgroups take heads of one run each
 };
 
@@ -138,11 +144,14 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t block = first_block + blockIdx.x;
-    const uint32_t place = block % (uint32_t)a.q_heads;
-    const int h = s.heads_apart ? (int)(place % 8 * (a.q_heads / 8) + place / 8) : (int)place;
-    const Tile tile(a, kRows * W, (int)(block / (uint32_t)a.q_heads));
+    // the workgroup's heads (of one key head) and each one's rows
+    const uint32_t runs = (uint32_t)(a.q_heads / s.heads), place = block % runs;
+    const int waves = W / s.heads;             // of a head
+    const int h0 = (s.heads_apart ? (int)(place % 8 * (runs / 8) + place / 8) : (int)place) * s.heads;
+    const int h = h0 + wave / waves;
+    const Tile tile(a, kRows * waves, (int)(block / runs));
     if (tile.b == -2) return;
-    const int row0 = kRows * wave;             // of the tile
+    const int row0 = kRows * (wave % waves);   // of the tile
     T* out = static_cast<T*>(a.out) + ((int64_t)(tile.first + tile.row0) * a.q_heads + h) * D;
     const int64_t out_row = (int64_t)a.q_heads * D;
     const Span keys = tile.b >= 0 ? Span(a.k_offsets != nullptr ? a.k_offsets : a.q_offsets, tile.b,
@@ -157,7 +166,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     };
     const int reach = tile.b >= 0 ? limit_of(tile.rows - 1) : 0;        // of the workgroup
     if (reach == 0) {                          // no keys: zeros
-        for (int i = threadIdx.x; i < tile.rows * kPieces; i += 64 * W)
+        for (int i = threadIdx.x % (64 * waves); i < tile.rows * kPieces; i += 64 * waves)
             *reinterpret_cast<u4*>(out + i / kPieces * out_row + i % kPieces * 8) = u4{0, 0, 0, 0};
         return;
     }
@@ -389,28 +398,24 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
 }
 
 // ------------------------------------------------------------------- host
-template <class T, int D, int W>
-hipError_t launch_shaped(const Args& s, hipStream_t stream) {
+template <class T, int D>
+hipError_t launch_typed(const Args& s, hipStream_t stream) {
     const cq_prompt_t& a = s.a;
     // every sequence's last tile may be a part of one, and so those of the rows
     // that belong to none
-    const int64_t tiles = a.q_tokens / (kRows * W) + a.batch + 2;
-    const __int128 grid = (__int128)tiles * a.q_heads;
+    const int64_t tiles = a.q_tokens / (kRows * kWaves / s.heads) + a.batch + 2;
+    const __int128 grid = (__int128)tiles * (a.q_heads / s.heads);
     if (grid > kMaxGrid) return hipErrorInvalidValue;
     return launch_parts((int64_t)grid, [&](dim3 blocks, uint32_t first) {
-        prompt_kernel<T, D, W><<<blocks, dim3(64 * W), 0, stream>>>(s, first);
-    }, 64 * W);
+        prompt_kernel<T, D, kWaves><<<blocks, dim3(64 * kWaves), 0, stream>>>(s, first);
+    });
 }
 
-// Four waves of 32 rows: two workgroups of 128 rows on a CU wait for their tiles and
-// barriers apart.  (Eight waves read half as many tiles, and lose at the diagonal,
-// where rows see half a tile; us, 4 and 8 waves: one sequence of 8192 tokens, 64/8
-// heads of 128, causal 1090 1113, all keys 1949 1925; 16 of up to 2048, 64/8: 518 598.)
 template <class T>
-hipError_t launch_typed(const Args& s, hipStream_t stream) {
-    if (s.a.head_dim == 64) return launch_shaped<T, 64, 4>(s, stream);
-    if (s.a.head_dim == 128) return launch_shaped<T, 128, 4>(s, stream);
-    return launch_shaped<T, 256, 4>(s, stream);
+hipError_t launch_head(const Args& s, hipStream_t stream) {
+    if (s.a.head_dim == 64) return launch_typed<T, 64>(s, stream);
+    if (s.a.head_dim == 128) return launch_typed<T, 128>(s, stream);
+    return launch_typed<T, 256>(s, stream);
 }
 
 }  // namespace
@@ -419,9 +424,14 @@ hipError_t launch_prompt(const cq_prompt_t& a, hipStream_t stream) {
     Args s{};
     s.a = a;
     s.group = a.q_heads / a.k_heads;
-    s.heads_apart = a.q_heads % 8 == 0;
-    return a.dtype == CQ_DTYPE_F16 ? launch_typed<_Float16>(s, stream)
-                                   : launch_typed<__bf16>(s, stream);
+    // where sequences are short of a workgroup's 128 rows, two or four heads of a key
+    // head share it (200 sequences of 40 tokens, 32/8 heads of 128, us: one head 98, two
+    // 66; of 20 tokens: one 92, four 37)
+    const int64_t rows = a.q_tokens / a.batch;
+    s.heads = rows <= 32 && s.group % 4 == 0 ? 4 : rows <= 64 && s.group % 2 == 0 ? 2 : 1;
+    s.heads_apart = a.q_heads / s.heads % 8 == 0;
+    return a.dtype == CQ_DTYPE_F16 ? launch_head<_Float16>(s, stream)
+                                   : launch_head<__bf16>(s, stream);
 }
 
 }  // namespace cq

@@ -26,6 +26,17 @@ int64_t count(py::handle o) {
     return n < 0 ? -1 : n;
 }
 
+// `n` elements of a contiguous 1-D tensor from element `from` on, as a tensor of the same
+// storage (a view without the dispatcher's work: about 0.1 us instead of an allocation's
+// 0.7).
+at::Tensor part_of(const at::Tensor& t, int64_t from, int64_t n) {
+    at::Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()),
+                                                               t.key_set(), t.dtype());
+    part.unsafeGetTensorImpl()->set_storage_offset(t.storage_offset() + from);
+    part.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return part;
+}
+
 class Calls {
 public:
     Calls(uintptr_t place, uintptr_t append_rows, uintptr_t prompt, uintptr_t last_error)
@@ -54,9 +65,11 @@ public:
             return py::none();
         const auto options = starts->options();
         at::Tensor slots = at::empty({tokens}, options.dtype(at::kLong));
-        at::Tensor positions = at::empty({tokens}, options);
-        at::Tensor offsets = at::empty({batch + 1}, options);
-        at::Tensor lengths = at::empty({batch}, options), gone = at::empty({1}, options);
+        // the others side by side
+        const at::Tensor all = at::empty({tokens + 2 * batch + 2}, options);
+        at::Tensor positions = part_of(all, 0, tokens), offsets = part_of(all, tokens, batch + 1);
+        at::Tensor lengths = part_of(all, tokens + batch + 1, batch);
+        at::Tensor gone = part_of(all, tokens + 2 * batch + 1, 1);
         auto data = [](const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
         cq_place_t a{};
         a.starts = data(*starts), a.counts = data(*counts), a.free_pages = data(*free);

@@ -58,6 +58,29 @@ def test_lengths_and_heads(att, dtype, d, lens, hq, h):
 
 
 @pytest.mark.parametrize("dtype,d", [("fp16", 128), ("bf16", 64), ("bf16", 256)])
+@pytest.mark.parametrize("hq,h", [(8, 2), (4, 1), (6, 3), (14, 7), (16, 2), (12, 3)])
+@pytest.mark.parametrize("lens", [[20] * 9 + [0, 1, 33], [50, 64, 3, 0, 65, 129], [1] * 40,
+                                  [300] + [5] * 30])
+def test_short_sequences_of_grouped_heads(att, dtype, d, hq, h, lens):
+    """Heads of a group share a workgroup where sequences are short, also with a
+    long one among them, keys ahead, rows of no sequence, and NaN that few rows see."""
+    rows = sum(lens)
+    q, k, v = _inputs(rows + 3, rows + 3, hq, h, d, dtype, 14)
+    offsets = _offsets(lens)
+    _check(att, q, k, v, offsets)
+    seen = [n + 7 * (i % 3) for i, n in enumerate(lens)]
+    q, k, v = _inputs(rows, sum(seen), hq, h, d, dtype, 15)
+    _check(att, q, k, v, offsets, _offsets(seen))
+    clean = att.prompt(q[:rows].cuda(), k[:rows].cuda(), v[:rows].cuda(), _ints(offsets)).cpu()
+    bad = offsets[1] - 1
+    v[bad, 0] = float("nan")
+    got = att.prompt(q[:rows].cuda(), k[:rows].cuda(), v[:rows].cuda(), _ints(offsets)).cpu()
+    assert bool(got[bad, :hq // h].isnan().all())
+    got[bad, :hq // h] = clean[bad, :hq // h]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dtype,d", [("fp16", 128), ("bf16", 64), ("bf16", 256)])
 def test_more_and_fewer_keys_than_queries(att, dtype, d):
     """Chunks with keys of earlier ones ahead; fewer keys than queries leave
     rows that see nothing."""
