@@ -78,6 +78,7 @@ struct Args {
     cq_prompt_t a;
     int32_t group;        // query heads per key head
     int32_t heads;        // of a workgroup
+    int32_t shift;        // log2 of a head's rows in a workgroup
     int32_t heads_apart;  // 1: neighbouring workgroups take heads of one run each
 };
 
@@ -89,40 +90,50 @@ __device__ __forceinline__ float half_fold(float v, F&& f) {
     return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
-// Rows of sequence b (of its queries or keys), within the tensor's.
-struct Span {
-    int first, count;
-    __device__ __forceinline__ Span(const int32_t* offsets, int b, int64_t rows) {
-        const int most = (int)rows;
-        first = max(0, min(offsets[b], most));
-        count = max(0, max(0, min(offsets[b + 1], most)) - first);
-    }
-};
-
-// A workgroup's tile of rows.  Part p of the rows (those ahead of the first sequence,
-// each sequence's, those behind the last) has the places from its first row / tile_rows
-// + p on, which are as many as its tiles or one more; so a bisection finds a place's
+// A workgroup's tile of rows, of 2^shift, and its sequence's keys.  Part p of the rows
+// (those ahead of the first sequence, each sequence's, those behind the last) has the
+// places from its first row / 2^shift + p on, which are as many as its tiles or one
+// more.  Of few sequences each lane looks at one, of more a bisection finds a place's
 // part.  The last places come first: of a sequence its last tile, which sees the most
 // keys.  (Sorting the sequences by length, in a search over all of them, gained nothing
-// and took 164 us instead of 104 for 200 sequences of 40 tokens.)
+// and took 164 us instead of 104 for 200 sequences of 40 tokens.)  Offsets are cut to
+// the tensors' rows.
 struct Tile {
-    int b, row0, rows, first;          // b = -1: of no sequence, -2: no rows
-    __device__ __forceinline__ Tile(const cq_prompt_t& a, int tile_rows, int index) {
-        const int most = (int)a.q_tokens;
-        const int place = most / tile_rows + a.batch + 1 - index;
+    int row0, rows, first;             // rows <= 0: none
+    int tokens, key0, keys;            // of the sequence; none for rows of no sequence
+    __device__ __forceinline__ Tile(const cq_prompt_t& a, int shift, int index, int lane) {
+        const int most = (int)a.q_tokens, most_keys = (int)a.k_tokens;
+        const int place = (most >> shift) + a.batch + 1 - index;
+        const int32_t* k_offsets = a.k_offsets != nullptr ? a.k_offsets : a.q_offsets;
         auto begin = [&](int part) {
-            return part == 0 ? 0 : part > a.batch + 1 ? most : max(0, min(a.q_offsets[part - 1], most));
+            return part <= 0 ? 0 : part > a.batch + 1 ? most : max(0, min(a.q_offsets[part - 1], most));
         };
-        int low = 0, high = a.batch + 2;       // the last part that begins here or before
-        while (high - low > 1) {
-            const int mid = low + (high - low) / 2;
-            if ((int64_t)begin(mid) / tile_rows + mid <= place) low = mid;
-            else high = mid;
+        auto key = [&](int b) { return max(0, min(k_offsets[max(0, min(b, a.batch))], most_keys)); };
+        int low = 0, end;
+        if (a.batch + 2 < 64) {
+            const int mine = begin(lane), mine_key = key(lane);
+            const uint64_t here = __ballot(lane <= a.batch + 1 && (mine >> shift) + lane <= place);
+            low = 63 - __builtin_clzll(here | 1);
+            first = __builtin_amdgcn_readlane(mine, low);
+            end = __builtin_amdgcn_readlane(mine, low + 1);
+            key0 = __builtin_amdgcn_readlane(mine_key, max(low - 1, 0));
+            keys = __builtin_amdgcn_readlane(mine_key, low);
+        } else {
+            int high = a.batch + 2;            // low: the last part that begins here or before
+            while (high - low > 1) {
+                const int mid = low + (high - low) / 2;
+                if ((int64_t)(begin(mid) >> shift) + mid <= place) low = mid;
+                else high = mid;
+            }
+            first = begin(low);
+            end = begin(low + 1);
+            key0 = key(low - 1);
+            keys = key(low);
         }
-        first = begin(low);
-        row0 = (place - first / tile_rows - low) * tile_rows;
-        rows = min(tile_rows, max(0, begin(low + 1) - first) - row0);
-        b = rows <= 0 ? -2 : low == 0 || low == a.batch + 1 ? -1 : low - 1;
+        tokens = max(0, end - first);
+        keys = low == 0 || low > a.batch ? 0 : max(0, keys - key0);
+        row0 = (place - (first >> shift) - low) << shift;
+        rows = min(1 << shift, tokens - row0);
     }
 };
 
@@ -149,22 +160,18 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     const int waves = W / s.heads;             // of a head
     const int h0 = (s.heads_apart ? (int)(place % 8 * (runs / 8) + place / 8) : (int)place) * s.heads;
     const int h = h0 + wave / waves;
-    const Tile tile(a, kRows * waves, (int)(block / runs));
-    if (tile.b == -2) return;
+    const Tile tile(a, s.shift, (int)(block / runs), lane);
+    if (tile.rows <= 0) return;
     const int row0 = kRows * (wave % waves);   // of the tile
     T* out = static_cast<T*>(a.out) + ((int64_t)(tile.first + tile.row0) * a.q_heads + h) * D;
     const int64_t out_row = (int64_t)a.q_heads * D;
-    const Span keys = tile.b >= 0 ? Span(a.k_offsets != nullptr ? a.k_offsets : a.q_offsets, tile.b,
-                                         a.k_tokens)
-                                  : Span(a.q_offsets, 0, 0);
-    const int tokens = tile.b >= 0 ? Span(a.q_offsets, tile.b, a.q_tokens).count : 0;
     // keys that row r of the tile sees
     auto limit_of = [&](int r) {
-        if (!a.causal) return keys.count;
-        const int64_t n = (int64_t)keys.count - tokens + tile.row0 + r + 1;
-        return (int)max((int64_t)0, min(n, (int64_t)keys.count));
+        if (!a.causal) return tile.keys;
+        const int64_t n = (int64_t)tile.keys - tile.tokens + tile.row0 + r + 1;
+        return (int)max((int64_t)0, min(n, (int64_t)tile.keys));
     };
-    const int reach = tile.b >= 0 ? limit_of(tile.rows - 1) : 0;        // of the workgroup
+    const int reach = limit_of(tile.rows - 1);         // of the workgroup
     if (reach == 0) {                          // no keys: zeros
         for (int i = threadIdx.x % (64 * waves); i < tile.rows * kPieces; i += 64 * waves)
             *reinterpret_cast<u4*>(out + i / kPieces * out_row + i % kPieces * 8) = u4{0, 0, 0, 0};
@@ -178,9 +185,9 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
 
     // the tiles of keys
     const int64_t k_row = a.k_token_stride * 2, v_row = a.v_token_stride * 2;      // bytes
-    const uint8_t* kp = static_cast<const uint8_t*>(a.k) + keys.first * k_row +
+    const uint8_t* kp = static_cast<const uint8_t*>(a.k) + tile.key0 * k_row +
                         (int64_t)(h / s.group) * a.k_head_stride * 2;
-    const uint8_t* vp = static_cast<const uint8_t*>(a.v) + keys.first * v_row +
+    const uint8_t* vp = static_cast<const uint8_t*>(a.v) + tile.key0 * v_row +
                         (int64_t)(h / s.group) * a.v_head_stride * 2;
     // where a row's pieces are turned to: K's reads take one piece of 16 rows, V's
     // four pieces of four rows
@@ -429,6 +436,7 @@ hipError_t launch_prompt(const cq_prompt_t& a, hipStream_t stream) {
     // 66; of 20 tokens: one 92, four 37)
     const int64_t rows = a.q_tokens / a.batch;
     s.heads = rows <= 32 && s.group % 4 == 0 ? 4 : rows <= 64 && s.group % 2 == 0 ? 2 : 1;
+    s.shift = __builtin_ctz((unsigned)(kRows * kWaves / s.heads));
     s.heads_apart = a.q_heads / s.heads % 8 == 0;
     return a.dtype == CQ_DTYPE_F16 ? launch_head<_Float16>(s, stream)
                                    : launch_head<__bf16>(s, stream);
