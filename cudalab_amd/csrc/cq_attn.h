@@ -1,6 +1,6 @@
 // Internal interface of the operators around attention: the C entry points
 // (cq_attn_capi.cpp) check a call's arguments and hand them on unchanged to
-// the launchers (cq_kvcache.hip, cq_attention.hip).
+// the launchers (cq_norm_rope.hip, cq_kvcache.hip, cq_attention.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>

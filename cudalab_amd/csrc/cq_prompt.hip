@@ -32,6 +32,13 @@
 //
 // Rows and keys lie wherever the offsets on the device say, so every workgroup
 // finds its tile of rows by itself.  Tiles that see the same keys run side by side.
+//
+// Bound by the softmax between the products: counters of one sequence of 8192 tokens,
+// 64/8 heads of 128, say 59% of the time in matrix instructions and 50% in vector ones,
+// at a clock that power has brought to 1.8 GHz.  That is 1.04 ms causal (1050 TFLOP/s,
+// a large plain product 1360 to 1560).  16 sequences of up to 2048, 32/32 heads of
+// 128, 290 us; five of up to 100, 28/4 heads of 64, 7 us.  Reading LDS one product
+// ahead, priorities for the waves in the products, and eight waves gained nothing.
 
 #include <algorithm>
 #include <type_traits>

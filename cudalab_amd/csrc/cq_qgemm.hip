@@ -33,7 +33,7 @@ __device__ __forceinline__ uint32_t magnitude(T x) {
 
 // One workgroup to a token; what it holds of the row (HOLD pieces of 8 elements a
 // thread) is read once, the rest again.  Codes need no clamp: x * inv lies within
-// 127 (1 + 2^-21).
+// 127 (1 + 2^-21).  Bound by memory: 4096 tokens of 8192 in fp16 19 us, 5.3 TB/s.
 template <class T, int HOLD>
 __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t stride, int64_t k,
                                                           int8_t* codes, float* scales, uint32_t first) {
@@ -132,7 +132,7 @@ __device__ __forceinline__ u4 below(u4 v, int at, int k) {
 // Rows that start at any byte, to rows of whole pieces of 16 (zeros behind their
 // ends).  A piece comes from the words around it that hold any of the row's bytes,
 // shifted: nothing else is read.  5003 rows of 4099: 13 us; a product with shifts
-// in its loads took 185 us of 777 tokens, this and the product of rows at words 60.
+// in its loads took 185 us of 777 tokens, this and the product of rows at words 47.
 __global__ __launch_bounds__(kBlock) void pack_kernel(const int8_t* from, int64_t stride,
                                                       int64_t rows, int k, int8_t* to, int pieces,
                                                       uint32_t first) {
@@ -321,8 +321,8 @@ __global__ __launch_bounds__(64 * WM * WN * KS, WM * WN * KS * STAGES > 8 ? 1 : 
     }
     // acc[n][m][j]: token 32 m + col, channel 32 n + 8 (j / 4) + 4 half + j % 4.  Of
     // types of 16 bits the halves of the wave change fours, so that a lane has eight
-    // channels side by side (4096 tokens, 11008 x
-    // 4096: 213 us with stores of 8 bytes, 199 with these).
+    // channels side by side (4096 tokens, 11008 x 4096: 213 us with stores of 8
+    // bytes, 199 with these).
     T* out = static_cast<T*>(a.out);
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
@@ -384,17 +384,18 @@ hipError_t launch_tiles(const Product& a, hipStream_t stream) {
 // smallest that does not give the 256 CUs more than one workgroup each.  (us, with
 // weights from memory, fp16 out:
 //   tile                      64x32 64x64 128x64 128x128 128x160 128x192 128x256 256x256
-//   35 tokens, 8192 x 8192     16.8  22.0   26     35                      55      94
-//   256 tokens, 4096 x 4096    15.8  12.3   15.6   19.7                    30      53
-//   256 tokens, 8192 x 8192    62    46     31.9   40                      58     105
-//   512 tokens, 8192 x 8192   121    85     62     43                      66     106
-//   777 tokens, 5003 x 4100    75    64     57     60      39.6    42.5    49      73
-//   512 tokens, 11008 x 4096                       49      49      33.3    37      59
-//   1500 tokens, 5000 x 4096                       56      50      56      39      60)
+//   35 tokens, 8192 x 8192     16.0  21.1   24.7   35      46      44      53      93
+//   256 tokens, 4096 x 4096    14.9  11.6   14.4   19.5    21.5    25.4    28.6    50
+//   256 tokens, 8192 x 8192    59    47     33.2   47      49      49      57     102
+//   512 tokens, 8192 x 8192   119    85     60     48      53      56      62     105
+//   777 tokens, 5003 x 4100    68    58     50     50      30.5    34.1    42      61
+//   512 tokens, 11008 x 4096   94    73     50     45      49      32.0    35      59
+//   1500 tokens, 5000 x 4096  122    83     65     50      49      54      38.1    60)
 // Where even the largest of these is too many, two workgroups of 128 x 128 to a CU, or
 // one of 256 x 256: per 128 codes a CU's pair takes 1.34 us (a workgroup alone 0.8),
-// the large one 2.07 us, in as many rounds as they need.  (4096 tokens, us: 11008 x 4096
-// 237, 211; 28672 x 8192 1022, 936.)
+// the large one 2.07 us, in as many rounds as they need.  (us: 4096 tokens, 11008 x 4096
+// 208, 194; 28672 x 8192 965, 888, of which the matrix units need 897 at the rate of
+// the library's largest product.)
 template <class T>
 hipError_t launch_typed(const Product& a, hipStream_t stream) {
     auto tiles = [&](int64_t m, int64_t n) {
