@@ -367,7 +367,10 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void prompt_kernel(Args s
     // tiles that every row of the workgroup sees all of, then the others
     const int tiles = (reach + kKeys - 1) / kKeys, whole = limit_of(0) / kKeys;
     auto next = [&](int t) {
-        __syncthreads();                       // tile t has come, t - 1 is done with
+        // this wave's loads of tile t have come and its reads of t - 1 are done, then
+        // everybody's (a barrier alone waits for neither: a wave that has no keys in
+        // t - 1 has not looked at any)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
     };
     int t = 0;

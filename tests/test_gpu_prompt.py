@@ -91,6 +91,17 @@ def test_more_and_fewer_keys_than_queries(att, dtype, d):
         _check(att, q, k, v, _offsets(lens), _offsets(seen), causal)
 
 
+@pytest.mark.parametrize("dtype,d", [("fp16", 128), ("bf16", 64), ("bf16", 256)])
+def test_waves_with_fewer_keys_than_others(att, dtype, d):
+    """Waves that have no rows, or whose rows see none of a tile's keys, load their
+    part of the next tile all the same, and the others wait for it."""
+    lens = [1, 5, 33, 65, 97, 33, 64, 128] * 12
+    keys = [194, 65, 130, 131, 300, 34, 129, 161] * 12
+    for seed in range(3):
+        q, k, v = _inputs(sum(lens), sum(keys), 8, 4, d, dtype, 40 + seed)
+        _check(att, q, k, v, _offsets(lens), _offsets(keys), what=f"seed {seed}")
+
+
 @pytest.mark.parametrize("dtype,d", [("fp16", 128), ("bf16", 128), ("fp16", 64), ("bf16", 256)])
 def test_many_rows(att, dtype, d):
     """Enough rows for the larger workgroups, of lengths that end anywhere."""
