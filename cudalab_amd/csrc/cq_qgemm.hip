@@ -256,8 +256,9 @@ __global__ __launch_bounds__(64 * WM * WN * KS, WM * WN * KS * STAGES > 8 ? 1 : 
     for (int i = 0; i < STAGES - 1; ++i) fetch(i);
     for (int step = 0; step < steps; ++step) {
         // the wave's loads of this step have come (those of the STAGES - 2 behind
-        // it may be on their way), then everybody's
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 2) * (kXLoads + kWLoads))
+        // it may be on their way) and its reads and writes of LDS are done, then
+        // everybody's
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * (kXLoads + kWLoads))
                      : "memory");
         const uint8_t* buf = sm + step % STAGES * kTileBytes;
         fetch(step + STAGES - 1);        // (zeros behind the last step: the count of loads stays)
