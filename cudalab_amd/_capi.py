@@ -221,6 +221,7 @@ SIGNATURES = {
     "cq_attention_workspace": (_i64, [ctypes.POINTER(CqKvCache),
                                       ctypes.POINTER(CqAttention)]),
     "cq_place": (ctypes.c_int, [ctypes.POINTER(CqPlace), _vp]),
+    "cq_place_held": (ctypes.c_int, [ctypes.POINTER(CqPlace), _vp, _vp, _vp]),
     "cq_kv_append_rows": (ctypes.c_int, [
         ctypes.POINTER(CqKvCache), ctypes.c_int, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64,
         _vp]),

@@ -120,6 +120,16 @@ class Placed(NamedTuple):
     taken: torch.Tensor        # int32 (1,): entries of the free list that are gone
 
 
+class PlacedHeld(NamedTuple):
+    """Placed, and the pages that each sequence holds then (place with `held`)."""
+    slots: torch.Tensor
+    positions: torch.Tensor
+    offsets: torch.Tensor
+    lengths: torch.Tensor
+    taken: torch.Tensor
+    held: torch.Tensor         # int32 (batch,)
+
+
 class AttentionExt:
     """Norms with rotation, the quantized cache and attention over it."""
 
@@ -131,7 +141,7 @@ class AttentionExt:
             "cq_attention_workspace", "cq_attention_tree", "cq_attention_tree_workspace",
             "cq_last_error")))
         self._step = mod and mod.StepCalls(*(_capi.entry_address(n) for n in (
-            "cq_place", "cq_kv_append_rows", "cq_prompt_attention", "cq_last_error")))
+            "cq_place", "cq_place_held", "cq_kv_append_rows", "cq_prompt_attention", "cq_last_error")))
 
     # ---- norms and rotation ----
     def qk_norm_rope(self, q: torch.Tensor, k: torch.Tensor,
@@ -324,7 +334,8 @@ class AttentionExt:
     # ---- packed batches ----
     def place(self, block_table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor,
               tokens: int, page_size: int, free_pages: torch.Tensor,
-              taken: Optional[torch.Tensor] = None) -> Placed:
+              taken: Optional[torch.Tensor] = None, *,
+              held: Optional[torch.Tensor] = None) -> Placed | PlacedHeld:
         """Pages, positions and slots for a packed batch of `tokens` rows in
         which sequence b adds counts[b] tokens to the starts[b] that it has.
 
@@ -337,12 +348,19 @@ class AttentionExt:
         call's `taken`.  A token without a page, or past the table, has slot -1,
         and so have rows behind the last sequence.  Tokens that do not fit
         `tokens` rows are not placed, and `lengths` does not count them.
-        Negative starts and counts are zero."""
+        Negative starts and counts are zero.
+
+        `held` int32 (batch,) says how many entries of its row a sequence owns
+        where those may be more than its start needs, as when drafted tokens were
+        given up: these entries are used before pages are taken from the list (without
+        it they are overwritten and their pages lost to the list).  The result is
+        then a PlacedHeld, whose `held` is the next call's, as its `taken` is; a
+        sequence whose pages go back to the list starts with 0."""
         if self._step is not None:
             got = self._step.place(block_table, starts, counts, tokens, page_size, free_pages,
-                                   taken)
+                                   taken, held)
             if got is not None:
-                return Placed(*got)
+                return Placed(*got) if held is None else PlacedHeld(*got)
         if not isinstance(block_table, torch.Tensor):
             _fail(f"block_table must be a tensor, got {type(block_table).__name__}")
         dev = block_table.device
@@ -357,12 +375,16 @@ class AttentionExt:
         _ints("free_pages", free_pages, (free_pages.numel(),), dev)
         if taken is not None:
             _ints("taken", taken, (1,), dev)
+        if held is not None:
+            _ints("held", held, (batch,), dev)
 
         def ints(n, dtype=torch.int32):
             return torch.empty(n, dtype=dtype, device=dev)
 
         p = Placed(ints(tokens, torch.int64), ints(tokens), ints(batch + 1), ints(batch),
                    ints(1))
+        if held is not None:
+            p = PlacedHeld(*p, ints(batch))
         if batch == 0:
             p.slots.fill_(-1)
             p.positions.zero_()
@@ -375,7 +397,9 @@ class AttentionExt:
             p.slots.data_ptr() or None, p.positions.data_ptr() or None, p.offsets.data_ptr(),
             p.lengths.data_ptr(), p.taken.data_ptr(), block_table.stride(0), tokens,
             free_pages.numel(), block_table.size(1), batch, page_size)
-        _check(_on_device(dev, lambda s: self._lib.cq_place(ctypes.byref(a), s)), "place")
+        _check(_on_device(dev, lambda s: self._lib.cq_place_held(
+            ctypes.byref(a), None if held is None else held.data_ptr(),
+            None if held is None else p.held.data_ptr(), s)), "place")
         return p
 
     def append_rows(self, cache: KVCache, k: torch.Tensor, v: torch.Tensor,

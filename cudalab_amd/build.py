@@ -46,8 +46,9 @@ LIB_PATH = LIB_DIR / LIB_NAME
 
 ARCH = "gfx950"
 SOURCES = ("cq_kernels.hip", "cq_quantize.hip", "cq_norm_rope.hip", "cq_kvcache.hip",
-           "cq_attention.hip", "cq_attention_tree.hip", "cq_place.hip", "cq_prompt.hip", "cq_qgemm.hip", "cq_capi.cpp",
-           "cq_attn_capi.cpp", "cq_step_capi.cpp")
+           "cq_attention.hip", "cq_attention_tree.hip", "cq_place.hip", "cq_prompt.hip",
+           "cq_qgemm.hip", "cq_capi.cpp", "cq_attn_capi.cpp", "cq_step_capi.cpp",
+           "cq_place_capi.cpp")
 # the Python binding of the eager fast path (host code only, built with the
 # host compiler against torch's headers; it calls the library by address)
 FAST_SOURCE = "cq_pyfast.cpp"

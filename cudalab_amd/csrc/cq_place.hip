@@ -2,8 +2,9 @@
 // (gfx950).
 //
 //   n_b      tokens that sequence b adds, offsets_b = n_0 + .. + n_{b-1}
-//   have_b   ceil(start_b / page) pages that it holds
-//   need_b   ceil((start_b + n_b) / page) - have_b pages that it gets,
+//   have_b   ceil(start_b / page) pages that it holds, or as many as the caller
+//            says, where those are more: pages taken for tokens that were given up
+//   need_b   max(0, ceil((start_b + n_b) / page) - have_b) pages that it gets,
 //   first_b  need_0 + .. + need_{b-1}, its place in the free list
 // and token t of the packed batch, in sequence b with offsets_b <= t, has the
 // position p = start_b + t - offsets_b, the page of column c = p / page (the
@@ -46,7 +47,8 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t cap, uint32_
     return v;
 }
 
-__global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, uint32_t first_block) {
+__global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, const int32_t* held_in,
+                                                       int32_t* held_out, uint32_t first_block) {
     __shared__ uint32_t sums[kBlock / 64];
     // of 256 sequences: where their tokens end, begin and start, and their pages
     __shared__ uint32_t end[kBlock], begin[kBlock], start[kBlock], have[kBlock], page0[kBlock];
@@ -59,10 +61,11 @@ __global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, uint32_t fi
     uint32_t placed = 0, pages = 0;            // of the sequences before these 256
     for (uint32_t base = 0; base < (uint32_t)a.batch; base += kBlock) {
         const uint32_t b = base + tid;
-        uint32_t n = 0, s = 0;
+        uint32_t n = 0, s = 0, own = 0;
         if (b < (uint32_t)a.batch) {
             n = (uint32_t)max(0, a.counts[b]);
             s = (uint32_t)max(0, a.starts[b]);
+            if (held_in != nullptr) own = (uint32_t)max(0, held_in[b]);
         }
         // what does not fit the call's tokens is not placed
         const uint32_t upto = min(placed + block_scan(min(n, tokens), tokens, sums), tokens);
@@ -71,7 +74,7 @@ __global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, uint32_t fi
         if (tid + 1 < kBlock) begin[tid + 1] = upto;
         __syncthreads();
         n = upto - begin[tid];
-        const uint32_t held = s / page + (s % page != 0);
+        const uint32_t held = max(s / page + (s % page != 0), own);
         const uint32_t last = min(s + n, room);
         const uint32_t want = last / page + (last % page != 0);
         const uint32_t need = n > 0 && want > held ? want - held : 0;
@@ -83,6 +86,13 @@ __global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, uint32_t fi
             if (b == 0) a.offsets[0] = 0;
             a.offsets[b + 1] = (int32_t)upto;
             a.lengths[b] = (int32_t)min(s + n, kMost);
+            if (held_out != nullptr) {         // of the pages it needs those that the list has
+                const uint64_t at = (uint64_t)taken + page0[tid];
+                const uint64_t left =
+                    (uint64_t)a.free_count > at ? (uint64_t)a.free_count - at : 0;
+                held_out[b] = (int32_t)min((uint64_t)held + min((uint64_t)need, left),
+                                           (uint64_t)kMost);
+            }
         }
         __syncthreads();
         const uint32_t lo = begin[0], hi = end[kBlock - 1];
@@ -129,11 +139,16 @@ __global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, uint32_t fi
 
 }  // namespace
 
-hipError_t launch_place(const cq_place_t& a, hipStream_t stream) {
+hipError_t launch_place_held(const cq_place_t& a, const int32_t* held_in, int32_t* held_out,
+                             hipStream_t stream) {
     const int64_t grid = std::max<int64_t>(1, (a.tokens + kTokens - 1) / kTokens);
     return launch_parts(grid, [&](dim3 blocks, uint32_t first) {
-        place_kernel<<<blocks, dim3(kBlock), 0, stream>>>(a, first);
+        place_kernel<<<blocks, dim3(kBlock), 0, stream>>>(a, held_in, held_out, first);
     });
+}
+
+hipError_t launch_place(const cq_place_t& a, hipStream_t stream) {
+    return launch_place_held(a, nullptr, nullptr, stream);
 }
 
 }  // namespace cq

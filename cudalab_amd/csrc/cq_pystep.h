@@ -39,20 +39,21 @@ at::Tensor part_of(const at::Tensor& t, int64_t from, int64_t n) {
 
 class Calls {
 public:
-    Calls(uintptr_t place, uintptr_t append_rows, uintptr_t prompt, uintptr_t last_error)
+    Calls(uintptr_t place, uintptr_t place_held, uintptr_t append_rows, uintptr_t prompt, uintptr_t last_error)
         : place_(reinterpret_cast<decltype(place_)>(place)),
+          place_held_(reinterpret_cast<decltype(place_held_)>(place_held)),
           append_rows_(reinterpret_cast<decltype(append_rows_)>(append_rows)),
           prompt_(reinterpret_cast<decltype(prompt_)>(prompt)),
           last_error_(reinterpret_cast<decltype(last_error_)>(last_error)) {}
 
-    // (slots, positions, offsets, lengths, taken), or None.
+    // (slots, positions, offsets, lengths, taken), with `held` also the next held, or None.
     py::object place(py::handle table_, py::handle starts_, py::handle counts_,
                      py::handle tokens_, py::handle page_, py::handle free_,
-                     py::handle taken_) const {
+                     py::handle taken_, py::handle held_) const {
         bool ok = true;
         const at::Tensor *table = tensor(table_, false, ok), *starts = tensor(starts_, false, ok);
         const at::Tensor *counts = tensor(counts_, false, ok), *free = tensor(free_, false, ok);
-        const at::Tensor* taken = tensor(taken_, true, ok);
+        const at::Tensor *taken = tensor(taken_, true, ok), *held = tensor(held_, true, ok);
         const int64_t tokens = count(tokens_), page = count(page_);
         if (!ok || table->dim() != 2 || !on_current(*table) || tokens < 0 || tokens > INT32_MAX ||
             page < 16 || page > 256)
@@ -61,12 +62,14 @@ public:
         const int64_t batch = table->size(0);
         if (batch < 1 || batch >= INT32_MAX || !table_ok(*table, batch, dev) ||
             !ints(*starts, batch, dev) || !ints(*counts, batch, dev) ||
-            !ints(*free, free->numel(), dev) || (taken != nullptr && !ints(*taken, 1, dev)))
+            !ints(*free, free->numel(), dev) || (taken != nullptr && !ints(*taken, 1, dev)) ||
+            (held != nullptr && !ints(*held, batch, dev)))
             return py::none();
         const auto options = starts->options();
         at::Tensor slots = at::empty({tokens}, options.dtype(at::kLong));
         // the others side by side
-        const at::Tensor all = at::empty({tokens + 2 * batch + 2}, options);
+        const at::Tensor all =
+            at::empty({tokens + (held != nullptr ? 3 : 2) * batch + 2}, options);
         at::Tensor positions = part_of(all, 0, tokens), offsets = part_of(all, tokens, batch + 1);
         at::Tensor lengths = part_of(all, tokens + batch + 1, batch);
         at::Tensor gone = part_of(all, tokens + 2 * batch + 1, 1);
@@ -84,6 +87,12 @@ public:
         a.table_cols = static_cast<int32_t>(table->size(1));
         a.batch = static_cast<int32_t>(batch);
         a.page_size = static_cast<int32_t>(page);
+        if (held != nullptr) {
+            at::Tensor owned = part_of(all, tokens + 2 * batch + 2, batch);
+            if (!done(place_held_(&a, data(*held), data(owned), stream_of(*table)), "place"))
+                return py::none();
+            return py::make_tuple(slots, positions, offsets, lengths, gone, owned);
+        }
         if (!done(place_(&a, stream_of(*table)), "place")) return py::none();
         return py::make_tuple(slots, positions, offsets, lengths, gone);
     }
@@ -171,6 +180,7 @@ private:
     }
 
     int (*place_)(const cq_place_t*, void*);
+    int (*place_held_)(const cq_place_t*, const int32_t*, int32_t*, void*);
     int (*append_rows_)(const cq_kv_cache_t*, int, int64_t, const int64_t*, const void*, int64_t,
                         int64_t, const void*, int64_t, int64_t, void*);
     int (*prompt_)(const cq_prompt_t*, void*);
@@ -276,7 +286,7 @@ void bind(py::module_& m) {
         .def("quantize", &Qgemm::quantize)
         .def("forward", &Qgemm::forward);
     py::class_<Calls>(m, "StepCalls")
-        .def(py::init<uintptr_t, uintptr_t, uintptr_t, uintptr_t>())
+        .def(py::init<uintptr_t, uintptr_t, uintptr_t, uintptr_t, uintptr_t>())
         .def("prompt", &Calls::prompt)
         .def("place", &Calls::place)
         .def("append_rows", &Calls::append_rows);

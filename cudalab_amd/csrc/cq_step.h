@@ -12,6 +12,9 @@ namespace cq {
 
 // cq_place.hip
 hipError_t launch_place(const cq_place_t& a, hipStream_t stream);
+// With counts of held pages, in and out (either may be null).
+hipError_t launch_place_held(const cq_place_t& a, const int32_t* held_in, int32_t* held_out,
+                             hipStream_t stream);
 
 // cq_kvcache.hip.  Element strides of k or v [tokens, heads, head_dim] (of
 // KvStrides `batch` is not used).

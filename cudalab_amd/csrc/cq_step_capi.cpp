@@ -13,53 +13,6 @@ using namespace cq::checks;
 
 namespace {
 
-// Whether a span written meets another operand of the call.
-template <int N, int M>
-bool meet(const Span (&out)[N], const Span (&in)[M]) {
-    for (int i = 0; i < N; ++i) {
-        for (int j = i + 1; j < N; ++j)
-            if (overlap(out[i], out[j])) return true;
-        for (const Span& x : in)
-            if (overlap(out[i], x)) return true;
-    }
-    return false;
-}
-
-int check_place(const cq_place_t& a) {
-    if (a.batch < 1 || a.batch == INT_MAX) return invalid("batch must be in [1, 2^31-2]");
-    if (a.tokens < 0 || a.tokens > INT_MAX) return invalid("tokens must be in [0, 2^31-1]");
-    if (a.page_size < 16 || a.page_size > 256 || (a.page_size & (a.page_size - 1)) != 0)
-        return invalid("page_size must be 16, 32, 64, 128 or 256");
-    if (a.free_count < 0 || a.free_count > (int64_t)1 << 40)
-        return invalid("free_count must be in [0, 2^40]");
-    int st = check_table(a.table, a.table_stride, a.table_cols, a.batch);
-    if (st != CQ_OK) return st;
-    if ((int64_t)a.table_cols * a.page_size > INT_MAX)
-        return invalid("table_cols * page_size must be below 2^31");
-    if (a.starts == nullptr || a.counts == nullptr || a.offsets == nullptr ||
-        a.lengths == nullptr || a.taken_out == nullptr ||
-        (a.free_count > 0 && a.free_pages == nullptr) ||
-        (a.tokens > 0 && (a.slots == nullptr || a.positions == nullptr)))
-        return invalid("null pointer argument");
-    for (const void* p : {(const void*)a.starts, (const void*)a.counts, (const void*)a.free_pages,
-                          (const void*)a.taken_in, (const void*)a.positions,
-                          (const void*)a.offsets, (const void*)a.lengths,
-                          (const void*)a.taken_out})
-        if (!aligned(p, 4)) return invalid("a pointer is not aligned to its element size");
-    if (!aligned(a.slots, 8)) return invalid("a pointer is not aligned to its element size");
-    const U batch = static_cast<U>(a.batch), tokens = static_cast<U>(a.tokens);
-    const Span out[] = {table_span(a.table, a.table_stride, a.table_cols, a.batch),
-                        Span(a.slots, tokens * 8),
-                        Span(a.positions, tokens * 4),
-                        Span(a.offsets, (batch + 1) * 4),
-                        Span(a.lengths, batch * 4),
-                        Span(a.taken_out, 4)};
-    const Span in[] = {Span(a.starts, batch * 4), Span(a.counts, batch * 4),
-                       Span(a.free_pages, static_cast<U>(a.free_count) * 4), Span(a.taken_in, 4)};
-    if (meet(out, in)) return invalid("an output overlaps another operand");
-    return CQ_OK;
-}
-
 bool stride_ok(int64_t n) { return n >= 0 && n <= (int64_t)1 << 40; }
 
 int check_append_rows(const cq_kv_cache_t& c, int dtype, int64_t tokens, const int64_t* slots,
@@ -249,7 +202,7 @@ int cq_prompt_attention(const cq_prompt_t* args, void* stream) {
 int cq_place(const cq_place_t* args, void* stream) {
     return guarded([&]() -> int {
         if (args == nullptr) return invalid("null pointer: args");
-        const int st = check_place(*args);
+        const int st = check_place(*args, nullptr, nullptr);
         if (st != CQ_OK) return st;
         return hip_status(cq::launch_place(*args, static_cast<hipStream_t>(stream)), "cq_place");
     });

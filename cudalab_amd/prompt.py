@@ -68,6 +68,8 @@ class PromptModel:
         """No tokens, all pages free."""
         self.lengths = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
         self.taken = torch.zeros(1, dtype=torch.int32, device=self.device)
+        # pages of each sequence: drafts that were given up leave theirs to the next
+        self.held = torch.zeros_like(self.lengths)
 
     def _product(self, name: str, layer: int, quantized) -> torch.Tensor:
         return self.gemm.forward(*quantized, *self.weights.layers[layer].w[name])
@@ -95,8 +97,8 @@ class PromptModel:
         """The first counts[b] tokens of each sequence, packed in x (rows, hidden)
         fp16; rows behind the last sequence are carried along and belong to none."""
         p = self.att.place(self.table, self.lengths, counts, x.size(0), PAGE, self.free,
-                           self.taken)
-        self.lengths, self.taken = p.lengths, p.taken
+                           self.taken, held=self.held)
+        self.lengths, self.taken, self.held = p.lengths, p.taken, p.held
         return self._layers(x, p.positions, p.slots, lambda cache, q, k, v:
                             self.att.prompt(q, k, v, p.offsets))[0]
 
@@ -106,8 +108,9 @@ class PromptModel:
         of its bits (tree int64 (batch, T, ceil(T / 64)))."""
         rows, T = x.size(0) * x.size(1), x.size(1)
         counts = torch.full_like(self.lengths, T)
-        p = self.att.place(self.table, self.lengths, counts, rows, PAGE, self.free, self.taken)
-        self.taken = p.taken
+        p = self.att.place(self.table, self.lengths, counts, rows, PAGE, self.free, self.taken,
+                           held=self.held)
+        self.taken, self.held = p.taken, p.held
         positions = (self.lengths[:, None] + depth).view(-1)
 
         def attend(cache, q, k, v):
@@ -174,13 +177,7 @@ def run(model: str = "7b", layers: int | None = None, batch: int = 4, tokens: in
     if drafts:
         tree, depth = chains(batch, drafts, 4)
         y = torch.randn(batch, drafts, cfg["hidden"], device="cuda").half()
-        taken = m.taken
-
-        def check():
-            m.taken = taken
-            m.check(y, tree, depth)
-
-        us = time_steps(check, steps, warmup)
+        us = time_steps(lambda: m.check(y, tree, depth), steps, warmup)
         res["check"] = {"drafts": drafts, "us_per_step": round(us, 1),
                         "us_per_layer": round(us / layers, 2),
                         "GBps_of_weights": round(weights * layers / us / 1e3, 1)}

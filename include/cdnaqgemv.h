@@ -600,6 +600,15 @@ typedef struct cq_place {
 } cq_place_t;
 int cq_place(const cq_place_t* args, void* stream);
 
+/* cq_place for sequences that own more entries of their rows than their starts
+ * need, as those do whose drafted tokens were given up: sequence b holds the first
+ * max(ceil(max(0, starts[b]) / page_size), held_in[b]) entries, and pages come from
+ * the list only beyond them.  held_out [batch] (or NULL) becomes the entries that
+ * it holds then (as far as the list had pages), the next call's held_in.  held_in
+ * [batch] NULL: as in cq_place. */
+int cq_place_held(const cq_place_t* args, const int32_t* held_in, int32_t* held_out,
+                  void* stream);
+
 /* cq_kv_append for packed rows of known slots: row t of k and v [tokens, heads,
  * head_dim] is quantized into slot slots[t] = page * page_size + offset of every
  * head.  A row whose slot is negative or past the last page is not written.  No
