@@ -122,9 +122,10 @@ class PromptModel:
 
     def accept(self, keep: torch.Tensor) -> None:
         """Of the last check's tokens those with keep[b, t], in their order, become
-        the sequences' next ones."""
+        the sequences' next ones, as many as `room` has places for."""
         rank = keep.long().cumsum(1) - 1
         at = self.lengths.long()[:, None] + rank
+        keep = keep & (at < self.room)
         page = self.table.long().gather(1, (at // PAGE).clamp(0, self.table.size(1) - 1))
         slots = torch.where(keep, page * PAGE + at % PAGE, -1).view(-1)
         for cache, (k, v) in zip(self.caches, self.drafts):

@@ -101,3 +101,28 @@ def test_rounds_until_the_room_is_full(cuda, bits):
             exact = codes.astype(np.float64) * scale.astype(np.float64)[..., None]
             assert there.all() and np.array_equal(got, exact.swapaxes(0, 1))
             assert len(codes) == n - prompt_lens[b]
+
+
+@pytest.mark.parametrize("room,n", [(128, 120), (120, 110), (128, 128), (100, 99)])
+def test_kept_drafts_past_the_room(cuda, room, n):
+    """Kept drafts that the room has no place for are dropped: the tokens before them
+    stay as they are, and the lengths count what is in the caches."""
+    from cudalab_amd.prompt import chains
+    T = 16
+    m = _model(2, room, layers=1)
+    announce(f"drafts past a room of {room}")
+    m.prompt(_x(n + 30, 1024, seed=30), _counts([n, 30]))
+    before = _pages_of(m.caches[0])
+    m.check(_x(2, T, 1024, seed=31), *chains(2, T, 1))
+    m.accept(torch.ones(2, T, dtype=torch.bool, device="cuda"))
+    assert m.lengths.tolist() == [room, 30 + T]
+    after, table = _pages_of(m.caches[0]), m.table.tolist()
+    (k, v), = m.drafts
+    for which, x in ((0, k), (1, v)):
+        for b, (had, has) in enumerate(((n, room), (30, 30 + T))):
+            old, _ = before.values(table[b], 0, had, which)
+            got, there = after.values(table[b], 0, has, which)
+            assert there.all() and np.array_equal(got[:, :had], old)
+            codes, scale = quantize(x.view(2, T, -1, 128)[b, :has - had].cpu().float().numpy(), 8)
+            exact = codes.astype(np.float64) * scale.astype(np.float64)[..., None]
+            assert np.array_equal(got[:, had:], exact.swapaxes(0, 1))
