@@ -369,7 +369,8 @@ class AttentionExt:
         _ints("starts", starts, (batch,), dev)
         _ints("counts", counts, (batch,), dev)
         _count("tokens", tokens)
-        if isinstance(page_size, bool) or page_size not in PAGE_SIZES:
+        if isinstance(page_size, bool) or not hasattr(page_size, "__index__") \
+                or page_size not in PAGE_SIZES:
             _fail(f"the page size must be one of {PAGE_SIZES}, got {page_size!r}")
         _gpu("free_pages", free_pages, dev)
         _ints("free_pages", free_pages, (free_pages.numel(),), dev)

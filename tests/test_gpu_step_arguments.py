@@ -1,0 +1,30 @@
+"""GPU tests of what the calls of a step of many tokens accept and refuse."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import announce
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def att(cuda):
+    from cudalab_amd.build import build
+    return build("attention")
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def test_a_page_size_that_is_no_whole_number(att):
+    """RuntimeError as for any other argument; numpy's whole numbers are ones."""
+    args = _ints([[0, 1], [2, 3]]), _ints([0, 0]), _ints([3, 4]), 9
+    for page in (16.0, np.float64(16), "16", None):
+        with pytest.raises(RuntimeError):
+            att.place(*args, page, _ints([5, 6]))
+    announce("place, the page size as numpy's")
+    assert att.place(*args, np.int64(16), _ints([5, 6])).taken.tolist() == [2]
