@@ -509,9 +509,10 @@ class AttentionExt:
             return out.zero_()
 
         def aligned(t, most):
-            # the kernels read 16 bytes of a head at once
-            if t.numel() == 0 or not (t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:2])
-                                      or t.stride(0) > most):
+            # the kernels read 16 bytes of a head at once (and the strides of no keys
+            # are checked like any others')
+            if not (t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:2])
+                    or t.stride(0) > most):
                 return t
             return torch.empty(t.shape, dtype=t.dtype, device=dev).copy_(t)
 

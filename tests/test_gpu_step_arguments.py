@@ -28,3 +28,16 @@ def test_a_page_size_that_is_no_whole_number(att):
             att.place(*args, page, _ints([5, 6]))
     announce("place, the page size as numpy's")
     assert att.place(*args, np.int64(16), _ints([5, 6])).taken.tolist() == [2]
+
+
+def test_no_keys_of_any_strides(att):
+    """Without keys rows are zeros, whatever the strides of nothing are."""
+    q = torch.randn(7, 4, 64, device="cuda").half()
+    none = _ints([0, 0])
+    wide = torch.zeros(3, 2, 67, device="cuda").half()
+    far = torch.zeros(1, dtype=torch.float16, device="cuda").as_strided((0, 2, 64),
+                                                                        (2 ** 25, 64, 1))
+    for kv in (wide[:0, :, 3:], wide[:0, :, :64], far):
+        announce(f"prompt without keys, strides {kv.stride()}")
+        got = att.prompt(q, kv, kv, _ints([0, 7]), k_offsets=none)
+        assert bool((got == 0).all())
