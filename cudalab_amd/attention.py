@@ -447,7 +447,8 @@ class AttentionExt:
                     offsets: torch.Tensor, out: torch.Tensor, *,
                     k_offsets: Optional[torch.Tensor] = None, causal: bool = True,
                     scale: Optional[float] = None) -> None:
-        """Attention of packed sequences into a given contiguous `out`.
+        """Attention of packed sequences into a given contiguous `out` that starts at
+        16 bytes.
 
         q (tokens, Hq, D), k and v (keys, H, D), float16 or bfloat16, as they are
         before they enter a cache: nothing is quantized.  Sequence b's n queries
@@ -553,7 +554,7 @@ class AttentionExt:
                      prefix: Optional[tuple[torch.Tensor, int]] = None,
                      scale: Optional[float] = None,
                      tree: Optional[torch.Tensor] = None) -> None:
-        """Attention into a given contiguous `out`.
+        """Attention into a given contiguous `out` that starts at 16 bytes.
 
         Sequence b holds lengths[b] tokens in the pages block_table[b]; the
         last counts[b] of them (all `tokens` if None) are the call's own: query

@@ -89,7 +89,7 @@ class QgemmExt:
     def forward_into(self, codes: torch.Tensor, scales: torch.Tensor, W_q: torch.Tensor,
                      scale: torch.Tensor, out: torch.Tensor) -> None:
         """The product into a given contiguous `out` (tokens, N), float16, bfloat16
-        or float32:
+        or float32, that starts at 16 bytes:
 
             out[t, n] = (sum_k codes[t, k] W_q[n, k]) * scales[t] * scale[n]
 

@@ -41,3 +41,21 @@ def test_no_keys_of_any_strides(att):
         announce(f"prompt without keys, strides {kv.stride()}")
         got = att.prompt(q, kv, kv, _ints([0, 7]), k_offsets=none)
         assert bool((got == 0).all())
+
+
+def test_outputs_off_16_bytes(att):
+    """An `out` that does not start at 16 bytes is refused, and stays as it was."""
+    from cudalab_amd.build import build
+    gemm = build("qgemm")
+    q = torch.randn(9, 2, 64, device="cuda").half()
+    flat = torch.full((9 * 2 * 64 + 8,), 7.0, dtype=torch.float16, device="cuda")
+    w = torch.ones(64, 32, dtype=torch.int8, device="cuda")
+    x, one = torch.ones(18, 32, dtype=torch.int8, device="cuda"), torch.ones(64, device="cuda")
+    for off in (1, 4):
+        out = flat[off:off + q.numel()].view(q.shape)
+        with pytest.raises(RuntimeError, match="16-byte"):
+            att.prompt_into(q, q, q, _ints([0, 9]), out)
+        with pytest.raises(RuntimeError, match="16-byte"):
+            gemm.forward_into(x, one[:18], w, one, out.view(18, 64))
+    torch.cuda.synchronize()
+    assert bool((flat == 7).all())
