@@ -21,14 +21,12 @@ int set_error(int code, const std::string& msg);
 constexpr int64_t kMaxGrid = 0x7FFFFFFF;
 constexpr int64_t kMaxLaunch = 0xFFFFFFFF / 256;
 
-// go(workgroups, first) for each launch of a call of `grid` workgroups of
-// `threads` (a multiple of 256).
+// go(workgroups, first) for each launch of a call of `grid` workgroups.
 template <class Go>
-hipError_t launch_parts(int64_t grid, Go&& go, int threads = 256) {
+hipError_t launch_parts(int64_t grid, Go&& go) {
     hipError_t e = hipSuccess;
-    const int64_t most = kMaxLaunch / (threads / 256);
-    for (int64_t first = 0; first < grid && e == hipSuccess; first += most) {
-        go(dim3((unsigned)std::min(grid - first, most)), (uint32_t)first);
+    for (int64_t first = 0; first < grid && e == hipSuccess; first += kMaxLaunch) {
+        go(dim3((unsigned)std::min(grid - first, kMaxLaunch)), (uint32_t)first);
         e = hipGetLastError();
     }
     return e;

@@ -72,12 +72,6 @@ __device__ __forceinline__ void load_to_lds(void* to, const void* base, int byte
         buffer_of(base, bytes), (__attribute__((address_space(3))) void*)to, 16, at, 0, 0, 0);
 }
 
-// 16 bytes of a buffer, to registers.
-__device__ __forceinline__ Vec<int, 4> load16(__amdgpu_buffer_rsrc_t from, int at) {
-    using i4 = Vec<int, 4>;
-    return __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0));
-}
-
 // Page of a table entry, or -1 for one outside the cache.
 __device__ __forceinline__ int64_t page_in(int32_t entry, int64_t pages) {
     return entry >= 0 && entry < pages ? (int64_t)entry : -1;
