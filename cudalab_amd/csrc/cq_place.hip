@@ -47,8 +47,10 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t cap, uint32_
     return v;
 }
 
-__global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, const int32_t* held_in,
-                                                       int32_t* held_out, uint32_t first_block) {
+// HELD: with counts of held pages (either may be null).
+template <bool HELD>
+__global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, uint32_t first_block,
+                                                       const int32_t* held_in, int32_t* held_out) {
     __shared__ uint32_t sums[kBlock / 64];
     // of 256 sequences: where their tokens end, begin and start, and their pages
     __shared__ uint32_t end[kBlock], begin[kBlock], start[kBlock], have[kBlock], page0[kBlock];
@@ -65,7 +67,7 @@ __global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, const int32
         if (b < (uint32_t)a.batch) {
             n = (uint32_t)max(0, a.counts[b]);
             s = (uint32_t)max(0, a.starts[b]);
-            if (held_in != nullptr) own = (uint32_t)max(0, held_in[b]);
+            if (HELD && held_in != nullptr) own = (uint32_t)max(0, held_in[b]);
         }
         // what does not fit the call's tokens is not placed
         const uint32_t upto = min(placed + block_scan(min(n, tokens), tokens, sums), tokens);
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(kBlock) void place_kernel(cq_place_t a, const int32
             if (b == 0) a.offsets[0] = 0;
             a.offsets[b + 1] = (int32_t)upto;
             a.lengths[b] = (int32_t)min(s + n, kMost);
-            if (held_out != nullptr) {         // of the pages it needs those that the list has
+            if (HELD && held_out != nullptr) {         // of the pages it needs those that the list has
                 const uint64_t at = (uint64_t)taken + page0[tid];
                 const uint64_t left =
                     (uint64_t)a.free_count > at ? (uint64_t)a.free_count - at : 0;
@@ -143,7 +145,10 @@ hipError_t launch_place_held(const cq_place_t& a, const int32_t* held_in, int32_
                              hipStream_t stream) {
     const int64_t grid = std::max<int64_t>(1, (a.tokens + kTokens - 1) / kTokens);
     return launch_parts(grid, [&](dim3 blocks, uint32_t first) {
-        place_kernel<<<blocks, dim3(kBlock), 0, stream>>>(a, held_in, held_out, first);
+        if (held_in != nullptr || held_out != nullptr)
+            place_kernel<true><<<blocks, dim3(kBlock), 0, stream>>>(a, first, held_in, held_out);
+        else
+            place_kernel<false><<<blocks, dim3(kBlock), 0, stream>>>(a, first, nullptr, nullptr);
     });
 }
 
