@@ -1307,8 +1307,12 @@ Shape shape_of(int64_t rows, int64_t units, int64_t keys, int d) {
 }
 
 // A tree's tokens are many rows of one sequence: where units of 256 rows would leave
-// half of the last one empty, units of 128 (16 sequences of up to 8000 keys, 48 tokens,
-// 64/8 heads of 128, INT8: 384 rows, us: 230 and 190).
+// half of the last one empty, units of 128, although more of them unpack each tile
+// (64/8 heads of 128, INT8, us with units of 256 and of 128:
+//   rows                               384       560       640       1152
+//   16 sequences of up to 8000 keys  242 191   348 292   350 296   573 529
+//   2 of up to 8000                   64  53    82  77    83  79   123 118
+//   64 of up to 1000                 220 195   345 282   358 297   598 520).
 Shape tree_shape_of(int64_t rows, int64_t units, int64_t keys, int d) {
     const Shape s = shape_of(rows, units, keys, d);
     return s.waves == 8 && (rows + 127) / 128 % 2 != 0 ? Shape{0, 4, 128, 2} : s;

@@ -21,9 +21,10 @@
 // with.  Pieces of 16 bytes are stored at places turned by the row, so that
 // neither read meets its own banks.
 //
-// Rounded to fewer than 32 bits: p to V's type before it multiplies (2^-11 of
-// each weight in fp16, 2^-8 in bf16; l is summed from the unrounded), and the
-// result.
+// Rounded to fewer than 32 bits: p to V's type before it multiplies, and the
+// result.  In bf16 that is off by up to 2^-8 of a weight; in fp16 by up to 2^-11 of
+// it, and where p is below 2^-14, a subnormal number there, by up to 2^-25 of the
+// weight at M (p below that is 0).  l is summed from the unrounded.
 //
 // A key that a row does not see has p = 0; so that an Inf or NaN in its V stays
 // out of the sums, tiles that some row sees only part of are looked through for
@@ -34,11 +35,12 @@
 // finds its tile of rows by itself.  Tiles that see the same keys run side by side.
 //
 // Bound by the softmax between the products: counters of one sequence of 8192 tokens,
-// 64/8 heads of 128, say 59% of the time in matrix instructions and 50% in vector ones,
-// at a clock that power has brought to 1.8 GHz.  That is 1.04 ms causal (1050 TFLOP/s,
-// a large plain product 1360 to 1560).  16 sequences of up to 2048, 32/32 heads of
-// 128, 290 us; five of up to 100, 28/4 heads of 64, 7 us.  Reading LDS one product
-// ahead, priorities for the waves in the products, and eight waves gained nothing.
+// 64/8 heads of 128, all keys seen, say 59% of the time in matrix instructions and 50%
+// in vector ones, at a clock that power has brought to 1.8 GHz.  It takes 1.97 ms
+// (1117 TFLOP/s; a large plain product 1360 to 1560), causal 1.02 ms (1080).  16
+// sequences of up to 2048, 32/32 heads of 128, 288 us; five of up to 100, 28/4 heads of
+// 64, 7 us.  Reading LDS one product ahead, priorities for the waves in the products,
+// and eight waves gained nothing.
 
 #include <algorithm>
 #include <type_traits>
@@ -103,8 +105,8 @@ __device__ __forceinline__ float half_fold(float v, F&& f) {
 // more.  Of few sequences each lane looks at one, of more a bisection finds a place's
 // part.  The last places come first: of a sequence its last tile, which sees the most
 // keys.  (Sorting the sequences by length, in a search over all of them, gained nothing
-// and took 164 us instead of 104 for 200 sequences of 40 tokens.)  Offsets are cut to
-// the tensors' rows.
+// and took 200 sequences of 40 tokens from 104 to 164 us, one head to a workgroup.)
+// Offsets are cut to the tensors' rows.
 struct Tile {
     int row0, rows, first;             // rows <= 0: none
     int tokens, key0, keys;            // of the sequence; none for rows of no sequence
@@ -443,7 +445,8 @@ hipError_t launch_prompt(const cq_prompt_t& a, hipStream_t stream) {
     s.group = a.q_heads / a.k_heads;
     // where sequences are short of a workgroup's 128 rows, two or four heads of a key
     // head share it (200 sequences of 40 tokens, 32/8 heads of 128, us: one head 98, two
-    // 66; of 20 tokens: one 92, four 37)
+    // 66; of 20 tokens: one 92, four 37; heads without groups have no such form, and 32/32
+    // heads take 103 and 95)
     const int64_t rows = a.q_tokens / a.batch;
     s.heads = rows <= 32 && s.group % 4 == 0 ? 4 : rows <= 64 && s.group % 2 == 0 ? 2 : 1;
     s.shift = __builtin_ctz((unsigned)(kRows * kWaves / s.heads));

@@ -33,7 +33,8 @@ __device__ __forceinline__ uint32_t magnitude(T x) {
 
 // One workgroup to a token; what it holds of the row (HOLD pieces of 8 elements a
 // thread) is read once, the rest again.  Codes need no clamp: x * inv lies within
-// 127 (1 + 2^-21).  Bound by memory: 4096 tokens of 8192 in fp16 19 us, 5.3 TB/s.
+// 127 (1 + 2^-21).  Bound by memory: 4096 tokens of 8192 in fp16 17.3 us, in fp32 28.8,
+// 5.8 TB/s.
 template <class T, int HOLD>
 __global__ __launch_bounds__(kBlock) void quantize_kernel(const T* x, int64_t stride, int64_t k,
                                                           int8_t* codes, float* scales, uint32_t first) {
@@ -395,15 +396,19 @@ hipError_t launch_tiles(const Product& a, hipStream_t stream) {
 // Where even the largest of these is too many, two workgroups of 128 x 128 to a CU, or
 // one of 256 x 256: per 128 codes a CU's pair takes 1.34 us (a workgroup alone 0.8),
 // the large one 2.07 us, in as many rounds as they need.  (us: 4096 tokens, 11008 x 4096
-// 208, 194; 28672 x 8192 965, 888, of which the matrix units need 897 at the rate of
-// the library's largest product.)
+// 208, 194; 28672 x 8192 965, 888 or 2170 TOP/s, where the library's product of that size
+// reaches 2210.)
+// By that rule 1 to 64 tokens take, us: 8192 x 8192 15.4 to 18.6, 8192 x 28672 49 to 59
+// (64x32, one workgroup to a CU); 16384 x 8192 40 to 46 (64x32, two to a CU, where 65
+// tokens take 34 by 128x64); 16448 x 8192 39 to 42 and 28672 x 8192 52 (128x128, 129 and
+// 224 workgroups; their weights alone 23 and 39); 1024 x 8192 11 (64x32, 32 workgroups).
 template <class T>
 hipError_t launch_typed(const Product& a, hipStream_t stream) {
     auto tiles = [&](int64_t m, int64_t n) {
         return ((a.tokens + m - 1) / m) * ((a.n + n - 1) / n);
     };
     constexpr int kCus = 256;
-    // (few tokens are bound by memory: two workgroups to a CU do no harm)
+    // (few tokens are bound by memory, and take it up to two workgroups to a CU)
     if (a.tokens <= 64 && tiles(64, 32) <= 2 * kCus)
         return launch_tiles<T, 64, 32, 1, 1, 4, 256, 4>(a, stream);
     if (tiles(64, 64) <= kCus) return launch_tiles<T, 64, 64, 1, 1, 4, 256, 3>(a, stream);
