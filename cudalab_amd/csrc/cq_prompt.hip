@@ -34,10 +34,12 @@
 // Rows and keys lie wherever the offsets on the device say, so every workgroup
 // finds its tile of rows by itself.  Tiles that see the same keys run side by side.
 //
-// Bound by the softmax between the products: counters of one sequence of 8192 tokens,
-// 64/8 heads of 128, all keys seen, say 59% of the time in matrix instructions and 50%
-// in vector ones, at a clock that power has brought to 1.8 GHz.  It takes 1.97 ms
-// (1117 TFLOP/s; a large plain product 1360 to 1560), causal 1.02 ms (1080).  16
+// Bound by the softmax between the products: counters of one causal sequence of 8192
+// tokens, 64/8 heads of 128, say 55% of the time in matrix instructions and 49% in vector
+// ones (all keys seen: 59 and 49), at a clock that power has brought to 1.5 to 1.8 GHz by
+// the card.  That is 1.02 ms (1080 TFLOP/s; a large plain product 1360 to 1560), all keys
+// 1.97 ms (1117).  Heads of 64 have half the products beside the same softmax (42 and 66%,
+// 0.62 ms), heads of 256 a single wave to a SIMD (29 and 30% at 4096 tokens, 0.76 ms).  16
 // sequences of up to 2048, 32/32 heads of 128, 288 us; five of up to 100, 28/4 heads of
 // 64, 7 us.  Reading LDS one product ahead, priorities for the waves in the products,
 // and eight waves gained nothing.
