@@ -94,8 +94,9 @@ class PromptModel:
         return x, kept
 
     def prompt(self, x: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
-        """The first counts[b] tokens of each sequence, packed in x (rows, hidden)
-        fp16; rows behind the last sequence are carried along and belong to none."""
+        """The first counts[b] tokens of each sequence (0 for one that has some: these
+        would see nothing that is in the caches), packed in x (rows, hidden) fp16;
+        rows behind the last sequence are carried along and belong to none."""
         p = self.att.place(self.table, self.lengths, counts, x.size(0), PAGE, self.free,
                            self.taken, held=self.held)
         self.lengths, self.taken, self.held = p.lengths, p.taken, p.held
